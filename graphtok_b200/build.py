@@ -24,7 +24,8 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC", "--shared", "--threads", "8",
     "-Xlinker", "--version-script=" + os.path.join(CSRC, "gtok.map"),
 ]
-SOURCES = ["encode_kernels.cu", "tiny_kernel.cu", "engine.cu", "gtok_abi.cc", "vocab_host.cc", "tables_build.cc", "nfc_host.cc", "host_text.cc"]
+SOURCES = ["encode_kernels.cu", "tiny_kernel.cu", "engine.cu", "gtok_abi.cc", "vocab_host.cc", "tables_build.cc", "nfc_host.cc", "host_text.cc",
+           "vocab_rows.cu", "vocab_loss.cu", "vocab_abi.cc"]
 
 
 def _newer(target, deps):
@@ -40,7 +41,7 @@ def source_hash():
     import hashlib
     h = hashlib.sha256()
     for name in sorted(os.listdir(CSRC)):
-        if name.endswith((".h", ".cu", ".cc", ".map")):
+        if name.endswith((".h", ".cu", ".cuh", ".cc", ".map")):
             with open(os.path.join(CSRC, name), "rb") as f:
                 h.update(name.encode() + b"\0" + f.read())
     with open(os.path.join(HERE, "..", "include", "gtok.h"), "rb") as f:

@@ -92,6 +92,10 @@ int32_t do_encode_batch(Handle* h, const uint8_t* concat_bytes, const uint32_t* 
 
 }  // namespace
 
+namespace gtok {
+void set_last_error(const char* message) { g_last_error = message; }
+}  // namespace gtok
+
 extern "C" {
 
 void* gtok_create(const char* vocab_json_path, uint32_t max_bytes) {

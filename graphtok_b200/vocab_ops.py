@@ -1,0 +1,384 @@
+"""Operators between token ids and a model, on torch tensors: embedding lookup, next-token cross entropy and distillation over
+the whole vocabulary, each with its gradient.
+
+They take ids as `Tokenizer.encode_to_device` and `encode_batch_to_device` leave them on the GPU, run as kernels of
+libgtok.so (`gtok_x_embed` and the entries after it in include/gtok.h, where the formulas are) on torch's current stream, and wait for
+nothing.  Every call makes its own outputs and workspace by torch's allocator, so calls may be captured into CUDA graphs and may
+run on several streams at once.
+
+    ids, offsets = tokenizer.encode_batch_to_device(texts)
+    hidden = model(embed(ids, table, scale=...))
+    loss = cross_entropy(hidden, out_table, next_targets(ids, offsets))
+    loss.backward()
+
+`embed`, `cross_entropy` and `distill` take part in autograd.  `embed_grad`, `cross_entropy_forward`, `cross_entropy_grad`,
+`distill_forward` and `distill_grad` are the same passes for programs that keep their own graph of them.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import GTokError, load_lib
+
+__all__ = ["embed", "embed_grad", "next_targets", "cross_entropy", "cross_entropy_forward", "cross_entropy_grad", "distill", "distill_forward", "distill_grad"]
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_IDS = {torch.int32: 32, torch.int64: 64}
+MAX_ENTRIES = 1024
+
+
+class _Matrix(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("stride", ctypes.c_int64), ("type", ctypes.c_int32)]
+
+
+class _Loss(ctypes.Structure):
+    _fields_ = [("hidden", _Matrix), ("weight", _Matrix), ("targets", ctypes.c_void_p), ("target_stride", ctypes.c_int64),
+                ("target_bits", ctypes.c_int32), ("entries", ctypes.c_int32), ("teacher_logits", _Matrix), ("ignore", ctypes.c_int64),
+                ("temperature", ctypes.c_float), ("mean", ctypes.c_int32), ("losses", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("total", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("grad_stride", ctypes.c_int64), ("d_hidden", _Matrix),
+                ("d_weight", _Matrix), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("cuda_stream", ctypes.c_void_p)]
+
+
+_bound = None
+
+
+def _lib():
+    global _bound
+    if _bound is None:
+        lib = load_lib()
+        vp, i32, i64, u64, mat = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.POINTER(_Matrix)
+        lib.gtok_x_embed.restype = i32
+        lib.gtok_x_embed.argtypes = [vp, i32, i64, mat, ctypes.c_float, mat, vp]
+        lib.gtok_x_embed_grad_workspace.restype = i64
+        lib.gtok_x_embed_grad_workspace.argtypes = [i64, i64, i64]
+        lib.gtok_x_embed_grad.restype = i32
+        lib.gtok_x_embed_grad.argtypes = [vp, i32, i64, mat, ctypes.c_float, mat, i32, vp, u64, vp]
+        lib.gtok_x_next_targets.restype = i32
+        lib.gtok_x_next_targets.argtypes = [vp, i64, vp, i64, vp, i32, vp, vp]
+        lib.gtok_x_vocab_loss_workspace.restype = i64
+        lib.gtok_x_vocab_loss_workspace.argtypes = [ctypes.POINTER(_Loss), i32]
+        for f in (lib.gtok_x_vocab_loss_forward, lib.gtok_x_vocab_loss_backward):
+            f.restype = i32
+            f.argtypes = [ctypes.POINTER(_Loss)]
+        _bound = lib
+    return _bound
+
+
+def _done(code, what):
+    if code < 0:
+        raise GTokError("%s returned %d: %s" % (what, code, _bound.gtok_x_last_error().decode("utf-8", "replace")))
+    return code
+
+
+def _on_gpu(device, **tensors):
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("%s must be a torch tensor" % name)
+        if t.layout is not torch.strided:
+            raise TypeError("%s must be a dense tensor" % name)
+        if t.device != device:
+            raise ValueError("%s is on %s, other arguments on %s" % (name, t.device, device))
+    if device.type != "cuda":
+        raise ValueError("tensors must be on the GPU, not on %s" % device)
+
+
+def _ids_of(name, t):
+    if t.dtype not in _IDS:
+        raise TypeError("%s must be int32 or int64, not %s" % (name, t.dtype))
+    return t.reshape(-1).contiguous()
+
+
+def _rows(t):
+    """`t` with its rows' elements next to one another (a copy only where they are not)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _matrix(t):
+    rows, cols = t.shape
+    return _Matrix(t.data_ptr(), rows, cols, t.stride(0) if rows > 1 else cols, _TYPES[t.dtype])
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _scale(scale):
+    scale = float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    return scale
+
+
+# ---- embedding -------------------------------------------------------------------
+def _table(name, t):
+    if t.dim() != 2:
+        raise ValueError("%s must have two dimensions" % name)
+    if t.dtype not in _TYPES:
+        raise TypeError("%s must be float32, bfloat16 or float16, not %s" % (name, t.dtype))
+    if t.shape[1] < 1:
+        raise ValueError("%s must have columns" % name)
+
+
+def _embed(ids, table, scale):
+    flat, rows = _ids_of("ids", ids), _rows(table)
+    with torch.cuda.device(table.device):
+        out = torch.empty((flat.numel(), table.shape[1]), dtype=table.dtype, device=table.device)
+        _done(_lib().gtok_x_embed(flat.data_ptr(), _IDS[flat.dtype], flat.numel(), _matrix(rows), scale, _matrix(out), _stream()), "gtok_x_embed")
+    return out.view(*ids.shape, table.shape[1])
+
+
+class _Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale):
+        ctx.save_for_backward(ids)
+        ctx.vocab, ctx.scale = table.shape[0], scale
+        return _embed(ids, table, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        ids, = ctx.saved_tensors
+        return None, embed_grad(ids, grad, ctx.vocab, scale=ctx.scale), None
+
+
+def embed(ids, table, scale=1.0):
+    """Rows of `table` [vocab, width] (float32, bfloat16 or float16) by id, times `scale`: a tensor of ids.shape + (width,).
+
+    ids: int32 or int64, any shape.  A negative id gives a row of zeros, one beyond the table a row of NaN; neither has a gradient."""
+    _on_gpu(getattr(table, "device", None) or torch.device("cpu"), table=table, ids=ids)
+    _table("table", table)
+    scale = _scale(scale)
+    if table.requires_grad and torch.is_grad_enabled():
+        return _Embed.apply(ids, table, scale)
+    return _embed(ids, table, scale)
+
+
+def embed_grad(ids, grad, vocab, scale=1.0, out=None, accumulate=False):
+    """Gradient of `embed`: [vocab, width] with, for each id, `scale` times the sum of the rows of `grad` (ids.shape + (width,)) that were
+    looked up from it, 0 for ids that were not.  The sum is in float32 and in the order of the ids, whatever they are.
+
+    out: where to write it, of grad's type.  With `accumulate` it is added to what `out` holds, as for a table that is an
+    output table too, and rows that are not asked for are not touched."""
+    _on_gpu(getattr(grad, "device", None) or torch.device("cpu"), grad=grad, ids=ids)
+    if grad.shape[:-1] != ids.shape or grad.dim() < 1:
+        raise ValueError("grad must have the shape of ids and one dimension more")
+    width, vocab = grad.shape[-1], int(vocab)
+    flat = _ids_of("ids", ids)
+    rows = _rows(grad.reshape(-1, width) if width else grad)
+    _table("grad", rows)
+    if vocab < 0:
+        raise ValueError("vocab must not be negative")
+    if accumulate and out is None:
+        raise ValueError("accumulate needs `out`")
+    scale = _scale(scale)
+    if out is not None:
+        _on_gpu(grad.device, out=out)
+        if out.shape != (vocab, width) or out.dtype != grad.dtype or (width > 1 and out.stride(1) != 1):
+            raise ValueError("out must be [vocab, width] of grad's type with the elements of a row next to one another")
+    with torch.cuda.device(grad.device):
+        if out is None:
+            out = torch.empty((vocab, width), dtype=grad.dtype, device=grad.device)
+        lib = _lib()
+        need = _done(lib.gtok_x_embed_grad_workspace(flat.numel(), vocab, width), "gtok_x_embed_grad_workspace")
+        work = torch.empty(need, dtype=torch.uint8, device=grad.device)
+        _done(lib.gtok_x_embed_grad(flat.data_ptr(), _IDS[flat.dtype], flat.numel(), _matrix(rows), scale, _matrix(out), int(bool(accumulate)),
+                                    work.data_ptr(), need, _stream()), "gtok_x_embed_grad")
+    return out
+
+
+# ---- targets ---------------------------------------------------------------------
+def next_targets(ids, offsets, loss_mask=None, ignore_index=-100):
+    """For packed documents as `Tokenizer.encode_batch_to_device` gives them (int32 ids, int32 n + 1 offsets): the id that follows each
+    position in its document, `ignore_index` at a document's last position, outside of all documents, and where the boolean
+    `loss_mask` (same length as ids) is false.  int32."""
+    _on_gpu(getattr(ids, "device", None) or torch.device("cpu"), ids=ids, offsets=offsets)
+    if ids.dtype != torch.int32 or ids.dim() != 1 or offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 1:
+        raise ValueError("ids and offsets must be one-dimensional and int32, offsets not empty")
+    if not -(1 << 31) <= ignore_index < 0:
+        raise ValueError("ignore_index must be negative, in 32 bits")
+    mask = None
+    if loss_mask is not None:
+        _on_gpu(ids.device, loss_mask=loss_mask)
+        if loss_mask.dtype != torch.bool or loss_mask.shape != ids.shape:
+            raise ValueError("loss_mask must be boolean and as long as ids")
+        mask = loss_mask.contiguous()
+    ids, offsets = ids.contiguous(), offsets.contiguous()
+    with torch.cuda.device(ids.device):
+        out = torch.empty_like(ids)
+        _done(_lib().gtok_x_next_targets(ids.data_ptr(), ids.numel(), offsets.data_ptr(), offsets.numel() - 1, mask.data_ptr() if mask is not None else None,
+                                         ignore_index, out.data_ptr(), _stream()), "gtok_x_next_targets")
+    return out
+
+
+# ---- losses over the vocabulary -----------------------------------------------------
+def _check_loss(hidden, weight, lead):
+    _on_gpu(getattr(hidden, "device", None) or torch.device("cpu"), hidden=hidden, weight=weight)
+    if hidden.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != hidden.dtype:
+        raise TypeError("hidden and weight must both be bfloat16 or both float16, not %s and %s" % (hidden.dtype, weight.dtype))
+    if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError("hidden must be [..., width] and weight [vocab, width]")
+    if hidden.shape[:-1] != lead:
+        raise ValueError("hidden and the targets differ in their leading dimensions")
+
+
+def _flat(hidden):
+    return _rows(hidden.reshape(-1, hidden.shape[-1]))
+
+
+class _Call:
+    """Arguments of one loss, checked, and what keeps their memory alive."""
+
+    def __init__(self, hidden, weight, targets=None, ignore_index=-100, teacher_ids=None, teacher_logits=None, temperature=1.0):
+        if teacher_ids is None:
+            ids = targets
+            _check_loss(hidden, weight, getattr(targets, "shape", None))
+        else:
+            ids = teacher_ids
+            _check_loss(hidden, weight, getattr(teacher_ids, "shape", (None,))[:-1])
+            _on_gpu(hidden.device, teacher_logits=teacher_logits)
+            if teacher_logits.shape != teacher_ids.shape or not 1 <= teacher_ids.shape[-1] <= MAX_ENTRIES:
+                raise ValueError("teacher_ids and teacher_logits must be [..., k] with k from 1 to %d" % MAX_ENTRIES)
+            if teacher_logits.dtype not in _TYPES:
+                raise TypeError("teacher_logits must be float32, bfloat16 or float16, not %s" % teacher_logits.dtype)
+        _on_gpu(hidden.device, ids=ids)
+        self.temperature = float(temperature)
+        if not (self.temperature > 0.0 and math.isfinite(self.temperature)):
+            raise ValueError("temperature must be positive and finite")
+        self.device, self.hidden, self.weight = hidden.device, _flat(hidden.detach()), _rows(weight.detach())
+        if self.weight.stride(0) < self.weight.shape[1] and self.weight.shape[0] > 1:
+            self.weight = self.weight.contiguous()
+        self.ids = _ids_of("targets" if teacher_ids is None else "teacher_ids", ids)
+        a = self.args = _Loss()
+        a.hidden, a.weight = _matrix(self.hidden), _matrix(self.weight)
+        a.targets, a.target_bits, a.ignore, a.temperature = self.ids.data_ptr(), _IDS[self.ids.dtype], int(ignore_index), self.temperature
+        if teacher_ids is not None:
+            k = teacher_ids.shape[-1]
+            self.logits = _rows(teacher_logits.detach().reshape(-1, k))
+            a.entries, a.target_stride, a.teacher_logits = k, k, _matrix(self.logits)
+
+    def _run(self, entry, backward):
+        a, lib = self.args, _lib()
+        need = _done(lib.gtok_x_vocab_loss_workspace(a, backward), "gtok_x_vocab_loss_workspace")
+        work = torch.empty(need, dtype=torch.uint8, device=self.device)
+        a.workspace, a.workspace_bytes, a.cuda_stream = work.data_ptr(), need, _stream()
+        _done(entry(a), entry.__name__)
+
+    def forward(self, reduction):
+        n = self.hidden.shape[0]
+        with torch.cuda.device(self.device):
+            losses, lse = torch.empty(n, dtype=torch.float32, device=self.device), torch.empty(n, dtype=torch.float32, device=self.device)
+            total = torch.empty((), dtype=torch.float32, device=self.device) if reduction != "none" else None
+            a = self.args
+            a.losses, a.lse, a.total, a.mean = losses.data_ptr(), lse.data_ptr(), total.data_ptr() if total is not None else None, reduction == "mean"
+            self._run(_lib().gtok_x_vocab_loss_forward, 0)
+        return (losses if total is None else total), lse
+
+    def backward(self, lse, grad, reduction, want_hidden, want_weight):
+        with torch.cuda.device(self.device):
+            a = self.args
+            lse, grad = lse.reshape(-1).contiguous(), grad.detach().reshape(-1)
+            a.lse, a.grad, a.mean = lse.data_ptr(), grad.data_ptr(), reduction == "mean"
+            a.grad_stride = grad.stride(0) if reduction == "none" and grad.numel() > 1 else 0
+            d_hidden = torch.empty(self.hidden.shape, dtype=self.hidden.dtype, device=self.device) if want_hidden else None
+            d_weight = torch.empty(self.weight.shape, dtype=self.weight.dtype, device=self.device) if want_weight else None
+            for name, t in (("d_hidden", d_hidden), ("d_weight", d_weight)):
+                if t is not None:
+                    setattr(a, name, _matrix(t))
+            self._run(_lib().gtok_x_vocab_loss_backward, 1)
+        return d_hidden, d_weight
+
+
+def _check_reduction(reduction):
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError("reduction must be 'mean', 'sum' or 'none'")
+
+
+def _check_grad(lse, grad, lead, reduction, device):
+    _check_reduction(reduction)
+    _on_gpu(device, lse=lse, grad=grad)
+    if lse.dtype != torch.float32 or grad.dtype != torch.float32:
+        raise TypeError("lse and grad must be float32")
+    if lse.shape != lead or grad.shape != (lead if reduction == "none" else ()):
+        raise ValueError("lse must have the targets' shape, grad that of the loss")
+
+
+class _LossFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, ids, teacher_logits, reduction, ignore_index, temperature):
+        loss, lse = _call(hidden, weight, ids, teacher_logits, ignore_index, temperature).forward(reduction)
+        ctx.save_for_backward(hidden, weight, ids, teacher_logits, lse)
+        ctx.rest = reduction, ignore_index, temperature
+        return loss.view(hidden.shape[:-1]) if reduction == "none" else loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        hidden, weight, ids, teacher_logits, lse = ctx.saved_tensors
+        reduction, ignore_index, temperature = ctx.rest
+        d_hidden, d_weight = _call(hidden, weight, ids, teacher_logits, ignore_index, temperature).backward(lse, grad, reduction, *ctx.needs_input_grad[:2])
+        return d_hidden.view(hidden.shape) if d_hidden is not None else None, d_weight, None, None, None, None, None
+
+
+def _call(hidden, weight, ids, teacher_logits, ignore_index, temperature):
+    if teacher_logits is None:
+        return _Call(hidden, weight, targets=ids, ignore_index=ignore_index, temperature=temperature)
+    return _Call(hidden, weight, teacher_ids=ids, teacher_logits=teacher_logits, temperature=temperature)
+
+
+def _loss(hidden, weight, ids, teacher_logits, reduction, ignore_index, temperature):
+    _check_reduction(reduction)
+    call = _call(hidden, weight, ids, teacher_logits, ignore_index, temperature)
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _LossFunction.apply(hidden, weight, ids, teacher_logits, reduction, ignore_index, temperature)
+    loss, _ = call.forward(reduction)
+    return loss.view(hidden.shape[:-1]) if reduction == "none" else loss
+
+
+def cross_entropy(hidden, weight, targets, reduction="mean", ignore_index=-100, temperature=1.0):
+    """Softmax cross entropy of the logits hidden @ weight.T / temperature against `targets`, without holding the logits.
+
+    hidden: [..., width], weight: [vocab, width], both bfloat16 or both float16; targets: int32 or int64 of hidden's leading shape.
+    Targets of `ignore_index`, or negative, carry no loss and no gradient; a target beyond the vocabulary gives NaN.
+    reduction: 'none' (float32 of the targets' shape), 'sum', or 'mean' over the rows that carry a loss (0 where none does)."""
+    return _loss(hidden, weight, targets, None, reduction, ignore_index, temperature)
+
+
+def cross_entropy_forward(hidden, weight, targets, reduction="none", ignore_index=-100, temperature=1.0):
+    """(loss, lse): what `cross_entropy` returns and the float32 logarithms of the rows' sums, which `cross_entropy_grad` takes."""
+    _check_reduction(reduction)
+    loss, lse = _call(hidden, weight, targets, None, ignore_index, temperature).forward(reduction)
+    return (loss.view(targets.shape) if reduction == "none" else loss), lse.view(targets.shape)
+
+
+def cross_entropy_grad(hidden, weight, targets, lse, grad, reduction="none", ignore_index=-100, temperature=1.0, want_hidden=True, want_weight=True):
+    """(d_hidden, d_weight) for the gradient `grad` of the loss (float32, of its shape); None for what is not wanted."""
+    call = _call(hidden, weight, targets, None, ignore_index, temperature)
+    _check_grad(lse, grad, targets.shape, reduction, hidden.device)
+    d_hidden, d_weight = call.backward(lse, grad, reduction, want_hidden, want_weight)
+    return d_hidden.view(hidden.shape) if d_hidden is not None else None, d_weight
+
+
+def distill(hidden, weight, teacher_ids, teacher_logits, temperature=1.0, reduction="mean"):
+    """Divergence of a student's softmax from a teacher's top logits, both over `temperature`, without holding the student's logits.
+
+    hidden, weight: as in `cross_entropy`.  teacher_ids (int32 or int64) and teacher_logits: [..., k], k up to 1024, in any order;
+    a negative id is no entry.  The teacher's probabilities are the softmax over a row's entries; a row without any carries no loss.
+    The customary factor temperature ** 2 is not applied.  There is no gradient for the teacher."""
+    return _loss(hidden, weight, teacher_ids, teacher_logits, reduction, -100, temperature)
+
+
+def distill_forward(hidden, weight, teacher_ids, teacher_logits, temperature=1.0, reduction="none"):
+    """(loss, lse), as `cross_entropy_forward`."""
+    _check_reduction(reduction)
+    loss, lse = _call(hidden, weight, teacher_ids, teacher_logits, -100, temperature).forward(reduction)
+    lead = hidden.shape[:-1]
+    return (loss.view(lead) if reduction == "none" else loss), lse.view(lead)
+
+
+def distill_grad(hidden, weight, teacher_ids, teacher_logits, lse, grad, temperature=1.0, reduction="none", want_hidden=True, want_weight=True):
+    """(d_hidden, d_weight), as `cross_entropy_grad`."""
+    call = _call(hidden, weight, teacher_ids, teacher_logits, -100, temperature)
+    _check_grad(lse, grad, hidden.shape[:-1], reduction, hidden.device)
+    d_hidden, d_weight = call.backward(lse, grad, reduction, want_hidden, want_weight)
+    return d_hidden.view(hidden.shape) if d_hidden is not None else None, d_weight

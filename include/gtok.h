@@ -200,6 +200,77 @@ int32_t gtok_x_take_bytes(void* handle, uint8_t* out);
 int32_t gtok_x_plan_chunks(void* handle, const uint8_t* text, uint64_t len, uint32_t n_parts, uint64_t* out_offsets);
 int32_t gtok_x_plan_documents(const uint32_t* doc_byte_offsets, uint32_t n_docs, uint32_t n_parts, uint32_t* out_doc_index);
 
+/* ---- between token ids and a model -----------------------------------------------
+ * No counterpart in the reference.  What a model does with token ids at its two ends that are as wide as the
+ * vocabulary: rows of the embedding table are looked up by id, and the hidden states of each position are
+ * compared with the id that follows there.  These entries work on device memory only, need no handle and no
+ * vocabulary file, allocate nothing, wait for nothing and read nothing back: the work is queued on `cuda_stream` (a
+ * cudaStream_t of the current device, NULL = its default stream), may be captured into a graph, and calls on different
+ * streams may overlap as long as each has a workspace of its own.  A workspace is device memory of at least the size
+ * that the _workspace entry answers, aligned to 256 bytes; nothing in it outlives the call's work.
+ * 0 or -1 (see gtok_x_last_error); sizes, types, strides and addresses are checked before anything is queued.
+ * Results do not depend on how the GPU schedules the work.  Sums are in fp32, rounded once to the output's type
+ * unless a comment says otherwise.  Outputs must not overlap inputs. */
+typedef struct {
+    void* data;              /* device memory */
+    int64_t rows, cols;
+    int64_t stride;          /* elements from a row to the next; elements of a row follow one another */
+    int32_t type;            /* 0 fp32, 1 bf16, 2 fp16 */
+} gtok_x_matrix;
+
+/* out[t, :] = scale * table[ids[t], :] for n ids of `id_bits` (32 or 64) bits.  A negative id gives a row of zeros,
+ * an id beyond the table a row of NaN. */
+int32_t gtok_x_embed(const void* ids, int32_t id_bits, int64_t n, const gtok_x_matrix* table, float scale, const gtok_x_matrix* out, void* cuda_stream);
+/* Its gradient: out[v, :] = scale * (sum of grad[t, :] over the t with ids[t] = v), summed in the order of the ids; rows that no
+ * id asks for become 0.  With `accumulate` the sums are added to what `out` holds (rounded once more) and other rows stay.
+ * Ids outside the table are left out. */
+int64_t gtok_x_embed_grad_workspace(int64_t n, int64_t vocab, int64_t width);
+int32_t gtok_x_embed_grad(const void* ids, int32_t id_bits, int64_t n, const gtok_x_matrix* grad, float scale, const gtok_x_matrix* out, int32_t accumulate,
+                          void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+/* Targets of packed documents, as gtok_x_encode_batch_to_device leaves them: out[i] = ids[i + 1] where i and i + 1 lie in the
+ * same document, else `ignore`; `ignore` also where loss_mask (may be NULL) is 0 and outside of all documents.
+ * doc_offsets: n_docs + 1 ascending places. */
+int32_t gtok_x_next_targets(const int32_t* ids, int64_t n, const int32_t* doc_offsets, int64_t n_docs, const uint8_t* loss_mask, int32_t ignore, int32_t* out,
+                            void* cuda_stream);
+
+/* Losses over the vocabulary from hidden states H [n, width] and an output table W [vocab, width] (both bf16 or both fp16),
+ * with logits Z = H W^T that are never held as a whole:
+ *   entries == 0   cross entropy: losses[i] = lse(z_i / T) - z_i[targets[i]] / T.  A negative target and `ignore` are no loss
+ *   entries > 0    distillation from a teacher's `entries` (at most 1024) top logits a row: ids in `targets` (rows
+ *                  `target_stride` apart; a negative id is no entry), logits of any type in teacher_logits.  With q the softmax of a row's
+ *                  logits / T, losses[i] = sum_k q_k (log q_k - z_i[id_k] / T + lse(z_i / T)); an id that comes twice counts twice.
+ *                  A row without entries, or with logits of -infinity only, is no loss
+ * Rows without a loss get 0 and leave no trace in any gradient, whatever H holds there; a target or entry beyond the vocabulary gives
+ * NaN as that row's loss and no gradient.  No factor T^2 is applied.
+ *   forward    writes losses[n], lse[n] (natural logarithm, of z / T) and, where `total` is given, the sum of the losses or,
+ *              with `mean`, their mean over the rows that have a loss (0 where none has)
+ *   backward   reads lse, and grad: the gradient of each loss (grad_stride elements apart, 0 for one that all share), or with
+ *              `mean` that of the mean.  Writes d_hidden and d_weight (either may have data = NULL).  dZ is rounded to the tables' type on its way
+ *              into the two products (fp16: scaled by a power of two and the largest gradient) */
+typedef struct {
+    gtok_x_matrix hidden, weight;
+    const void* targets;
+    int64_t target_stride;
+    int32_t target_bits;     /* 32 or 64 */
+    int32_t entries;
+    gtok_x_matrix teacher_logits;
+    int64_t ignore;
+    float temperature;
+    int32_t mean;
+    float* losses;
+    float* lse;
+    float* total;
+    const float* grad;
+    int64_t grad_stride;
+    gtok_x_matrix d_hidden, d_weight;
+    void* workspace;
+    uint64_t workspace_bytes;
+    void* cuda_stream;
+} gtok_x_vocab_loss;
+int64_t gtok_x_vocab_loss_workspace(const gtok_x_vocab_loss* args, int32_t backward);   /* addresses in `args` but the tables' are not looked at */
+int32_t gtok_x_vocab_loss_forward(const gtok_x_vocab_loss* args);
+int32_t gtok_x_vocab_loss_backward(const gtok_x_vocab_loss* args);
+
 #ifdef __cplusplus
 }
 #endif
