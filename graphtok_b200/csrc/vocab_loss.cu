@@ -38,61 +38,67 @@ constexpr int kGroup = 16;              // row tiles that share a sweep over the
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// The matrix instruction's sums are cut off, not rounded: each step of 16 elements takes the logit towards 0, by 2^-26 of its final
+// value on average (measured on random and on coherent rows alike: 1.9e-6 to 2.1e-6 of it at a width of 2048, 4.0e-6 to 4.2e-6 at
+// 4096).  Logits are scaled up by that much.
+inline float cut_off(int width) { return 1.f + static_cast<float>((width + 15) / 16) * 0x1p-26f; }
+
 // Scalars in device memory that the kernels hand to one another.
 struct Shared {
     int active;          // rows with a loss
     int error;           // a wait ran out
+    int splits;          // hidden gradient: parts of a piece's columns that are summed apart
+    unsigned joined;     // blocks of join_kernel that are done
     float row_scale;     // gradient of row i, times this, is what dZ carries of it ...
     float unscale;       // ... and the products times this are the gradients
 };
 
 enum { kForward = 0, kDelta = 1, kHiddenGrad = 2, kWeightGrad = 3 };
 
+struct Entry { int id; float share; };        // what a row's softmax should be at `id`; ascending in a row, INT_MAX after the last
+struct RowInfo { float lse2, factor; };       // of an active row: lse in powers of 2; what dZ is multiplied by
+
 struct Product {
     Shared* shared;
-    const int* rows;           // place of each active row
     int n_rows;                // rows of the padded arrays (a multiple of kTile)
     int vocab, width;
     int first, count;          // first column of this piece, its columns
     int entries;
-    const int* entry_ids;      // [n, entries], ascending in a row, INT_MAX after the last
-    const float* entry_share;  // q; NULL: 1
+    const Entry* entry;        // [active][entries]
+    const RowInfo* info;       // backward: [active]
     float exponent;            // log2(e) / T
     float2* partial;           // forward: (maximum, sum) of [half tile of columns][row]
-    float* entry_logits;       // forward: [n, entries]
-    const float* lse;          // [n]
-    const float* grad;
-    int64_t grad_stride;
-    int splits;                // hidden gradient: parts of the piece's columns that are summed apart
-    bool add;                  // ... onto what earlier pieces left
-    void* direct;              // weight gradient, where its rows are no lines of whole 16 bytes: written by the threads
-    int64_t direct_stride;
+    float* entry_logits;       // forward: [active][entries]
+    bool add;                  // hidden gradient: onto what earlier pieces left
+    bool direct;               // weight gradient, where its rows are no lines of whole 16 bytes: written by the threads
+    uint16_t* out;             // weight gradient
+    int64_t out_stride;
 };
 
 struct Place { int m, n, k0, k1, split; };     // tile of the output, blocks of the summed dimension
 
 template <int MODE>
-__device__ __forceinline__ int tile_count(const Product& p, int active) {
+__device__ __forceinline__ int tile_count(const Product& p, int active, int splits) {
     const int row_tiles = (active + kTile - 1) / kTile, col_tiles = (p.count + kTile - 1) / kTile, width_tiles = (p.width + kTile - 1) / kTile;
-    if (MODE == kHiddenGrad) return row_tiles * width_tiles * p.splits;
+    if (MODE == kHiddenGrad) return row_tiles * width_tiles * splits;
     if (MODE == kWeightGrad) return active ? col_tiles * width_tiles : 0;
     return row_tiles * col_tiles;
 }
 
 template <int MODE>
-__device__ __forceinline__ Place tile_place(const Product& p, int active, int t) {
+__device__ __forceinline__ Place tile_place(const Product& p, int active, int splits, int t) {
     const int row_tiles = (active + kTile - 1) / kTile, col_tiles = (p.count + kTile - 1) / kTile, width_tiles = (p.width + kTile - 1) / kTile;
     Place q;
     q.k0 = 0;
     q.split = 0;
     if (MODE == kHiddenGrad) {
-        const int blocks = (p.count + kDepth - 1) / kDepth;
+        const int blocks = (p.count + kDepth - 1) / kDepth;      // fewer in the last piece; a split may then be left without any
         q.split = t / (row_tiles * width_tiles);
         t -= q.split * row_tiles * width_tiles;
         q.m = t / width_tiles;
         q.n = t - q.m * width_tiles;
-        q.k0 = static_cast<int>(static_cast<int64_t>(blocks) * q.split / p.splits);
-        q.k1 = static_cast<int>(static_cast<int64_t>(blocks) * (q.split + 1) / p.splits);
+        q.k0 = static_cast<int>(static_cast<int64_t>(blocks) * q.split / splits);
+        q.k1 = static_cast<int>(static_cast<int64_t>(blocks) * (q.split + 1) / splits);
     } else if (MODE == kWeightGrad) {
         q.m = t / width_tiles;
         q.n = t - q.m * width_tiles;
@@ -129,24 +135,47 @@ __device__ __forceinline__ uint16_t pack1(float a) {
     }
 }
 
-// A thread's way through the entries of its row, in ascending order of their ids.
-struct Entries {
-    int64_t at = 0, end = 0;
-    int next = INT_MAX;
-    __device__ __forceinline__ void begin(const Product& p, int row, int column) {
-        at = static_cast<int64_t>(row) * p.entries;
-        end = at + p.entries;
-        int64_t lo = at, hi = end;            // first entry at or behind `column`
-        while (lo < hi) {
-            const int64_t mid = (lo + hi) >> 1;
-            if (p.entry_ids[mid] < column) lo = mid + 1; else hi = mid;
-        }
-        at = lo;
-        next = at < end ? p.entry_ids[at] : INT_MAX;
+// A row's entries from a column on.  The first of them is searched for while the tile before is worked on, a step at a time, so that
+// the loads' latency is not waited for: each step looks at seven entries at once, and four steps do for kMaxEntries.
+struct Ahead {
+    const Entry* list;
+    int lo, hi, column;
+    bool there;
+    Entry next, then;          // the entry that comes next, and the one after it
+    RowInfo info;
+    __device__ __forceinline__ Entry get(const Product& p, int i) const { return i < p.entries ? list[i] : Entry{INT_MAX, 0.f}; }
+    __device__ __forceinline__ void begin(const Product& p, int m, bool live, int from, bool with_info) {
+        list = p.entry + static_cast<int64_t>(m) * p.entries;
+        lo = 0;
+        hi = live ? p.entries : 0;
+        column = from;
+        there = !live;
+        next = then = Entry{INT_MAX, 0.f};
+        info = RowInfo{0.f, 0.f};
+        if (with_info && live) info = p.info[m];
     }
     __device__ __forceinline__ void step(const Product& p) {
-        ++at;
-        next = at < end ? p.entry_ids[at] : INT_MAX;
+        if (there) return;
+        if (lo < hi) {
+            const int s = (hi - lo + 7) >> 3;
+            int c = 0;
+#pragma unroll
+            for (int k = 1; k < 8; ++k) {
+                const int at = lo + k * s - 1;
+                c += at < hi && list[at].id < column;
+            }
+            lo += c * s;
+            hi = min(hi, lo + s - 1);
+            if (lo < hi) return;
+        }
+        next = get(p, lo);
+        then = get(p, lo + 1);
+        there = true;
+    }
+    __device__ __forceinline__ void advance(const Product& p) {
+        ++lo;
+        next = then;
+        then = get(p, lo + 1);
     }
 };
 
@@ -185,8 +214,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     uint32_t tmem;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
 
-    const int active = p.shared->active;
-    const int tiles = tile_count<MODE>(p, active);
+    after_previous();
+    const int active = p.shared->active, splits = MODE == kHiddenGrad ? p.shared->splits : 1;
+    const int tiles = tile_count<MODE>(p, active, splits);
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     bool ok = true;
 
@@ -195,7 +225,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint32_t full_of_pair = in_block(full, 0);
             uint32_t it = 0;
             for (int t = pair; t < tiles && ok; t += pairs) {
-                const Place q = tile_place<MODE>(p, active, t);
+                const Place q = tile_place<MODE>(p, active, splits, t);
                 const int am = q.m * kTile + rank * 128, bn = q.n * kTile + rank * 128 + ((MODE == kForward || MODE == kDelta) ? p.first : 0);
                 const int bk = MODE == kHiddenGrad ? p.first : 0;
                 for (int k = q.k0; k < q.k1; ++k, ++it) {
@@ -219,8 +249,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (rank == 0 && elect()) {
             constexpr uint32_t kind = mma_kind(BF16, kAcrossA, kAcrossB);
             uint32_t it = 0, acc = 0;
-            for (int t = pair; t < tiles && ok; t += pairs, ++acc) {
-                const Place q = tile_place<MODE>(p, active, t);
+            for (int t = pair; t < tiles && ok; t += pairs) {
+                const Place q = tile_place<MODE>(p, active, splits, t);
+                if (q.k0 >= q.k1) continue;
                 if (!bar_wait(acc_empty + 8 * (acc & 1), ((acc >> 1) & 1) ^ 1)) { ok = false; break; }
                 fence_after();
                 for (int k = q.k0; k < q.k1; ++k, ++it) {
@@ -235,43 +266,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     mma_commit(empty + 8 * s);
                 }
                 if (ok) mma_commit(acc_full + 8 * (acc & 1));
+                ++acc;
             }
         }
     } else if (warp >= 4) {
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const uint32_t lines = staging + (warp - 4) * kStagingBytes;
         const uint32_t line = lines + lane * 128;
+        constexpr bool kRows = MODE == kForward || MODE == kDelta;
+        const float unscale = MODE == kWeightGrad ? p.shared->unscale : 0.f;
+        Ahead ahead;
+        auto look_ahead = [&](int t) {
+            if (t >= tiles) t = pair;                  // (no further tile: anything that is in bounds)
+            const Place q = tile_place<MODE>(p, active, splits, t);
+            const int m = q.m * kTile + rank * 128 + quarter * 32 + lane;
+            ahead.begin(p, m, m < active, p.first + q.n * kTile + half * 128, MODE == kDelta);
+        };
+        if (kRows && pair < tiles) look_ahead(pair);
         uint32_t acc = 0;
-        for (int t = pair; t < tiles; t += pairs, ++acc) {
-            const Place q = tile_place<MODE>(p, active, t);
+        for (int t = pair; t < tiles; t += pairs) {
+            const Place q = tile_place<MODE>(p, active, splits, t);
+            if (q.k0 >= q.k1) continue;
             const int m = q.m * kTile + rank * 128 + quarter * 32 + lane;       // this thread's line of the tile
             const int column = q.n * kTile + half * 128;                        // of the output; of the piece where columns are the vocabulary's
             const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (acc & 1) * 256 + half * 128;
-            Entries e;
-            float lse2 = 0.f, f = 0.f;
-            bool live = true;
-            if (MODE == kForward || MODE == kDelta) {
-                live = m < active;
-                if (live) {
-                    const int row = p.rows[m];
-                    e.begin(p, row, p.first + column);
-                    if (MODE == kDelta) {
-                        lse2 = p.lse[row] * kLog2e;
-                        f = p.grad[row * p.grad_stride] * p.shared->row_scale;
-                    }
-                }
+            const bool live = m < active;
+            Ahead e;
+            if (kRows) {
+                while (!ahead.there) ahead.step(p);
+                e = ahead;
+                look_ahead(t + pairs);
             }
-            if (MODE == kWeightGrad) f = p.shared->unscale;
             ok = __all_sync(~0u, bar_wait(acc_full + 8 * (acc & 1), (acc >> 1) & 1));
             if (!ok) break;
             fence_after();
-            if constexpr (MODE == kForward) {
-                float high = -INFINITY, sum = 0.f;
-#pragma unroll 1
-                for (int c = 0; c < 128; c += 32) {
-                    float v[32];
-                    tmem_load(from + c, v);
-                    const int at = p.first + column + c;
+            float va[32], vb[32];
+            float high = -INFINITY, sum = 0.f;
+            // What becomes of 32 columns from `c` on.
+            auto work = [&](float (&v)[32], int c) {
+                const int at = p.first + column + c;
+                if constexpr (MODE == kForward) {
                     if (at + 32 > p.vocab) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = at + i < p.vocab ? v[i] : -INFINITY;
@@ -287,83 +321,72 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) part[i & 3] += exp2_fast(fmaf(v[i], p.exponent, -from_top));
                     sum += (part[0] + part[1]) + (part[2] + part[3]);
-                    while (e.next < at + 32) {
-                        const int j = e.next - at;
+                    while (e.next.id < at + 32) {
+                        const int j = e.next.id - at;
                         float z = 0.f;
 #pragma unroll
                         for (int i = 0; i < 32; ++i) z = i == j ? v[i] : z;
-                        p.entry_logits[e.at] = z;
-                        e.step(p);
+                        p.entry_logits[static_cast<int64_t>(m) * p.entries + e.lo] = z;
+                        e.advance(p);
                     }
+                    ahead.step(p);
                     __syncwarp();
-                }
-                if (live) p.partial[static_cast<int64_t>(q.n * 2 + half) * p.n_rows + m] = make_float2(high, sum);
-            } else if constexpr (MODE == kDelta || MODE == kWeightGrad) {
-                // 64 columns of 16 bits make a line
-#pragma unroll 1
-                for (int c = 0; c < 128; c += 64) {
-                    if (lane == 0) stores_read();
-                    __syncwarp();
-#pragma unroll 1
-                    for (int d = 0; d < 64; d += 32) {
-                        float v[32];
-                        tmem_load(from + c + d, v);
-                        if constexpr (MODE == kDelta) {
-                            const int at = p.first + column + c + d;
+                } else if constexpr (MODE == kDelta || MODE == kWeightGrad) {
+                    // 64 columns of 16 bits make a line
+                    if (MODE == kDelta) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = f * exp2_fast(fmaf(v[i], p.exponent, -lse2));
-                            while (e.next < at + 32) {
-                                const int j = e.next - at;
-                                const float share = p.entry_share ? p.entry_share[e.at] * f : f;
+                        for (int i = 0; i < 32; ++i) v[i] = e.info.factor * exp2_fast(fmaf(v[i], p.exponent, -e.info.lse2));
+                        while (e.next.id < at + 32) {
+                            const int j = e.next.id - at;
+                            const float share = e.next.share * e.info.factor;
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) v[i] -= i == j ? share : 0.f;
-                                e.step(p);
+                            for (int i = 0; i < 32; ++i) v[i] -= i == j ? share : 0.f;
+                            e.advance(p);
+                        }
+                        ahead.step(p);
+                        __syncwarp();
+                        if (!live || at + 32 > p.vocab) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = live && at + i < p.vocab ? v[i] : 0.f;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] *= unscale;
+                        if (p.direct) {
+                            if (m < p.count) {
+                                uint16_t* to = p.out + static_cast<int64_t>(p.first + m) * p.out_stride;
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                    if (column + c + i < p.width) to[column + c + i] = pack1<BF16>(v[i]);
                             }
                             __syncwarp();
-                            if (!live || at + 32 > p.vocab) {
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) v[i] = live && at + i < p.vocab ? v[i] : 0.f;
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] *= f;
-                            if (p.direct) {
-                                const int row = q.m * kTile + static_cast<int>(rank) * 128 + quarter * 32 + lane;
-                                if (row < p.count) {
-                                    uint16_t* to = static_cast<uint16_t*>(p.direct) + static_cast<int64_t>(p.first + row) * p.direct_stride;
-#pragma unroll
-                                    for (int i = 0; i < 32; ++i)
-                                        if (column + c + d + i < p.width) to[column + c + d + i] = pack1<BF16>(v[i]);
-                                }
-                                continue;
-                            }
-                        }
-#pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            const uint32_t to = line + (((d >> 3) + g) ^ (lane & 7)) * 16;
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pack2<BF16>(v[8 * g], v[8 * g + 1])),
-                                         "r"(pack2<BF16>(v[8 * g + 2], v[8 * g + 3])), "r"(pack2<BF16>(v[8 * g + 4], v[8 * g + 5])),
-                                         "r"(pack2<BF16>(v[8 * g + 6], v[8 * g + 7]))
-                                         : "memory");
+                            return;
                         }
                     }
-                    if (MODE == kWeightGrad && p.direct) continue;
-                    smem_to_async();
-                    __syncwarp();
-                    if (lane == 0) {
-                        const int row = q.m * kTile + static_cast<int>(rank) * 128 + quarter * 32;
-                        if (MODE == kDelta) store_tile(&map_out, lines, column + c, row);
-                        else if (column + c < p.width && row < p.count) store_tile(&map_out, lines, column + c, p.first + row);
-                        stores_commit();
+                    if ((c & 32) == 0) {
+                        if (lane == 0) stores_read();
+                        __syncwarp();
                     }
-                }
-            } else {
-                // 32 columns of fp32 make a line
-#pragma unroll 1
-                for (int c = 0; c < 128; c += 32) {
-                    if (column + c >= p.width) break;
-                    float v[32];
-                    tmem_load(from + c, v);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const uint32_t to = line + ((((c & 32) >> 3) + g) ^ (lane & 7)) * 16;
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pack2<BF16>(v[8 * g], v[8 * g + 1])),
+                                     "r"(pack2<BF16>(v[8 * g + 2], v[8 * g + 3])), "r"(pack2<BF16>(v[8 * g + 4], v[8 * g + 5])),
+                                     "r"(pack2<BF16>(v[8 * g + 6], v[8 * g + 7]))
+                                     : "memory");
+                    }
+                    if (c & 32) {
+                        smem_to_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            const int x = column + c - 32, row = m - lane;
+                            if (MODE == kDelta) store_tile(&map_out, lines, x, row);
+                            else if (x < p.width && row < p.count) store_tile(&map_out, lines, x, p.first + row);
+                            stores_commit();
+                        }
+                    }
+                } else {
+                    // 32 columns of fp32 make a line
                     if (lane == 0) stores_read();
                     __syncwarp();
 #pragma unroll
@@ -376,21 +399,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     smem_to_async();
                     __syncwarp();
                     if (lane == 0) {
-                        const int row = q.split * p.n_rows + q.m * kTile + static_cast<int>(rank) * 128 + quarter * 32;
-                        if (p.add) add_tile(&map_out, lines, column + c, row); else store_tile(&map_out, lines, column + c, row);
+                        const int row = q.split * ((active + kTile - 1) / kTile * kTile) + m;
+                        if (column + c < p.width) {
+                            if (p.add) add_tile(&map_out, lines, column + c, row); else store_tile(&map_out, lines, column + c, row);
+                        }
                         stores_commit();
                     }
                 }
+            };
+            tmem_load(from, va);
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 64) {
+                tmem_wait(va);
+                tmem_load(from + c + 32, vb);
+                work(va, c);
+                tmem_wait(vb);
+                if (c == 0) {
+                    tmem_load(from + 64, va);
+                } else {              // all taken out: the next tile but one may be summed there
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive_cluster(in_block(acc_empty + 8 * (acc & 1), 0));
+                }
+                work(vb, c + 32);
             }
-            fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive_cluster(in_block(acc_empty + 8 * (acc & 1), 0));
+            if (MODE == kForward && live) p.partial[static_cast<int64_t>(q.n * 2 + half) * p.n_rows + m] = make_float2(high, sum);
+            ++acc;
         }
         if (lane == 0) stores_done();
     }
     if (!ok) atomicExch(&p.shared->error, 1);
     __syncwarp();
+    let_next_begin();
     __syncthreads();
+    if (MODE == kWeightGrad) {
+        if (active == 0) {       // no product, no gradient
+            for (int64_t r = p.first + blockIdx.x; r < p.first + p.count; r += gridDim.x)
+                for (int i = threadIdx.x; i < p.width; i += kThreads) p.out[r * p.out_stride + i] = 0;
+        }
+        if (threadIdx.x == 0 && *static_cast<volatile int*>(&p.shared->error)) p.out[0] = BF16 ? 0x7FC0 : 0x7E00;
+    }
     fence_before();
     cluster_sync();
     fence_after();
@@ -407,16 +455,20 @@ __device__ __forceinline__ float load_value(const void* data, int type, int64_t 
     if (type == kF16) return __half2float(static_cast<const __half*>(data)[i]);
     return static_cast<const float*>(data)[i];
 }
+// Maximum that keeps NaN.
+__device__ __forceinline__ float max_nan(float a, float b) { return a != a || b != b ? a + b : fmaxf(a, b); }
 
-constexpr int kNone = -1, kBad = -2;      // what a row without a loss has in place of its first entry
+constexpr int kNone = -1, kBad = -2;      // a row without a loss: nothing wanted of it; something beyond the vocabulary
 
-// A teacher's rows: entries sorted by id (ties by place), their softmax beside them.  One block a row.
-__global__ void teacher_kernel(Ids ids, Matrix logits, int entries, int room, int vocab, float inv_temperature, int* entry_ids, float* entry_share, int* first) {
+// A teacher's rows: entries sorted by id (ties by place) with their softmax.  One block a row.
+__global__ void teacher_kernel(Ids ids, Matrix logits, int entries, int room, int vocab, float inv_temperature, Entry* entry, int* state) {
     extern __shared__ uint8_t smem_raw[];
     uint64_t* key = reinterpret_cast<uint64_t*>(smem_raw);
     float* share = reinterpret_cast<float*>(key + room);
     __shared__ float red[32];
     __shared__ int bad;
+    after_previous();
+    let_next_begin();
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, threads = blockDim.x;
     if (tid == 0) bad = 0;
@@ -432,20 +484,19 @@ __global__ void teacher_kernel(Ids ids, Matrix logits, int entries, int room, in
         }
         key[k] = (static_cast<uint64_t>(id >= 0 && id < vocab ? static_cast<uint32_t>(id) : 0x7FFFFFFFu) << 32) | static_cast<uint32_t>(k);
         share[k] = l;
-        top = l != l ? l : fmaxf(top, l);
+        top = max_nan(top, l);
     }
-    // maximum, then sum, over the block
     auto over_block = [&](float x, bool max_of) {
 #pragma unroll
         for (int d = 16; d; d >>= 1) {
             const float y = __shfl_xor_sync(~0u, x, d);
-            x = max_of ? (x != x || y != y ? x + y : fmaxf(x, y)) : x + y;
+            x = max_of ? max_nan(x, y) : x + y;
         }
         __syncthreads();
         if ((tid & 31) == 0) red[tid >> 5] = x;
         __syncthreads();
         x = red[0];
-        for (int w = 1; w < (threads >> 5); ++w) x = max_of ? (x != x || red[w] != red[w] ? x + red[w] : fmaxf(x, red[w])) : x + red[w];
+        for (int w = 1; w < (threads >> 5); ++w) x = max_of ? max_nan(x, red[w]) : x + red[w];
         return x;
     };
     top = over_block(top, true);
@@ -466,226 +517,307 @@ __global__ void teacher_kernel(Ids ids, Matrix logits, int entries, int room, in
             }
         }
     __syncthreads();
-    for (int k = tid; k < entries; k += threads) {
-        entry_ids[row * entries + k] = static_cast<int>(key[k] >> 32);
-        entry_share[row * entries + k] = share[static_cast<uint32_t>(key[k])] / sum;
-    }
-    if (tid == 0) first[row] = bad ? kBad : none ? kNone : 0;
+    for (int k = tid; k < entries; k += threads)
+        entry[row * entries + k] = Entry{static_cast<int>(key[k] >> 32), share[static_cast<uint32_t>(key[k])] / sum};
+    if (tid == 0) state[row] = bad ? kBad : none ? kNone : 0;
 }
 
-// Which rows have a loss: their places in order, behind them those of the others; and the scale of the gradients.  One block.
-__global__ void __launch_bounds__(1024) rows_kernel(Ids targets, int64_t ignore, int vocab, int n, const int* first, int* entry_ids, int* rows, Shared* shared,
-                                                    float* losses, float* lse, const float* grad, int64_t grad_stride, bool grad_of_mean, float inv_temperature,
-                                                    bool half) {
+// Time in ns of the hidden gradient's part of a piece in `s` splits: `outs` tiles of it over `blocks` steps of the summed dimension.  A step
+// of a tile takes 270, beginning and ending one 700, and each split costs its way to memory and back.
+__host__ __device__ inline int64_t split_time(int s, int64_t outs, int blocks, int pairs) {
+    if (s > 1 && s * 8 > blocks) return INT64_MAX;
+    return (outs * s + pairs - 1) / pairs * (270 * blocks / s + 700) + 90 * s * outs;
+}
+constexpr int kMaxSplits = 32;
+
+struct RowsArgs {
+    Ids targets;
+    int64_t ignore;
+    int vocab, n;
+    const int* state;            // of a teacher's rows; NULL: from the targets
+    Entry* entry;                // of the targets, the active rows' together
+    int* rows;
+    Shared* shared;
+    float *losses, *lse;         // forward
+    const float* grad;           // backward
+    int64_t grad_stride;
+    bool grad_of_mean, half;
+    float inv_temperature;
+    int width_tiles, blocks, pairs;
+};
+
+// Which rows have a loss: their places in order, behind them those of the others; and the scale of the gradients.  One block, 256 rows
+// a warp at a time.
+__global__ void __launch_bounds__(1024) rows_kernel(const __grid_constant__ RowsArgs a) {
     constexpr int kEach = 8;
     __shared__ int warp_sum[32];
     __shared__ float warp_top[32];
-    __shared__ int done;
+    after_previous();
+    let_next_begin();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) done = 0;
-    __syncthreads();
     float top = 0.f;
-    for (int base = 0; base < n; base += 1024 * kEach) {
-        const int at = base + tid * kEach;
-        uint32_t bits = 0;
+    int done = 0;
+    for (int base = 0; base < a.n; base += 1024 * kEach) {
+        const int at = base + warp * 32 * kEach + lane;
+        int id[kEach];              // or the state of a row without a loss
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            if (at + i >= n) break;
-            int state;
-            if (first) {
-                state = first[at + i];
+            const int row = at + 32 * i;
+            id[i] = kNone;
+            if (row >= a.n) continue;
+            if (a.state) {
+                id[i] = a.state[row];
             } else {
-                const int64_t id = load_id(targets.data, targets.bits, at + i);
-                state = id < 0 || id == ignore ? kNone : id >= vocab ? kBad : 0;
-                entry_ids[at + i] = state < 0 ? INT_MAX : static_cast<int>(id);
-            }
-            if (state >= 0) {
-                bits |= 1u << i;
-                if (grad) {
-                    const float g = fabsf(grad[(at + i) * grad_stride]);
-                    top = g != g || top != top ? g + top : fmaxf(top, g);
-                }
-            } else if (losses) {
-                losses[at + i] = state == kBad ? __int_as_float(0x7FC00000) : 0.f;
-                lse[at + i] = 0.f;
+                const int64_t t = load_id(a.targets.data, a.targets.bits, row);
+                id[i] = t < 0 || t == a.ignore ? kNone : t >= a.vocab ? kBad : static_cast<int>(t);
             }
         }
-        const int mine = __popc(bits);
-        int before = mine;
+        uint32_t live[kEach];
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int row = at + 32 * i;
+            live[i] = __ballot_sync(~0u, id[i] >= 0);
+            mine += __popc(live[i]);
+            if (row < a.n && id[i] < 0 && a.losses) {
+                a.losses[row] = id[i] == kBad ? __int_as_float(0x7FC00000) : 0.f;
+                a.lse[row] = 0.f;
+            }
+            if (id[i] >= 0 && a.grad) top = max_nan(top, fabsf(a.grad[row * a.grad_stride]));
+        }
+        if (lane == 0) warp_sum[warp] = mine;
+        __syncthreads();
+        int x = warp_sum[lane];
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int y = __shfl_up_sync(~0u, before, d);
-            if (lane >= d) before += y;
+            const int y = __shfl_up_sync(~0u, x, d);
+            if (lane >= d) x += y;
         }
-        if (lane == 31) warp_sum[warp] = before;
-        __syncthreads();
-        if (warp == 0) {
-            int x = warp_sum[lane];
+        int to = done + __shfl_sync(~0u, x, warp) - mine;
+        done += __shfl_sync(~0u, x, 31);
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int y = __shfl_up_sync(~0u, x, d);
-                if (lane >= d) x += y;
+        for (int i = 0; i < kEach; ++i) {
+            const int row = at + 32 * i, before = to + __popc(live[i] & ((1u << lane) - 1));
+            to += __popc(live[i]);
+            if (row >= a.n) continue;
+            if (id[i] >= 0) {
+                a.rows[before] = row;
+                if (!a.state) a.entry[before] = Entry{id[i], 1.f};
+            } else {
+                a.rows[a.n - 1 - (row - before)] = row;
             }
-            warp_sum[lane] = x;
         }
-        __syncthreads();
-        int to = done + before - mine + (warp ? warp_sum[warp - 1] : 0);
-        int out = at - to;                    // rows without a loss before this thread's
-        for (int i = 0; i < kEach && at + i < n; ++i) {
-            if (bits >> i & 1) rows[to++] = at + i; else rows[n - 1 - out++] = at + i;
-        }
-        __syncthreads();
-        if (tid == 0) done += warp_sum[31];
         __syncthreads();
     }
 #pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        const float y = __shfl_xor_sync(~0u, top, d);
-        top = top != top || y != y ? top + y : fmaxf(top, y);
-    }
+    for (int d = 16; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, d));
     if (lane == 0) warp_top[warp] = top;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < 32; ++w) top = top != top || warp_top[w] != warp_top[w] ? top + warp_top[w] : fmaxf(top, warp_top[w]);
-        shared->active = done;
-        shared->error = 0;
-        if (grad) {
-            // dZ is kept with the largest row gradient as 1 (bf16: its range is fp32's) or as 2^15, so that fp16 holds probabilities
-            // down to 2^-29 in full precision and nothing above 2^16.
-            const float unit = half ? 32768.f : 1.f;
-            shared->row_scale = top == 0.f ? 0.f : unit / top;
-            shared->unscale = top / unit * inv_temperature / (grad_of_mean ? fmaxf(static_cast<float>(done), 1.f) : 1.f);
-        }
+    if (warp) return;
+    top = warp_top[lane];
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, d));
+    // each lane the time of one number of splits
+    const int64_t time = split_time(lane + 1, static_cast<int64_t>((done + kTile - 1) / kTile) * a.width_tiles, a.blocks, a.pairs);
+    int64_t least = time;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) least = min(least, __shfl_xor_sync(~0u, least, d));
+    const int splits = __ffs(__ballot_sync(~0u, time == least));
+    if (lane == 0) {
+        Shared s;
+        s.active = done;
+        s.error = 0;
+        s.joined = 0;
+        s.splits = splits;
+        // dZ is kept with the largest row gradient as 1 (bf16: its range is fp32's) or as 2^15, so that fp16 holds probabilities
+        // down to 2^-29 in full precision and nothing above 2^16.
+        const float unit = a.half ? 32768.f : 1.f;
+        s.row_scale = top == 0.f ? 0.f : unit / top;
+        s.unscale = top / unit * a.inv_temperature / (a.grad_of_mean ? fmaxf(static_cast<float>(done), 1.f) : 1.f);
+        *a.shared = s;
     }
 }
 
-// Rows `rows[0 .. active)` (all `n` where rows is NULL) copied together, lines of `cols` rounded up to whole 16 bytes; lines up to the next whole tile become 0.
-__global__ void gather_kernel(const uint16_t* src, int64_t stride, int cols, const int* rows, const Shared* shared, int n, uint16_t* dst, int dst_cols, bool wide) {
-    const int active = rows ? shared->active : n;
-    const int end = rows ? (active + kTile - 1) / kTile * kTile : n;
-    const int lines = dst_cols / 8;
+struct GatherArgs {
+    const uint16_t* src;
+    int64_t stride;
+    int cols;
+    const int* rows;             // NULL: all n
+    const Shared* shared;
+    int n;
+    uint16_t* dst;
+    int dst_cols;
+    bool wide;
+    int entries;                 // of a teacher
+    const Entry* entry_from;
+    Entry* entry_to;
+    RowInfo* info;               // backward
+    const float *lse, *grad;
+    int64_t grad_stride;
+};
+
+// The active rows copied together, lines of `cols` rounded up to whole 16 bytes; lines up to the next whole tile become 0.  One block a row.
+__global__ void __launch_bounds__(128) gather_kernel(const __grid_constant__ GatherArgs a) {
+    after_previous();
+    let_next_begin();
+    const int active = a.rows ? a.shared->active : a.n;
+    const int end = a.rows ? (active + kTile - 1) / kTile * kTile : a.n;
+    const int lines = a.dst_cols / 8;
     for (int64_t j = blockIdx.x; j < end; j += gridDim.x) {
-        const uint16_t* from = j < active ? src + (rows ? rows[j] : j) * stride : nullptr;
-        uint4* to = reinterpret_cast<uint4*>(dst + j * dst_cols);
-        for (int i = threadIdx.x; i < lines; i += blockDim.x) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (from && wide) {
-                v = __ldg(reinterpret_cast<const uint4*>(from) + i);
-            } else if (from) {
-                uint32_t w[4] = {0, 0, 0, 0};
+        const int64_t row = j < active ? (a.rows ? a.rows[j] : j) : 0;
+        const uint16_t* from = j < active ? a.src + row * a.stride : nullptr;
+        uint4* to = reinterpret_cast<uint4*>(a.dst + j * a.dst_cols);
+        if (from && a.wide) {
+            for (int i = threadIdx.x; i < lines; i += 4 * 128) {
+                uint4 v[4];
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (8 * i + k < cols) w[k >> 1] |= static_cast<uint32_t>(from[8 * i + k]) << (16 * (k & 1));
-                v = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int k = 0; k < 4; ++k)
+                    if (i + 128 * k < lines) v[k] = __ldg(reinterpret_cast<const uint4*>(from) + i + 128 * k);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (i + 128 * k < lines) to[i + 128 * k] = v[k];
             }
-            to[i] = v;
+        } else {
+            for (int i = threadIdx.x; i < lines; i += 128) {
+                uint32_t w[4] = {0, 0, 0, 0};
+                if (from)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (8 * i + k < a.cols) w[k >> 1] |= static_cast<uint32_t>(from[8 * i + k]) << (16 * (k & 1));
+                to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+        if (j < active) {
+            for (int i = threadIdx.x; i < a.entries; i += 128) a.entry_to[j * a.entries + i] = a.entry_from[row * a.entries + i];
+            if (a.info && threadIdx.x == 0) a.info[j] = RowInfo{a.lse[row] * kLog2e, a.grad[row * a.grad_stride] * a.shared->row_scale};
         }
     }
 }
 
 // ---- and afterwards ---------------------------------------------------------------
 
-// Joins the half tiles' maxima and sums of 32 rows a block and takes the losses.
-__global__ void __launch_bounds__(512) join_kernel(const float2* partial, int parts, int n_rows, const Shared* shared, const int* rows, int entries,
-                                                   const int* entry_ids, const float* entry_share, const float* entry_logits, float exponent,
-                                                   float inv_temperature, float* losses, float* lse) {
-    __shared__ float2 piece[16][32];
-    const int active = shared->active;
+struct JoinArgs {
+    const float2* partial;
+    int parts, n_rows;
+    Shared* shared;
+    const int* rows;
+    int n, entries;
+    const Entry* entry;
+    const float* entry_logits;
+    float exponent, inv_temperature;
+    float *losses, *lse, *total;
+    bool mean;
+};
+
+// Joins the half tiles' maxima and sums of 32 rows a block and takes the losses; the last block to end adds them up, in the same order always.
+__global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ JoinArgs a) {
+    __shared__ float2 piece[32][33];
+    __shared__ float red[32];
+    __shared__ bool last;
+    after_previous();
+    let_next_begin();
+    const int active = a.shared->active;
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
     for (int base = blockIdx.x * 32; base < active; base += gridDim.x * 32) {
         const int m = base + x;
         float high = -INFINITY, sum = 0.f;
-        if (m < active)
-            for (int k = y; k < parts; k += 16) {
-                const float2 v = partial[static_cast<int64_t>(k) * n_rows + m];
-                const float top = fmaxf(high, v.x), ref = top == -INFINITY ? 0.f : top;
-                sum = sum * exp2_fast((high - ref) * exponent) + v.y * exp2_fast((v.x - ref) * exponent);
+        if (m < active) {
+            for (int k = y; k < a.parts; k += 32 * 8) {
+                float2 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[i] = k + 32 * i < a.parts ? a.partial[static_cast<int64_t>(k + 32 * i) * a.n_rows + m] : make_float2(-INFINITY, 0.f);
+                float top = high;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, v[i].x);
+                const float ref = top == -INFINITY ? 0.f : top;
+                sum *= exp2_fast((high - ref) * a.exponent);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += v[i].y * exp2_fast((v[i].x - ref) * a.exponent);
                 high = top;
             }
+        }
         __syncthreads();
         piece[y][x] = make_float2(high, sum);
         __syncthreads();
-        // 16 threads a row again, now beside one another
-        const int row_of = threadIdx.x >> 4, k = threadIdx.x & 15;
-        float2 v = piece[k][row_of];
+        // a warp a row, its 32 parts beside one another
+        const float2 v = piece[x][y];
         float top = v.x;
 #pragma unroll
-        for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
         const float ref = top == -INFINITY ? 0.f : top;
-        float total = v.y * exp2_fast((v.x - ref) * exponent);
+        float total = v.y * exp2_fast((v.x - ref) * a.exponent);
 #pragma unroll
-        for (int d = 8; d; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
-        const float row_lse = ref * inv_temperature + logf(total);
-        if (base + row_of < active) {
-            const int row = rows[base + row_of];
+        for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
+        const float row_lse = ref * a.inv_temperature + logf(total);
+        const int j = base + y;
+        if (j < active) {
             float loss = 0.f;
-            for (int i = k; i < entries; i += 16) {
-                const int64_t at = static_cast<int64_t>(row) * entries + i;
-                if (entry_ids[at] == INT_MAX) continue;
-                const float q = entry_share ? entry_share[at] : 1.f;
-                if (q != 0.f) loss += q * ((entry_share ? logf(q) : 0.f) + (row_lse - entry_logits[at] * inv_temperature));
+            for (int i = x; i < a.entries; i += 32) {
+                const int64_t at = static_cast<int64_t>(j) * a.entries + i;
+                const Entry e = a.entry[at];
+                if (e.id != INT_MAX && e.share != 0.f) loss += e.share * (logf(e.share) + (row_lse - a.entry_logits[at] * a.inv_temperature));
             }
 #pragma unroll
-            for (int d = 8; d; d >>= 1) loss += __shfl_xor_sync(0xFFFFu << (threadIdx.x & 16), loss, d);
-            if (k == 0) {
-                const bool failed = shared->error != 0;
-                losses[row] = failed ? __int_as_float(0x7FC00000) : loss;
-                lse[row] = row_lse;
+            for (int d = 16; d; d >>= 1) loss += __shfl_xor_sync(~0u, loss, d);
+            if (x == 0) {
+                const int row = a.rows[j];
+                a.losses[row] = a.shared->error ? __int_as_float(0x7FC00000) : loss;
+                a.lse[row] = row_lse;
             }
         }
     }
-}
-
-// Sum or mean of the losses, one block: sums of every 1024th, then over the block, always in the same order.
-__global__ void __launch_bounds__(1024) total_kernel(const float* losses, int n, const Shared* shared, bool mean, float* total) {
-    __shared__ float red[32];
+    if (!a.total) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(&a.shared->joined, 1u) == gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
     float sum = 0.f;
-    for (int i = threadIdx.x; i < n; i += 1024) sum += losses[i];
+    for (int i = threadIdx.x; i < a.n; i += 1024) sum += __ldcg(a.losses + i);
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
+    if (x == 0) red[y] = sum;
     __syncthreads();
-    if (threadIdx.x < 32) {
-        sum = red[threadIdx.x];
+    if (y) return;
+    sum = red[x];
 #pragma unroll
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-        if (threadIdx.x == 0) *total = mean ? sum / fmaxf(static_cast<float>(shared->active), 1.f) : sum;
-    }
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+    if (x == 0) *a.total = a.mean ? sum / fmaxf(static_cast<float>(active), 1.f) : sum;
 }
 
-// Hidden gradient: the splits' sums in order, scaled, each row back at its place; rows without a loss get 0.
+// Hidden gradient: the splits' sums in order, scaled, each row back at its place; rows without a loss get 0.  Eight columns a thread.
 template <bool BF16>
-__global__ void hidden_grad_kernel(const float* part, int splits, int n_rows, int part_cols, const Shared* shared, const int* rows, int n, int cols, uint16_t* out,
-                                   int64_t stride, bool wide) {
-    const int active = shared->active;
+__global__ void __launch_bounds__(256) hidden_grad_kernel(const float* part, int part_cols, const Shared* shared, const int* rows, int n, int cols, uint16_t* out,
+                                                          int64_t stride, bool wide) {
+    after_previous();
+    const int active = shared->active, splits = shared->splits;
+    const int64_t apart = static_cast<int64_t>((active + kTile - 1) / kTile * kTile) * part_cols;
     const float unscale = shared->error ? __int_as_float(0x7FC00000) : shared->unscale;
-    for (int64_t j = blockIdx.x; j < n; j += gridDim.x) {
-        uint16_t* to = out + rows[j] * stride;
-        for (int i = threadIdx.x * 4; i < cols; i += blockDim.x * 4) {
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (j < active) {
-                for (int s = 0; s < splits; ++s) {
-                    const float4 w = *reinterpret_cast<const float4*>(part + (static_cast<int64_t>(s) * n_rows + j) * part_cols + i);
-                    v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
-                }
-                v.x *= unscale; v.y *= unscale; v.z *= unscale; v.w *= unscale;
+    const int lines = (cols + 7) / 8;
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < static_cast<int64_t>(n) * lines; u += static_cast<int64_t>(gridDim.x) * 256) {
+        const int j = static_cast<int>(u / lines), i = static_cast<int>(u - static_cast<int64_t>(j) * lines) * 8;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (j < active) {
+            const float* from = part + static_cast<int64_t>(j) * part_cols + i;
+            for (int s = 0; s < splits; ++s, from += apart) {
+                const float4 a = *reinterpret_cast<const float4*>(from), b = *reinterpret_cast<const float4*>(from + 4);
+                v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+                v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
             }
-            if (wide) {
-                *reinterpret_cast<uint2*>(to + i) = make_uint2(pack2<BF16>(v.x, v.y), pack2<BF16>(v.z, v.w));
-            } else {
-                const float each[4] = {v.x, v.y, v.z, v.w};
-                for (int k = 0; k < 4 && i + k < cols; ++k) to[i + k] = pack1<BF16>(each[k]);
-            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] *= unscale;
+        }
+        uint16_t* to = out + rows[j] * stride + i;
+        if (wide) {
+            *reinterpret_cast<uint4*>(to) = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i + k < cols) to[k] = pack1<BF16>(v[k]);
         }
     }
-}
-
-// The table's gradient where no row has a loss (the products have nothing to do then), and NaN in it after a wait that ran out.
-__global__ void no_rows_kernel(const Shared* shared, uint16_t* out, int64_t rows, int cols, int64_t stride, uint16_t nan) {
-    if (shared->error && blockIdx.x == 0 && threadIdx.x == 0) out[0] = nan;
-    if (shared->active) return;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-        for (int i = threadIdx.x; i < cols; i += blockDim.x) out[r * stride + i] = 0;
 }
 
 // ---- host -------------------------------------------------------------------------
@@ -693,29 +825,32 @@ __global__ void no_rows_kernel(const Shared* shared, uint16_t* out, int64_t rows
 inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 inline int64_t div_up(int64_t x, int64_t by) { return (x + by - 1) / by; }
 
-struct Plan {
-    int n, n_rows, vocab, width, cols, entries;     // cols: width in whole 16 bytes
-    bool copy_weight;
-    int piece, splits;                              // backward: columns a piece, parts of a piece summed apart
-    uint64_t shared, rows, entry_ids, entry_share, first, entry_logits, hidden, weight, partial, delta, sums, bytes;
-};
-
 int multiprocessors() {
     int device = 0, count = 148;
     if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device);
     return count;
 }
 
+struct Plan {
+    int n, n_rows, vocab, width, cols, entries;     // cols: width in whole 16 bytes
+    int pairs;
+    bool copy_weight;
+    int piece;                                      // backward: columns a piece
+    int64_t sum_rows;                               // rows of the hidden gradient's parts, however many rows are active
+    uint64_t shared, rows, entry, entry_raw, state, info, entry_logits, hidden, weight, partial, delta, sums, bytes;
+};
+
 constexpr int64_t kDeltaBytes = 256 << 20;          // of a piece's dZ
 
 Plan make_plan(const LossCall& c, bool backward) {
     Plan p{};
     p.n = static_cast<int>(c.hidden.rows);
-    p.n_rows = static_cast<int>(round_up(std::max<int64_t>(c.hidden.rows, 1), kTile));
+    p.n_rows = static_cast<int>(round_up(c.hidden.rows, kTile));
     p.vocab = static_cast<int>(c.weight.rows);
     p.width = static_cast<int>(c.hidden.cols);
     p.cols = static_cast<int>(round_up(p.width, 8));
     p.entries = c.entries ? c.entries : 1;
+    p.pairs = multiprocessors() / 2;
     p.copy_weight = p.width % 8 || c.weight.stride % 8 || reinterpret_cast<uintptr_t>(c.weight.data) % 16;
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) {
@@ -726,29 +861,31 @@ Plan make_plan(const LossCall& c, bool backward) {
     const int64_t listed = static_cast<int64_t>(p.n) * p.entries;
     p.shared = take(sizeof(Shared));
     p.rows = take(4ull * p.n);
-    p.entry_ids = take(4ull * listed);
+    p.entry = take(sizeof(Entry) * listed);
     if (c.entries) {
-        p.entry_share = take(4ull * listed);
-        p.first = take(4ull * p.n);
+        p.entry_raw = take(sizeof(Entry) * listed);
+        p.state = take(4ull * p.n);
     }
     p.hidden = take(2ull * p.n_rows * p.cols);
     if (p.copy_weight) p.weight = take(2ull * p.vocab * p.cols);
+    const int64_t tiles = div_up(p.vocab, kTile);
     if (!backward) {
         p.entry_logits = take(4ull * listed);
-        p.partial = take(8ull * 2 * div_up(p.vocab, kTile) * p.n_rows);
+        p.partial = take(8ull * 2 * tiles * p.n_rows);
     } else {
-        const int64_t tiles = div_up(p.vocab, kTile), room = std::max<int64_t>(1, kDeltaBytes / (2ll * kTile * p.n_rows));
-        const int64_t pieces = div_up(tiles, room);
-        p.piece = static_cast<int>(div_up(tiles, pieces) * kTile);
-        const int64_t outs = static_cast<int64_t>(p.n_rows / kTile) * div_up(p.width, kTile), pairs = 74;
-        p.splits = 1;
-        double best = 1e30;
-        for (int s = 1; s <= 32 && s * 512 <= p.piece; ++s) {
-            const double waves = static_cast<double>(div_up(outs * s, pairs)) / s + 0.01 * s;
-            if (waves < best - 1e-9) { best = waves; p.splits = s; }
+        p.info = take(sizeof(RowInfo) * p.n);
+        const int64_t room = std::max<int64_t>(1, kDeltaBytes / (2ll * kTile * p.n_rows));
+        p.piece = static_cast<int>(div_up(tiles, div_up(tiles, room)) * kTile);
+        const int64_t width_tiles = div_up(p.cols, kTile);
+        for (int64_t t = 1; t <= p.n_rows / kTile; ++t)
+        {
+            int splits = 1;
+            for (int k = 2; k <= kMaxSplits; ++k)
+                if (split_time(k, t * width_tiles, p.piece / kDepth, p.pairs) < split_time(splits, t * width_tiles, p.piece / kDepth, p.pairs)) splits = k;
+            p.sum_rows = std::max(p.sum_rows, t * kTile * splits);
         }
         p.delta = take(2ull * p.n_rows * p.piece);
-        p.sums = take(4ull * p.splits * p.n_rows * p.cols);
+        p.sums = take(4ull * p.sum_rows * p.cols);
     }
     p.bytes = at;
     return p;
@@ -776,13 +913,27 @@ bool tile_map(CUtensorMap* map, int type, const void* data, int64_t rows, int64_
                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Launches that may begin before the kernel in front of them on the stream has ended (see after_previous).
+template <typename... Params, typename... Args>
+cudaError_t launch(void (*kernel)(Params...), int64_t blocks, int threads, int smem, cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(blocks));
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...);
+}
+
 template <int MODE>
-cudaError_t launch_product(bool bf16, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const Product& p, cudaStream_t stream) {
+cudaError_t launch_product(bool bf16, int pairs, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const Product& p, cudaStream_t stream) {
     auto* kernel = bf16 ? product_kernel<MODE, true> : product_kernel<MODE, false>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-    if (e != cudaSuccess) return e;
-    kernel<<<multiprocessors() / 2 * 2, kThreads, kSmemBytes, stream>>>(a, b, out, p);
-    return cudaGetLastError();
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes)) return e;
+    return launch(kernel, 2 * pairs, kThreads, kSmemBytes, stream, a, b, out, p);
 }
 
 struct Prepared {
@@ -790,8 +941,6 @@ struct Prepared {
     char* at;
     Shared* shared;
     int* rows;
-    const uint16_t* weight;
-    int64_t weight_stride;
     Product product;
     CUtensorMap hidden_map, weight_map;
 };
@@ -806,48 +955,82 @@ const char* prepare(const LossCall& c, bool backward, Prepared& w) {
     w.at = static_cast<char*>(c.workspace);
     w.shared = reinterpret_cast<Shared*>(w.at + p.shared);
     w.rows = reinterpret_cast<int*>(w.at + p.rows);
-    int* entry_ids = reinterpret_cast<int*>(w.at + p.entry_ids);
-    float* entry_share = c.entries ? reinterpret_cast<float*>(w.at + p.entry_share) : nullptr;
-    int* first = c.entries ? reinterpret_cast<int*>(w.at + p.first) : nullptr;
-    const float inv_temperature = 1.f / c.temperature;
+    Entry *entry = reinterpret_cast<Entry*>(w.at + p.entry), *entry_raw = reinterpret_cast<Entry*>(w.at + p.entry_raw);
+    int* state = reinterpret_cast<int*>(w.at + p.state);
+    RowInfo* info = backward ? reinterpret_cast<RowInfo*>(w.at + p.info) : nullptr;
+    const float inv_temperature = 1.f / c.temperature;      // of the teacher's logits and the gradient; the student's: see cut_off
     if (c.entries) {
         int room = 2;
         while (room < c.entries) room *= 2;
-        teacher_kernel<<<p.n, std::min(256, std::max(32, room / 2)), room * 12, c.stream>>>(c.targets, c.teacher, c.entries, room, p.vocab, inv_temperature, entry_ids,
-                                                                                             entry_share, first);
+        if (cudaError_t e = launch(teacher_kernel, p.n, std::min(256, std::max(32, room / 2)), room * 12, c.stream, c.targets, c.teacher, c.entries, room, p.vocab,
+                                   inv_temperature, entry_raw, state))
+            return cuda_error(e);
     }
-    rows_kernel<<<1, 1024, 0, c.stream>>>(c.targets, c.ignore, p.vocab, p.n, first, entry_ids, w.rows, w.shared, backward ? nullptr : c.losses,
-                                          backward ? nullptr : c.lse, backward ? c.grad : nullptr, c.grad_stride, c.grad_of_mean, inv_temperature,
-                                          c.hidden.type == kF16);
-    uint16_t* hidden = reinterpret_cast<uint16_t*>(w.at + p.hidden);
-    const bool wide = p.width % 8 == 0 && c.hidden.stride % 8 == 0 && reinterpret_cast<uintptr_t>(c.hidden.data) % 16 == 0;
-    gather_kernel<<<std::min(p.n_rows, 148 * 16), 128, 0, c.stream>>>(static_cast<const uint16_t*>(c.hidden.data), c.hidden.stride, p.width, w.rows, w.shared, p.n, hidden,
-                                                                      p.cols, wide);
-    w.weight = static_cast<const uint16_t*>(c.weight.data);
-    w.weight_stride = c.weight.stride;
+    RowsArgs r{};
+    r.targets = c.targets;
+    r.ignore = c.ignore;
+    r.vocab = p.vocab;
+    r.n = p.n;
+    r.state = c.entries ? state : nullptr;
+    r.entry = entry;
+    r.rows = w.rows;
+    r.shared = w.shared;
+    r.losses = backward ? nullptr : c.losses;
+    r.lse = backward ? nullptr : c.lse;
+    r.grad = backward ? c.grad : nullptr;
+    r.grad_stride = c.grad_stride;
+    r.grad_of_mean = c.grad_of_mean;
+    r.half = c.hidden.type == kF16;
+    r.inv_temperature = inv_temperature;
+    r.width_tiles = static_cast<int>(div_up(p.cols, kTile));
+    r.blocks = p.piece / kDepth;
+    r.pairs = p.pairs;
+    if (cudaError_t e = launch(rows_kernel, 1, 1024, 0, c.stream, r)) return cuda_error(e);
+    const void* weight = c.weight.data;
+    int64_t weight_stride = c.weight.stride;
+    GatherArgs g{};
     if (p.copy_weight) {
-        uint16_t* copy = reinterpret_cast<uint16_t*>(w.at + p.weight);
-        gather_kernel<<<148 * 16, 128, 0, c.stream>>>(w.weight, c.weight.stride, p.width, nullptr, w.shared, p.vocab, copy, p.cols, false);
-        w.weight = copy;
-        w.weight_stride = p.cols;
+        g.src = static_cast<const uint16_t*>(weight);
+        g.stride = weight_stride;
+        g.cols = p.width;
+        g.n = p.vocab;
+        g.dst = reinterpret_cast<uint16_t*>(w.at + p.weight);
+        g.dst_cols = p.cols;
+        if (cudaError_t e = launch(gather_kernel, std::min(p.vocab, 148 * 16), 128, 0, c.stream, g)) return cuda_error(e);
+        weight = g.dst;
+        weight_stride = p.cols;
     }
-    if (!tile_map(&w.hidden_map, c.hidden.type, hidden, p.n_rows, p.cols, p.cols, 64) ||
-        !tile_map(&w.weight_map, c.hidden.type, w.weight, p.vocab, p.cols, w.weight_stride, 64))
+    g.src = static_cast<const uint16_t*>(c.hidden.data);
+    g.stride = c.hidden.stride;
+    g.cols = p.width;
+    g.rows = w.rows;
+    g.shared = w.shared;
+    g.n = p.n;
+    g.dst = reinterpret_cast<uint16_t*>(w.at + p.hidden);
+    g.dst_cols = p.cols;
+    g.wide = p.width % 8 == 0 && c.hidden.stride % 8 == 0 && reinterpret_cast<uintptr_t>(c.hidden.data) % 16 == 0;
+    g.entries = c.entries;
+    g.entry_from = entry_raw;
+    g.entry_to = entry;
+    g.info = info;
+    g.lse = c.lse;
+    g.grad = c.grad;
+    g.grad_stride = c.grad_stride;
+    if (cudaError_t e = launch(gather_kernel, std::min(p.n_rows, 148 * 16), 128, 0, c.stream, g)) return cuda_error(e);
+    if (!tile_map(&w.hidden_map, c.hidden.type, g.dst, p.n_rows, p.cols, p.cols, 64) || !tile_map(&w.weight_map, c.hidden.type, weight, p.vocab, p.cols, weight_stride, 64))
         return "a tensor map was refused";
     Product& q = w.product;
     q = Product{};
     q.shared = w.shared;
-    q.rows = w.rows;
     q.n_rows = p.n_rows;
     q.vocab = p.vocab;
     q.width = p.cols;
     q.count = p.vocab;
     q.entries = p.entries;
-    q.entry_ids = entry_ids;
-    q.entry_share = entry_share;
-    q.exponent = kLog2e / c.temperature;
-    q.splits = 1;
-    return cuda_error(cudaGetLastError());
+    q.entry = entry;
+    q.info = info;
+    q.exponent = kLog2e / c.temperature * cut_off(p.width);
+    return nullptr;
 }
 
 }  // namespace
@@ -862,12 +1045,24 @@ const char* loss_forward(const LossCall& c) {
     Product& q = w.product;
     q.partial = reinterpret_cast<float2*>(w.at + p.partial);
     q.entry_logits = reinterpret_cast<float*>(w.at + p.entry_logits);
-    if (cudaError_t e = launch_product<kForward>(c.hidden.type == kBF16, w.hidden_map, w.weight_map, w.hidden_map, q, c.stream)) return cuda_error(e);
-    join_kernel<<<static_cast<int>(std::min<int64_t>(div_up(p.n, 32), 148 * 4)), 512, 0, c.stream>>>(
-        q.partial, static_cast<int>(2 * div_up(p.vocab, kTile)), p.n_rows, w.shared, w.rows, p.entries, q.entry_ids, q.entry_share, q.entry_logits, q.exponent,
-        1.f / c.temperature, c.losses, c.lse);
-    if (c.total) total_kernel<<<1, 1024, 0, c.stream>>>(c.losses, p.n, w.shared, c.mean, c.total);
-    return cuda_error(cudaGetLastError());
+    if (cudaError_t e = launch_product<kForward>(c.hidden.type == kBF16, p.pairs, w.hidden_map, w.weight_map, w.hidden_map, q, c.stream)) return cuda_error(e);
+    JoinArgs j{};
+    j.partial = q.partial;
+    j.parts = static_cast<int>(2 * div_up(p.vocab, kTile));
+    j.n_rows = p.n_rows;
+    j.shared = w.shared;
+    j.rows = w.rows;
+    j.n = p.n;
+    j.entries = p.entries;
+    j.entry = q.entry;
+    j.entry_logits = q.entry_logits;
+    j.exponent = q.exponent;
+    j.inv_temperature = 1.f / c.temperature * cut_off(p.width);
+    j.losses = c.losses;
+    j.lse = c.lse;
+    j.total = c.total;
+    j.mean = c.mean;
+    return cuda_error(launch(join_kernel, std::min<int64_t>(div_up(p.n, 32), 148 * 2), 1024, 0, c.stream, j));
 }
 
 const char* loss_backward(const LossCall& c) {
@@ -883,7 +1078,7 @@ const char* loss_backward(const LossCall& c) {
     float* sums = reinterpret_cast<float*>(w.at + p.sums);
     CUtensorMap delta_map, delta_out, sums_out, weight_out;
     if (!tile_map(&delta_map, c.hidden.type, delta, p.n_rows, p.piece, p.piece, 64) || !tile_map(&delta_out, c.hidden.type, delta, p.n_rows, p.piece, p.piece, 32) ||
-        !tile_map(&sums_out, kF32, sums, static_cast<int64_t>(p.splits) * p.n_rows, p.cols, p.cols, 32))
+        !tile_map(&sums_out, kF32, sums, p.sum_rows, p.cols, p.cols, 32))
         return "a tensor map was refused";
     uint16_t* d_weight = static_cast<uint16_t*>(const_cast<void*>(c.d_weight.data));
     const bool direct = d_weight && (p.width % 8 || c.d_weight.stride % 8 || reinterpret_cast<uintptr_t>(d_weight) % 16);
@@ -896,32 +1091,25 @@ const char* loss_backward(const LossCall& c) {
         Product q = w.product;
         q.first = first;
         q.count = std::min(p.piece, p.vocab - first);
-        q.lse = c.lse;
-        q.grad = c.grad;
-        q.grad_stride = c.grad_stride;
-        if (cudaError_t e = launch_product<kDelta>(bf16, w.hidden_map, w.weight_map, delta_out, q, c.stream)) return cuda_error(e);
+        if (cudaError_t e = launch_product<kDelta>(bf16, p.pairs, w.hidden_map, w.weight_map, delta_out, q, c.stream)) return cuda_error(e);
         if (c.d_hidden.data) {
-            q.splits = p.splits;
             q.add = first > 0;
-            if (cudaError_t e = launch_product<kHiddenGrad>(bf16, delta_map, w.weight_map, sums_out, q, c.stream)) return cuda_error(e);
+            if (cudaError_t e = launch_product<kHiddenGrad>(bf16, p.pairs, delta_map, w.weight_map, sums_out, q, c.stream)) return cuda_error(e);
         }
         if (d_weight) {
-            q.splits = 1;
-            q.add = false;
-            q.direct = direct ? d_weight : nullptr;
-            q.direct_stride = c.d_weight.stride;
-            if (direct) q.width = p.width;
-            if (cudaError_t e = launch_product<kWeightGrad>(bf16, delta_map, w.hidden_map, weight_out, q, c.stream)) return cuda_error(e);
+            q.direct = direct;
+            q.out = d_weight;
+            q.out_stride = c.d_weight.stride;
+            q.width = p.width;
+            if (cudaError_t e = launch_product<kWeightGrad>(bf16, p.pairs, delta_map, w.hidden_map, weight_out, q, c.stream)) return cuda_error(e);
         }
     }
-    if (c.d_hidden.data) {
-        uint16_t* out = static_cast<uint16_t*>(const_cast<void*>(c.d_hidden.data));
-        const bool wide = p.width % 4 == 0 && c.d_hidden.stride % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0;
-        auto* kernel = bf16 ? hidden_grad_kernel<true> : hidden_grad_kernel<false>;
-        kernel<<<std::min(p.n, 148 * 16), 256, 0, c.stream>>>(sums, p.splits, p.n_rows, p.cols, w.shared, w.rows, p.n, p.width, out, c.d_hidden.stride, wide);
-    }
-    if (d_weight) no_rows_kernel<<<148 * 4, 256, 0, c.stream>>>(w.shared, d_weight, p.vocab, p.width, c.d_weight.stride, bf16 ? 0x7FC0 : 0x7E00);
-    return cuda_error(cudaGetLastError());
+    if (!c.d_hidden.data) return nullptr;
+    uint16_t* out = static_cast<uint16_t*>(const_cast<void*>(c.d_hidden.data));
+    const bool wide = p.width % 8 == 0 && c.d_hidden.stride % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    const int64_t blocks = std::min<int64_t>(div_up(static_cast<int64_t>(p.n) * div_up(p.width, 8), 256), 148 * 32);
+    return cuda_error(launch(bf16 ? hidden_grad_kernel<true> : hidden_grad_kernel<false>, blocks, 256, 0, c.stream, sums, p.cols, w.shared, w.rows, p.n, p.width, out,
+                             c.d_hidden.stride, wide));
 }
 
 }  // namespace gtok
