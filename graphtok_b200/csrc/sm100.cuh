@@ -139,10 +139,5 @@ __device__ __forceinline__ float exp2_fast(float x) {     // the hardware's 2^x,
     return y;
 }
 
-// ---- launches that overlap the end of the one before --------------------------------
-// A kernel launched so may begin while the one before it on the stream still runs; what it reads of that one's it reads behind this.
-__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 }  // namespace sm100
 }  // namespace gtok

@@ -15,6 +15,7 @@
 // Rows without a loss (ignored targets, no teacher entries) are left out before the products: the others are copied together, so
 // neither time nor NaN of masked positions is carried along.
 #include "sm100.cuh"
+#include "vocab_launch.cuh"
 #include "vocab_ops.h"
 
 #include <algorithm>
@@ -911,22 +912,6 @@ bool tile_map(CUtensorMap* map, int type, const void* data, int64_t rows, int64_
     const CUtensorMapDataType kind = type == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     return encode_fn()(map, kind, 2, const_cast<void*>(data), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// Launches that may begin before the kernel in front of them on the stream has ended (see after_previous).
-template <typename... Params, typename... Args>
-cudaError_t launch(void (*kernel)(Params...), int64_t blocks, int threads, int smem, cudaStream_t stream, Args&&... args) {
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(static_cast<unsigned>(blocks));
-    config.blockDim = dim3(threads);
-    config.dynamicSmemBytes = smem;
-    config.stream = stream;
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...);
 }
 
 template <int MODE>

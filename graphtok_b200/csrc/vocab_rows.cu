@@ -1,10 +1,12 @@
 // Rows of a table by token id: the embedding lookup, its gradient, and the ids that follow in packed documents.
+#include "vocab_launch.cuh"
 #include "vocab_ops.h"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace gtok {
 namespace {
@@ -29,36 +31,78 @@ struct alignas(sizeof(T) * N) Lump {
 };
 
 // ---- lookup ---------------------------------------------------------------------
-// out[t, :] = scale * table[id_t, :]; a negative id gives a row of zeros, an id beyond the table a row of NaN.  Bound by memory: each
-// thread has four lumps under way.
+// out[t, :] = scale * table[id_t, :]; a negative id gives a row of zeros, an id beyond the table a row of NaN.  Bound by memory.  The output is
+// cut into lumps whatever its width; each thread has four of them, 256 apart, under way at once, and writes past the caches, which are
+// better used for rows that are asked for again.
 template <typename T, int N>
-__global__ void __launch_bounds__(256) embed_kernel(const void* ids, int bits, int64_t n, const T* table, int64_t vocab, int64_t stride, int lumps, float scale, T* out,
+__device__ __forceinline__ void scale_lump(Lump<T, N>& v, float scale) {
+    if constexpr (N == 8) {             // two elements of 16 bits at a time
+        using Pair = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+        Pair* pair = reinterpret_cast<Pair*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same_v<T, __half>) {
+                const float2 f = __half22float2(pair[i]);
+                pair[i] = __floats2half2_rn(scale * f.x, scale * f.y);
+            } else {
+                const float2 f = __bfloat1622float2(pair[i]);
+                pair[i] = __floats2bfloat162_rn(scale * f.x, scale * f.y);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v.v[i] = from_float<T>(scale * to_float<T>(v.v[i]));
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void write_past(Lump<T, N>* to, const Lump<T, N>& v) {
+    if constexpr (sizeof(Lump<T, N>) == 16) __stcs(reinterpret_cast<uint4*>(to), reinterpret_cast<const uint4&>(v));
+    else *to = v;
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(256) embed_kernel(const void* ids, int bits, int64_t n, const T* table, int64_t vocab, int64_t stride, uint32_t lumps, float scale, T* out,
                                                     int64_t out_stride) {
     using L = Lump<T, N>;
-    for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; t < n; t += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-        const int64_t id = load_id(ids, bits, t);
-        const bool known = id >= 0 && id < vocab;
-        const L* from = reinterpret_cast<const L*>(table + (known ? id : 0) * stride);
-        L* to = reinterpret_cast<L*>(out + t * out_stride);
-        const T other = from_float<T>(id < 0 ? 0.f : __int_as_float(0x7FC00000));
-        for (int i = threadIdx.x; i < lumps; i += 4 * blockDim.x) {
-            L v[4];
+    constexpr int kEach = 4;
+    after_previous();
+    let_next_begin();
+    const int64_t blocks = (n * lumps + 256 * kEach - 1) / (256 * kEach);
+    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+        const int64_t t0 = block * (256 * kEach) / lumps;
+        const uint32_t first = static_cast<uint32_t>(block * (256 * kEach) - t0 * lumps) + threadIdx.x;
+        int64_t t[kEach], id[kEach];
+        uint32_t col[kEach];
+        L v[kEach];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (known && i + k * static_cast<int>(blockDim.x) < lumps) v[k] = from[i + k * blockDim.x];
+        for (int k = 0; k < kEach; ++k) {
+            const uint32_t down = (first + 256 * k) / lumps;
+            col[k] = first + 256 * k - down * lumps;
+            t[k] = t0 + down;
+            id[k] = t[k] < n ? load_id(ids, bits, t[k]) : -1;
+        }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (i + k * static_cast<int>(blockDim.x) >= lumps) break;
+        for (int k = 0; k < kEach; ++k)
+            if (id[k] >= 0 && id[k] < vocab) v[k] = reinterpret_cast<const L*>(table + id[k] * stride)[col[k]];
 #pragma unroll
-                for (int e = 0; e < N; ++e) v[k].v[e] = known ? from_float<T>(scale * to_float<T>(v[k].v[e])) : other;
-                to[i + k * blockDim.x] = v[k];
+        for (int k = 0; k < kEach; ++k) {
+            if (t[k] >= n) continue;
+            if (id[k] >= 0 && id[k] < vocab) {
+                scale_lump(v[k], scale);
+            } else {
+                const T other = from_float<T>(id[k] < 0 ? 0.f : __int_as_float(0x7FC00000));
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[k].v[e] = other;
             }
+            write_past(reinterpret_cast<L*>(out + t[k] * out_stride) + col[k], v[k]);
         }
     }
 }
 
 // ---- the ids that follow ----------------------------------------------------------
 __global__ void next_kernel(const int32_t* ids, int64_t n, const int32_t* offsets, int64_t n_docs, const uint8_t* loss_mask, int32_t ignore, int32_t* out) {
+    after_previous();
+    let_next_begin();
     const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= n) return;
     int64_t lo = 0, hi = n_docs + 1;              // offsets at or before i
@@ -73,107 +117,238 @@ __global__ void next_kernel(const int32_t* ids, int64_t n, const int32_t* offset
 // ---- the lookup's gradient ----------------------------------------------------------
 // The places of the ids are sorted by id (radix sort, stable), so that the rows to be summed for one id follow one another in the
 // order of the text and their sum does not depend on how the GPU runs.  Runs of equal ids differ from one place to tens of thousands;
-// the sorted places are therefore cut into chunks of 32 whatever they hold, and runs across chunks are joined from fp32 partial sums.
+// the sorted places are therefore cut into chunks of 32 (8, where that makes too few warps) whatever they hold, and runs across chunks are
+// joined from fp32 partial sums.
+//
+// Most of the gradient's bytes are rows that no id asks for.  The sort is a few short launches that leave memory idle: further blocks of
+// the same launches write these zeros meanwhile.
 constexpr int kDigit = 9, kBins = 1 << kDigit;
-constexpr int kSortThreads = 256, kSortEach = 8, kSortTile = kSortThreads * kSortEach;
-constexpr int kChunk = 32;
+constexpr int kSortThreads = 256, kSortEach = 8, kSortTile = kSortThreads * kSortEach, kSortWarps = kSortThreads / 32;
+constexpr int kChunk = 32, kShortChunk = 8;
 
 struct Key { uint32_t id, place; };
 
-// First pass: keys from the ids (those outside the table sort behind it), and which rows of the table occur.
-__device__ __forceinline__ uint32_t key_of(const void* ids, int bits, int64_t i, uint32_t vocab) {
-    const int64_t id = load_id(ids, bits, i);
-    return id >= 0 && id < vocab ? static_cast<uint32_t>(id) : vocab;
+struct SortArgs {
+    const void* ids;
+    int bits;
+    int64_t n;
+    uint32_t vocab;
+    int tiles, shift, passes;
+    const Key* in;
+    Key* out;
+    uint32_t *counts, *seen;       // seen: a bit for each row that an id asks for
+    // rows that a launch's further blocks clear where no id asks for them
+    char* rows;
+    int64_t row_bytes, row_stride;
+    int64_t from, to;
+    int unit;                      // bytes written together: 16, or an element
+};
+
+// Ids outside the table sort behind it.
+__device__ __forceinline__ uint32_t key_of(const SortArgs& a, int64_t i) {
+    const int64_t id = load_id(a.ids, a.bits, i);
+    return id >= 0 && id < a.vocab ? static_cast<uint32_t>(id) : a.vocab;
+}
+
+template <typename U>
+__device__ __forceinline__ void clear_row(char* row, int64_t bytes, int lane) {
+    U zero;
+    memset(&zero, 0, sizeof(U));
+    for (int64_t i = lane; i < bytes / static_cast<int64_t>(sizeof(U)); i += 32) reinterpret_cast<U*>(row)[i] = zero;
+}
+// Warp `self` of `warps` clears its share of the rows [a.from, a.to).  `seen` begins at the bit of row `first`.
+__device__ __forceinline__ void clear_rows(const SortArgs& a, const uint32_t* seen, int64_t first, int64_t from, int64_t to, int64_t self, int64_t warps) {
+    const int lane = threadIdx.x & 31;
+    for (int64_t r = from + self; r < to; r += warps) {
+        const int64_t bit = r - first;
+        if (seen[bit >> 5] >> (bit & 31) & 1) continue;
+        char* row = a.rows + r * a.row_stride;
+        if (a.unit == 16) clear_row<uint4>(row, a.row_bytes, lane);
+        else if (a.unit == 4) clear_row<uint32_t>(row, a.row_bytes, lane);
+        else clear_row<uint16_t>(row, a.row_bytes, lane);
+    }
+}
+__device__ __forceinline__ void clear_share(const SortArgs& a) {
+    clear_rows(a, a.seen, 0, a.from, a.to, static_cast<int64_t>(blockIdx.x - a.tiles) * kSortWarps + (threadIdx.x >> 5),
+               static_cast<int64_t>(gridDim.x - a.tiles) * kSortWarps);
 }
 
 template <bool FIRST>
-__global__ void __launch_bounds__(kSortThreads) count_kernel(const void* ids, int bits, const Key* in, int64_t n, uint32_t vocab, int shift, uint32_t* counts,
-                                                             uint32_t* seen) {
+__global__ void __launch_bounds__(kSortThreads) count_kernel(const __grid_constant__ SortArgs a) {
     __shared__ uint32_t bin[kBins];
+    after_previous();
+    let_next_begin();
+    if (!FIRST && static_cast<int>(blockIdx.x) >= a.tiles) return clear_share(a);
     for (int b = threadIdx.x; b < kBins; b += kSortThreads) bin[b] = 0;
     __syncthreads();
     const int64_t from = static_cast<int64_t>(blockIdx.x) * kSortTile;
-    for (int i = threadIdx.x; i < kSortTile && from + i < n; i += kSortThreads) {
-        const uint32_t key = FIRST ? key_of(ids, bits, from + i, vocab) : in[from + i].id;
-        atomicAdd(&bin[key >> shift & (kBins - 1)], 1u);
-        if (FIRST && key < vocab) atomicOr(&seen[key >> 5], 1u << (key & 31));
+    uint32_t key[kSortEach];
+#pragma unroll
+    for (int i = 0; i < kSortEach; ++i) {
+        const int64_t at = from + i * kSortThreads + threadIdx.x;
+        if (at < a.n) key[i] = FIRST ? key_of(a, at) : a.in[at].id;
+    }
+#pragma unroll
+    for (int i = 0; i < kSortEach; ++i) {
+        if (from + i * kSortThreads + threadIdx.x >= a.n) continue;
+        atomicAdd(&bin[key[i] >> a.shift & (kBins - 1)], 1u);
+        if (FIRST && key[i] < a.vocab) atomicOr(&a.seen[key[i] >> 5], 1u << (key[i] & 31));
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < kBins; b += kSortThreads) counts[static_cast<int64_t>(blockIdx.x) * kBins + b] = bin[b];
+    for (int b = threadIdx.x; b < kBins; b += kSortThreads) a.counts[static_cast<int64_t>(blockIdx.x) * kBins + b] = bin[b];
 }
 
-template <bool FIRST>
-__global__ void __launch_bounds__(kSortThreads) scatter_kernel(const void* ids, int bits, const Key* in, int64_t n, uint32_t vocab, int shift, const uint32_t* counts,
-                                                               Key* out) {
-    constexpr int kWarps = kSortThreads / 32;
-    __shared__ uint32_t base[kBins];
-    __shared__ uint16_t warp_bin[kWarps][kBins];
-    __shared__ uint32_t warp_sum[kWarps];
+struct SortSpace {
+    uint32_t base[kBins];
+    uint16_t warp_bin[kSortWarps][kBins];
+    uint32_t warp_sum[kSortWarps];
+};
+
+// Places of a tile's keys (256 a warp, in order) after one digit: `key` to s.base[bin] + s.warp_bin[warp][bin] + rank.  With `all` and `mine`, the
+// keys of a thread's two bins in all tiles and in those before; without, the tile is all there is.
+__device__ __forceinline__ void rank_keys(SortSpace& s, const Key (&key)[kSortEach], const bool (&here)[kSortEach], uint16_t (&rank)[kSortEach], int shift,
+                                          bool alone, uint32_t all0, uint32_t all1, uint32_t mine0, uint32_t mine1) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    for (int b = tid; b < kWarps * kBins; b += kSortThreads) (&warp_bin[0][0])[b] = 0;
-    // where this tile's keys of each bin begin: all smaller bins, and the same bin in the tiles before
-    uint32_t all[2], mine[2];
+    __syncthreads();
+    for (int b = tid; b < kSortWarps * kBins; b += kSortThreads) (&s.warp_bin[0][0])[b] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSortEach; ++i) {
+        const uint32_t b = here[i] ? key[i].id >> shift & (kBins - 1) : kBins;
+        const uint32_t same = __match_any_sync(~0u, b);
+        const uint16_t seen = here[i] ? s.warp_bin[warp][b] : 0;
+        __syncwarp();
+        rank[i] = seen + __popc(same & ((1u << lane) - 1));
+        if (here[i] && (same & ((1u << lane) - 1)) == 0) s.warp_bin[warp][b] = seen + __popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+    uint32_t total[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        uint32_t sum = 0, before = 0;
-        for (uint32_t t = 0; t < gridDim.x; ++t) {
-            const uint32_t c = counts[static_cast<int64_t>(t) * kBins + 2 * tid + k];
-            before += t < blockIdx.x ? c : 0;
-            sum += c;
+        uint32_t run = 0;
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) {
+            const uint32_t c = s.warp_bin[w][2 * tid + k];
+            s.warp_bin[w][2 * tid + k] = static_cast<uint16_t>(run);
+            run += c;
         }
-        all[k] = sum;
-        mine[k] = before;
+        total[k] = run;
     }
-    uint32_t scan = all[0] + all[1];
+    if (alone) { all0 = total[0]; all1 = total[1]; }
+    uint32_t scan = all0 + all1;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const uint32_t y = __shfl_up_sync(~0u, scan, d);
         if (lane >= d) scan += y;
     }
-    if (lane == 31) warp_sum[warp] = scan;
+    if (lane == 31) s.warp_sum[warp] = scan;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) scan += warp_sum[w];
-    base[2 * tid] = scan - all[0] - all[1] + mine[0];
-    base[2 * tid + 1] = scan - all[1] + mine[1];
-    // each warp takes its 256 keys in order; a key's rank among those of its bin
+    for (int w = 0; w < warp; ++w) scan += s.warp_sum[w];
+    s.base[2 * tid] = scan - all0 - all1 + mine0;
+    s.base[2 * tid + 1] = scan - all1 + mine1;
+    __syncthreads();
+}
+
+template <bool FIRST>
+__global__ void __launch_bounds__(kSortThreads) scatter_kernel(const __grid_constant__ SortArgs a) {
+    __shared__ SortSpace s;
+    after_previous();
+    let_next_begin();
+    if (static_cast<int>(blockIdx.x) >= a.tiles) return clear_share(a);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t from = static_cast<int64_t>(blockIdx.x) * kSortTile + warp * 32 * kSortEach;
     Key key[kSortEach];
+    bool here[kSortEach];
     uint16_t rank[kSortEach];
 #pragma unroll
     for (int i = 0; i < kSortEach; ++i) {
         const int64_t at = from + i * 32 + lane;
-        key[i] = Key{0xFFFFFFFFu, 0};
-        if (at < n) key[i] = FIRST ? Key{key_of(ids, bits, at, vocab), static_cast<uint32_t>(at)} : in[at];
+        here[i] = at < a.n;
+        key[i] = here[i] ? (FIRST ? Key{key_of(a, at), static_cast<uint32_t>(at)} : a.in[at]) : Key{0xFFFFFFFFu, 0};
     }
+    // how many keys of this thread's two bins there are: in all tiles, and in those before this one
+    uint2 all = make_uint2(0, 0), mine = make_uint2(0, 0);
+    const uint2* counts = reinterpret_cast<const uint2*>(a.counts);
+    for (int t = 0; t < a.tiles; t += 8) {
+        uint2 c[8];
 #pragma unroll
-    for (int i = 0; i < kSortEach; ++i) {
-        const bool here = from + i * 32 + lane < n;
-        const uint32_t b = here ? key[i].id >> shift & (kBins - 1) : kBins;
-        const uint32_t same = __match_any_sync(~0u, b);
-        uint16_t seen = here ? warp_bin[warp][b] : 0;
-        __syncwarp();
-        rank[i] = seen + __popc(same & ((1u << lane) - 1));
-        if (here && (same & ((1u << lane) - 1)) == 0) warp_bin[warp][b] = seen + __popc(same);
-        __syncwarp();
-    }
-    __syncthreads();
-    for (int b = tid; b < kBins; b += kSortThreads) {
-        uint32_t sum = base[b];
-        base[b] = sum;
-        uint32_t run = 0;
+        for (int k = 0; k < 8; ++k) c[k] = t + k < a.tiles ? counts[static_cast<int64_t>(t + k) * (kBins / 2) + tid] : make_uint2(0, 0);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const uint32_t c = warp_bin[w][b];
-            warp_bin[w][b] = static_cast<uint16_t>(run);
-            run += c;
+        for (int k = 0; k < 8; ++k) {
+            if (t + k < static_cast<int>(blockIdx.x)) { mine.x += c[k].x; mine.y += c[k].y; }
+            all.x += c[k].x;
+            all.y += c[k].y;
         }
     }
-    __syncthreads();
+    rank_keys(s, key, here, rank, a.shift, false, all.x, all.y, mine.x, mine.y);
 #pragma unroll
     for (int i = 0; i < kSortEach; ++i) {
-        if (from + i * 32 + lane >= n) continue;
-        const uint32_t b = key[i].id >> shift & (kBins - 1);
-        out[base[b] + warp_bin[warp][b] + rank[i]] = key[i];
+        if (!here[i]) continue;
+        const uint32_t b = key[i].id >> a.shift & (kBins - 1);
+        a.out[s.base[b] + s.warp_bin[warp][b] + rank[i]] = key[i];
+    }
+}
+
+// All of the sort where the ids make one tile: block 0 sorts, digit after digit, the others clear a share of the rows.  Each of those finds
+// out for itself which of its rows are asked for.
+constexpr int kOwnRows = 4096;          // rows whose bits a block has room for
+__global__ void __launch_bounds__(kSortThreads) one_tile_kernel(const __grid_constant__ SortArgs a) {
+    __shared__ union {
+        struct { SortSpace space; Key key[kSortTile]; } sort;
+        uint32_t seen[kOwnRows / 32];
+    } s;
+    after_previous();
+    let_next_begin();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (blockIdx.x > 0) {
+        const int64_t blocks = gridDim.x - 1, self = blockIdx.x - 1;
+        const int64_t share = min((a.to - a.from + blocks - 1) / blocks, static_cast<int64_t>(kOwnRows));
+        for (int64_t from = a.from + self * share; from < a.to; from += blocks * share) {
+            const int64_t to = min(from + share, a.to);
+            __syncthreads();
+            for (int i = tid; i < kOwnRows / 32; i += kSortThreads) s.seen[i] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kSortEach; ++i) {
+                const int at = i * kSortThreads + tid;
+                if (at >= a.n) continue;
+                const int64_t id = key_of(a, at);
+                if (id >= from && id < to) atomicOr(&s.seen[(id - from) >> 5], 1u << ((id - from) & 31));
+            }
+            __syncthreads();
+            clear_rows(a, s.seen, from, from, to, warp, kSortWarps);
+        }
+        return;
+    }
+    for (int64_t i = tid; i < (a.vocab + 31) / 32; i += kSortThreads) a.seen[i] = 0;
+    Key key[kSortEach];
+    bool here[kSortEach];
+    uint16_t rank[kSortEach];
+#pragma unroll
+    for (int i = 0; i < kSortEach; ++i) {
+        const int at = warp * 32 * kSortEach + i * 32 + lane;
+        here[i] = at < a.n;
+        key[i] = here[i] ? Key{key_of(a, at), static_cast<uint32_t>(at)} : Key{0xFFFFFFFFu, 0};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSortEach; ++i)
+        if (here[i] && key[i].id < a.vocab) atomicOr(&a.seen[key[i].id >> 5], 1u << (key[i].id & 31));
+    for (int pass = 0; pass < a.passes; ++pass) {
+        rank_keys(s.sort.space, key, here, rank, pass * kDigit, true, 0, 0, 0, 0);
+        Key* to = pass + 1 < a.passes ? s.sort.key : a.out;
+#pragma unroll
+        for (int i = 0; i < kSortEach; ++i) {
+            if (!here[i]) continue;
+            const uint32_t b = key[i].id >> (pass * kDigit) & (kBins - 1);
+            to[s.sort.space.base[b] + s.sort.space.warp_bin[warp][b] + rank[i]] = key[i];
+        }
+        if (pass + 1 == a.passes) break;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kSortEach; ++i)
+            if (here[i]) key[i] = s.sort.key[warp * 32 * kSortEach + i * 32 + lane];
     }
 }
 
@@ -188,20 +363,23 @@ __device__ __forceinline__ void put_row(T* out, int64_t at, const float (&sum)[N
     *to = v;
 }
 
-// Sums of the runs in a chunk, one warp a chunk and 32 lumps of columns; rows that no id asks for become 0 (unless summed onto `out`).
+// Sums of the runs in a chunk, one warp a chunk and 32 lumps of columns; then a share of the rows to be cleared.
 template <typename T, int N>
 __global__ void __launch_bounds__(256) sum_kernel(const Key* keys, int64_t n, uint32_t vocab, const T* grad, int64_t stride, int lumps, float scale, T* out,
-                                                  int64_t out_stride, bool accumulate, float* partial, int64_t partial_cols, int slices, const uint32_t* seen) {
+                                                  int64_t out_stride, bool accumulate, float* partial, int64_t partial_cols, int slices,
+                                                  int in_chunk, const __grid_constant__ SortArgs sort) {
+    after_previous();
+    let_next_begin();
     using L = Lump<T, N>;
     const int lane = threadIdx.x & 31;
     const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32), self = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5);
-    const int64_t chunks = (n + kChunk - 1) / kChunk;
+    const int64_t chunks = (n + in_chunk - 1) / in_chunk;
     for (int64_t u = self; u < chunks * slices; u += warps) {
         const int64_t chunk = u / slices;
         const int col = (static_cast<int>(u - chunk * slices) * 32 + lane);
         const bool here = col < lumps;
-        const int64_t from = chunk * kChunk;
-        const int count = static_cast<int>(min(static_cast<int64_t>(kChunk), n - from));
+        const int64_t from = chunk * in_chunk;
+        const int count = static_cast<int>(min(static_cast<int64_t>(in_chunk), n - from));
         const Key mine = lane < count ? keys[from + lane] : Key{0xFFFFFFFFu, 0};
         const uint32_t before = from > 0 ? keys[from - 1].id : 0xFFFFFFFEu, after = from + count < n ? keys[from + count].id : 0xFFFFFFFEu;
         float sum[N];
@@ -251,42 +429,53 @@ __global__ void __launch_bounds__(256) sum_kernel(const Key* keys, int64_t n, ui
             }
         }
     }
-    if (accumulate) return;
-    L zero;
-#pragma unroll
-    for (int e = 0; e < N; ++e) zero.v[e] = from_float<T>(0.f);
-    for (int64_t r = self; r < vocab; r += warps) {
-        if (seen[r >> 5] >> (r & 31) & 1) continue;
-        L* to = reinterpret_cast<L*>(out + r * out_stride);
-        for (int i = lane; i < lumps; i += 32) to[i] = zero;
-    }
+    clear_rows(sort, sort.seen, 0, sort.from, sort.to, self, warps);
 }
 
 // Runs across chunks: the warp of the chunk where one begins adds its parts up, in order.
 template <typename T, int N>
 __global__ void __launch_bounds__(256) join_runs_kernel(const Key* keys, int64_t n, uint32_t vocab, int lumps, float scale, T* out, int64_t out_stride, bool accumulate,
-                                                        const float* partial, int64_t partial_cols, int slices) {
+                                                        const float* partial, int64_t partial_cols, int slices, int in_chunk,
+                                                        const __grid_constant__ SortArgs sort) {
+    using F = Lump<float, N>;
+    after_previous();
+    let_next_begin();
     const int lane = threadIdx.x & 31;
     const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32), self = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5);
-    const int64_t chunks = (n + kChunk - 1) / kChunk;
+    const int64_t chunks = (n + in_chunk - 1) / in_chunk;
     for (int64_t u = self; u < (chunks - 1) * slices; u += warps) {
         const int64_t chunk = u / slices;
-        const int64_t from = chunk * kChunk, next = from + kChunk;
-        const uint32_t run = keys[next - 1].id;
-        if (run >= vocab || keys[next].id != run) continue;
-        const bool front = keys[from].id == run;
-        if (front && from > 0 && keys[from - 1].id == run) continue;       // it began earlier
+        const int64_t from = chunk * in_chunk, next = from + in_chunk;
+        const uint32_t run = keys[next - 1].id, behind = keys[next].id, head = keys[from].id, before = from > 0 ? keys[from - 1].id : 0xFFFFFFFEu;
+        if (run >= vocab || behind != run) continue;
+        const bool front = head == run;
+        if (front && before == run) continue;       // it began earlier
         const int64_t col = static_cast<int64_t>(u - chunk * slices) * 32 + lane;
-        if (col >= lumps) continue;
-        float sum[N];
+        const bool here = col < lumps;
+        F sum{};
+        if (here) sum = *reinterpret_cast<const F*>(partial + (chunk * 2 + (front ? 0 : 1)) * partial_cols + col * N);
+        // 32 chunks further on at a time: how many of them the run reaches, then their parts with several loads under way
+        for (int64_t c = chunk + 1;; c += 32) {
+            const uint32_t begins = c + lane < chunks ? keys[(c + lane) * in_chunk].id : 0xFFFFFFFEu;
+            const uint32_t other = __ballot_sync(~0u, begins != run);
+            const int count = other ? __ffs(other) - 1 : 32;
+            for (int i = 0; i < count; i += 8) {
+                F v[8];
 #pragma unroll
-        for (int e = 0; e < N; ++e) sum[e] = partial[(chunk * 2 + (front ? 0 : 1)) * partial_cols + col * N + e];
-        for (int64_t c = chunk + 1; c < chunks && keys[c * kChunk].id == run; ++c) {
+                for (int k = 0; k < 8; ++k)
+                    if (here && i + k < count) v[k] = *reinterpret_cast<const F*>(partial + (c + i + k) * 2 * partial_cols + col * N);
 #pragma unroll
-            for (int e = 0; e < N; ++e) sum[e] += partial[(c * 2) * partial_cols + col * N + e];
+                for (int k = 0; k < 8; ++k) {
+                    if (!here || i + k >= count) break;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) sum.v[e] += v[k].v[e];
+                }
+            }
+            if (other) break;
         }
-        put_row<T, N>(out, run * out_stride + col * N, sum, scale, accumulate);
+        if (here) put_row<T, N>(out, run * out_stride + col * N, sum.v, scale, accumulate);
     }
+    clear_rows(sort, sort.seen, 0, sort.from, sort.to, self, warps);
 }
 
 inline int64_t div_up(int64_t x, int64_t by) { return (x + by - 1) / by; }
@@ -301,27 +490,24 @@ bool wide_rows(const Matrix& m) {
 
 template <typename T, int N>
 const char* embed_typed(const Ids& ids, int64_t n, const Matrix& table, float scale, const Matrix& out, cudaStream_t stream) {
-    const int lumps = static_cast<int>(table.cols / N);
-    int x = 32;
-    while (x < 256 && x * 4 < lumps) x *= 2;
-    const dim3 block(x, 256 / x);
-    const int64_t blocks = div_up(n, block.y);
-    embed_kernel<T, N><<<static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 20)), block, 0, stream>>>(ids.data, ids.bits, n, static_cast<const T*>(table.data), table.rows,
-                                                                                                   table.stride, lumps, scale,
-                                                                                                   static_cast<T*>(const_cast<void*>(out.data)), out.stride);
-    const cudaError_t e = cudaGetLastError();
+    const int64_t lumps = table.cols / N;
+    const cudaError_t e = launch(embed_kernel<T, N>, std::min<int64_t>(div_up(n * lumps, 1024), 1 << 30), 256, 0, stream, ids.data, ids.bits, n,
+                                 static_cast<const T*>(table.data), table.rows, table.stride, static_cast<uint32_t>(lumps), scale,
+                                 static_cast<T*>(const_cast<void*>(out.data)), out.stride);
     return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 
 struct GradPlan {
     int64_t tiles, chunks;
+    int in_chunk;
     uint64_t seen, counts, a, b, partial, bytes;
     int passes;
 };
 GradPlan grad_plan(int64_t n, int64_t vocab, int64_t width) {
     GradPlan p;
     p.tiles = div_up(n, kSortTile);
-    p.chunks = div_up(n, kChunk);
+    p.in_chunk = div_up(n, kChunk) * div_up(width, 256) < 148 * 32 ? kShortChunk : kChunk;      // (256: a warp's columns of 16 bits)
+    p.chunks = div_up(n, p.in_chunk);
     p.passes = 1;
     while (p.passes * kDigit < 32 && (vocab >> (p.passes * kDigit))) ++p.passes;
     uint64_t at = 0;
@@ -340,18 +526,23 @@ GradPlan grad_plan(int64_t n, int64_t vocab, int64_t width) {
 }
 
 template <typename T, int N>
-void sum_typed(const Key* keys, int64_t n, const Matrix& grad, float scale, const Matrix& out, bool accumulate, float* partial, const uint32_t* seen, const GradPlan& p,
-               cudaStream_t stream) {
+cudaError_t sum_typed(const Key* keys, int64_t n, const Matrix& grad, float scale, const Matrix& out, bool accumulate, float* partial, SortArgs sort, const GradPlan& p,
+                      int64_t rows_at_once, int64_t all, cudaStream_t stream) {
     const int lumps = static_cast<int>(grad.cols / N), slices = static_cast<int>(div_up(lumps, 32));
     const int64_t cols = round_up(grad.cols, 8);
     T* to = static_cast<T*>(const_cast<void*>(out.data));
-    const int64_t units = std::max(p.chunks * slices, accumulate ? 0 : out.rows);
-    const unsigned blocks = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(div_up(units, 8), 148 * 8)));
-    sum_kernel<T, N><<<blocks, 256, 0, stream>>>(keys, n, static_cast<uint32_t>(out.rows), static_cast<const T*>(grad.data), grad.stride, lumps, scale, to, out.stride,
-                                                 accumulate, partial, cols, slices, seen);
-    if (p.chunks > 1)
-        join_runs_kernel<T, N><<<static_cast<unsigned>(std::min<int64_t>(div_up(p.chunks * slices, 8), 148 * 8)), 256, 0, stream>>>(
-            keys, n, static_cast<uint32_t>(out.rows), lumps, scale, to, out.stride, accumulate, partial, cols, slices);
+    const uint32_t vocab = static_cast<uint32_t>(out.rows);
+    auto blocks = [&](int64_t sums) { return std::min<int64_t>(div_up(std::max<int64_t>(1, std::max(sums, sort.to - sort.from)), 8), 148 * 8); };
+    sort.from = sort.to;
+    sort.to = p.chunks < 2 ? all : std::max(sort.from, all - rows_at_once);
+    if (cudaError_t e = launch(sum_kernel<T, N>, blocks(p.chunks * slices), 256, 0, stream, keys, n, vocab, static_cast<const T*>(grad.data), grad.stride, lumps, scale, to,
+                               out.stride, accumulate, partial, cols, slices, p.in_chunk, sort))
+        return e;
+    if (p.chunks < 2) return cudaSuccess;
+    sort.from = sort.to;
+    sort.to = all;
+    return launch(join_runs_kernel<T, N>, blocks((p.chunks - 1) * slices), 256, 0, stream, keys, n, vocab, lumps, scale, to, out.stride, accumulate,
+                  partial, cols, slices, p.in_chunk, sort);
 }
 
 }  // namespace
@@ -373,44 +564,65 @@ const char* embed_grad(const Ids& ids, int64_t n, const Matrix& grad, float scal
     const GradPlan p = grad_plan(n, out.rows, out.cols);
     if (workspace_bytes < p.bytes) return "the workspace is too small";
     char* at = static_cast<char*>(workspace);
-    uint32_t* seen = reinterpret_cast<uint32_t*>(at + p.seen);
-    uint32_t* counts = reinterpret_cast<uint32_t*>(at + p.counts);
-    Key *from = reinterpret_cast<Key*>(at + p.a), *to = reinterpret_cast<Key*>(at + p.b);
+    Key *keys = reinterpret_cast<Key*>(at + p.a), *other = reinterpret_cast<Key*>(at + p.b);
     float* partial = reinterpret_cast<float*>(at + p.partial);
-    const uint32_t vocab = static_cast<uint32_t>(out.rows);
-    cudaMemsetAsync(seen, 0, div_up(out.rows, 32) * 4, stream);
-    if (n) {
-        const unsigned tiles = static_cast<unsigned>(p.tiles);
-        count_kernel<true><<<tiles, kSortThreads, 0, stream>>>(ids.data, ids.bits, nullptr, n, vocab, 0, counts, seen);
-        scatter_kernel<true><<<tiles, kSortThreads, 0, stream>>>(ids.data, ids.bits, nullptr, n, vocab, 0, counts, from);
-        for (int pass = 1; pass < p.passes; ++pass) {
-            count_kernel<false><<<tiles, kSortThreads, 0, stream>>>(nullptr, 0, from, n, vocab, pass * kDigit, counts, nullptr);
-            scatter_kernel<false><<<tiles, kSortThreads, 0, stream>>>(nullptr, 0, from, n, vocab, pass * kDigit, counts, to);
-            std::swap(from, to);
+    const bool wide = wide_rows(grad) && wide_rows(out);
+    const int size = element(out.type);
+    SortArgs s{};
+    s.ids = ids.data;
+    s.bits = ids.bits;
+    s.n = n;
+    s.vocab = static_cast<uint32_t>(out.rows);
+    s.tiles = static_cast<int>(p.tiles);
+    s.passes = p.passes;
+    s.counts = reinterpret_cast<uint32_t*>(at + p.counts);
+    s.seen = reinterpret_cast<uint32_t*>(at + p.seen);
+    s.rows = static_cast<char*>(const_cast<void*>(out.data));
+    s.row_bytes = out.cols * size;
+    s.row_stride = out.stride * size;
+    s.unit = wide_rows(out) ? 16 : size;
+    // Rows cleared beside the other work of a launch: what memory takes in the time of a launch of the sort, some 8 us.
+    const int64_t rows_at_once = std::max<int64_t>(1, (48 << 20) / s.row_bytes), all = accumulate ? 0 : out.rows;
+    auto clearing = [&](int64_t blocks) {
+        s.from = s.to;
+        s.to = std::min(all, s.from + rows_at_once);
+        return blocks + std::min<int64_t>(div_up(s.to - s.from, kSortWarps), 148 * 6);
+    };
+    cudaError_t e = cudaSuccess;
+    if (p.tiles == 1) {
+        s.out = keys;
+        s.to = std::min(all, 2 * rows_at_once);
+        e = launch(one_tile_kernel, 1 + std::min<int64_t>(div_up(s.to, kSortWarps), 148 * 6), kSortThreads, 0, stream, s);
+    } else {
+        e = cudaMemsetAsync(s.seen, 0, div_up(out.rows, 32) * 4, stream);
+        for (int pass = 0; pass < p.passes && p.tiles && e == cudaSuccess; ++pass) {
+            s.in = keys;
+            s.out = pass ? other : keys;
+            s.shift = pass * kDigit;
+            e = pass ? launch(count_kernel<false>, clearing(p.tiles), kSortThreads, 0, stream, s) : launch(count_kernel<true>, p.tiles, kSortThreads, 0, stream, s);
+            if (e != cudaSuccess) break;
+            e = launch(pass ? scatter_kernel<false> : scatter_kernel<true>, clearing(p.tiles), kSortThreads, 0, stream, s);
+            if (pass) std::swap(keys, other);
         }
     }
-    const bool wide = wide_rows(grad) && wide_rows(out);
+    if (e != cudaSuccess) return cudaGetErrorString(e);
     switch (out.type) {
         case kF32:
-            wide ? sum_typed<float, 4>(from, n, grad, scale, out, accumulate, partial, seen, p, stream) : sum_typed<float, 1>(from, n, grad, scale, out, accumulate, partial, seen, p, stream);
+            e = (wide ? sum_typed<float, 4> : sum_typed<float, 1>)(keys, n, grad, scale, out, accumulate, partial, s, p, rows_at_once, all, stream);
             break;
         case kBF16:
-            wide ? sum_typed<__nv_bfloat16, 8>(from, n, grad, scale, out, accumulate, partial, seen, p, stream)
-                 : sum_typed<__nv_bfloat16, 1>(from, n, grad, scale, out, accumulate, partial, seen, p, stream);
+            e = (wide ? sum_typed<__nv_bfloat16, 8> : sum_typed<__nv_bfloat16, 1>)(keys, n, grad, scale, out, accumulate, partial, s, p, rows_at_once, all, stream);
             break;
         default:
-            wide ? sum_typed<__half, 8>(from, n, grad, scale, out, accumulate, partial, seen, p, stream)
-                 : sum_typed<__half, 1>(from, n, grad, scale, out, accumulate, partial, seen, p, stream);
+            e = (wide ? sum_typed<__half, 8> : sum_typed<__half, 1>)(keys, n, grad, scale, out, accumulate, partial, s, p, rows_at_once, all, stream);
     }
-    const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 
 const char* next_targets(const int32_t* ids, int64_t n, const int32_t* offsets, int64_t n_docs, const uint8_t* loss_mask, int32_t ignore, int32_t* out,
                          cudaStream_t stream) {
     if (n == 0) return nullptr;
-    next_kernel<<<static_cast<unsigned>(div_up(n, 256)), 256, 0, stream>>>(ids, n, offsets, n_docs, loss_mask, ignore, out);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch(next_kernel, div_up(n, 256), 256, 0, stream, ids, n, offsets, n_docs, loss_mask, ignore, out);
     return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 
