@@ -71,22 +71,34 @@ def _done(code, what):
     return code
 
 
-def _on_gpu(device, **tensors):
-    for name, t in tensors.items():
+def _on_gpu(first, **others):
+    """Index of the GPU that all of them are on."""
+    for name, t in others.items():
         if not isinstance(t, torch.Tensor):
             raise TypeError("%s must be a torch tensor" % name)
+    device = first.device if isinstance(first, torch.Tensor) else None
+    for name, t in others.items():
         if t.layout is not torch.strided:
             raise TypeError("%s must be a dense tensor" % name)
         if t.device != device:
             raise ValueError("%s is on %s, other arguments on %s" % (name, t.device, device))
     if device.type != "cuda":
         raise ValueError("tensors must be on the GPU, not on %s" % device)
+    return device.index
+
+
+def _there(index, f, *args):
+    """f(*args) with GPU `index` current."""
+    if torch.cuda.current_device() == index:
+        return f(*args)
+    with torch.cuda.device(index):
+        return f(*args)
 
 
 def _ids_of(name, t):
     if t.dtype not in _IDS:
         raise TypeError("%s must be int32 or int64, not %s" % (name, t.dtype))
-    return t.reshape(-1).contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _rows(t):
@@ -99,8 +111,11 @@ def _matrix(t):
     return _Matrix(t.data_ptr(), rows, cols, t.stride(0) if rows > 1 else cols, _TYPES[t.dtype])
 
 
-def _stream():
-    return torch.cuda.current_stream().cuda_stream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)       # (a tenth of the time of the public way)
+
+
+def _stream(index):
+    return _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream
 
 
 def _scale(scale):
@@ -120,12 +135,13 @@ def _table(name, t):
         raise ValueError("%s must have columns" % name)
 
 
-def _embed(ids, table, scale):
-    flat, rows = _ids_of("ids", ids), _rows(table)
-    with torch.cuda.device(table.device):
-        out = torch.empty((flat.numel(), table.shape[1]), dtype=table.dtype, device=table.device)
-        _done(_lib().gtok_x_embed(flat.data_ptr(), _IDS[flat.dtype], flat.numel(), _matrix(rows), scale, _matrix(out), _stream()), "gtok_x_embed")
-    return out.view(*ids.shape, table.shape[1])
+def _embed(ids, table, scale, index):
+    flat, rows, width = _ids_of("ids", ids), _rows(table), table.shape[1]
+    out = table.new_empty(ids.shape + (width,), requires_grad=False)
+    n = flat.numel()
+    to = _Matrix(out.data_ptr(), n, width, width, _TYPES[table.dtype])
+    _done(_lib().gtok_x_embed(flat.data_ptr(), _IDS[flat.dtype], n, _matrix(rows), scale, to, _stream(index)), "gtok_x_embed")
+    return out
 
 
 class _Embed(torch.autograd.Function):
@@ -133,7 +149,7 @@ class _Embed(torch.autograd.Function):
     def forward(ctx, ids, table, scale):
         ctx.save_for_backward(ids)
         ctx.vocab, ctx.scale = table.shape[0], scale
-        return _embed(ids, table, scale)
+        return _there(table.get_device(), _embed, ids, table, scale, table.get_device())
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -146,12 +162,12 @@ def embed(ids, table, scale=1.0):
     """Rows of `table` [vocab, width] (float32, bfloat16 or float16) by id, times `scale`: a tensor of ids.shape + (width,).
 
     ids: int32 or int64, any shape.  A negative id gives a row of zeros, one beyond the table a row of NaN; neither has a gradient."""
-    _on_gpu(getattr(table, "device", None) or torch.device("cpu"), table=table, ids=ids)
+    index = _on_gpu(table, table=table, ids=ids)
     _table("table", table)
     scale = _scale(scale)
     if table.requires_grad and torch.is_grad_enabled():
         return _Embed.apply(ids, table, scale)
-    return _embed(ids, table, scale)
+    return _there(index, _embed, ids, table, scale, index)
 
 
 def embed_grad(ids, grad, vocab, scale=1.0, out=None, accumulate=False):
@@ -160,12 +176,12 @@ def embed_grad(ids, grad, vocab, scale=1.0, out=None, accumulate=False):
 
     out: where to write it, of grad's type.  With `accumulate` it is added to what `out` holds, as for a table that is an
     output table too, and rows that are not asked for are not touched."""
-    _on_gpu(getattr(grad, "device", None) or torch.device("cpu"), grad=grad, ids=ids)
-    if grad.shape[:-1] != ids.shape or grad.dim() < 1:
+    index = _on_gpu(grad, grad=grad, ids=ids)
+    if grad.dim() < 1 or grad.shape[:-1] != ids.shape:
         raise ValueError("grad must have the shape of ids and one dimension more")
     width, vocab = grad.shape[-1], int(vocab)
     flat = _ids_of("ids", ids)
-    rows = _rows(grad.reshape(-1, width) if width else grad)
+    rows = _rows(grad if grad.dim() == 2 else grad.reshape(flat.numel(), width))
     _table("grad", rows)
     if vocab < 0:
         raise ValueError("vocab must not be negative")
@@ -173,17 +189,20 @@ def embed_grad(ids, grad, vocab, scale=1.0, out=None, accumulate=False):
         raise ValueError("accumulate needs `out`")
     scale = _scale(scale)
     if out is not None:
-        _on_gpu(grad.device, out=out)
+        _on_gpu(grad, out=out)
         if out.shape != (vocab, width) or out.dtype != grad.dtype or (width > 1 and out.stride(1) != 1):
             raise ValueError("out must be [vocab, width] of grad's type with the elements of a row next to one another")
-    with torch.cuda.device(grad.device):
-        if out is None:
-            out = torch.empty((vocab, width), dtype=grad.dtype, device=grad.device)
-        lib = _lib()
-        need = _done(lib.gtok_x_embed_grad_workspace(flat.numel(), vocab, width), "gtok_x_embed_grad_workspace")
-        work = torch.empty(need, dtype=torch.uint8, device=grad.device)
-        _done(lib.gtok_x_embed_grad(flat.data_ptr(), _IDS[flat.dtype], flat.numel(), _matrix(rows), scale, _matrix(out), int(bool(accumulate)),
-                                    work.data_ptr(), need, _stream()), "gtok_x_embed_grad")
+    return _there(index, _embed_grad, flat, rows, vocab, scale, out, accumulate, index)
+
+
+def _embed_grad(flat, rows, vocab, scale, out, accumulate, index):
+    lib, n, width = _lib(), flat.numel(), rows.shape[1]
+    if out is None:
+        out = rows.new_empty((vocab, width), requires_grad=False)
+    need = _done(lib.gtok_x_embed_grad_workspace(n, vocab, width), "gtok_x_embed_grad_workspace")
+    work = torch.empty(need, dtype=torch.uint8, device=rows.device)
+    _done(lib.gtok_x_embed_grad(flat.data_ptr(), _IDS[flat.dtype], n, _matrix(rows), scale, _matrix(out), bool(accumulate), work.data_ptr(), need,
+                                _stream(index)), "gtok_x_embed_grad")
     return out
 
 
@@ -192,100 +211,103 @@ def next_targets(ids, offsets, loss_mask=None, ignore_index=-100):
     """For packed documents as `Tokenizer.encode_batch_to_device` gives them (int32 ids, int32 n + 1 offsets): the id that follows each
     position in its document, `ignore_index` at a document's last position, outside of all documents, and where the boolean
     `loss_mask` (same length as ids) is false.  int32."""
-    _on_gpu(getattr(ids, "device", None) or torch.device("cpu"), ids=ids, offsets=offsets)
+    index = _on_gpu(ids, ids=ids, offsets=offsets)
     if ids.dtype != torch.int32 or ids.dim() != 1 or offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 1:
         raise ValueError("ids and offsets must be one-dimensional and int32, offsets not empty")
     if not -(1 << 31) <= ignore_index < 0:
         raise ValueError("ignore_index must be negative, in 32 bits")
-    mask = None
     if loss_mask is not None:
-        _on_gpu(ids.device, loss_mask=loss_mask)
+        _on_gpu(ids, loss_mask=loss_mask)
         if loss_mask.dtype != torch.bool or loss_mask.shape != ids.shape:
             raise ValueError("loss_mask must be boolean and as long as ids")
-        mask = loss_mask.contiguous()
-    ids, offsets = ids.contiguous(), offsets.contiguous()
-    with torch.cuda.device(ids.device):
-        out = torch.empty_like(ids)
-        _done(_lib().gtok_x_next_targets(ids.data_ptr(), ids.numel(), offsets.data_ptr(), offsets.numel() - 1, mask.data_ptr() if mask is not None else None,
-                                         ignore_index, out.data_ptr(), _stream()), "gtok_x_next_targets")
+        loss_mask = loss_mask.contiguous()
+    return _there(index, _next_targets, ids.contiguous(), offsets.contiguous(), loss_mask, int(ignore_index), index)
+
+
+def _next_targets(ids, offsets, mask, ignore_index, index):
+    out = torch.empty_like(ids)
+    _done(_lib().gtok_x_next_targets(ids.data_ptr(), ids.numel(), offsets.data_ptr(), offsets.numel() - 1, mask.data_ptr() if mask is not None else None,
+                                     ignore_index, out.data_ptr(), _stream(index)), "gtok_x_next_targets")
     return out
 
 
 # ---- losses over the vocabulary -----------------------------------------------------
-def _check_loss(hidden, weight, lead):
-    _on_gpu(getattr(hidden, "device", None) or torch.device("cpu"), hidden=hidden, weight=weight)
-    if hidden.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != hidden.dtype:
-        raise TypeError("hidden and weight must both be bfloat16 or both float16, not %s and %s" % (hidden.dtype, weight.dtype))
-    if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:
-        raise ValueError("hidden must be [..., width] and weight [vocab, width]")
-    if hidden.shape[:-1] != lead:
-        raise ValueError("hidden and the targets differ in their leading dimensions")
-
-
 def _flat(hidden):
-    return _rows(hidden.reshape(-1, hidden.shape[-1]))
+    return _rows(hidden if hidden.dim() == 2 else hidden.reshape(hidden.shape[:-1].numel(), hidden.shape[-1]))
 
 
 class _Call:
-    """Arguments of one loss, checked, and what keeps their memory alive."""
+    """Arguments of one loss, checked, and what keeps their memory alive.  `teacher_logits` is None for cross entropy."""
 
-    def __init__(self, hidden, weight, targets=None, ignore_index=-100, teacher_ids=None, teacher_logits=None, temperature=1.0):
-        if teacher_ids is None:
-            ids = targets
-            _check_loss(hidden, weight, getattr(targets, "shape", None))
+    def __init__(self, hidden, weight, ids, teacher_logits, ignore_index, temperature):
+        if teacher_logits is None:
+            what, lead = "targets", getattr(ids, "shape", None)
+            self.index = _on_gpu(hidden, hidden=hidden, weight=weight, targets=ids)
         else:
-            ids = teacher_ids
-            _check_loss(hidden, weight, getattr(teacher_ids, "shape", (None,))[:-1])
-            _on_gpu(hidden.device, teacher_logits=teacher_logits)
-            if teacher_logits.shape != teacher_ids.shape or not 1 <= teacher_ids.shape[-1] <= MAX_ENTRIES:
+            what, lead = "teacher_ids", getattr(ids, "shape", (None,))[:-1]
+            self.index = _on_gpu(hidden, hidden=hidden, weight=weight, teacher_ids=ids, teacher_logits=teacher_logits)
+            if ids.dim() < 1 or teacher_logits.shape != ids.shape or not 1 <= ids.shape[-1] <= MAX_ENTRIES:
                 raise ValueError("teacher_ids and teacher_logits must be [..., k] with k from 1 to %d" % MAX_ENTRIES)
             if teacher_logits.dtype not in _TYPES:
                 raise TypeError("teacher_logits must be float32, bfloat16 or float16, not %s" % teacher_logits.dtype)
-        _on_gpu(hidden.device, ids=ids)
-        self.temperature = float(temperature)
-        if not (self.temperature > 0.0 and math.isfinite(self.temperature)):
+        if hidden.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != hidden.dtype:
+            raise TypeError("hidden and weight must both be bfloat16 or both float16, not %s and %s" % (hidden.dtype, weight.dtype))
+        if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:
+            raise ValueError("hidden must be [..., width] and weight [vocab, width]")
+        if hidden.shape[:-1] != lead:
+            raise ValueError("hidden and %s differ in their leading dimensions" % what)
+        temperature = float(temperature)
+        if not (temperature > 0.0 and math.isfinite(temperature)):
             raise ValueError("temperature must be positive and finite")
-        self.device, self.hidden, self.weight = hidden.device, _flat(hidden.detach()), _rows(weight.detach())
+        self.hidden, self.weight, self.ids = _flat(hidden), _rows(weight), _ids_of(what, ids)
         if self.weight.stride(0) < self.weight.shape[1] and self.weight.shape[0] > 1:
             self.weight = self.weight.contiguous()
-        self.ids = _ids_of("targets" if teacher_ids is None else "teacher_ids", ids)
         a = self.args = _Loss()
         a.hidden, a.weight = _matrix(self.hidden), _matrix(self.weight)
-        a.targets, a.target_bits, a.ignore, a.temperature = self.ids.data_ptr(), _IDS[self.ids.dtype], int(ignore_index), self.temperature
-        if teacher_ids is not None:
-            k = teacher_ids.shape[-1]
-            self.logits = _rows(teacher_logits.detach().reshape(-1, k))
+        a.targets, a.target_bits, a.ignore, a.temperature = self.ids.data_ptr(), _IDS[ids.dtype], ignore_index, temperature
+        if teacher_logits is not None:
+            k = ids.shape[-1]
+            self.logits = _flat(teacher_logits)
             a.entries, a.target_stride, a.teacher_logits = k, k, _matrix(self.logits)
 
     def _run(self, entry, backward):
-        a, lib = self.args, _lib()
-        need = _done(lib.gtok_x_vocab_loss_workspace(a, backward), "gtok_x_vocab_loss_workspace")
-        work = torch.empty(need, dtype=torch.uint8, device=self.device)
-        a.workspace, a.workspace_bytes, a.cuda_stream = work.data_ptr(), need, _stream()
+        a = self.args
+        need = _done(_lib().gtok_x_vocab_loss_workspace(a, backward), "gtok_x_vocab_loss_workspace")
+        work = torch.empty(need, dtype=torch.uint8, device=self.hidden.device)
+        a.workspace, a.workspace_bytes, a.cuda_stream = work.data_ptr(), need, _stream(self.index)
         _done(entry(a), entry.__name__)
 
     def forward(self, reduction):
-        n = self.hidden.shape[0]
-        with torch.cuda.device(self.device):
-            losses, lse = torch.empty(n, dtype=torch.float32, device=self.device), torch.empty(n, dtype=torch.float32, device=self.device)
-            total = torch.empty((), dtype=torch.float32, device=self.device) if reduction != "none" else None
-            a = self.args
-            a.losses, a.lse, a.total, a.mean = losses.data_ptr(), lse.data_ptr(), total.data_ptr() if total is not None else None, reduction == "mean"
-            self._run(_lib().gtok_x_vocab_loss_forward, 0)
-        return (losses if total is None else total), lse
+        return _there(self.index, self._forward, reduction)
+
+    def _forward(self, reduction):
+        a, n, device = self.args, self.hidden.shape[0], self.hidden.device
+        losses, lse = torch.empty(n, dtype=torch.float32, device=device), torch.empty(n, dtype=torch.float32, device=device)
+        a.losses, a.lse = losses.data_ptr(), lse.data_ptr()
+        if reduction != "none":
+            total = torch.empty((), dtype=torch.float32, device=device)
+            a.total, a.mean, losses = total.data_ptr(), reduction == "mean", total
+        self._run(_lib().gtok_x_vocab_loss_forward, 0)
+        return losses, lse
 
     def backward(self, lse, grad, reduction, want_hidden, want_weight):
-        with torch.cuda.device(self.device):
-            a = self.args
-            lse, grad = lse.reshape(-1).contiguous(), grad.detach().reshape(-1)
-            a.lse, a.grad, a.mean = lse.data_ptr(), grad.data_ptr(), reduction == "mean"
-            a.grad_stride = grad.stride(0) if reduction == "none" and grad.numel() > 1 else 0
-            d_hidden = torch.empty(self.hidden.shape, dtype=self.hidden.dtype, device=self.device) if want_hidden else None
-            d_weight = torch.empty(self.weight.shape, dtype=self.weight.dtype, device=self.device) if want_weight else None
-            for name, t in (("d_hidden", d_hidden), ("d_weight", d_weight)):
-                if t is not None:
-                    setattr(a, name, _matrix(t))
-            self._run(_lib().gtok_x_vocab_loss_backward, 1)
+        return _there(self.index, self._backward, lse, grad, reduction, want_hidden, want_weight)
+
+    def _backward(self, lse, grad, reduction, want_hidden, want_weight):
+        a = self.args
+        lse = lse.contiguous()
+        if reduction == "none":
+            grad = grad if grad.dim() == 1 else grad.reshape(-1)
+            a.grad_stride = grad.stride(0) if grad.numel() > 1 else 0
+        a.lse, a.grad, a.mean = lse.data_ptr(), grad.data_ptr(), reduction == "mean"
+        d_hidden = d_weight = None
+        if want_hidden:
+            d_hidden = self.hidden.new_empty(self.hidden.shape, requires_grad=False)
+            a.d_hidden = _matrix(d_hidden)
+        if want_weight:
+            d_weight = self.weight.new_empty(self.weight.shape, requires_grad=False)
+            a.d_weight = _matrix(d_weight)
+        self._run(_lib().gtok_x_vocab_loss_backward, 1)
         return d_hidden, d_weight
 
 
@@ -294,9 +316,9 @@ def _check_reduction(reduction):
         raise ValueError("reduction must be 'mean', 'sum' or 'none'")
 
 
-def _check_grad(lse, grad, lead, reduction, device):
+def _check_grad(lse, grad, lead, reduction, hidden):
     _check_reduction(reduction)
-    _on_gpu(device, lse=lse, grad=grad)
+    _on_gpu(hidden, lse=lse, grad=grad)
     if lse.dtype != torch.float32 or grad.dtype != torch.float32:
         raise TypeError("lse and grad must be float32")
     if lse.shape != lead or grad.shape != (lead if reduction == "none" else ()):
@@ -305,10 +327,10 @@ def _check_grad(lse, grad, lead, reduction, device):
 
 class _LossFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, ids, teacher_logits, reduction, ignore_index, temperature):
-        loss, lse = _call(hidden, weight, ids, teacher_logits, ignore_index, temperature).forward(reduction)
+    def forward(ctx, call, hidden, weight, ids, teacher_logits, reduction):
+        loss, lse = call.forward(reduction)
         ctx.save_for_backward(hidden, weight, ids, teacher_logits, lse)
-        ctx.rest = reduction, ignore_index, temperature
+        ctx.rest = reduction, call.args.ignore, call.args.temperature
         return loss.view(hidden.shape[:-1]) if reduction == "none" else loss
 
     @staticmethod
@@ -316,21 +338,17 @@ class _LossFunction(torch.autograd.Function):
     def backward(ctx, grad):
         hidden, weight, ids, teacher_logits, lse = ctx.saved_tensors
         reduction, ignore_index, temperature = ctx.rest
-        d_hidden, d_weight = _call(hidden, weight, ids, teacher_logits, ignore_index, temperature).backward(lse, grad, reduction, *ctx.needs_input_grad[:2])
-        return d_hidden.view(hidden.shape) if d_hidden is not None else None, d_weight, None, None, None, None, None
-
-
-def _call(hidden, weight, ids, teacher_logits, ignore_index, temperature):
-    if teacher_logits is None:
-        return _Call(hidden, weight, targets=ids, ignore_index=ignore_index, temperature=temperature)
-    return _Call(hidden, weight, teacher_ids=ids, teacher_logits=teacher_logits, temperature=temperature)
+        _, want_hidden, want_weight, _, _, _ = ctx.needs_input_grad
+        call = _Call(hidden, weight, ids, teacher_logits, ignore_index, temperature)
+        d_hidden, d_weight = call.backward(lse, grad, reduction, want_hidden, want_weight)
+        return None, d_hidden.view(hidden.shape) if want_hidden else None, d_weight, None, None, None
 
 
 def _loss(hidden, weight, ids, teacher_logits, reduction, ignore_index, temperature):
     _check_reduction(reduction)
-    call = _call(hidden, weight, ids, teacher_logits, ignore_index, temperature)
+    call = _Call(hidden, weight, ids, teacher_logits, ignore_index, temperature)
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        return _LossFunction.apply(hidden, weight, ids, teacher_logits, reduction, ignore_index, temperature)
+        return _LossFunction.apply(call, hidden, weight, ids, teacher_logits, reduction)
     loss, _ = call.forward(reduction)
     return loss.view(hidden.shape[:-1]) if reduction == "none" else loss
 
@@ -347,14 +365,14 @@ def cross_entropy(hidden, weight, targets, reduction="mean", ignore_index=-100, 
 def cross_entropy_forward(hidden, weight, targets, reduction="none", ignore_index=-100, temperature=1.0):
     """(loss, lse): what `cross_entropy` returns and the float32 logarithms of the rows' sums, which `cross_entropy_grad` takes."""
     _check_reduction(reduction)
-    loss, lse = _call(hidden, weight, targets, None, ignore_index, temperature).forward(reduction)
+    loss, lse = _Call(hidden, weight, targets, None, ignore_index, temperature).forward(reduction)
     return (loss.view(targets.shape) if reduction == "none" else loss), lse.view(targets.shape)
 
 
 def cross_entropy_grad(hidden, weight, targets, lse, grad, reduction="none", ignore_index=-100, temperature=1.0, want_hidden=True, want_weight=True):
     """(d_hidden, d_weight) for the gradient `grad` of the loss (float32, of its shape); None for what is not wanted."""
-    call = _call(hidden, weight, targets, None, ignore_index, temperature)
-    _check_grad(lse, grad, targets.shape, reduction, hidden.device)
+    call = _Call(hidden, weight, targets, None, ignore_index, temperature)
+    _check_grad(lse, grad, targets.shape, reduction, hidden)
     d_hidden, d_weight = call.backward(lse, grad, reduction, want_hidden, want_weight)
     return d_hidden.view(hidden.shape) if d_hidden is not None else None, d_weight
 
@@ -365,20 +383,23 @@ def distill(hidden, weight, teacher_ids, teacher_logits, temperature=1.0, reduct
     hidden, weight: as in `cross_entropy`.  teacher_ids (int32 or int64) and teacher_logits: [..., k], k up to 1024, in any order;
     a negative id is no entry.  The teacher's probabilities are the softmax over a row's entries; a row without any carries no loss.
     The customary factor temperature ** 2 is not applied.  There is no gradient for the teacher."""
+    _on_gpu(hidden, teacher_logits=teacher_logits)
     return _loss(hidden, weight, teacher_ids, teacher_logits, reduction, -100, temperature)
 
 
 def distill_forward(hidden, weight, teacher_ids, teacher_logits, temperature=1.0, reduction="none"):
     """(loss, lse), as `cross_entropy_forward`."""
     _check_reduction(reduction)
-    loss, lse = _call(hidden, weight, teacher_ids, teacher_logits, -100, temperature).forward(reduction)
+    _on_gpu(hidden, teacher_logits=teacher_logits)
+    loss, lse = _Call(hidden, weight, teacher_ids, teacher_logits, -100, temperature).forward(reduction)
     lead = hidden.shape[:-1]
     return (loss.view(lead) if reduction == "none" else loss), lse.view(lead)
 
 
 def distill_grad(hidden, weight, teacher_ids, teacher_logits, lse, grad, temperature=1.0, reduction="none", want_hidden=True, want_weight=True):
     """(d_hidden, d_weight), as `cross_entropy_grad`."""
-    call = _call(hidden, weight, teacher_ids, teacher_logits, -100, temperature)
-    _check_grad(lse, grad, hidden.shape[:-1], reduction, hidden.device)
+    _on_gpu(hidden, teacher_logits=teacher_logits)
+    call = _Call(hidden, weight, teacher_ids, teacher_logits, -100, temperature)
+    _check_grad(lse, grad, hidden.shape[:-1], reduction, hidden)
     d_hidden, d_weight = call.backward(lse, grad, reduction, want_hidden, want_weight)
     return d_hidden.view(hidden.shape) if d_hidden is not None else None, d_weight
