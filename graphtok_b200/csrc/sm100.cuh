@@ -100,7 +100,7 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(static_cast<uint16_t>(3))
                  : "memory");
 }
-// 256 x 256 x 16: each block holds half of A's rows, half of B's columns and the accumulator of its rows.
+// 256 x columns x 16: each block holds half of A's rows, half of B's columns and the accumulator of its rows.
 __device__ __forceinline__ void mma(uint32_t acc, uint64_t a, uint64_t b, uint32_t kind, bool add) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(acc), "l"(a), "l"(b), "r"(kind),
                  "r"(static_cast<uint32_t>(add))
@@ -112,8 +112,8 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, bool lines_across) {
     const uint64_t lead = lines_across ? 8192 >> 4 : 1;
     return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (lead << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-__host__ __device__ constexpr uint32_t mma_kind(bool bf16, bool a_across, bool b_across) {
-    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_across ? 1u : 0u) << 15) | ((b_across ? 1u : 0u) << 16) | ((256u >> 3) << 17) |
+__device__ __forceinline__ uint32_t mma_kind(bool bf16, bool a_across, bool b_across, uint32_t columns) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_across ? 1u : 0u) << 15) | ((b_across ? 1u : 0u) << 16) | ((columns >> 3) << 17) |
            ((256u >> 4) << 24);
 }
 // 32 lanes (this warp's quarter) x 32 columns of fp32 on their way; they are there after tmem_wait of the same registers.

@@ -30,7 +30,17 @@ int device() {
         cudaGetLastError();
         return refuse("no GPU");
     }
-    return major == 10 ? d : refuse("the current device is no B200");
+    if (major != 10) return refuse("the current device is no B200");
+    // A thread that has called nothing yet, such as one of torch's for backward passes, has no context for the driver's calls until this.
+    static thread_local int ready = -1;
+    if (ready != d) {
+        if (cudaSetDevice(d) != cudaSuccess) {
+            cudaGetLastError();
+            return refuse("the current device cannot be used");
+        }
+        ready = d;
+    }
+    return d;
 }
 
 // An address that the current device's kernels may use: its own memory, or memory that it shares with the host.
@@ -116,7 +126,7 @@ gtok::LossCall loss_call(const gtok_x_vocab_loss* a) {
     c.mean = a->mean != 0;
     c.grad = a->grad;
     c.grad_stride = a->grad_stride;
-    c.grad_of_mean = a->mean != 0;
+    c.kept = a->kept;
     c.d_hidden = matrix(a->d_hidden);
     c.d_weight = matrix(a->d_weight);
     c.workspace = a->workspace;
@@ -125,18 +135,23 @@ gtok::LossCall loss_call(const gtok_x_vocab_loss* a) {
     return c;
 }
 
-const char* check_loss(const gtok_x_vocab_loss* a, int d) {
+// `values`: hidden states and targets are read, not only what a forward pass kept of them.
+const char* check_loss(const gtok_x_vocab_loss* a, int d, bool values) {
     if (const char* e = check_sizes(a)) return e;
-    if (const char* e = check(&a->hidden, d)) return e;
     if (const char* e = check(&a->weight, d)) return e;
     if (a->weight.rows > 1 && a->weight.stride < a->weight.cols) return "rows of the table lie over one another";
-    if (a->entries) {
+    if (values) {
+        if (const char* e = check(&a->hidden, d)) return e;
         if (const char* e = check_ids(a->targets, a->target_bits, a->hidden.rows, d)) return e;
-        if (const char* e = check(&a->teacher_logits, d)) return e;
-        if (a->teacher_logits.rows != a->hidden.rows || a->teacher_logits.cols != a->entries) return "the teacher's logits have another shape than its ids";
-        if (a->target_stride < 0) return "the stride of the teacher's ids is out of range";
-    } else if (const char* e = check_ids(a->targets, a->target_bits, a->hidden.rows, d)) {
-        return e;
+        if (a->entries) {
+            if (const char* e = check(&a->teacher_logits, d)) return e;
+            if (a->teacher_logits.rows != a->hidden.rows || a->teacher_logits.cols != a->entries) return "the teacher's logits have another shape than its ids";
+            if (a->target_stride < 0) return "the stride of the teacher's ids is out of range";
+        }
+    }
+    if (a->kept && a->hidden.rows) {
+        if (reinterpret_cast<uintptr_t>(a->kept) % 256 || !usable(a->kept, d)) return "`kept` is not aligned to 256 bytes or not in the current device's memory";
+        if (a->kept_bytes < gtok::loss_kept(loss_call(a))) return "`kept` is too small";
     }
     return nullptr;
 }
@@ -203,12 +218,18 @@ int64_t gtok_x_vocab_loss_workspace(const gtok_x_vocab_loss* args, int32_t backw
     return static_cast<int64_t>(gtok::loss_workspace(loss_call(args), backward != 0));
 }
 
+int64_t gtok_x_vocab_loss_kept(const gtok_x_vocab_loss* args) {
+    if (!args) return refuse("arguments are missing");
+    if (const char* e = check_sizes(args)) return refuse(e);
+    return static_cast<int64_t>(gtok::loss_kept(loss_call(args)));
+}
+
 int32_t gtok_x_vocab_loss_forward(const gtok_x_vocab_loss* args) {
     try {
         const int d = device();
         if (d < 0) return -1;
         if (!args) return refuse("arguments are missing");
-        if (const char* e = check_loss(args, d)) return refuse(e);
+        if (const char* e = check_loss(args, d, true)) return refuse(e);
         if (args->hidden.rows && (!args->losses || !args->lse || !usable(args->losses, d) || !usable(args->lse, d)))
             return refuse("losses or lse are missing or not in the current device's memory");
         if (args->total && !usable(args->total, d)) return refuse("the total is not in the current device's memory");
@@ -223,7 +244,7 @@ int32_t gtok_x_vocab_loss_backward(const gtok_x_vocab_loss* args) {
         const int d = device();
         if (d < 0) return -1;
         if (!args) return refuse("arguments are missing");
-        if (const char* e = check_loss(args, d)) return refuse(e);
+        if (const char* e = check_loss(args, d, !args->kept)) return refuse(e);
         if (!args->d_hidden.data && !args->d_weight.data) return 0;
         if (args->hidden.rows && (!args->lse || !args->grad || !usable(args->lse, d) || !usable(args->grad, d)))
             return refuse("lse or the losses' gradient are missing or not in the current device's memory");

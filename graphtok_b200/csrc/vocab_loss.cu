@@ -29,12 +29,10 @@ using namespace sm100;
 
 constexpr int kTile = 256;              // rows and columns of a pair's tile
 constexpr int kDepth = 64;              // elements of the summed dimension a stage holds: one 128-byte line
-constexpr int kStages = 6;
 constexpr int kStageBytes = 32768;      // 128 x 64 of either operand
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;
 constexpr int kStagingBytes = 4096;     // a warp's 32 lines of 128 bytes on their way out
-constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpilogueWarps * kStagingBytes + 256;
 constexpr int kGroup = 16;              // row tiles that share a sweep over the vocabulary: 16 x 256 rows stay in L2
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -48,16 +46,30 @@ inline float cut_off(int width) { return 1.f + static_cast<float>((width + 15) /
 struct Shared {
     int active;          // rows with a loss
     int error;           // a wait ran out
-    int splits;          // hidden gradient: parts of a piece's columns that are summed apart
     unsigned joined;     // blocks of join_kernel that are done
-    float row_scale;     // gradient of row i, times this, is what dZ carries of it ...
-    float unscale;       // ... and the products times this are the gradients
+    int splits;          // hidden gradient: parts of a piece's columns that are summed apart
+    float unscale;       // gradients are the products times this
 };
 
 enum { kForward = 0, kDelta = 1, kHiddenGrad = 2, kWeightGrad = 3 };
 
+// The forward pass writes no tiles and has its room for another stage.
+__host__ __device__ constexpr int stages(int mode) { return mode == kForward ? 7 : 6; }
+__host__ __device__ constexpr int smem_bytes(int mode) { return 1024 + stages(mode) * kStageBytes + (mode == kForward ? 0 : kEpilogueWarps * kStagingBytes) + 256; }
+
 struct Entry { int id; float share; };        // what a row's softmax should be at `id`; ascending in a row, INT_MAX after the last
 struct RowInfo { float lse2, factor; };       // of an active row: lse in powers of 2; what dZ is multiplied by
+
+// The hidden gradient's parts and where their sums go.
+struct HiddenOut {
+    const float* part;         // NULL: nothing to do
+    int part_cols;
+    const int* rows;
+    int n, cols;
+    uint16_t* out;
+    int64_t stride;
+    bool wide;                 // rows of `out` are lines of whole 16 bytes
+};
 
 struct Product {
     Shared* shared;
@@ -74,46 +86,55 @@ struct Product {
     bool direct;               // weight gradient, where its rows are no lines of whole 16 bytes: written by the threads
     uint16_t* out;             // weight gradient
     int64_t out_stride;
+    HiddenOut hidden_out;      // weight gradient of the last piece: what its idle warps may finish meanwhile
 };
 
 struct Place { int m, n, k0, k1, split; };     // tile of the output, blocks of the summed dimension
 
+// How one product is cut into tiles.
 template <int MODE>
-__device__ __forceinline__ int tile_count(const Product& p, int active, int splits) {
-    const int row_tiles = (active + kTile - 1) / kTile, col_tiles = (p.count + kTile - 1) / kTile, width_tiles = (p.width + kTile - 1) / kTile;
-    if (MODE == kHiddenGrad) return row_tiles * width_tiles * splits;
-    if (MODE == kWeightGrad) return active ? col_tiles * width_tiles : 0;
-    return row_tiles * col_tiles;
-}
-
-template <int MODE>
-__device__ __forceinline__ Place tile_place(const Product& p, int active, int splits, int t) {
-    const int row_tiles = (active + kTile - 1) / kTile, col_tiles = (p.count + kTile - 1) / kTile, width_tiles = (p.width + kTile - 1) / kTile;
-    Place q;
-    q.k0 = 0;
-    q.split = 0;
-    if (MODE == kHiddenGrad) {
-        const int blocks = (p.count + kDepth - 1) / kDepth;      // fewer in the last piece; a split may then be left without any
-        q.split = t / (row_tiles * width_tiles);
-        t -= q.split * row_tiles * width_tiles;
-        q.m = t / width_tiles;
-        q.n = t - q.m * width_tiles;
-        q.k0 = static_cast<int>(static_cast<int64_t>(blocks) * q.split / splits);
-        q.k1 = static_cast<int>(static_cast<int64_t>(blocks) * (q.split + 1) / splits);
-    } else if (MODE == kWeightGrad) {
-        q.m = t / width_tiles;
-        q.n = t - q.m * width_tiles;
-        q.k1 = (active + kDepth - 1) / kDepth;
-    } else {
-        const int group = t / (kGroup * col_tiles);
-        const int first = group * kGroup, rows = min(kGroup, row_tiles - first);
-        t -= first * col_tiles;
-        q.n = t / rows;
-        q.m = first + t - q.n * rows;
-        q.k1 = (p.width + kDepth - 1) / kDepth;
+struct Tiling {
+    int row_tiles, col_tiles, width_tiles, splits, blocks, tiles;
+    __device__ __forceinline__ Tiling(const Product& p, int active, int splits_) : splits(splits_) {
+        row_tiles = (active + kTile - 1) / kTile;
+        width_tiles = (p.width + kTile - 1) / kTile;
+        col_tiles = (p.count + kTile - 1) / kTile;
+        if (MODE == kHiddenGrad) {
+            blocks = (p.count + kDepth - 1) / kDepth;        // fewer in the last piece; a split may then be left without any
+            tiles = row_tiles * width_tiles * splits;
+        } else if (MODE == kWeightGrad) {
+            blocks = (active + kDepth - 1) / kDepth;
+            tiles = active ? col_tiles * width_tiles : 0;
+        } else {
+            blocks = (p.width + kDepth - 1) / kDepth;
+            tiles = row_tiles * col_tiles;
+        }
     }
-    return q;
-}
+    __device__ __forceinline__ Place place(int t) const {
+        Place q;
+        q.k0 = 0;
+        q.k1 = blocks;
+        q.split = 0;
+        if (MODE == kHiddenGrad) {
+            q.split = t / (row_tiles * width_tiles);
+            t -= q.split * row_tiles * width_tiles;
+            q.m = t / width_tiles;
+            q.n = t - q.m * width_tiles;
+            q.k0 = static_cast<int>(static_cast<int64_t>(blocks) * q.split / splits);
+            q.k1 = static_cast<int>(static_cast<int64_t>(blocks) * (q.split + 1) / splits);
+        } else if (MODE == kWeightGrad) {
+            q.m = t / width_tiles;
+            q.n = t - q.m * width_tiles;
+        } else {
+            const int group = t / (kGroup * col_tiles);
+            const int first = group * kGroup, rows = min(kGroup, row_tiles - first);
+            t -= first * col_tiles;
+            q.n = t / rows;
+            q.m = first + t - q.n * rows;
+        }
+        return q;
+    }
+};
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -180,6 +201,69 @@ struct Ahead {
     }
 };
 
+// Hidden gradient: the splits' sums in order, scaled, each row back at its place; rows without a loss get 0.  Eight columns a thread.
+template <bool BF16>
+__device__ __forceinline__ void finish_hidden(const HiddenOut& h, const Shared* shared, int64_t self, int64_t threads) {
+    const int active = shared->active, splits = shared->splits;
+    const int64_t apart = static_cast<int64_t>((active + kTile - 1) / kTile * kTile) * h.part_cols;
+    const float unscale = shared->error ? __int_as_float(0x7FC00000) : shared->unscale;
+    const int lines = (h.cols + 7) / 8;
+    const int64_t units = static_cast<int64_t>(h.n) * lines;
+    constexpr int kUnits = 2, kParts = 4;             // on their way at once
+    for (int64_t u = self; u < units; u += kUnits * threads) {
+        float v[kUnits][8];
+        const float* from[kUnits];
+        bool sums[kUnits];
+        int j[kUnits], i[kUnits];
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+            const int64_t at = min(u + k * threads, units - 1);
+            j[k] = static_cast<int>(at / lines);
+            i[k] = static_cast<int>(at - static_cast<int64_t>(j[k]) * lines) * 8;
+            sums[k] = u + k * threads < units && j[k] < active;
+            from[k] = h.part + static_cast<int64_t>(j[k]) * h.part_cols + i[k];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] = 0.f;
+        }
+        for (int s = 0; s < splits; s += kParts) {
+            float4 a[kUnits][kParts], b[kUnits][kParts];
+#pragma unroll
+            for (int k = 0; k < kUnits; ++k)
+#pragma unroll
+                for (int d = 0; d < kParts; ++d)
+                    if (sums[k] && s + d < splits) {
+                        a[k][d] = *reinterpret_cast<const float4*>(from[k] + (s + d) * apart);
+                        b[k][d] = *reinterpret_cast<const float4*>(from[k] + (s + d) * apart + 4);
+                    }
+#pragma unroll
+            for (int k = 0; k < kUnits; ++k)
+#pragma unroll
+                for (int d = 0; d < kParts; ++d)
+                    if (sums[k] && s + d < splits) {
+                        v[k][0] += a[k][d].x; v[k][1] += a[k][d].y; v[k][2] += a[k][d].z; v[k][3] += a[k][d].w;
+                        v[k][4] += b[k][d].x; v[k][5] += b[k][d].y; v[k][6] += b[k][d].z; v[k][7] += b[k][d].w;
+                    }
+        }
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+            if (u + k * threads >= units) break;
+            if (sums[k]) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[k][e] *= unscale;
+            }
+            uint16_t* to = h.out + h.rows[j[k]] * h.stride + i[k];
+            if (h.wide) {
+                *reinterpret_cast<uint4*>(to) =
+                    make_uint4(pack2<BF16>(v[k][0], v[k][1]), pack2<BF16>(v[k][2], v[k][3]), pack2<BF16>(v[k][4], v[k][5]), pack2<BF16>(v[k][6], v[k][7]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (i[k] + e < h.cols) to[e] = pack1<BF16>(v[k][e]);
+            }
+        }
+    }
+}
+
 // A persistent product: one pair of blocks an SM pair, tiles handed out in turn.  Warp 0 of each block copies its half of the operands
 // in, warp 1 of the first block issues the matrix instructions for both, eight warps of each block take the accumulators out while the
 // next tile is summed into the other half of tensor memory.
@@ -188,10 +272,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out,
                    const __grid_constant__ Product p) {
     constexpr bool kAcrossA = MODE == kWeightGrad, kAcrossB = MODE >= kHiddenGrad;     // operand's lines run across the summed dimension
+    constexpr bool kRows = MODE == kForward || MODE == kDelta;                          // the tile is one of logits
+    constexpr int kStages = stages(MODE);
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_addr(smem_raw) + 1023) & ~1023u;
     const uint32_t staging = base + kStages * kStageBytes;
-    const uint32_t bars = staging + kEpilogueWarps * kStagingBytes;
+    const uint32_t bars = staging + (MODE == kForward ? 0 : kEpilogueWarps * kStagingBytes);
     const uint32_t full = bars, empty = bars + 8 * kStages, acc_full = empty + 8 * kStages, acc_empty = acc_full + 16, tmem_at = acc_empty + 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -217,8 +303,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     after_previous();
     const int active = p.shared->active, splits = MODE == kHiddenGrad ? p.shared->splits : 1;
-    const int tiles = tile_count<MODE>(p, active, splits);
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const Tiling<MODE> tiling(p, active, splits);
+    const int tiles = tiling.tiles;
     bool ok = true;
 
     if (warp == 0) {
@@ -226,17 +313,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint32_t full_of_pair = in_block(full, 0);
             uint32_t it = 0;
             for (int t = pair; t < tiles && ok; t += pairs) {
-                const Place q = tile_place<MODE>(p, active, splits, t);
-                const int am = q.m * kTile + rank * 128, bn = q.n * kTile + rank * 128 + ((MODE == kForward || MODE == kDelta) ? p.first : 0);
+                const Place q = tiling.place(t);
+                const int am = q.m * kTile + rank * 128, bn = q.n * kTile + rank * 128 + (kRows ? p.first : 0);
                 const int bk = MODE == kHiddenGrad ? p.first : 0;
+                // Boxes of 64 rows that hold no active row are left out: what lies in their place only reaches rows that nobody reads.
+                const int boxes = MODE == kWeightGrad ? 2 : max(0, min(2, (active - am + 63) / 64));
+                const int all_boxes = MODE == kWeightGrad ? 4 : max(0, min(4, (active - q.m * kTile + 63) / 64));
                 for (int k = q.k0; k < q.k1; ++k, ++it) {
                     const uint32_t s = it % kStages;
                     if (!bar_wait(empty + 8 * s, ((it / kStages) & 1) ^ 1)) { ok = false; break; }
                     const uint32_t a = base + s * kStageBytes, b = a + kStageBytes / 2, bar = full_of_pair + 8 * s;
-                    if (rank == 0) bar_expect(full + 8 * s, 2 * kStageBytes);
+                    if (rank == 0) bar_expect(full + 8 * s, (4 + all_boxes) * 8192);
                     const int x = k * kDepth;
-                    load_tile(a, &map_a, kAcrossA ? am : x, kAcrossA ? x : am, bar);
-                    load_tile(a + 8192, &map_a, kAcrossA ? am + 64 : x, kAcrossA ? x : am + 64, bar);
+                    if (boxes > 0) load_tile(a, &map_a, kAcrossA ? am : x, kAcrossA ? x : am, bar);
+                    if (boxes > 1) load_tile(a + 8192, &map_a, kAcrossA ? am + 64 : x, kAcrossA ? x : am + 64, bar);
                     load_tile(b, &map_b, kAcrossB ? bn : x, kAcrossB ? x + bk : bn, bar);
                     load_tile(b + 8192, &map_b, kAcrossB ? bn + 64 : x, kAcrossB ? x + bk : bn + 64, bar);
                 }
@@ -248,10 +338,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 1) {
         if (rank == 0 && elect()) {
-            constexpr uint32_t kind = mma_kind(BF16, kAcrossA, kAcrossB);
+            const uint32_t kind = mma_kind(BF16, kAcrossA, kAcrossB, kTile);
             uint32_t it = 0, acc = 0;
             for (int t = pair; t < tiles && ok; t += pairs) {
-                const Place q = tile_place<MODE>(p, active, splits, t);
+                const Place q = tiling.place(t);
                 if (q.k0 >= q.k1) continue;
                 if (!bar_wait(acc_empty + 8 * (acc & 1), ((acc >> 1) & 1) ^ 1)) { ok = false; break; }
                 fence_after();
@@ -270,23 +360,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 ++acc;
             }
         }
-    } else if (warp >= 4) {
+    } else if (warp < 4) {
+        if (MODE == kWeightGrad && p.hidden_out.part)
+            finish_hidden<BF16>(p.hidden_out, p.shared, static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x - 64, static_cast<int64_t>(gridDim.x) * 64);
+    } else {
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const uint32_t lines = staging + (warp - 4) * kStagingBytes;
         const uint32_t line = lines + lane * 128;
-        constexpr bool kRows = MODE == kForward || MODE == kDelta;
         const float unscale = MODE == kWeightGrad ? p.shared->unscale : 0.f;
         Ahead ahead;
         auto look_ahead = [&](int t) {
             if (t >= tiles) t = pair;                  // (no further tile: anything that is in bounds)
-            const Place q = tile_place<MODE>(p, active, splits, t);
+            const Place q = tiling.place(t);
             const int m = q.m * kTile + rank * 128 + quarter * 32 + lane;
             ahead.begin(p, m, m < active, p.first + q.n * kTile + half * 128, MODE == kDelta);
         };
         if (kRows && pair < tiles) look_ahead(pair);
         uint32_t acc = 0;
+        float high = -INFINITY, sum = 0.f;          // forward: of a row in this tile; where all tiles are of the same rows, in all so far
         for (int t = pair; t < tiles; t += pairs) {
-            const Place q = tile_place<MODE>(p, active, splits, t);
+            const Place q = tiling.place(t);
             if (q.k0 >= q.k1) continue;
             const int m = q.m * kTile + rank * 128 + quarter * 32 + lane;       // this thread's line of the tile
             const int column = q.n * kTile + half * 128;                        // of the output; of the piece where columns are the vocabulary's
@@ -302,7 +395,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (!ok) break;
             fence_after();
             float va[32], vb[32];
-            float high = -INFINITY, sum = 0.f;
+            if (tiling.row_tiles > 1) {
+                high = -INFINITY;
+                sum = 0.f;
+            }
             // What becomes of 32 columns from `c` on.
             auto work = [&](float (&v)[32], int c) {
                 const int at = p.first + column + c;
@@ -408,6 +504,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                 }
             };
+            // Lines without an active row, of which nothing is asked; dZ is read in steps of 64 rows, and they are 0 up to there.
+            const bool idle = MODE == kDelta ? m - lane >= (active + kDepth - 1) / kDepth * kDepth : MODE != kWeightGrad && m - lane >= active;
+            if (idle) {
+                if (lane == 0) bar_arrive_cluster(in_block(acc_empty + 8 * (acc & 1), 0));
+                ++acc;
+                continue;
+            }
             tmem_load(from, va);
 #pragma unroll 1
             for (int c = 0; c < 128; c += 64) {
@@ -424,8 +527,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
                 work(vb, c + 32);
             }
-            if (MODE == kForward && live) p.partial[static_cast<int64_t>(q.n * 2 + half) * p.n_rows + m] = make_float2(high, sum);
+            if (MODE == kForward && live && tiling.row_tiles > 1) p.partial[static_cast<int64_t>(q.n * 2 + half) * p.n_rows + m] = make_float2(high, sum);
             ++acc;
+        }
+        if (MODE == kForward && tiling.row_tiles == 1 && pair < tiles) {
+            const int m = rank * 128 + quarter * 32 + lane;
+            if (m < active) p.partial[static_cast<int64_t>(pair * 2 + half) * p.n_rows + m] = make_float2(high, sum);
         }
         if (lane == 0) stores_done();
     }
@@ -540,23 +647,15 @@ struct RowsArgs {
     int* rows;
     Shared* shared;
     float *losses, *lse;         // forward
-    const float* grad;           // backward
-    int64_t grad_stride;
-    bool grad_of_mean, half;
-    float inv_temperature;
-    int width_tiles, blocks, pairs;
 };
 
-// Which rows have a loss: their places in order, behind them those of the others; and the scale of the gradients.  One block, 256 rows
-// a warp at a time.
+// Which rows have a loss: their places in order, behind them those of the others.  One block, 256 rows a warp at a time.
 __global__ void __launch_bounds__(1024) rows_kernel(const __grid_constant__ RowsArgs a) {
     constexpr int kEach = 8;
     __shared__ int warp_sum[32];
-    __shared__ float warp_top[32];
     after_previous();
     let_next_begin();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    float top = 0.f;
     int done = 0;
     for (int base = 0; base < a.n; base += 1024 * kEach) {
         const int at = base + warp * 32 * kEach + lane;
@@ -584,7 +683,6 @@ __global__ void __launch_bounds__(1024) rows_kernel(const __grid_constant__ Rows
                 a.losses[row] = id[i] == kBad ? __int_as_float(0x7FC00000) : 0.f;
                 a.lse[row] = 0.f;
             }
-            if (id[i] >= 0 && a.grad) top = max_nan(top, fabsf(a.grad[row * a.grad_stride]));
         }
         if (lane == 0) warp_sum[warp] = mine;
         __syncthreads();
@@ -610,31 +708,76 @@ __global__ void __launch_bounds__(1024) rows_kernel(const __grid_constant__ Rows
         }
         __syncthreads();
     }
+    if (tid == 0) {
+        Shared s{};
+        s.active = done;
+        *a.shared = s;
+    }
+}
+
+struct ScaleArgs {
+    const Shared* from;          // of the forward pass, or of what has just been prepared
+    Shared* shared;
+    const int* rows;
+    RowInfo* info;
+    const float *lse, *grad;
+    int64_t grad_stride;
+    bool grad_of_mean, half;
+    float inv_temperature;
+    int width_tiles, blocks, pairs;
+};
+
+// The scale of the gradients, each active row's part of it, and the number of the hidden gradient's splits.  One block.
+__global__ void __launch_bounds__(1024) scale_kernel(const __grid_constant__ ScaleArgs a) {
+    __shared__ float warp_top[32];
+    after_previous();
+    let_next_begin();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int active = a.from->active;
+    float top = 0.f;
+    for (int base = tid; base < active; base += 8 * 1024) {
+        float g[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = base + 1024 * i < active ? fabsf(a.grad[a.rows[base + 1024 * i] * a.grad_stride]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max_nan(top, g[i]);
+    }
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, d));
     if (lane == 0) warp_top[warp] = top;
     __syncthreads();
-    if (warp) return;
     top = warp_top[lane];
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, d));
+    // dZ is kept with the largest row gradient as 1 (bf16: its range is fp32's) or as 2^15, so that fp16 holds probabilities
+    // down to 2^-29 in full precision and nothing above 2^16.
+    const float unit = a.half ? 32768.f : 1.f;
+    const float row_scale = top == 0.f ? 0.f : unit / top;
+    for (int base = tid; base < active; base += 8 * 1024) {
+        RowInfo r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (base + 1024 * i >= active) break;
+            const int row = a.rows[base + 1024 * i];
+            r[i] = RowInfo{a.lse[row] * kLog2e, a.grad[row * a.grad_stride] * row_scale};
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (base + 1024 * i < active) a.info[base + 1024 * i] = r[i];
+    }
+    if (warp) return;
     // each lane the time of one number of splits
-    const int64_t time = split_time(lane + 1, static_cast<int64_t>((done + kTile - 1) / kTile) * a.width_tiles, a.blocks, a.pairs);
+    const int64_t time = split_time(lane + 1, static_cast<int64_t>((active + kTile - 1) / kTile) * a.width_tiles, a.blocks, a.pairs);
     int64_t least = time;
 #pragma unroll
     for (int d = 16; d; d >>= 1) least = min(least, __shfl_xor_sync(~0u, least, d));
     const int splits = __ffs(__ballot_sync(~0u, time == least));
     if (lane == 0) {
-        Shared s;
-        s.active = done;
-        s.error = 0;
-        s.joined = 0;
+        Shared s{};
+        s.active = active;
+        s.error = a.from->error;
         s.splits = splits;
-        // dZ is kept with the largest row gradient as 1 (bf16: its range is fp32's) or as 2^15, so that fp16 holds probabilities
-        // down to 2^-29 in full precision and nothing above 2^16.
-        const float unit = a.half ? 32768.f : 1.f;
-        s.row_scale = top == 0.f ? 0.f : unit / top;
-        s.unscale = top / unit * a.inv_temperature / (a.grad_of_mean ? fmaxf(static_cast<float>(done), 1.f) : 1.f);
+        s.unscale = top / unit * a.inv_temperature / (a.grad_of_mean ? fmaxf(static_cast<float>(active), 1.f) : 1.f);
         *a.shared = s;
     }
 }
@@ -652,17 +795,15 @@ struct GatherArgs {
     int entries;                 // of a teacher
     const Entry* entry_from;
     Entry* entry_to;
-    RowInfo* info;               // backward
-    const float *lse, *grad;
-    int64_t grad_stride;
 };
 
-// The active rows copied together, lines of `cols` rounded up to whole 16 bytes; lines up to the next whole tile become 0.  One block a row.
+// The active rows copied together, lines of `cols` rounded up to whole 16 bytes; up to the next multiple of 64, in which they are read, there are
+// lines of 0.  One block a row.
 __global__ void __launch_bounds__(128) gather_kernel(const __grid_constant__ GatherArgs a) {
     after_previous();
     let_next_begin();
     const int active = a.rows ? a.shared->active : a.n;
-    const int end = a.rows ? (active + kTile - 1) / kTile * kTile : a.n;
+    const int end = a.rows ? (active + kDepth - 1) / kDepth * kDepth : a.n;
     const int lines = a.dst_cols / 8;
     for (int64_t j = blockIdx.x; j < end; j += gridDim.x) {
         const int64_t row = j < active ? (a.rows ? a.rows[j] : j) : 0;
@@ -688,10 +829,8 @@ __global__ void __launch_bounds__(128) gather_kernel(const __grid_constant__ Gat
                 to[i] = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
-        if (j < active) {
+        if (j < active)
             for (int i = threadIdx.x; i < a.entries; i += 128) a.entry_to[j * a.entries + i] = a.entry_from[row * a.entries + i];
-            if (a.info && threadIdx.x == 0) a.info[j] = RowInfo{a.lse[row] * kLog2e, a.grad[row * a.grad_stride] * a.shared->row_scale};
-        }
     }
 }
 
@@ -699,7 +838,7 @@ __global__ void __launch_bounds__(128) gather_kernel(const __grid_constant__ Gat
 
 struct JoinArgs {
     const float2* partial;
-    int parts, n_rows;
+    int vocab, pairs, n_rows;
     Shared* shared;
     const int* rows;
     int n, entries;
@@ -719,15 +858,27 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Join
     let_next_begin();
     const int active = a.shared->active;
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int tiles = (a.vocab + kTile - 1) / kTile, parts = 2 * (active > kTile ? tiles : min(tiles, a.pairs));
     for (int base = blockIdx.x * 32; base < active; base += gridDim.x * 32) {
-        const int m = base + x;
+        const int m = base + x, j = base + y;
+        // what the second half of the work needs, on its way during the first
+        Entry e{INT_MAX, 0.f};
+        float logit = 0.f;
+        int row = 0;
+        if (j < active) {
+            row = a.rows[j];
+            if (x < a.entries) {
+                e = a.entry[static_cast<int64_t>(j) * a.entries + x];
+                logit = a.entry_logits[static_cast<int64_t>(j) * a.entries + x];
+            }
+        }
         float high = -INFINITY, sum = 0.f;
         if (m < active) {
-            for (int k = y; k < a.parts; k += 32 * 8) {
+            for (int k = y; k < parts; k += 32 * 8) {
                 float2 v[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    v[i] = k + 32 * i < a.parts ? a.partial[static_cast<int64_t>(k + 32 * i) * a.n_rows + m] : make_float2(-INFINITY, 0.f);
+                    v[i] = k + 32 * i < parts ? a.partial[static_cast<int64_t>(k + 32 * i) * a.n_rows + m] : make_float2(-INFINITY, 0.f);
                 float top = high;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) top = fmaxf(top, v[i].x);
@@ -751,18 +902,18 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Join
 #pragma unroll
         for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
         const float row_lse = ref * a.inv_temperature + logf(total);
-        const int j = base + y;
         if (j < active) {
             float loss = 0.f;
             for (int i = x; i < a.entries; i += 32) {
-                const int64_t at = static_cast<int64_t>(j) * a.entries + i;
-                const Entry e = a.entry[at];
-                if (e.id != INT_MAX && e.share != 0.f) loss += e.share * (logf(e.share) + (row_lse - a.entry_logits[at] * a.inv_temperature));
+                if (i >= 32) {
+                    e = a.entry[static_cast<int64_t>(j) * a.entries + i];
+                    logit = a.entry_logits[static_cast<int64_t>(j) * a.entries + i];
+                }
+                if (e.id != INT_MAX && e.share != 0.f) loss += e.share * (logf(e.share) + (row_lse - logit * a.inv_temperature));
             }
 #pragma unroll
             for (int d = 16; d; d >>= 1) loss += __shfl_xor_sync(~0u, loss, d);
             if (x == 0) {
-                const int row = a.rows[j];
                 a.losses[row] = a.shared->error ? __int_as_float(0x7FC00000) : loss;
                 a.lse[row] = row_lse;
             }
@@ -788,37 +939,11 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Join
     if (x == 0) *a.total = a.mean ? sum / fmaxf(static_cast<float>(active), 1.f) : sum;
 }
 
-// Hidden gradient: the splits' sums in order, scaled, each row back at its place; rows without a loss get 0.  Eight columns a thread.
+// The hidden gradient where the table's product does not finish it.
 template <bool BF16>
-__global__ void __launch_bounds__(256) hidden_grad_kernel(const float* part, int part_cols, const Shared* shared, const int* rows, int n, int cols, uint16_t* out,
-                                                          int64_t stride, bool wide) {
+__global__ void __launch_bounds__(256) hidden_grad_kernel(const __grid_constant__ HiddenOut h, const Shared* shared) {
     after_previous();
-    const int active = shared->active, splits = shared->splits;
-    const int64_t apart = static_cast<int64_t>((active + kTile - 1) / kTile * kTile) * part_cols;
-    const float unscale = shared->error ? __int_as_float(0x7FC00000) : shared->unscale;
-    const int lines = (cols + 7) / 8;
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < static_cast<int64_t>(n) * lines; u += static_cast<int64_t>(gridDim.x) * 256) {
-        const int j = static_cast<int>(u / lines), i = static_cast<int>(u - static_cast<int64_t>(j) * lines) * 8;
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (j < active) {
-            const float* from = part + static_cast<int64_t>(j) * part_cols + i;
-            for (int s = 0; s < splits; ++s, from += apart) {
-                const float4 a = *reinterpret_cast<const float4*>(from), b = *reinterpret_cast<const float4*>(from + 4);
-                v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-                v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] *= unscale;
-        }
-        uint16_t* to = out + rows[j] * stride + i;
-        if (wide) {
-            *reinterpret_cast<uint4*>(to) = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (i + k < cols) to[k] = pack1<BF16>(v[k]);
-        }
-    }
+    finish_hidden<BF16>(h, shared, static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, static_cast<int64_t>(gridDim.x) * 256);
 }
 
 // ---- host -------------------------------------------------------------------------
@@ -838,7 +963,10 @@ struct Plan {
     bool copy_weight;
     int piece;                                      // backward: columns a piece
     int64_t sum_rows;                               // rows of the hidden gradient's parts, however many rows are active
-    uint64_t shared, rows, entry, entry_raw, state, info, entry_logits, hidden, weight, partial, delta, sums, bytes;
+    // what a forward pass may leave for the backward one
+    uint64_t shared, rows, entry, hidden, kept_bytes;
+    // and the rest of the workspace
+    uint64_t entry_raw, state, info, own_shared, entry_logits, weight, partial, delta, sums, bytes;
 };
 
 constexpr int64_t kDeltaBytes = 256 << 20;          // of a piece's dZ
@@ -863,23 +991,25 @@ Plan make_plan(const LossCall& c, bool backward) {
     p.shared = take(sizeof(Shared));
     p.rows = take(4ull * p.n);
     p.entry = take(sizeof(Entry) * listed);
-    if (c.entries) {
+    p.hidden = take(2ull * p.n_rows * p.cols);
+    p.kept_bytes = at;
+    if (c.kept) at = 0;
+    if (c.entries && !(backward && c.kept)) {
         p.entry_raw = take(sizeof(Entry) * listed);
         p.state = take(4ull * p.n);
     }
-    p.hidden = take(2ull * p.n_rows * p.cols);
     if (p.copy_weight) p.weight = take(2ull * p.vocab * p.cols);
     const int64_t tiles = div_up(p.vocab, kTile);
     if (!backward) {
         p.entry_logits = take(4ull * listed);
-        p.partial = take(8ull * 2 * tiles * p.n_rows);
+        p.partial = take(8ull * 2 * std::max<int64_t>(tiles, p.pairs) * p.n_rows);
     } else {
+        p.own_shared = take(sizeof(Shared));
         p.info = take(sizeof(RowInfo) * p.n);
         const int64_t room = std::max<int64_t>(1, kDeltaBytes / (2ll * kTile * p.n_rows));
         p.piece = static_cast<int>(div_up(tiles, div_up(tiles, room)) * kTile);
         const int64_t width_tiles = div_up(p.cols, kTile);
-        for (int64_t t = 1; t <= p.n_rows / kTile; ++t)
-        {
+        for (int64_t t = 1; t <= p.n_rows / kTile; ++t) {
             int splits = 1;
             for (int k = 2; k <= kMaxSplits; ++k)
                 if (split_time(k, t * width_tiles, p.piece / kDepth, p.pairs) < split_time(splits, t * width_tiles, p.piece / kDepth, p.pairs)) splits = k;
@@ -917,39 +1047,55 @@ bool tile_map(CUtensorMap* map, int type, const void* data, int64_t rows, int64_
 template <int MODE>
 cudaError_t launch_product(bool bf16, int pairs, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const Product& p, cudaStream_t stream) {
     auto* kernel = bf16 ? product_kernel<MODE, true> : product_kernel<MODE, false>;
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes)) return e;
-    return launch(kernel, 2 * pairs, kThreads, kSmemBytes, stream, a, b, out, p);
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(MODE))) return e;
+    return launch(kernel, 2 * pairs, kThreads, smem_bytes(MODE), stream, a, b, out, p);
 }
 
 struct Prepared {
     Plan plan;
-    char* at;
+    char *at, *kept;
     Shared* shared;
     int* rows;
-    Product product;
-    CUtensorMap hidden_map, weight_map;
+    Entry* entry;
+    uint16_t* hidden;
+    const void* weight;
+    int64_t weight_stride;
 };
 
 const char* cuda_error(cudaError_t e) { return e == cudaSuccess ? nullptr : cudaGetErrorString(e); }
 
-const char* prepare(const LossCall& c, bool backward, Prepared& w) {
-    w.plan = make_plan(c, backward);
+// Addresses in the workspace; the table copied where its rows are no lines of whole 16 bytes; and, unless `given`, the active rows.
+cudaError_t prepare(const LossCall& c, bool backward, bool given, Prepared& w) {
     const Plan& p = w.plan;
-    if (c.workspace_bytes < p.bytes) return "the workspace is too small";
-    if (!encode_fn()) return "the driver has no tiled copies";
     w.at = static_cast<char*>(c.workspace);
-    w.shared = reinterpret_cast<Shared*>(w.at + p.shared);
-    w.rows = reinterpret_cast<int*>(w.at + p.rows);
-    Entry *entry = reinterpret_cast<Entry*>(w.at + p.entry), *entry_raw = reinterpret_cast<Entry*>(w.at + p.entry_raw);
+    w.kept = c.kept ? static_cast<char*>(c.kept) : w.at;
+    w.shared = reinterpret_cast<Shared*>(w.kept + p.shared);
+    w.rows = reinterpret_cast<int*>(w.kept + p.rows);
+    w.entry = reinterpret_cast<Entry*>(w.kept + p.entry);
+    w.hidden = reinterpret_cast<uint16_t*>(w.kept + p.hidden);
+    w.weight = c.weight.data;
+    w.weight_stride = c.weight.stride;
+    GatherArgs g{};
+    if (p.copy_weight) {
+        g.src = static_cast<const uint16_t*>(w.weight);
+        g.stride = w.weight_stride;
+        g.cols = p.width;
+        g.n = p.vocab;
+        g.dst = reinterpret_cast<uint16_t*>(w.at + p.weight);
+        g.dst_cols = p.cols;
+        if (cudaError_t e = launch(gather_kernel, std::min(p.vocab, 148 * 16), 128, 0, c.stream, g)) return e;
+        w.weight = g.dst;
+        w.weight_stride = p.cols;
+    }
+    if (given) return cudaSuccess;
+    Entry* entry_raw = reinterpret_cast<Entry*>(w.at + p.entry_raw);
     int* state = reinterpret_cast<int*>(w.at + p.state);
-    RowInfo* info = backward ? reinterpret_cast<RowInfo*>(w.at + p.info) : nullptr;
-    const float inv_temperature = 1.f / c.temperature;      // of the teacher's logits and the gradient; the student's: see cut_off
     if (c.entries) {
         int room = 2;
         while (room < c.entries) room *= 2;
         if (cudaError_t e = launch(teacher_kernel, p.n, std::min(256, std::max(32, room / 2)), room * 12, c.stream, c.targets, c.teacher, c.entries, room, p.vocab,
-                                   inv_temperature, entry_raw, state))
-            return cuda_error(e);
+                                   1.f / c.temperature, entry_raw, state))
+            return e;
     }
     RowsArgs r{};
     r.targets = c.targets;
@@ -957,83 +1103,63 @@ const char* prepare(const LossCall& c, bool backward, Prepared& w) {
     r.vocab = p.vocab;
     r.n = p.n;
     r.state = c.entries ? state : nullptr;
-    r.entry = entry;
+    r.entry = w.entry;
     r.rows = w.rows;
     r.shared = w.shared;
     r.losses = backward ? nullptr : c.losses;
     r.lse = backward ? nullptr : c.lse;
-    r.grad = backward ? c.grad : nullptr;
-    r.grad_stride = c.grad_stride;
-    r.grad_of_mean = c.grad_of_mean;
-    r.half = c.hidden.type == kF16;
-    r.inv_temperature = inv_temperature;
-    r.width_tiles = static_cast<int>(div_up(p.cols, kTile));
-    r.blocks = p.piece / kDepth;
-    r.pairs = p.pairs;
-    if (cudaError_t e = launch(rows_kernel, 1, 1024, 0, c.stream, r)) return cuda_error(e);
-    const void* weight = c.weight.data;
-    int64_t weight_stride = c.weight.stride;
-    GatherArgs g{};
-    if (p.copy_weight) {
-        g.src = static_cast<const uint16_t*>(weight);
-        g.stride = weight_stride;
-        g.cols = p.width;
-        g.n = p.vocab;
-        g.dst = reinterpret_cast<uint16_t*>(w.at + p.weight);
-        g.dst_cols = p.cols;
-        if (cudaError_t e = launch(gather_kernel, std::min(p.vocab, 148 * 16), 128, 0, c.stream, g)) return cuda_error(e);
-        weight = g.dst;
-        weight_stride = p.cols;
-    }
+    if (cudaError_t e = launch(rows_kernel, 1, 1024, 0, c.stream, r)) return e;
     g.src = static_cast<const uint16_t*>(c.hidden.data);
     g.stride = c.hidden.stride;
     g.cols = p.width;
     g.rows = w.rows;
     g.shared = w.shared;
     g.n = p.n;
-    g.dst = reinterpret_cast<uint16_t*>(w.at + p.hidden);
+    g.dst = w.hidden;
     g.dst_cols = p.cols;
     g.wide = p.width % 8 == 0 && c.hidden.stride % 8 == 0 && reinterpret_cast<uintptr_t>(c.hidden.data) % 16 == 0;
     g.entries = c.entries;
     g.entry_from = entry_raw;
-    g.entry_to = entry;
-    g.info = info;
-    g.lse = c.lse;
-    g.grad = c.grad;
-    g.grad_stride = c.grad_stride;
-    if (cudaError_t e = launch(gather_kernel, std::min(p.n_rows, 148 * 16), 128, 0, c.stream, g)) return cuda_error(e);
-    if (!tile_map(&w.hidden_map, c.hidden.type, g.dst, p.n_rows, p.cols, p.cols, 64) || !tile_map(&w.weight_map, c.hidden.type, weight, p.vocab, p.cols, weight_stride, 64))
-        return "a tensor map was refused";
-    Product& q = w.product;
-    q = Product{};
+    g.entry_to = w.entry;
+    return launch(gather_kernel, std::min(p.n_rows, 148 * 16), 128, 0, c.stream, g);
+}
+
+Product product_of(const LossCall& c, const Prepared& w) {
+    Product q{};
     q.shared = w.shared;
-    q.n_rows = p.n_rows;
-    q.vocab = p.vocab;
-    q.width = p.cols;
-    q.count = p.vocab;
-    q.entries = p.entries;
-    q.entry = entry;
-    q.info = info;
-    q.exponent = kLog2e / c.temperature * cut_off(p.width);
-    return nullptr;
+    q.n_rows = w.plan.n_rows;
+    q.vocab = w.plan.vocab;
+    q.width = w.plan.cols;
+    q.count = w.plan.vocab;
+    q.entries = w.plan.entries;
+    q.entry = w.entry;
+    q.exponent = kLog2e / c.temperature * cut_off(w.plan.width);
+    return q;
 }
 
 }  // namespace
 
 uint64_t loss_workspace(const LossCall& c, bool backward) { return c.hidden.rows ? make_plan(c, backward).bytes : 0; }
+uint64_t loss_kept(const LossCall& c) { return c.hidden.rows ? make_plan(c, false).kept_bytes : 0; }
 
 const char* loss_forward(const LossCall& c) {
     if (c.hidden.rows == 0) return c.total ? cuda_error(cudaMemsetAsync(c.total, 0, 4, c.stream)) : nullptr;
+    if (!encode_fn()) return "the driver has no tiled copies";
     Prepared w;
-    if (const char* e = prepare(c, false, w)) return e;
+    w.plan = make_plan(c, false);
     const Plan& p = w.plan;
-    Product& q = w.product;
+    if (cudaError_t e = prepare(c, false, false, w)) return cuda_error(e);
+    CUtensorMap hidden_map, weight_map;
+    if (!tile_map(&hidden_map, c.hidden.type, w.hidden, p.n_rows, p.cols, p.cols, 64) || !tile_map(&weight_map, c.hidden.type, w.weight, p.vocab, p.cols, w.weight_stride, 64))
+        return "a tensor map was refused";
+    Product q = product_of(c, w);
     q.partial = reinterpret_cast<float2*>(w.at + p.partial);
     q.entry_logits = reinterpret_cast<float*>(w.at + p.entry_logits);
-    if (cudaError_t e = launch_product<kForward>(c.hidden.type == kBF16, p.pairs, w.hidden_map, w.weight_map, w.hidden_map, q, c.stream)) return cuda_error(e);
+    if (cudaError_t e = launch_product<kForward>(c.hidden.type == kBF16, p.pairs, hidden_map, weight_map, hidden_map, q, c.stream)) return cuda_error(e);
     JoinArgs j{};
     j.partial = q.partial;
-    j.parts = static_cast<int>(2 * div_up(p.vocab, kTile));
+    j.vocab = p.vocab;
+    j.pairs = p.pairs;
     j.n_rows = p.n_rows;
     j.shared = w.shared;
     j.rows = w.rows;
@@ -1056,45 +1182,79 @@ const char* loss_backward(const LossCall& c) {
         if (!c.d_weight.data) return nullptr;
         return cuda_error(cudaMemset2DAsync(const_cast<void*>(c.d_weight.data), c.d_weight.stride * 2, 0, c.d_weight.cols * 2, c.d_weight.rows, c.stream));
     }
+    if (!encode_fn()) return "the driver has no tiled copies";
     Prepared w;
-    if (const char* e = prepare(c, true, w)) return e;
+    w.plan = make_plan(c, true);
     const Plan& p = w.plan;
+    if (cudaError_t e = prepare(c, true, c.kept != nullptr, w)) return cuda_error(e);
     uint16_t* delta = reinterpret_cast<uint16_t*>(w.at + p.delta);
     float* sums = reinterpret_cast<float*>(w.at + p.sums);
-    CUtensorMap delta_map, delta_out, sums_out, weight_out;
-    if (!tile_map(&delta_map, c.hidden.type, delta, p.n_rows, p.piece, p.piece, 64) || !tile_map(&delta_out, c.hidden.type, delta, p.n_rows, p.piece, p.piece, 32) ||
-        !tile_map(&sums_out, kF32, sums, p.sum_rows, p.cols, p.cols, 32))
-        return "a tensor map was refused";
     uint16_t* d_weight = static_cast<uint16_t*>(const_cast<void*>(c.d_weight.data));
     const bool direct = d_weight && (p.width % 8 || c.d_weight.stride % 8 || reinterpret_cast<uintptr_t>(d_weight) % 16);
+    // operands come in boxes of 64 lines, results leave in boxes of 32
+    CUtensorMap hidden_map, weight_map, delta_map, delta_out, sums_out, weight_out;
+    if (!tile_map(&hidden_map, c.hidden.type, w.hidden, p.n_rows, p.cols, p.cols, 64) ||
+        !tile_map(&weight_map, c.hidden.type, w.weight, p.vocab, p.cols, w.weight_stride, 64) ||
+        !tile_map(&delta_map, c.hidden.type, delta, p.n_rows, p.piece, p.piece, 64) || !tile_map(&delta_out, c.hidden.type, delta, p.n_rows, p.piece, p.piece, 32) ||
+        !tile_map(&sums_out, kF32, sums, p.sum_rows, p.cols, p.cols, 32))
+        return "a tensor map was refused";
     if (d_weight && !direct) {
         if (!tile_map(&weight_out, c.hidden.type, d_weight, p.vocab, p.width, c.d_weight.stride, 32)) return "a tensor map was refused";
     } else {
         weight_out = delta_out;
     }
+    ScaleArgs a{};
+    a.from = w.shared;
+    a.shared = reinterpret_cast<Shared*>(w.at + p.own_shared);
+    a.rows = w.rows;
+    a.info = reinterpret_cast<RowInfo*>(w.at + p.info);
+    a.lse = c.lse;
+    a.grad = c.grad;
+    a.grad_stride = c.grad_stride;
+    a.grad_of_mean = c.mean;
+    a.half = !bf16;
+    a.inv_temperature = 1.f / c.temperature;
+    a.width_tiles = static_cast<int>(div_up(p.cols, kTile));
+    a.blocks = p.piece / kDepth;
+    a.pairs = p.pairs;
+    if (cudaError_t e = launch(scale_kernel, 1, 1024, 0, c.stream, a)) return cuda_error(e);
+    HiddenOut h{};
+    if (c.d_hidden.data) {
+        h.part = sums;
+        h.part_cols = p.cols;
+        h.rows = w.rows;
+        h.n = p.n;
+        h.cols = p.width;
+        h.out = static_cast<uint16_t*>(const_cast<void*>(c.d_hidden.data));
+        h.stride = c.d_hidden.stride;
+        h.wide = p.width % 8 == 0 && h.stride % 8 == 0 && reinterpret_cast<uintptr_t>(h.out) % 16 == 0;
+    }
+    // A small hidden gradient is finished by idle warps of the last product, which hides it (6 to 8 us of 280); a large one takes those few
+    // warps longer than the product (4,099 x 1024 in 5 splits: 40 us more than the kernel of its own, which takes 8).
+    const int64_t lines = static_cast<int64_t>(p.n) * div_up(p.width, 8);
+    const bool within = d_weight && lines <= 16ll * 64 * 2 * p.pairs;
     for (int first = 0; first < p.vocab; first += p.piece) {
-        Product q = w.product;
+        Product q = product_of(c, w);
+        q.shared = a.shared;
+        q.info = a.info;
         q.first = first;
         q.count = std::min(p.piece, p.vocab - first);
-        if (cudaError_t e = launch_product<kDelta>(bf16, p.pairs, w.hidden_map, w.weight_map, delta_out, q, c.stream)) return cuda_error(e);
+        if (cudaError_t e = launch_product<kDelta>(bf16, p.pairs, hidden_map, weight_map, delta_out, q, c.stream)) return cuda_error(e);
         if (c.d_hidden.data) {
             q.add = first > 0;
-            if (cudaError_t e = launch_product<kHiddenGrad>(bf16, p.pairs, delta_map, w.weight_map, sums_out, q, c.stream)) return cuda_error(e);
+            if (cudaError_t e = launch_product<kHiddenGrad>(bf16, p.pairs, delta_map, weight_map, sums_out, q, c.stream)) return cuda_error(e);
         }
         if (d_weight) {
             q.direct = direct;
             q.out = d_weight;
             q.out_stride = c.d_weight.stride;
             q.width = p.width;
-            if (cudaError_t e = launch_product<kWeightGrad>(bf16, p.pairs, delta_map, w.hidden_map, weight_out, q, c.stream)) return cuda_error(e);
+            if (within && first + p.piece >= p.vocab) q.hidden_out = h;
+            if (cudaError_t e = launch_product<kWeightGrad>(bf16, p.pairs, delta_map, hidden_map, weight_out, q, c.stream)) return cuda_error(e);
         }
     }
-    if (!c.d_hidden.data) return nullptr;
-    uint16_t* out = static_cast<uint16_t*>(const_cast<void*>(c.d_hidden.data));
-    const bool wide = p.width % 8 == 0 && c.d_hidden.stride % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-    const int64_t blocks = std::min<int64_t>(div_up(static_cast<int64_t>(p.n) * div_up(p.width, 8), 256), 148 * 32);
-    return cuda_error(launch(bf16 ? hidden_grad_kernel<true> : hidden_grad_kernel<false>, blocks, 256, 0, c.stream, sums, p.cols, w.shared, w.rows, p.n, p.width, out,
-                             c.d_hidden.stride, wide));
+    if (!c.d_hidden.data || within) return nullptr;
+    return cuda_error(launch(bf16 ? hidden_grad_kernel<true> : hidden_grad_kernel<false>, std::min<int64_t>(div_up(lines, 512), 148 * 16), 256, 0, c.stream, h, a.shared));
 }
 
 }  // namespace gtok

@@ -30,11 +30,11 @@ struct LossCall {
     float* losses = nullptr;     // forward: [n]
     float* lse = nullptr;        // forward, written; backward, read: [n]
     float* total = nullptr;      // forward, optional: their sum,
-    bool mean = false;           // or the mean over the rows that have a loss
-    const float* grad = nullptr; // backward: of `losses` (grad_stride 1, or 0 for one value), or of the mean
+    bool mean = false;           // or the mean over the rows that have a loss; backward: `grad` is of that mean
+    const float* grad = nullptr; // backward: of `losses`, grad_stride apart, or of their sum or mean (grad_stride 0)
     int64_t grad_stride = 1;
-    bool grad_of_mean = false;
     Matrix d_hidden, d_weight;   // backward, either may have no data
+    void* kept = nullptr;        // optional: what the forward pass leaves there the backward one does not do again
     void* workspace = nullptr;
     uint64_t workspace_bytes = 0;
     cudaStream_t stream = nullptr;
@@ -44,6 +44,7 @@ constexpr int kMaxEntries = 1024;
 
 // NULL or an error message.  Arguments are checked by the caller; `stream` must belong to the current device.
 uint64_t loss_workspace(const LossCall& c, bool backward);
+uint64_t loss_kept(const LossCall& c);
 const char* loss_forward(const LossCall& c);
 const char* loss_backward(const LossCall& c);
 

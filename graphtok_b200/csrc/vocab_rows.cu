@@ -34,36 +34,61 @@ struct alignas(sizeof(T) * N) Lump {
 // out[t, :] = scale * table[id_t, :]; a negative id gives a row of zeros, an id beyond the table a row of NaN.  Bound by memory.  The output is
 // cut into lumps whatever its width; each thread has four of them, 256 apart, under way at once, and writes past the caches, which are
 // better used for rows that are asked for again.
+// A lump as it is loaded and stored; its elements unpacked only where they are added (kept apart, eight take twice the registers).
+template <typename T, int N> struct RawOf { using type = T; };
+template <> struct RawOf<float, 4> { using type = uint4; };
+template <> struct RawOf<__nv_bfloat16, 8> { using type = uint4; };
+template <> struct RawOf<__half, 8> { using type = uint4; };
 template <typename T, int N>
-__device__ __forceinline__ void scale_lump(Lump<T, N>& v, float scale) {
-    if constexpr (N == 8) {             // two elements of 16 bits at a time
-        using Pair = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
-        Pair* pair = reinterpret_cast<Pair*>(&v);
+__device__ __forceinline__ void unpack(float (&f)[N], const typename RawOf<T, N>::type& raw) {
+    if constexpr (N == 8) {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (std::is_same_v<T, __half>) {
-                const float2 f = __half22float2(pair[i]);
-                pair[i] = __floats2half2_rn(scale * f.x, scale * f.y);
-            } else {
-                const float2 f = __bfloat1622float2(pair[i]);
-                pair[i] = __floats2bfloat162_rn(scale * f.x, scale * f.y);
+                const float2 p = __half22float2(reinterpret_cast<const __half2&>(w[i]));
+                f[2 * i] = p.x; f[2 * i + 1] = p.y;
+            } else {              // bf16 is the upper half of fp32
+                f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
             }
         }
+    } else if constexpr (N == 4) {
+        f[0] = __uint_as_float(raw.x); f[1] = __uint_as_float(raw.y); f[2] = __uint_as_float(raw.z); f[3] = __uint_as_float(raw.w);
     } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v.v[i] = from_float<T>(scale * to_float<T>(v.v[i]));
+        f[0] = to_float<T>(raw);
     }
 }
 template <typename T, int N>
-__device__ __forceinline__ void write_past(Lump<T, N>* to, const Lump<T, N>& v) {
-    if constexpr (sizeof(Lump<T, N>) == 16) __stcs(reinterpret_cast<uint4*>(to), reinterpret_cast<const uint4&>(v));
+__device__ __forceinline__ typename RawOf<T, N>::type pack(const float (&f)[N]) {
+    if constexpr (N == 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same_v<T, __half>) {
+                const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+                w[i] = reinterpret_cast<const uint32_t&>(p);
+            } else {
+                const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+                w[i] = reinterpret_cast<const uint32_t&>(p);
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    } else if constexpr (N == 4) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    } else {
+        return from_float<T>(f[0]);
+    }
+}
+template <typename Raw>
+__device__ __forceinline__ void write_past(Raw* to, const Raw& v) {
+    if constexpr (sizeof(Raw) == 16) __stcs(to, v);
     else *to = v;
 }
 
 template <typename T, int N>
 __global__ void __launch_bounds__(256) embed_kernel(const void* ids, int bits, int64_t n, const T* table, int64_t vocab, int64_t stride, uint32_t lumps, float scale, T* out,
                                                     int64_t out_stride) {
-    using L = Lump<T, N>;
+    using Raw = typename RawOf<T, N>::type;
     constexpr int kEach = 4;
     after_previous();
     let_next_begin();
@@ -73,7 +98,7 @@ __global__ void __launch_bounds__(256) embed_kernel(const void* ids, int bits, i
         const uint32_t first = static_cast<uint32_t>(block * (256 * kEach) - t0 * lumps) + threadIdx.x;
         int64_t t[kEach], id[kEach];
         uint32_t col[kEach];
-        L v[kEach];
+        Raw v[kEach];
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
             const uint32_t down = (first + 256 * k) / lumps;
@@ -83,18 +108,20 @@ __global__ void __launch_bounds__(256) embed_kernel(const void* ids, int bits, i
         }
 #pragma unroll
         for (int k = 0; k < kEach; ++k)
-            if (id[k] >= 0 && id[k] < vocab) v[k] = reinterpret_cast<const L*>(table + id[k] * stride)[col[k]];
+            if (id[k] >= 0 && id[k] < vocab) v[k] = reinterpret_cast<const Raw*>(table + id[k] * stride)[col[k]];
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
             if (t[k] >= n) continue;
+            float f[N];
             if (id[k] >= 0 && id[k] < vocab) {
-                scale_lump(v[k], scale);
-            } else {
-                const T other = from_float<T>(id[k] < 0 ? 0.f : __int_as_float(0x7FC00000));
+                unpack<T, N>(f, v[k]);
 #pragma unroll
-                for (int e = 0; e < N; ++e) v[k].v[e] = other;
+                for (int e = 0; e < N; ++e) f[e] *= scale;
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) f[e] = id[k] < 0 ? 0.f : __int_as_float(0x7FC00000);
             }
-            write_past(reinterpret_cast<L*>(out + t[k] * out_stride) + col[k], v[k]);
+            write_past(reinterpret_cast<Raw*>(out + t[k] * out_stride) + col[k], pack<T, N>(f));
         }
     }
 }
@@ -121,7 +148,7 @@ __global__ void next_kernel(const int32_t* ids, int64_t n, const int32_t* offset
 // joined from fp32 partial sums.
 //
 // Most of the gradient's bytes are rows that no id asks for.  The sort is a few short launches that leave memory idle: further blocks of
-// the same launches write these zeros meanwhile.
+// the same launches write these zeros meanwhile (the first two, before it is known which rows are asked for, all of a share).
 constexpr int kDigit = 9, kBins = 1 << kDigit;
 constexpr int kSortThreads = 256, kSortEach = 8, kSortTile = kSortThreads * kSortEach, kSortWarps = kSortThreads / 32;
 constexpr int kChunk = 32, kShortChunk = 8;
@@ -156,20 +183,20 @@ __device__ __forceinline__ void clear_row(char* row, int64_t bytes, int lane) {
     memset(&zero, 0, sizeof(U));
     for (int64_t i = lane; i < bytes / static_cast<int64_t>(sizeof(U)); i += 32) reinterpret_cast<U*>(row)[i] = zero;
 }
-// Warp `self` of `warps` clears its share of the rows [a.from, a.to).  `seen` begins at the bit of row `first`.
+// Warp `self` of `warps` clears its share of the rows [a.from, a.to).  `seen` begins at the bit of row `first`; without it, all of them.
 __device__ __forceinline__ void clear_rows(const SortArgs& a, const uint32_t* seen, int64_t first, int64_t from, int64_t to, int64_t self, int64_t warps) {
     const int lane = threadIdx.x & 31;
     for (int64_t r = from + self; r < to; r += warps) {
         const int64_t bit = r - first;
-        if (seen[bit >> 5] >> (bit & 31) & 1) continue;
+        if (seen && (seen[bit >> 5] >> (bit & 31) & 1)) continue;
         char* row = a.rows + r * a.row_stride;
         if (a.unit == 16) clear_row<uint4>(row, a.row_bytes, lane);
         else if (a.unit == 4) clear_row<uint32_t>(row, a.row_bytes, lane);
         else clear_row<uint16_t>(row, a.row_bytes, lane);
     }
 }
-__device__ __forceinline__ void clear_share(const SortArgs& a) {
-    clear_rows(a, a.seen, 0, a.from, a.to, static_cast<int64_t>(blockIdx.x - a.tiles) * kSortWarps + (threadIdx.x >> 5),
+__device__ __forceinline__ void clear_share(const SortArgs& a, bool all) {
+    clear_rows(a, all ? nullptr : a.seen, 0, a.from, a.to, static_cast<int64_t>(blockIdx.x - a.tiles) * kSortWarps + (threadIdx.x >> 5),
                static_cast<int64_t>(gridDim.x - a.tiles) * kSortWarps);
 }
 
@@ -178,7 +205,13 @@ __global__ void __launch_bounds__(kSortThreads) count_kernel(const __grid_consta
     __shared__ uint32_t bin[kBins];
     after_previous();
     let_next_begin();
-    if (!FIRST && static_cast<int>(blockIdx.x) >= a.tiles) return clear_share(a);
+    if (static_cast<int>(blockIdx.x) >= a.tiles) {
+        if (FIRST) {
+            const int64_t threads = static_cast<int64_t>(gridDim.x - a.tiles) * kSortThreads;
+            for (int64_t i = static_cast<int64_t>(blockIdx.x - a.tiles) * kSortThreads + threadIdx.x; i < (a.vocab + 31) / 32; i += threads) a.seen[i] = 0;
+        }
+        return clear_share(a, FIRST);
+    }
     for (int b = threadIdx.x; b < kBins; b += kSortThreads) bin[b] = 0;
     __syncthreads();
     const int64_t from = static_cast<int64_t>(blockIdx.x) * kSortTile;
@@ -192,7 +225,6 @@ __global__ void __launch_bounds__(kSortThreads) count_kernel(const __grid_consta
     for (int i = 0; i < kSortEach; ++i) {
         if (from + i * kSortThreads + threadIdx.x >= a.n) continue;
         atomicAdd(&bin[key[i] >> a.shift & (kBins - 1)], 1u);
-        if (FIRST && key[i] < a.vocab) atomicOr(&a.seen[key[i] >> 5], 1u << (key[i] & 31));
     }
     __syncthreads();
     for (int b = threadIdx.x; b < kBins; b += kSortThreads) a.counts[static_cast<int64_t>(blockIdx.x) * kBins + b] = bin[b];
@@ -255,7 +287,7 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(const __grid_cons
     __shared__ SortSpace s;
     after_previous();
     let_next_begin();
-    if (static_cast<int>(blockIdx.x) >= a.tiles) return clear_share(a);
+    if (static_cast<int>(blockIdx.x) >= a.tiles) return clear_share(a, FIRST);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t from = static_cast<int64_t>(blockIdx.x) * kSortTile + warp * 32 * kSortEach;
     Key key[kSortEach];
@@ -286,6 +318,7 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(const __grid_cons
     for (int i = 0; i < kSortEach; ++i) {
         if (!here[i]) continue;
         const uint32_t b = key[i].id >> a.shift & (kBins - 1);
+        if (FIRST && key[i].id < a.vocab) atomicOr(&a.seen[key[i].id >> 5], 1u << (key[i].id & 31));
         a.out[s.base[b] + s.warp_bin[warp][b] + rank[i]] = key[i];
     }
 }
@@ -354,26 +387,33 @@ __global__ void __launch_bounds__(kSortThreads) one_tile_kernel(const __grid_con
 
 template <typename T, int N>
 __device__ __forceinline__ void put_row(T* out, int64_t at, const float (&sum)[N], float scale, bool accumulate) {
-    using L = Lump<T, N>;
-    L* to = reinterpret_cast<L*>(out + at);
-    L v;
-    if (accumulate) v = *to;
+    using Raw = typename RawOf<T, N>::type;
+    Raw* to = reinterpret_cast<Raw*>(out + at);
+    float v[N];
+    if (accumulate) {
+        unpack<T, N>(v, *to);
 #pragma unroll
-    for (int e = 0; e < N; ++e) v.v[e] = from_float<T>(accumulate ? to_float<T>(v.v[e]) + scale * sum[e] : scale * sum[e]);
-    *to = v;
+        for (int e = 0; e < N; ++e) v[e] += scale * sum[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = scale * sum[e];
+    }
+    *to = pack<T, N>(v);
 }
 
 // Sums of the runs in a chunk, one warp a chunk and 32 lumps of columns; then a share of the rows to be cleared.
+constexpr int kFlight = 4;      // (8: more registers, fewer warps, slower by a tenth)
 template <typename T, int N>
-__global__ void __launch_bounds__(256) sum_kernel(const Key* keys, int64_t n, uint32_t vocab, const T* grad, int64_t stride, int lumps, float scale, T* out,
+__global__ void __launch_bounds__(256, 3) sum_kernel(const Key* keys, int64_t n, uint32_t vocab, const T* grad, int64_t stride, int lumps, float scale, T* out,
                                                   int64_t out_stride, bool accumulate, float* partial, int64_t partial_cols, int slices,
                                                   int in_chunk, const __grid_constant__ SortArgs sort) {
     after_previous();
     let_next_begin();
-    using L = Lump<T, N>;
-    const int lane = threadIdx.x & 31;
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32), self = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5);
+    using Raw = typename RawOf<T, N>::type;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32), self = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + warp;
     const int64_t chunks = (n + in_chunk - 1) / in_chunk;
+    if (warp & 1) clear_rows(sort, sort.seen, 0, sort.from, sort.to, self, warps);      // half of the warps write while the others read
     for (int64_t u = self; u < chunks * slices; u += warps) {
         const int64_t chunk = u / slices;
         const int col = (static_cast<int>(u - chunk * slices) * 32 + lane);
@@ -387,49 +427,47 @@ __global__ void __launch_bounds__(256) sum_kernel(const Key* keys, int64_t n, ui
         for (int e = 0; e < N; ++e) sum[e] = 0.f;
         uint32_t run = __shfl_sync(~0u, mine.id, 0);
         bool open = run == before;                 // the run began in an earlier chunk
-        bool whole_front = true;                   // it begins where the chunk does
-        for (int i = 0; i < count; i += 8) {
-            L v[8];
+        int slot = 0;                              // of its part; 1 behind the first run
+        auto put = [&](bool to_partial) {
+            if (!here || run >= vocab) return;
+            if (to_partial) {
+                float* to = partial + (chunk * 2 + slot) * partial_cols + static_cast<int64_t>(col) * N;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const uint32_t id = __shfl_sync(~0u, mine.id, (i + k) & 31), place = __shfl_sync(~0u, mine.place, (i + k) & 31);
-                if (here && i + k < count && id < vocab) v[k] = reinterpret_cast<const L*>(grad + static_cast<int64_t>(place) * stride)[col];
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                if (i + k >= count) break;
-                const uint32_t id = __shfl_sync(~0u, mine.id, i + k);
-                if (id != run) {
-                    if (here && run < vocab) {
-                        if (open) {
-#pragma unroll
-                            for (int e = 0; e < N; ++e) partial[(chunk * 2) * partial_cols + static_cast<int64_t>(col) * N + e] = sum[e];
-                        } else {
-                            put_row<T, N>(out, run * out_stride + static_cast<int64_t>(col) * N, sum, scale, accumulate);
-                        }
-                    }
-#pragma unroll
-                    for (int e = 0; e < N; ++e) sum[e] = 0.f;
-                    run = id;
-                    open = whole_front = false;
-                }
-                if (here && id < vocab) {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) sum[e] += to_float<T>(v[k].v[e]);
-                }
-            }
-        }
-        if (here && run < vocab) {
-            if (open || run == after) {
-                const int64_t slot = chunk * 2 + (whole_front ? 0 : 1);
-#pragma unroll
-                for (int e = 0; e < N; ++e) partial[slot * partial_cols + static_cast<int64_t>(col) * N + e] = sum[e];
+                for (int e = 0; e < N; ++e) to[e] = sum[e];
             } else {
                 put_row<T, N>(out, run * out_stride + static_cast<int64_t>(col) * N, sum, scale, accumulate);
             }
+        };
+        for (int i = 0; i < count; i += kFlight) {
+            Raw v[kFlight];
+#pragma unroll
+            for (int k = 0; k < kFlight; ++k) {
+                const uint32_t id = __shfl_sync(~0u, mine.id, (i + k) & 31), place = __shfl_sync(~0u, mine.place, (i + k) & 31);
+                if (here && i + k < count && id < vocab) v[k] = reinterpret_cast<const Raw*>(grad + static_cast<int64_t>(place) * stride)[col];
+            }
+#pragma unroll
+            for (int k = 0; k < kFlight; ++k) {
+                if (i + k >= count) break;
+                const uint32_t id = __shfl_sync(~0u, mine.id, i + k);
+                if (id != run) {
+                    put(open);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) sum[e] = 0.f;
+                    run = id;
+                    open = false;
+                    slot = 1;
+                }
+                if (here && id < vocab) {
+                    float f[N];
+                    unpack<T, N>(f, v[k]);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) sum[e] += f[e];
+                }
+            }
         }
+        put(open || run == after);
     }
-    clear_rows(sort, sort.seen, 0, sort.from, sort.to, self, warps);
+    if (!(warp & 1)) clear_rows(sort, sort.seen, 0, sort.from, sort.to, self, warps);
 }
 
 // Runs across chunks: the warp of the chunk where one begins adds its parts up, in order.
@@ -581,8 +619,8 @@ const char* embed_grad(const Ids& ids, int64_t n, const Matrix& grad, float scal
     s.row_bytes = out.cols * size;
     s.row_stride = out.stride * size;
     s.unit = wide_rows(out) ? 16 : size;
-    // Rows cleared beside the other work of a launch: what memory takes in the time of a launch of the sort, some 8 us.
-    const int64_t rows_at_once = std::max<int64_t>(1, (48 << 20) / s.row_bytes), all = accumulate ? 0 : out.rows;
+    // Rows cleared beside the other work of a launch: what memory takes in the time of a launch of the sort, some 11 us.
+    const int64_t rows_at_once = std::max<int64_t>(1, (72 << 20) / s.row_bytes), all = accumulate ? 0 : out.rows;
     auto clearing = [&](int64_t blocks) {
         s.from = s.to;
         s.to = std::min(all, s.from + rows_at_once);
@@ -594,16 +632,17 @@ const char* embed_grad(const Ids& ids, int64_t n, const Matrix& grad, float scal
         s.to = std::min(all, 2 * rows_at_once);
         e = launch(one_tile_kernel, 1 + std::min<int64_t>(div_up(s.to, kSortWarps), 148 * 6), kSortThreads, 0, stream, s);
     } else {
-        e = cudaMemsetAsync(s.seen, 0, div_up(out.rows, 32) * 4, stream);
         for (int pass = 0; pass < p.passes && p.tiles && e == cudaSuccess; ++pass) {
             s.in = keys;
             s.out = pass ? other : keys;
             s.shift = pass * kDigit;
-            e = pass ? launch(count_kernel<false>, clearing(p.tiles), kSortThreads, 0, stream, s) : launch(count_kernel<true>, p.tiles, kSortThreads, 0, stream, s);
+            // (one block at least to clear `seen`)
+            e = launch(pass ? count_kernel<false> : count_kernel<true>, std::max(clearing(p.tiles), p.tiles + 1), kSortThreads, 0, stream, s);
             if (e != cudaSuccess) break;
             e = launch(pass ? scatter_kernel<false> : scatter_kernel<true>, clearing(p.tiles), kSortThreads, 0, stream, s);
             if (pass) std::swap(keys, other);
         }
+        if (!p.tiles) e = cudaMemsetAsync(s.seen, 0, div_up(out.rows, 32) * 4, stream);
     }
     if (e != cudaSuccess) return cudaGetErrorString(e);
     switch (out.type) {

@@ -37,7 +37,7 @@ class _Loss(ctypes.Structure):
                 ("target_bits", ctypes.c_int32), ("entries", ctypes.c_int32), ("teacher_logits", _Matrix), ("ignore", ctypes.c_int64),
                 ("temperature", ctypes.c_float), ("mean", ctypes.c_int32), ("losses", ctypes.c_void_p), ("lse", ctypes.c_void_p),
                 ("total", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("grad_stride", ctypes.c_int64), ("d_hidden", _Matrix),
-                ("d_weight", _Matrix), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("cuda_stream", ctypes.c_void_p)]
+                ("d_weight", _Matrix), ("kept", ctypes.c_void_p), ("kept_bytes", ctypes.c_uint64), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("cuda_stream", ctypes.c_void_p)]
 
 
 _bound = None
@@ -58,6 +58,8 @@ def _lib():
         lib.gtok_x_next_targets.argtypes = [vp, i64, vp, i64, vp, i32, vp, vp]
         lib.gtok_x_vocab_loss_workspace.restype = i64
         lib.gtok_x_vocab_loss_workspace.argtypes = [ctypes.POINTER(_Loss), i32]
+        lib.gtok_x_vocab_loss_kept.restype = i64
+        lib.gtok_x_vocab_loss_kept.argtypes = [ctypes.POINTER(_Loss)]
         for f in (lib.gtok_x_vocab_loss_forward, lib.gtok_x_vocab_loss_backward):
             f.restype = i32
             f.argtypes = [ctypes.POINTER(_Loss)]
@@ -259,34 +261,56 @@ class _Call:
         temperature = float(temperature)
         if not (temperature > 0.0 and math.isfinite(temperature)):
             raise ValueError("temperature must be positive and finite")
-        self.hidden, self.weight, self.ids = _flat(hidden), _rows(weight), _ids_of(what, ids)
-        if self.weight.stride(0) < self.weight.shape[1] and self.weight.shape[0] > 1:
-            self.weight = self.weight.contiguous()
+        self.hidden, self.ids = _flat(hidden), _ids_of(what, ids)
         a = self.args = _Loss()
-        a.hidden, a.weight = _matrix(self.hidden), _matrix(self.weight)
+        a.hidden = _matrix(self.hidden)
+        self._take(weight)
         a.targets, a.target_bits, a.ignore, a.temperature = self.ids.data_ptr(), _IDS[ids.dtype], ignore_index, temperature
         if teacher_logits is not None:
             k = ids.shape[-1]
             self.logits = _flat(teacher_logits)
             a.entries, a.target_stride, a.teacher_logits = k, k, _matrix(self.logits)
 
+    def _take(self, weight):
+        self.weight = _rows(weight)
+        if self.weight.stride(0) < self.weight.shape[1] and self.weight.shape[0] > 1:
+            self.weight = self.weight.contiguous()
+        self.args.weight = _matrix(self.weight)
+
+    def _keep(self, kept):
+        self.kept = kept
+        self.args.kept, self.args.kept_bytes = kept.data_ptr(), kept.numel()
+
+    def let_go(self):
+        """Forgets the tensors, for a call that waits for its backward pass; `again` is that pass's."""
+        self.hidden = self.ids = self.logits = self.weight = self.kept = None
+
+    def again(self, weight, kept):
+        call = object.__new__(_Call)
+        call.index, call.args = self.index, _Loss.from_buffer_copy(self.args)
+        call._take(weight)
+        call._keep(kept)
+        return call
+
     def _run(self, entry, backward):
         a = self.args
         need = _done(_lib().gtok_x_vocab_loss_workspace(a, backward), "gtok_x_vocab_loss_workspace")
-        work = torch.empty(need, dtype=torch.uint8, device=self.hidden.device)
+        work = torch.empty(need, dtype=torch.uint8, device=self.weight.device)
         a.workspace, a.workspace_bytes, a.cuda_stream = work.data_ptr(), need, _stream(self.index)
         _done(entry(a), entry.__name__)
 
-    def forward(self, reduction):
-        return _there(self.index, self._forward, reduction)
+    def forward(self, reduction, keep=False):
+        return _there(self.index, self._forward, reduction, keep)
 
-    def _forward(self, reduction):
+    def _forward(self, reduction, keep):
         a, n, device = self.args, self.hidden.shape[0], self.hidden.device
         losses, lse = torch.empty(n, dtype=torch.float32, device=device), torch.empty(n, dtype=torch.float32, device=device)
         a.losses, a.lse = losses.data_ptr(), lse.data_ptr()
         if reduction != "none":
             total = torch.empty((), dtype=torch.float32, device=device)
             a.total, a.mean, losses = total.data_ptr(), reduction == "mean", total
+        if keep:
+            self._keep(torch.empty(_done(_lib().gtok_x_vocab_loss_kept(a), "gtok_x_vocab_loss_kept"), dtype=torch.uint8, device=device))
         self._run(_lib().gtok_x_vocab_loss_forward, 0)
         return losses, lse
 
@@ -302,7 +326,7 @@ class _Call:
         a.lse, a.grad, a.mean = lse.data_ptr(), grad.data_ptr(), reduction == "mean"
         d_hidden = d_weight = None
         if want_hidden:
-            d_hidden = self.hidden.new_empty(self.hidden.shape, requires_grad=False)
+            d_hidden = self.weight.new_empty((a.hidden.rows, a.hidden.cols), requires_grad=False)
             a.d_hidden = _matrix(d_hidden)
         if want_weight:
             d_weight = self.weight.new_empty(self.weight.shape, requires_grad=False)
@@ -326,29 +350,30 @@ def _check_grad(lse, grad, lead, reduction, hidden):
 
 
 class _LossFunction(torch.autograd.Function):
+    """Keeps the forward pass's copy of the rows that have a loss in place of the hidden states."""
+
     @staticmethod
-    def forward(ctx, call, hidden, weight, ids, teacher_logits, reduction):
-        loss, lse = call.forward(reduction)
-        ctx.save_for_backward(hidden, weight, ids, teacher_logits, lse)
-        ctx.rest = reduction, call.args.ignore, call.args.temperature
+    def forward(ctx, call, hidden, weight, reduction):
+        loss, lse = call.forward(reduction, keep=True)
+        ctx.save_for_backward(weight, lse, call.kept)
+        ctx.call, ctx.reduction, ctx.shape = call, reduction, hidden.shape
+        call.let_go()
         return loss.view(hidden.shape[:-1]) if reduction == "none" else loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        hidden, weight, ids, teacher_logits, lse = ctx.saved_tensors
-        reduction, ignore_index, temperature = ctx.rest
-        _, want_hidden, want_weight, _, _, _ = ctx.needs_input_grad
-        call = _Call(hidden, weight, ids, teacher_logits, ignore_index, temperature)
-        d_hidden, d_weight = call.backward(lse, grad, reduction, want_hidden, want_weight)
-        return None, d_hidden.view(hidden.shape) if want_hidden else None, d_weight, None, None, None
+        weight, lse, kept = ctx.saved_tensors
+        _, want_hidden, want_weight, _ = ctx.needs_input_grad
+        d_hidden, d_weight = ctx.call.again(weight, kept).backward(lse, grad, ctx.reduction, want_hidden, want_weight)
+        return None, d_hidden.view(ctx.shape) if want_hidden else None, d_weight, None
 
 
 def _loss(hidden, weight, ids, teacher_logits, reduction, ignore_index, temperature):
     _check_reduction(reduction)
     call = _Call(hidden, weight, ids, teacher_logits, ignore_index, temperature)
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        return _LossFunction.apply(call, hidden, weight, ids, teacher_logits, reduction)
+        return _LossFunction.apply(call, hidden, weight, reduction)
     loss, _ = call.forward(reduction)
     return loss.view(hidden.shape[:-1]) if reduction == "none" else loss
 

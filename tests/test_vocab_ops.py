@@ -3,6 +3,7 @@
 How far a result may be off is counted from roundings: u = eps / 2 of a type is half a step relative to the value.  A sum of tensor-core
 products loses at most a step of fp32 (2^-23) of its largest partial sum every 16 elements."""
 import math
+import threading
 
 import pytest
 import torch
@@ -540,6 +541,32 @@ def test_on_another_stream_and_captured(ops):
         torch.cuda.synchronize()
         for got in [eager] + [outs for _, outs in graphs]:
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_from_a_thread_of_its_own(ops):
+    """A backward pass in a thread that has not used the GPU yet, as torch's own for backward passes; two at once, and one a second time."""
+    hidden, weight, targets, g = make(44, 40, 1000, 64, BF16, masked=0)
+    losses, lse = ops.cross_entropy_forward(hidden, weight, targets)
+    want = ops.cross_entropy_grad(hidden, weight, targets, lse, g)
+    h, w = hidden.clone().requires_grad_(), weight.clone().requires_grad_()
+    loss = ops.cross_entropy(h, w, targets, reduction="none")
+    torch.cuda.synchronize()
+    got = [None] * 3
+    def run(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got[i] = ops.cross_entropy_grad(hidden, weight, targets, lse, g) if i else torch.autograd.grad(loss, (h, w), g, retain_graph=True)
+        stream.synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    h.detach().zero_()                  # the graph keeps what it needs of it
+    got.append(torch.autograd.grad(loss, (h, w), g))
+    torch.cuda.synchronize()
+    for pair in got:
+        assert all(torch.equal(a, b) for a, b in zip(pair, want))
 
 
 def test_refusals(ops):
