@@ -631,12 +631,13 @@ __global__ void teacher_kernel(Ids ids, Matrix logits, int entries, int room, in
 }
 
 // Time in ns of the hidden gradient's part of a piece in `s` splits: `outs` tiles of it over `blocks` steps of the summed dimension.  A step
-// of a tile takes 270, beginning and ending one 700, and each split costs its way to memory and back.
+// of a tile takes 270, beginning and ending one 700, and each split costs its way to memory and back.  No more splits than make eight rounds of
+// the pairs, and eight steps each: they would gain nothing, and their sums take room.  (The best of 32 is looked for, by a lane each.)
+constexpr int kSplitRounds = 8;
 __host__ __device__ inline int64_t split_time(int s, int64_t outs, int blocks, int pairs) {
-    if (s > 1 && s * 8 > blocks) return INT64_MAX;
+    if (s > 1 && (s * 8 > blocks || outs * s > kSplitRounds * pairs)) return INT64_MAX;
     return (outs * s + pairs - 1) / pairs * (270 * blocks / s + 700) + 90 * s * outs;
 }
-constexpr int kMaxSplits = 32;
 
 struct RowsArgs {
     Ids targets;
@@ -752,7 +753,8 @@ __global__ void __launch_bounds__(1024) scale_kernel(const __grid_constant__ Sca
     // dZ is kept with the largest row gradient as 1 (bf16: its range is fp32's) or as 2^15, so that fp16 holds probabilities
     // down to 2^-29 in full precision and nothing above 2^16.
     const float unit = a.half ? 32768.f : 1.f;
-    const float row_scale = top == 0.f ? 0.f : unit / top;
+    top = top < 0x1p-100f ? 0x1p-100f : top;
+    const float row_scale = unit / top;
     for (int base = tid; base < active; base += 8 * 1024) {
         RowInfo r[8];
 #pragma unroll
@@ -1009,12 +1011,7 @@ Plan make_plan(const LossCall& c, bool backward) {
         const int64_t room = std::max<int64_t>(1, kDeltaBytes / (2ll * kTile * p.n_rows));
         p.piece = static_cast<int>(div_up(tiles, div_up(tiles, room)) * kTile);
         const int64_t width_tiles = div_up(p.cols, kTile);
-        for (int64_t t = 1; t <= p.n_rows / kTile; ++t) {
-            int splits = 1;
-            for (int k = 2; k <= kMaxSplits; ++k)
-                if (split_time(k, t * width_tiles, p.piece / kDepth, p.pairs) < split_time(splits, t * width_tiles, p.piece / kDepth, p.pairs)) splits = k;
-            p.sum_rows = std::max(p.sum_rows, t * kTile * splits);
-        }
+        p.sum_rows = std::max<int64_t>(p.n_rows, kSplitRounds * p.pairs / width_tiles * kTile);
         p.delta = take(2ull * p.n_rows * p.piece);
         p.sums = take(4ull * p.sum_rows * p.cols);
     }

@@ -230,6 +230,44 @@ __global__ void __launch_bounds__(kSortThreads) count_kernel(const __grid_consta
     for (int b = threadIdx.x; b < kBins; b += kSortThreads) a.counts[static_cast<int64_t>(blockIdx.x) * kBins + b] = bin[b];
 }
 
+// Many tiles: their counts of each bin become sums over the tiles before, and a row behind them the totals.  32 bins a block.
+constexpr int kFewTiles = 32;           // up to here each tile adds them up by itself; 4 steps of loads, as long as this launch
+__global__ void __launch_bounds__(1024) prefix_kernel(uint32_t* counts, int64_t tiles) {
+    constexpr int kEach = 8;
+    __shared__ uint32_t sums[32][33];
+    after_previous();
+    let_next_begin();
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    uint32_t* column = counts + blockIdx.x * 32 + x;
+    uint32_t done = 0;
+    for (int64_t base = 0; base < tiles; base += 32 * kEach) {
+        uint32_t c[kEach], mine = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int64_t t = base + y * kEach + i;
+            c[i] = t < tiles ? column[t * kBins] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) mine += c[i];
+        __syncthreads();
+        sums[y][x] = mine;
+        __syncthreads();
+        uint32_t before = done;
+        for (int r = 0; r < 32; ++r) {
+            const uint32_t v = sums[r][x];
+            if (r < y) before += v;
+            done += v;
+        }
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int64_t t = base + y * kEach + i;
+            if (t < tiles) column[t * kBins] = before;
+            before += c[i];
+        }
+    }
+    if (y == 0) column[tiles * kBins] = done;
+}
+
 struct SortSpace {
     uint32_t base[kBins];
     uint16_t warp_bin[kSortWarps][kBins];
@@ -302,7 +340,11 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(const __grid_cons
     // how many keys of this thread's two bins there are: in all tiles, and in those before this one
     uint2 all = make_uint2(0, 0), mine = make_uint2(0, 0);
     const uint2* counts = reinterpret_cast<const uint2*>(a.counts);
-    for (int t = 0; t < a.tiles; t += 8) {
+    if (a.tiles > kFewTiles) {
+        mine = counts[static_cast<int64_t>(blockIdx.x) * (kBins / 2) + tid];
+        all = counts[static_cast<int64_t>(a.tiles) * (kBins / 2) + tid];
+    }
+    for (int t = 0; t < a.tiles && a.tiles <= kFewTiles; t += 8) {
         uint2 c[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) c[k] = t + k < a.tiles ? counts[static_cast<int64_t>(t + k) * (kBins / 2) + tid] : make_uint2(0, 0);
@@ -443,7 +485,11 @@ __global__ void __launch_bounds__(256, 3) sum_kernel(const Key* keys, int64_t n,
 #pragma unroll
             for (int k = 0; k < kFlight; ++k) {
                 const uint32_t id = __shfl_sync(~0u, mine.id, (i + k) & 31), place = __shfl_sync(~0u, mine.place, (i + k) & 31);
-                if (here && i + k < count && id < vocab) v[k] = reinterpret_cast<const Raw*>(grad + static_cast<int64_t>(place) * stride)[col];
+                if (here && i + k < count && id < vocab) {
+                    v[k] = reinterpret_cast<const Raw*>(grad + static_cast<int64_t>(place) * stride)[col];
+                    // what a run's sum will be added to comes nearer meanwhile
+                    if (accumulate) asm volatile("prefetch.global.L2 [%0];" ::"l"(out + id * out_stride + static_cast<int64_t>(col) * N));
+                }
             }
 #pragma unroll
             for (int k = 0; k < kFlight; ++k) {
@@ -555,7 +601,7 @@ GradPlan grad_plan(int64_t n, int64_t vocab, int64_t width) {
         return from;
     };
     p.seen = take(div_up(vocab, 32) * 4);
-    p.counts = take(p.tiles * kBins * 4);
+    p.counts = take((p.tiles + 1) * kBins * 4);
     p.a = take(n * sizeof(Key));
     p.b = take(n * sizeof(Key));
     p.partial = take(static_cast<uint64_t>(p.chunks) * 2 * round_up(width, 8) * 4);
@@ -638,6 +684,7 @@ const char* embed_grad(const Ids& ids, int64_t n, const Matrix& grad, float scal
             s.shift = pass * kDigit;
             // (one block at least to clear `seen`)
             e = launch(pass ? count_kernel<false> : count_kernel<true>, std::max(clearing(p.tiles), p.tiles + 1), kSortThreads, 0, stream, s);
+            if (e == cudaSuccess && p.tiles > kFewTiles) e = launch(prefix_kernel, kBins / 32, 1024, 0, stream, s.counts, p.tiles);
             if (e != cudaSuccess) break;
             e = launch(pass ? scatter_kernel<false> : scatter_kernel<true>, clearing(p.tiles), kSortThreads, 0, stream, s);
             if (pass) std::swap(keys, other);
