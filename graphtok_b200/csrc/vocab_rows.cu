@@ -150,7 +150,7 @@ __global__ void next_kernel(const int32_t* ids, int64_t n, const int32_t* offset
 // Most of the gradient's bytes are rows that no id asks for.  The sort is a few short launches that leave memory idle: further blocks of
 // the same launches write these zeros meanwhile (the first two, before it is known which rows are asked for, all of a share).
 constexpr int kDigit = 9, kBins = 1 << kDigit;
-constexpr int kSortThreads = 256, kSortEach = 8, kSortTile = kSortThreads * kSortEach, kSortWarps = kSortThreads / 32;
+constexpr int kSortThreads = kBins, kSortEach = 4, kSortTile = kSortThreads * kSortEach, kSortWarps = kSortThreads / 32;
 constexpr int kChunk = 32, kShortChunk = 8;
 
 struct Key { uint32_t id, place; };
@@ -274,13 +274,14 @@ struct SortSpace {
     uint32_t warp_sum[kSortWarps];
 };
 
-// Places of a tile's keys (256 a warp, in order) after one digit: `key` to s.base[bin] + s.warp_bin[warp][bin] + rank.  With `all` and `mine`, the
-// keys of a thread's two bins in all tiles and in those before; without, the tile is all there is.
+// Places of a tile's keys (128 a warp, in order) after one digit: `key` to s.base[bin] + s.warp_bin[warp][bin] + rank.  `all` and `before`: keys of this
+// thread's bin in all tiles and in those before; with `alone` the tile is all there is.
 __device__ __forceinline__ void rank_keys(SortSpace& s, const Key (&key)[kSortEach], const bool (&here)[kSortEach], uint16_t (&rank)[kSortEach], int shift,
-                                          bool alone, uint32_t all0, uint32_t all1, uint32_t mine0, uint32_t mine1) {
+                                          bool alone, uint32_t all, uint32_t before) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     __syncthreads();
-    for (int b = tid; b < kSortWarps * kBins; b += kSortThreads) (&s.warp_bin[0][0])[b] = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) s.warp_bin[w][tid] = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kSortEach; ++i) {
@@ -293,20 +294,15 @@ __device__ __forceinline__ void rank_keys(SortSpace& s, const Key (&key)[kSortEa
         __syncwarp();
     }
     __syncthreads();
-    uint32_t total[2];
+    uint32_t total = 0;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        uint32_t run = 0;
-#pragma unroll
-        for (int w = 0; w < kSortWarps; ++w) {
-            const uint32_t c = s.warp_bin[w][2 * tid + k];
-            s.warp_bin[w][2 * tid + k] = static_cast<uint16_t>(run);
-            run += c;
-        }
-        total[k] = run;
+    for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = s.warp_bin[w][tid];
+        s.warp_bin[w][tid] = static_cast<uint16_t>(total);
+        total += c;
     }
-    if (alone) { all0 = total[0]; all1 = total[1]; }
-    uint32_t scan = all0 + all1;
+    if (alone) all = total;
+    uint32_t scan = all;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const uint32_t y = __shfl_up_sync(~0u, scan, d);
@@ -314,9 +310,10 @@ __device__ __forceinline__ void rank_keys(SortSpace& s, const Key (&key)[kSortEa
     }
     if (lane == 31) s.warp_sum[warp] = scan;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) scan += s.warp_sum[w];
-    s.base[2 * tid] = scan - all0 - all1 + mine0;
-    s.base[2 * tid + 1] = scan - all1 + mine1;
+    uint32_t low = lane < warp ? s.warp_sum[lane] : 0;          // kSortWarps are no more than the lanes
+#pragma unroll
+    for (int d = 16; d; d >>= 1) low += __shfl_xor_sync(~0u, low, d);
+    s.base[tid] = low + scan - all + before;
     __syncthreads();
 }
 
@@ -337,25 +334,23 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(const __grid_cons
         here[i] = at < a.n;
         key[i] = here[i] ? (FIRST ? Key{key_of(a, at), static_cast<uint32_t>(at)} : a.in[at]) : Key{0xFFFFFFFFu, 0};
     }
-    // how many keys of this thread's two bins there are: in all tiles, and in those before this one
-    uint2 all = make_uint2(0, 0), mine = make_uint2(0, 0);
-    const uint2* counts = reinterpret_cast<const uint2*>(a.counts);
+    // how many keys of this thread's bin there are: in all tiles, and in those before this one
+    uint32_t all = 0, before = 0;
     if (a.tiles > kFewTiles) {
-        mine = counts[static_cast<int64_t>(blockIdx.x) * (kBins / 2) + tid];
-        all = counts[static_cast<int64_t>(a.tiles) * (kBins / 2) + tid];
+        before = a.counts[static_cast<int64_t>(blockIdx.x) * kBins + tid];
+        all = a.counts[static_cast<int64_t>(a.tiles) * kBins + tid];
     }
     for (int t = 0; t < a.tiles && a.tiles <= kFewTiles; t += 8) {
-        uint2 c[8];
+        uint32_t c[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) c[k] = t + k < a.tiles ? counts[static_cast<int64_t>(t + k) * (kBins / 2) + tid] : make_uint2(0, 0);
+        for (int k = 0; k < 8; ++k) c[k] = t + k < a.tiles ? a.counts[static_cast<int64_t>(t + k) * kBins + tid] : 0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            if (t + k < static_cast<int>(blockIdx.x)) { mine.x += c[k].x; mine.y += c[k].y; }
-            all.x += c[k].x;
-            all.y += c[k].y;
+            if (t + k < static_cast<int>(blockIdx.x)) before += c[k];
+            all += c[k];
         }
     }
-    rank_keys(s, key, here, rank, a.shift, false, all.x, all.y, mine.x, mine.y);
+    rank_keys(s, key, here, rank, a.shift, false, all, before);
 #pragma unroll
     for (int i = 0; i < kSortEach; ++i) {
         if (!here[i]) continue;
@@ -411,7 +406,7 @@ __global__ void __launch_bounds__(kSortThreads) one_tile_kernel(const __grid_con
     for (int i = 0; i < kSortEach; ++i)
         if (here[i] && key[i].id < a.vocab) atomicOr(&a.seen[key[i].id >> 5], 1u << (key[i].id & 31));
     for (int pass = 0; pass < a.passes; ++pass) {
-        rank_keys(s.sort.space, key, here, rank, pass * kDigit, true, 0, 0, 0, 0);
+        rank_keys(s.sort.space, key, here, rank, pass * kDigit, true, 0, 0);
         Key* to = pass + 1 < a.passes ? s.sort.key : a.out;
 #pragma unroll
         for (int i = 0; i < kSortEach; ++i) {
@@ -452,10 +447,9 @@ __global__ void __launch_bounds__(256, 3) sum_kernel(const Key* keys, int64_t n,
     after_previous();
     let_next_begin();
     using Raw = typename RawOf<T, N>::type;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32), self = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + warp;
+    const int lane = threadIdx.x & 31;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x / 32), self = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5);
     const int64_t chunks = (n + in_chunk - 1) / in_chunk;
-    if (warp & 1) clear_rows(sort, sort.seen, 0, sort.from, sort.to, self, warps);      // half of the warps write while the others read
     for (int64_t u = self; u < chunks * slices; u += warps) {
         const int64_t chunk = u / slices;
         const int col = (static_cast<int>(u - chunk * slices) * 32 + lane);
@@ -513,7 +507,7 @@ __global__ void __launch_bounds__(256, 3) sum_kernel(const Key* keys, int64_t n,
         }
         put(open || run == after);
     }
-    if (!(warp & 1)) clear_rows(sort, sort.seen, 0, sort.from, sort.to, self, warps);
+    clear_rows(sort, sort.seen, 0, sort.from, sort.to, self, warps);
 }
 
 // Runs across chunks: the warp of the chunk where one begins adds its parts up, in order.
@@ -665,18 +659,20 @@ const char* embed_grad(const Ids& ids, int64_t n, const Matrix& grad, float scal
     s.row_bytes = out.cols * size;
     s.row_stride = out.stride * size;
     s.unit = wide_rows(out) ? 16 : size;
-    // Rows cleared beside the other work of a launch: what memory takes in the time of a launch of the sort, some 11 us.
-    const int64_t rows_at_once = std::max<int64_t>(1, (72 << 20) / s.row_bytes), all = accumulate ? 0 : out.rows;
+    // Rows cleared beside the other work of a launch.  Beside the sort of many tiles 140 MB: more than fits into the sort's own time, but sums and
+    // clearing together go slower than either (16,384 ids of 4096 onto 128,256 rows: 239 us with 40 MB, 220 with 140, 228 with 260).  One tile is
+    // sorted in the time of 80 MB.
+    const int64_t rows_at_once = std::max<int64_t>(1, ((p.tiles == 1 ? 40 : 140) << 20) / s.row_bytes), all = accumulate ? 0 : out.rows;
     auto clearing = [&](int64_t blocks) {
         s.from = s.to;
         s.to = std::min(all, s.from + rows_at_once);
-        return blocks + std::min<int64_t>(div_up(s.to - s.from, kSortWarps), 148 * 6);
+        return blocks + std::min<int64_t>(div_up(s.to - s.from, kSortWarps), 148 * 4);
     };
     cudaError_t e = cudaSuccess;
     if (p.tiles == 1) {
         s.out = keys;
         s.to = std::min(all, 2 * rows_at_once);
-        e = launch(one_tile_kernel, 1 + std::min<int64_t>(div_up(s.to, kSortWarps), 148 * 6), kSortThreads, 0, stream, s);
+        e = launch(one_tile_kernel, 1 + std::min<int64_t>(div_up(s.to, kSortWarps), 148 * 4), kSortThreads, 0, stream, s);
     } else {
         for (int pass = 0; pass < p.passes && p.tiles && e == cudaSuccess; ++pass) {
             s.in = keys;
