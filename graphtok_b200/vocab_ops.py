@@ -75,18 +75,25 @@ def _done(code, what):
 
 def _on_gpu(first, **others):
     """Index of the GPU that all of them are on."""
+    try:
+        index = first.get_device()
+        for t in others.values():
+            if not (t.is_cuda and t.get_device() == index and t.layout is torch.strided):
+                break
+        else:
+            return index
+    except (AttributeError, RuntimeError):
+        pass
     for name, t in others.items():
         if not isinstance(t, torch.Tensor):
             raise TypeError("%s must be a torch tensor" % name)
-    device = first.device if isinstance(first, torch.Tensor) else None
-    for name, t in others.items():
         if t.layout is not torch.strided:
             raise TypeError("%s must be a dense tensor" % name)
+    device = getattr(first, "device", None)
+    for name, t in others.items():
         if t.device != device:
             raise ValueError("%s is on %s, other arguments on %s" % (name, t.device, device))
-    if device.type != "cuda":
-        raise ValueError("tensors must be on the GPU, not on %s" % device)
-    return device.index
+    raise ValueError("tensors must be on the GPU, not on %s" % device)
 
 
 def _there(index, f, *args):
@@ -138,11 +145,12 @@ def _table(name, t):
 
 
 def _embed(ids, table, scale, index):
-    flat, rows, width = _ids_of("ids", ids), _rows(table), table.shape[1]
-    out = table.new_empty(ids.shape + (width,), requires_grad=False)
-    n = flat.numel()
-    to = _Matrix(out.data_ptr(), n, width, width, _TYPES[table.dtype])
-    _done(_lib().gtok_x_embed(flat.data_ptr(), _IDS[flat.dtype], n, _matrix(rows), scale, to, _stream(index)), "gtok_x_embed")
+    flat, rows = _ids_of("ids", ids), _rows(table)
+    n, width, kind = flat.numel(), table.shape[1], _TYPES[table.dtype]
+    out = table.new_empty((*ids.shape, width))
+    code = _lib().gtok_x_embed(flat.data_ptr(), _IDS[flat.dtype], n, _matrix(rows), scale, _Matrix(out.data_ptr(), n, width, width, kind), _stream(index))
+    if code:
+        _done(code, "gtok_x_embed")
     return out
 
 
@@ -200,7 +208,7 @@ def embed_grad(ids, grad, vocab, scale=1.0, out=None, accumulate=False):
 def _embed_grad(flat, rows, vocab, scale, out, accumulate, index):
     lib, n, width = _lib(), flat.numel(), rows.shape[1]
     if out is None:
-        out = rows.new_empty((vocab, width), requires_grad=False)
+        out = rows.new_empty((vocab, width))
     need = _done(lib.gtok_x_embed_grad_workspace(n, vocab, width), "gtok_x_embed_grad_workspace")
     work = torch.empty(need, dtype=torch.uint8, device=rows.device)
     _done(lib.gtok_x_embed_grad(flat.data_ptr(), _IDS[flat.dtype], n, _matrix(rows), scale, _matrix(out), bool(accumulate), work.data_ptr(), need,
@@ -326,10 +334,10 @@ class _Call:
         a.lse, a.grad, a.mean = lse.data_ptr(), grad.data_ptr(), reduction == "mean"
         d_hidden = d_weight = None
         if want_hidden:
-            d_hidden = self.weight.new_empty((a.hidden.rows, a.hidden.cols), requires_grad=False)
+            d_hidden = self.weight.new_empty((a.hidden.rows, a.hidden.cols))
             a.d_hidden = _matrix(d_hidden)
         if want_weight:
-            d_weight = self.weight.new_empty(self.weight.shape, requires_grad=False)
+            d_weight = self.weight.new_empty(self.weight.shape)
             a.d_weight = _matrix(d_weight)
         self._run(_lib().gtok_x_vocab_loss_backward, 1)
         return d_hidden, d_weight
