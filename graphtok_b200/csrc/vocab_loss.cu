@@ -639,81 +639,132 @@ __host__ __device__ inline int64_t split_time(int s, int64_t outs, int blocks, i
     return (outs * s + pairs - 1) / pairs * (270 * blocks / s + 700) + 90 * s * outs;
 }
 
+// Lines of `cols` elements, eight at a time by the lanes of a warp; elements up to the next whole 16 bytes become 0, and all of them without `from`.
+// `wide`: `from` begins at whole 16 bytes, and so do its lines.
+__device__ __forceinline__ void copy_line(const uint16_t* from, int cols, bool wide, uint16_t* to, int to_cols) {
+    const int lane = threadIdx.x & 31, lines = to_cols / 8;
+    if (from && wide) {
+        for (int i = lane; i < lines; i += 8 * 32) {
+            uint4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i + 32 * k < lines) v[k] = __ldg(reinterpret_cast<const uint4*>(from) + i + 32 * k);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i + 32 * k < lines) reinterpret_cast<uint4*>(to)[i + 32 * k] = v[k];
+        }
+        return;
+    }
+    for (int i = lane; i < lines; i += 32) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (from)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (8 * i + k < cols) w[k >> 1] |= static_cast<uint32_t>(from[8 * i + k]) << (16 * (k & 1));
+        reinterpret_cast<uint4*>(to)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
 struct RowsArgs {
     Ids targets;
     int64_t ignore;
     int vocab, n;
+    int each;                    // rows a block
     const int* state;            // of a teacher's rows; NULL: from the targets
-    Entry* entry;                // of the targets, the active rows' together
+    const Entry* entry_from;     // of a teacher
+    int entries;
+    Entry* entry;                // the active rows' together
     int* rows;
     Shared* shared;
     float *losses, *lse;         // forward
+    const uint16_t* src;         // hidden states
+    int64_t stride;
+    int cols;
+    bool wide;
+    uint16_t* dst;
+    int dst_cols;
+
+    // Target, 0 for a teacher's row, or what it has in place of a loss.
+    __device__ __forceinline__ int of(int row) const {
+        if (state) return state[row];
+        const int64_t t = load_id(targets.data, targets.bits, row);
+        return t < 0 || t == ignore ? kNone : t >= vocab ? kBad : static_cast<int>(t);
+    }
 };
 
-// Which rows have a loss: their places in order, behind them those of the others.  One block, 256 rows a warp at a time.
-__global__ void __launch_bounds__(1024) rows_kernel(const __grid_constant__ RowsArgs a) {
-    constexpr int kEach = 8;
-    __shared__ int warp_sum[32];
+// The rows that have a loss, together and in order, with their entries and places; behind their places those of the others.  Up to the next
+// multiple of 64, in which they are read, there are lines of 0 behind them.  Each block counts the active rows before its own (at most kRowBlocks
+// blocks do that, so it is never much), which takes less than a launch that counts for all: 37 rows, 9 -> 5 us.
+constexpr int kRowBlocks = 2048;
+__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ RowsArgs a) {
+    __shared__ int part[2][8];
     after_previous();
     let_next_begin();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int done = 0;
-    for (int base = 0; base < a.n; base += 1024 * kEach) {
-        const int at = base + warp * 32 * kEach + lane;
-        int id[kEach];              // or the state of a row without a loss
+    const int first = blockIdx.x * a.each, last = min(first + a.each, a.n);
+    int before = 0, active = 0;
+    for (int base = 0; base < a.n; base += 8 * 256) {
+        int id[8];
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int row = at + 32 * i;
-            id[i] = kNone;
-            if (row >= a.n) continue;
-            if (a.state) {
-                id[i] = a.state[row];
-            } else {
-                const int64_t t = load_id(a.targets.data, a.targets.bits, row);
-                id[i] = t < 0 || t == a.ignore ? kNone : t >= a.vocab ? kBad : static_cast<int>(t);
-            }
-        }
-        uint32_t live[kEach];
-        int mine = 0;
+        for (int k = 0; k < 8; ++k) id[k] = base + k * 256 + tid < a.n ? a.of(base + k * 256 + tid) : kNone;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int row = at + 32 * i;
-            live[i] = __ballot_sync(~0u, id[i] >= 0);
-            mine += __popc(live[i]);
-            if (row < a.n && id[i] < 0 && a.losses) {
-                a.losses[row] = id[i] == kBad ? __int_as_float(0x7FC00000) : 0.f;
-                a.lse[row] = 0.f;
-            }
+        for (int k = 0; k < 8; ++k) {
+            active += id[k] >= 0;
+            before += id[k] >= 0 && base + k * 256 + tid < first;
         }
-        if (lane == 0) warp_sum[warp] = mine;
-        __syncthreads();
-        int x = warp_sum[lane];
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int y = __shfl_up_sync(~0u, x, d);
-            if (lane >= d) x += y;
-        }
-        int to = done + __shfl_sync(~0u, x, warp) - mine;
-        done += __shfl_sync(~0u, x, 31);
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int row = at + 32 * i, before = to + __popc(live[i] & ((1u << lane) - 1));
-            to += __popc(live[i]);
-            if (row >= a.n) continue;
-            if (id[i] >= 0) {
-                a.rows[before] = row;
-                if (!a.state) a.entry[before] = Entry{id[i], 1.f};
-            } else {
-                a.rows[a.n - 1 - (row - before)] = row;
-            }
-        }
-        __syncthreads();
     }
-    if (tid == 0) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        before += __shfl_xor_sync(~0u, before, d);
+        active += __shfl_xor_sync(~0u, active, d);
+    }
+    if (lane == 0) {
+        part[0][warp] = before;
+        part[1][warp] = active;
+    }
+    __syncthreads();
+    before = active = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        before += part[0][w];
+        active += part[1][w];
+    }
+    if (blockIdx.x == 0 && tid == 0) {
         Shared s{};
-        s.active = done;
+        s.active = active;
         *a.shared = s;
     }
+    for (int base = first; base < last; base += 32) {
+        const int own = base + lane < last ? a.of(base + lane) : kNone;
+        const uint32_t live = __ballot_sync(~0u, own >= 0);
+        for (int i = warp; i < 32 && base + i < last; i += 8) {
+            const int row = base + i, id = __shfl_sync(~0u, own, i), to = before + __popc(live & ((1u << i) - 1));
+            if (id >= 0) {
+                copy_line(a.src + row * a.stride, a.cols, a.wide, a.dst + static_cast<int64_t>(to) * a.dst_cols, a.dst_cols);
+                for (int k = lane; k < a.entries; k += 32) a.entry[static_cast<int64_t>(to) * a.entries + k] = a.entry_from[static_cast<int64_t>(row) * a.entries + k];
+                if (lane == 0) {
+                    a.rows[to] = row;
+                    if (!a.state) a.entry[to] = Entry{id, 1.f};
+                }
+            } else if (lane == 0) {
+                a.rows[a.n - 1 - (row - to)] = row;
+                if (a.losses) {
+                    a.losses[row] = id == kBad ? __int_as_float(0x7FC00000) : 0.f;
+                    a.lse[row] = 0.f;
+                }
+            }
+        }
+        before += __popc(live);
+    }
+    for (int j = active + blockIdx.x * 8 + warp; j < (active + kDepth - 1) / kDepth * kDepth; j += gridDim.x * 8)
+        copy_line(nullptr, a.cols, a.wide, a.dst + static_cast<int64_t>(j) * a.dst_cols, a.dst_cols);
+}
+
+// A table whose rows are no lines of whole 16 bytes, as such.  A warp a row.
+__global__ void __launch_bounds__(256) table_kernel(const uint16_t* src, int64_t stride, int rows, int cols, uint16_t* dst, int dst_cols) {
+    after_previous();
+    let_next_begin();
+    for (int64_t r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) copy_line(src + r * stride, cols, false, dst + r * dst_cols, dst_cols);
 }
 
 struct ScaleArgs {
@@ -781,58 +832,6 @@ __global__ void __launch_bounds__(1024) scale_kernel(const __grid_constant__ Sca
         s.splits = splits;
         s.unscale = top / unit * a.inv_temperature / (a.grad_of_mean ? fmaxf(static_cast<float>(active), 1.f) : 1.f);
         *a.shared = s;
-    }
-}
-
-struct GatherArgs {
-    const uint16_t* src;
-    int64_t stride;
-    int cols;
-    const int* rows;             // NULL: all n
-    const Shared* shared;
-    int n;
-    uint16_t* dst;
-    int dst_cols;
-    bool wide;
-    int entries;                 // of a teacher
-    const Entry* entry_from;
-    Entry* entry_to;
-};
-
-// The active rows copied together, lines of `cols` rounded up to whole 16 bytes; up to the next multiple of 64, in which they are read, there are
-// lines of 0.  One block a row.
-__global__ void __launch_bounds__(128) gather_kernel(const __grid_constant__ GatherArgs a) {
-    after_previous();
-    let_next_begin();
-    const int active = a.rows ? a.shared->active : a.n;
-    const int end = a.rows ? (active + kDepth - 1) / kDepth * kDepth : a.n;
-    const int lines = a.dst_cols / 8;
-    for (int64_t j = blockIdx.x; j < end; j += gridDim.x) {
-        const int64_t row = j < active ? (a.rows ? a.rows[j] : j) : 0;
-        const uint16_t* from = j < active ? a.src + row * a.stride : nullptr;
-        uint4* to = reinterpret_cast<uint4*>(a.dst + j * a.dst_cols);
-        if (from && a.wide) {
-            for (int i = threadIdx.x; i < lines; i += 4 * 128) {
-                uint4 v[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (i + 128 * k < lines) v[k] = __ldg(reinterpret_cast<const uint4*>(from) + i + 128 * k);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (i + 128 * k < lines) to[i + 128 * k] = v[k];
-            }
-        } else {
-            for (int i = threadIdx.x; i < lines; i += 128) {
-                uint32_t w[4] = {0, 0, 0, 0};
-                if (from)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        if (8 * i + k < a.cols) w[k >> 1] |= static_cast<uint32_t>(from[8 * i + k]) << (16 * (k & 1));
-                to[i] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
-        if (j < active)
-            for (int i = threadIdx.x; i < a.entries; i += 128) a.entry_to[j * a.entries + i] = a.entry_from[row * a.entries + i];
     }
 }
 
@@ -1072,16 +1071,12 @@ cudaError_t prepare(const LossCall& c, bool backward, bool given, Prepared& w) {
     w.hidden = reinterpret_cast<uint16_t*>(w.kept + p.hidden);
     w.weight = c.weight.data;
     w.weight_stride = c.weight.stride;
-    GatherArgs g{};
     if (p.copy_weight) {
-        g.src = static_cast<const uint16_t*>(w.weight);
-        g.stride = w.weight_stride;
-        g.cols = p.width;
-        g.n = p.vocab;
-        g.dst = reinterpret_cast<uint16_t*>(w.at + p.weight);
-        g.dst_cols = p.cols;
-        if (cudaError_t e = launch(gather_kernel, std::min(p.vocab, 148 * 16), 128, 0, c.stream, g)) return e;
-        w.weight = g.dst;
+        uint16_t* copy = reinterpret_cast<uint16_t*>(w.at + p.weight);
+        if (cudaError_t e = launch(table_kernel, std::min<int64_t>(div_up(p.vocab, 8), 148 * 8), 256, 0, c.stream, static_cast<const uint16_t*>(w.weight), w.weight_stride,
+                                   p.vocab, p.width, copy, p.cols))
+            return e;
+        w.weight = copy;
         w.weight_stride = p.cols;
     }
     if (given) return cudaSuccess;
@@ -1099,26 +1094,22 @@ cudaError_t prepare(const LossCall& c, bool backward, bool given, Prepared& w) {
     r.ignore = c.ignore;
     r.vocab = p.vocab;
     r.n = p.n;
+    r.each = static_cast<int>(std::max<int64_t>(8, div_up(p.n, kRowBlocks)));
     r.state = c.entries ? state : nullptr;
+    r.entry_from = entry_raw;
+    r.entries = c.entries;
     r.entry = w.entry;
     r.rows = w.rows;
     r.shared = w.shared;
     r.losses = backward ? nullptr : c.losses;
     r.lse = backward ? nullptr : c.lse;
-    if (cudaError_t e = launch(rows_kernel, 1, 1024, 0, c.stream, r)) return e;
-    g.src = static_cast<const uint16_t*>(c.hidden.data);
-    g.stride = c.hidden.stride;
-    g.cols = p.width;
-    g.rows = w.rows;
-    g.shared = w.shared;
-    g.n = p.n;
-    g.dst = w.hidden;
-    g.dst_cols = p.cols;
-    g.wide = p.width % 8 == 0 && c.hidden.stride % 8 == 0 && reinterpret_cast<uintptr_t>(c.hidden.data) % 16 == 0;
-    g.entries = c.entries;
-    g.entry_from = entry_raw;
-    g.entry_to = w.entry;
-    return launch(gather_kernel, std::min(p.n_rows, 148 * 16), 128, 0, c.stream, g);
+    r.src = static_cast<const uint16_t*>(c.hidden.data);
+    r.stride = c.hidden.stride;
+    r.cols = p.width;
+    r.wide = p.width % 8 == 0 && c.hidden.stride % 8 == 0 && reinterpret_cast<uintptr_t>(c.hidden.data) % 16 == 0;
+    r.dst = w.hidden;
+    r.dst_cols = p.cols;
+    return launch(rows_kernel, div_up(p.n, r.each), 256, 0, c.stream, r);
 }
 
 Product product_of(const LossCall& c, const Prepared& w) {
