@@ -104,7 +104,8 @@ const char* check_sizes(const gtok_x_vocab_loss* a) {
     if ((h.type != gtok::kBF16 && h.type != gtok::kF16) || h.type != w.type) return "hidden states and table are both bf16 or both fp16";
     if (h.cols != w.cols) return "hidden states and table have different widths";
     if (h.cols < 1 || h.cols > (1 << 16)) return "the width is out of range";
-    if (h.rows < 0 || h.rows > kMostRows || w.rows < 1 || w.rows > kMostRows) return "rows or vocabulary are out of range";
+    // (a tile of the table's gradient sums over all rows, and is waited for in the kernel: 2^28 of them take a second)
+    if (h.rows < 0 || h.rows > (1ll << 28) || w.rows < 1 || w.rows > kMostRows) return "rows or vocabulary are out of range";
     if ((h.rows / 256 + 1) * (w.rows / 256 + 1) > (1 << 28)) return "rows times vocabulary are out of range";
     if (a->entries < 0 || a->entries > gtok::kMaxEntries) return "a teacher's row has 1 to 1024 entries";
     if (!(a->temperature > 0.f) || !std::isfinite(a->temperature) || !std::isfinite(1.f / a->temperature)) return "the temperature must be positive";

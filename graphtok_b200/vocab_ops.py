@@ -12,7 +12,9 @@ run on several streams at once.
     loss.backward()
 
 `embed`, `cross_entropy` and `distill` take part in autograd.  `embed_grad`, `cross_entropy_forward`, `cross_entropy_grad`,
-`distill_forward` and `distill_grad` are the same passes for programs that keep their own graph of them.
+`distill_forward` and `distill_grad` are the same passes without autograd.  A step that is captured into a CUDA graph takes these: autograd's
+nodes for the gradients of leaves belong to the stream that first used them, and a backward pass of torch's that is captured on
+another one while they live fails.
 """
 import ctypes
 import math

@@ -272,7 +272,7 @@ typedef struct {
     uint64_t workspace_bytes;
     void* cuda_stream;
 } gtok_x_vocab_loss;
-int64_t gtok_x_vocab_loss_workspace(const gtok_x_vocab_loss* args, int32_t backward);   /* addresses in `args` but the tables' are not looked at */
+int64_t gtok_x_vocab_loss_workspace(const gtok_x_vocab_loss* args, int32_t backward);   /* of the addresses it goes by weight's alignment and by whether `kept` is given */
 int64_t gtok_x_vocab_loss_kept(const gtok_x_vocab_loss* args);
 int32_t gtok_x_vocab_loss_forward(const gtok_x_vocab_loss* args);
 int32_t gtok_x_vocab_loss_backward(const gtok_x_vocab_loss* args);
