@@ -1,7 +1,7 @@
 """What the extension `_host` does, by ctypes alone: for an installation without it (no Python or numpy headers
 where it was built, or an interpreter it was not built for).
 
-The same four functions with the same arguments and answers, over the calls of gtok.h that take one run of
+The same functions with the same arguments and answers, over the calls of gtok.h that take one run of
 bytes: a str is encoded by the interpreter and a batch is joined first, which the extension does without.
 """
 import ctypes
@@ -9,6 +9,11 @@ import ctypes
 import numpy as np
 
 MOST_BYTES = 0xFFFFFF00          # beyond it a length does not fit the calls; they answer -3 for longer texts
+
+
+class Matrix(ctypes.Structure):
+    """gtok_x_matrix of gtok.h."""
+    _fields_ = [("data", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("stride", ctypes.c_int64), ("type", ctypes.c_int32)]
 
 
 def as_bytes(text):
@@ -101,6 +106,9 @@ class CtypesHost:
             if n != -2:
                 break
         return n if n < 0 else (out, n, doc)
+
+    def embed(self, ids, bits, n, table, rows, cols, stride, kind, scale, out, stream):
+        return self.lib.gtok_x_embed(ids, bits, n, Matrix(table, rows, cols, stride, kind), scale, Matrix(out, n, cols, cols, kind), stream)
 
     def decode(self, handle, ids):
         return None              # the caller goes by an array, as for an `ids` that the extension does not take

@@ -38,12 +38,13 @@ struct Lib {
     decltype(&gtok_x_decode_room) decode_room;
     decltype(&gtok_x_decode_run) decode_run;
     decltype(&gtok_x_take_bytes) take_bytes;
+    decltype(&gtok_x_embed) embed;
 } lib;
 bool bound = false;
 struct Need { const char* name; void* at; };
 #define GTOK_NEED(f) {"gtok_x_" #f, &lib.f}
 const Need kNeeds[] = {GTOK_NEED(set_max_bytes), GTOK_NEED(result_stream), GTOK_NEED(measure), GTOK_NEED(encode_measured), GTOK_NEED(take_ids), GTOK_NEED(decode_room),
-                       GTOK_NEED(decode_run), GTOK_NEED(take_bytes)};
+                       GTOK_NEED(decode_run), GTOK_NEED(take_bytes), GTOK_NEED(embed)};
 
 // bind(address): address(name) -> where that call of gtok.h is in the loaded library.
 PyObject* py_bind(PyObject*, PyObject* address) {
@@ -373,6 +374,24 @@ PyObject* py_users(PyObject*, PyObject* change) {
     Py_RETURN_NONE;
 }
 
+// embed(ids, id bits, n, table, rows, columns, stride, type, scale, out, stream): gtok_x_embed of integers, whose rows of `out` follow one another.
+PyObject* py_embed(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+    if (!bound || n_args != 11) {
+        PyErr_SetString(PyExc_TypeError, "embed takes eleven numbers");
+        return nullptr;
+    }
+    const auto number = [&](int i) { return static_cast<int64_t>(PyLong_AsLongLong(args[i])); };
+    const auto address = [&](int i) { return PyLong_AsVoidPtr(args[i]); };
+    gtok_x_matrix table{address(3), number(4), number(5), number(6), static_cast<int32_t>(number(7))};
+    gtok_x_matrix out{address(9), number(2), table.cols, table.cols, table.type};
+    const void* ids = address(0);
+    void* stream = address(10);
+    const int32_t bits = static_cast<int32_t>(number(1));
+    const float scale = static_cast<float>(PyFloat_AsDouble(args[8]));
+    if (PyErr_Occurred()) return nullptr;
+    return PyLong_FromLong(lib.embed(ids, bits, out.rows, &table, scale, &out, stream));
+}
+
 PyMethodDef kMethods[] = {
     {"users", py_users, METH_O, "users(change): tokenizers opened (+1) or closed (-1); memory of dropped results is kept while one is open"},
     {"bind", py_bind, METH_O, "bind(address): address(name) -> address of that call of gtok.h in the loaded library"},
@@ -382,6 +401,8 @@ PyMethodDef kMethods[] = {
     {"encode_to_device", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_encode_to_device)), METH_FASTCALL,
      "encode_to_device(handle, text or tuple, grow, make, queue) -> (tensor, id count, offsets or None), or an error code"},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_decode)), METH_FASTCALL, "decode(handle, ids) -> bytes, None, or an error code"},
+    {"embed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_embed)), METH_FASTCALL,
+     "embed(ids, id bits, n, table, rows, columns, stride, type, scale, out, stream) -> 0 or an error code"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "Python objects to and from libgtok's calls in steps.", -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -22,16 +22,13 @@ import math
 import torch
 
 from . import GTokError, load_lib
+from .ctypes_host import Matrix as _Matrix
 
 __all__ = ["embed", "embed_grad", "next_targets", "cross_entropy", "cross_entropy_forward", "cross_entropy_grad", "distill", "distill_forward", "distill_grad"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _IDS = {torch.int32: 32, torch.int64: 64}
 MAX_ENTRIES = 1024
-
-
-class _Matrix(ctypes.Structure):
-    _fields_ = [("data", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("stride", ctypes.c_int64), ("type", ctypes.c_int32)]
 
 
 class _Loss(ctypes.Structure):
@@ -148,9 +145,10 @@ def _table(name, t):
 
 def _embed(ids, table, scale, index):
     flat, rows = _ids_of("ids", ids), _rows(table)
-    n, width, kind = flat.numel(), table.shape[1], _TYPES[table.dtype]
+    vocab, width = table.shape
     out = table.new_empty((*ids.shape, width))
-    code = _lib().gtok_x_embed(flat.data_ptr(), _IDS[flat.dtype], n, _matrix(rows), scale, _Matrix(out.data_ptr(), n, width, width, kind), _stream(index))
+    code = _lib().host.embed(flat.data_ptr(), _IDS[flat.dtype], flat.numel(), rows.data_ptr(), vocab, width, rows.stride(0) if vocab > 1 else width,
+                             _TYPES[table.dtype], scale, out.data_ptr(), _stream(index))
     if code:
         _done(code, "gtok_x_embed")
     return out

@@ -425,6 +425,19 @@ def test_embed(ops, n, vocab, width, dtype, scale):
         assert torch.equal(ops.embed(ids, other, scale=scale), got)
 
 
+def test_embed_without_the_extension(ops):
+    """The lookup by ctypes gives what it gives by the extension, whichever of the two the installation has."""
+    from graphtok_b200.ctypes_host import CtypesHost
+    lib, table = ops._lib(), randn(gen(5), 300, 72).to(F16)
+    ids = torch.randint(-1, 301, (100,), generator=gen(6), device="cuda")
+    host, want = lib.host, ops.embed(ids, table, scale=0.3)
+    lib.host = CtypesHost(lib)
+    try:
+        assert torch.equal(ops.embed(ids, table, scale=0.3).view(torch.int16), want.view(torch.int16))
+    finally:
+        lib.host = host
+
+
 def test_embed_beyond_the_table(ops):
     table = randn(gen(1), 300, 64).to(BF16)
     ids = torch.tensor([0, 300, 299, 2 ** 40, -2 ** 40, 2 ** 31 + 5], device="cuda")
