@@ -8,7 +8,7 @@
 // Cross entropy is the second form with one entry of q = 1 a row, and runs as that.
 //
 // Forward: one matrix product whose epilogue reduces each 256 x 256 tile of Z, as it leaves the accumulators, to a running maximum and
-// sum per row (and takes the entries' logits out); a small kernel joins the tiles' pairs.  Backward: per piece of the vocabulary, the
+// sum per row (and takes the entries' logits out); a small kernel joins the tiles' pairs.  Up to 64 rows have a form of their own (few_kernel).  Backward: per piece of the vocabulary, the
 // tile of Z is computed again and becomes dZ in 16 bits, from which two more products give the piece's part of dH and its rows of dW.
 // A piece's dZ is the only thing in memory that grows with n x vocab.
 //
@@ -277,8 +277,7 @@ __device__ __forceinline__ void finish_hidden(const HiddenOut& h, const Shared* 
 // L2 for each 8.4 MFLOP, which L2 just gives at the full rate (13 TB/s); both operands come through TMA in 128-byte lines, whichever way they
 // run, so nothing is ever transposed in memory.  Epilogues work from registers: 32 columns of a row a thread and step, the next 32 on their way.
 // Tensor pipe in use (2,048 rows, 128,256 x 1024): forward 97 %, delta 92, hidden gradient 94, weight gradient 94.  Forward of 4,093 rows against
-// 128,256 x 4096 in 2.52 ms: 1.7 PFLOP/s, 1.04 of what a library product of 8192^3 measured; of 37 rows against 151,665 x 2048 in 105 us, the time of
-// reading the table at 5.9 TB/s.
+// 128,256 x 4096 in 2.52 ms: 1.7 PFLOP/s, 1.04 of what a library product of 8192^3 measured.
 template <int MODE, bool BF16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out,
@@ -328,17 +327,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const Place q = tiling.place(t);
                 const int am = q.m * kTile + rank * 128, bn = q.n * kTile + rank * 128 + (kRows ? p.first : 0);
                 const int bk = MODE == kHiddenGrad ? p.first : 0;
-                // Boxes of 64 rows that hold no active row are left out: what lies in their place only reaches rows that nobody reads.
-                const int boxes = MODE == kWeightGrad ? 2 : max(0, min(2, (active - am + 63) / 64));
-                const int all_boxes = MODE == kWeightGrad ? 4 : max(0, min(4, (active - q.m * kTile + 63) / 64));
+                // Boxes of 64 rows that hold no active row are taken from beyond the array, which gives zeros: nothing is read for them, and products
+                // with zeros take less power.
+                const int am0 = MODE == kWeightGrad || am < active ? am : p.n_rows, am1 = MODE == kWeightGrad || am + 64 < active ? am + 64 : p.n_rows;
                 for (int k = q.k0; k < q.k1; ++k, ++it) {
                     const uint32_t s = it % kStages;
                     if (!bar_wait(empty + 8 * s, ((it / kStages) & 1) ^ 1)) { ok = false; break; }
                     const uint32_t a = base + s * kStageBytes, b = a + kStageBytes / 2, bar = full_of_pair + 8 * s;
-                    if (rank == 0) bar_expect(full + 8 * s, (4 + all_boxes) * 8192);
+                    if (rank == 0) bar_expect(full + 8 * s, 2 * kStageBytes);
                     const int x = k * kDepth;
-                    if (boxes > 0) load_tile(a, &map_a, kAcrossA ? am : x, kAcrossA ? x : am, bar);
-                    if (boxes > 1) load_tile(a + 8192, &map_a, kAcrossA ? am + 64 : x, kAcrossA ? x : am + 64, bar);
+                    load_tile(a, &map_a, kAcrossA ? am0 : x, kAcrossA ? x : am0, bar);
+                    load_tile(a + 8192, &map_a, kAcrossA ? am1 : x, kAcrossA ? x : am1, bar);
                     load_tile(b, &map_b, kAcrossB ? bn : x, kAcrossB ? x + bk : bn, bar);
                     load_tile(b + 8192, &map_b, kAcrossB ? bn + 64 : x, kAcrossB ? x + bk : bn + 64, bar);
                 }
@@ -565,6 +564,159 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     cluster_sync();
     fence_after();
     if (warp == 2) tmem_free(tmem, 512);
+}
+
+// Forward of a few rows (cross entropy): the table's rows are the ones that go down the tile, 256 of them a pair, and the hidden states the columns,
+// as many as there are, so that the matrix instructions cost what the rows ask for and not 256 of them.  A thread keeps maximum and sum of
+// each of its columns over all its tiles and joins them with its warp's at the end.
+//
+// Bound by reading the table; stages of 20 KB leave room for ten of them on their way.  37 rows against 151,665 x 2048: 98 us, 6.4 TB/s, as a copy.
+// With the rows down the tile it was 105 alone, and 130 in a loop, where 256 rows of products for 37 asked for more power than there is.
+constexpr int kFewRows = 64, kFewStages = 10, kFewStageBytes = 16384 + kFewRows / 2 * 128;
+constexpr int kFewSmem = 1024 + kFewStages * kFewStageBytes + 256;
+
+struct Few {
+    Shared* shared;
+    int vocab, width, columns;       // columns: a multiple of 16
+    int n_rows;
+    const Entry* entry;
+    float exponent;
+    float2* partial;                 // of [pair, block, quarter of lanes][row]
+    float* entry_logits;
+};
+
+template <bool BF16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    few_kernel(const __grid_constant__ CUtensorMap map_weight, const __grid_constant__ CUtensorMap map_hidden, const __grid_constant__ Few p) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_addr(smem_raw) + 1023) & ~1023u;
+    const uint32_t full = base + kFewStages * kFewStageBytes, empty = full + 8 * kFewStages, acc_full = empty + 8 * kFewStages, acc_empty = acc_full + 16,
+                   tmem_at = acc_empty + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kFewStages; ++s) {
+            bar_init(full + 8 * s, 1);
+            bar_init(empty + 8 * s, 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            bar_init(acc_full + 8 * s, 1);
+            bar_init(acc_empty + 8 * s, 2 * kEpilogueWarps);
+        }
+        bar_init_fence();
+    }
+    if (warp == 2) tmem_alloc(tmem_at, 2 * kFewRows);
+    __syncthreads();
+    fence_before();
+    cluster_sync();
+    fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
+    after_previous();
+    const int active = p.shared->active, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int tiles = active ? (p.vocab + kTile - 1) / kTile : 0, blocks = (p.width + kDepth - 1) / kDepth;
+    const int mine = p.columns / 2;          // of the columns: the rows of the hidden states that a block copies, and those that a warp takes out
+    bool ok = true;
+
+    if (warp == 0) {
+        if (elect()) {
+            const uint32_t full_of_pair = in_block(full, 0);
+            uint32_t it = 0;
+            for (int t = pair; t < tiles && ok; t += pairs) {
+                const int row = t * kTile + rank * 128;
+                for (int k = 0; k < blocks; ++k, ++it) {
+                    const uint32_t s = it % kFewStages;
+                    if (!bar_wait(empty + 8 * s, ((it / kFewStages) & 1) ^ 1)) { ok = false; break; }
+                    const uint32_t a = base + s * kFewStageBytes, bar = full_of_pair + 8 * s;
+                    if (rank == 0) bar_expect(full + 8 * s, 2 * 16384 + p.columns * 128);
+                    load_tile(a, &map_weight, k * kDepth, row, bar);
+                    load_tile(a + 8192, &map_weight, k * kDepth, row + 64, bar);
+                    load_tile(a + 16384, &map_hidden, k * kDepth, rank * mine, bar);
+                }
+            }
+            for (uint32_t i = it < kFewStages ? 0 : it - kFewStages; i < it && ok; ++i) ok = bar_wait(empty + 8 * (i % kFewStages), (i / kFewStages) & 1);
+            if (!ok) {
+                const uint64_t from = nanoseconds();
+                while (nanoseconds() - from < 2000000ull) __nanosleep(1000);
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && elect()) {
+            const uint32_t kind = mma_kind(BF16, false, false, p.columns);
+            uint32_t it = 0, acc = 0;
+            for (int t = pair; t < tiles && ok; t += pairs, ++acc) {
+                if (!bar_wait(acc_empty + 8 * (acc & 1), ((acc >> 1) & 1) ^ 1)) { ok = false; break; }
+                fence_after();
+                for (int k = 0; k < blocks; ++k, ++it) {
+                    const uint32_t s = it % kFewStages;
+                    if (!bar_wait(full + 8 * s, (it / kFewStages) & 1)) { ok = false; break; }
+                    fence_after();
+                    const uint32_t a = base + s * kFewStageBytes, b = a + 16384;
+#pragma unroll
+                    for (int j = 0; j < kDepth / 16; ++j)
+                        mma(tmem + (acc & 1) * kFewRows, operand(a + j * 32, false), operand(b + j * 32, false), kind, k > 0 || j > 0);
+                    mma_commit(empty + 8 * s);
+                }
+                if (ok) mma_commit(acc_full + 8 * (acc & 1));
+            }
+        }
+    } else if (warp >= 4) {
+        const int quarter = warp & 3, half = (warp - 4) >> 2, first = half * mine;
+        float high[32], sum[32];
+        int target[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            high[i] = -INFINITY;
+            sum[i] = 0.f;
+            target[i] = i < mine && first + i < active ? p.entry[first + i].id : INT_MAX;
+        }
+        uint32_t acc = 0;
+        for (int t = pair; t < tiles; t += pairs, ++acc) {
+            ok = __all_sync(~0u, bar_wait(acc_full + 8 * (acc & 1), (acc >> 1) & 1));
+            if (!ok) break;
+            fence_after();
+            float v[32];
+            tmem_load(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (acc & 1) * kFewRows + first, v);
+            tmem_wait(v);
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive_cluster(in_block(acc_empty + 8 * (acc & 1), 0));
+            const int id = t * kTile + rank * 128 + quarter * 32 + lane;
+            if (id < p.vocab) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    if (i >= mine) break;
+                    if (target[i] == id) p.entry_logits[first + i] = v[i];
+                    const float top = fmaxf(high[i], v[i]), from_top = top == -INFINITY ? 0.f : top * p.exponent;
+                    sum[i] = sum[i] * exp2_fast(fmaf(high[i], p.exponent, -from_top)) + exp2_fast(fmaf(v[i], p.exponent, -from_top));
+                    high[i] = top;
+                }
+            }
+            __syncwarp();
+        }
+        if (pair < tiles) {
+            float2* to = p.partial + static_cast<int64_t>((pair * 2 + rank) * 4 + quarter) * p.n_rows + first;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                if (i >= mine) break;
+                float top = high[i];
+#pragma unroll
+                for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+                float all = sum[i] * exp2_fast(fmaf(high[i], p.exponent, top == -INFINITY ? 0.f : -top * p.exponent));
+#pragma unroll
+                for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(~0u, all, d);
+                if (lane == i) to[i] = make_float2(top, all);
+            }
+        }
+    }
+    if (!ok) atomicExch(&p.shared->error, 1);
+    __syncwarp();
+    let_next_begin();
+    __syncthreads();
+    fence_before();
+    cluster_sync();
+    fence_after();
+    if (warp == 2) tmem_free(tmem, 2 * kFewRows);
 }
 
 // ---- what the products need beforehand ------------------------------------------
@@ -856,6 +1008,7 @@ __global__ void __launch_bounds__(1024) scale_kernel(const __grid_constant__ Sca
 struct JoinArgs {
     const float2* partial;
     int vocab, pairs, n_rows;
+    bool few;                    // of few_kernel
     Shared* shared;
     const int* rows;
     int n, entries;
@@ -876,7 +1029,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Join
     let_next_begin();
     const int active = a.shared->active;
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    const int tiles = (a.vocab + kTile - 1) / kTile, parts = 2 * (active > kTile ? tiles : min(tiles, a.pairs));
+    const int tiles = (a.vocab + kTile - 1) / kTile, parts = a.few ? 8 * min(tiles, a.pairs) : 2 * (active > kTile ? tiles : min(tiles, a.pairs));
     for (int base = blockIdx.x * 32; base < active; base += gridDim.x * 32) {
         const int m = base + x, j = base + y;
         // what the second half of the work needs, on its way during the first
@@ -1022,7 +1175,7 @@ Plan make_plan(const LossCall& c, bool backward) {
     const int64_t tiles = div_up(p.vocab, kTile);
     if (!backward) {
         p.entry_logits = take(4ull * listed);
-        p.partial = take(8ull * 2 * std::max<int64_t>(tiles, p.pairs) * p.n_rows);
+        p.partial = take(8ull * std::max<int64_t>(2 * tiles, 8 * p.pairs) * p.n_rows);
     } else {
         p.own_shared = take(sizeof(Shared));
         p.info = take(sizeof(RowInfo) * p.n);
@@ -1156,17 +1309,38 @@ const char* loss_forward(const LossCall& c) {
     w.plan = make_plan(c, false);
     const Plan& p = w.plan;
     if (cudaError_t e = prepare(c, false, false, w)) return cuda_error(e);
-    CUtensorMap hidden_map, weight_map;
-    if (!tile_map(&hidden_map, c.hidden.type, w.hidden, p.n_rows, p.cols, p.cols, 64) || !tile_map(&weight_map, c.hidden.type, w.weight, p.vocab, p.cols, w.weight_stride, 64))
-        return "a tensor map was refused";
     Product q = product_of(c, w);
     q.partial = reinterpret_cast<float2*>(w.at + p.partial);
     q.entry_logits = reinterpret_cast<float*>(w.at + p.entry_logits);
-    if (cudaError_t e = launch_product<kForward>(c.hidden.type == kBF16, p.pairs, hidden_map, weight_map, hidden_map, q, c.stream)) return cuda_error(e);
+    const bool bf16 = c.hidden.type == kBF16, few = p.n <= kFewRows && !c.entries;
+    const int columns = static_cast<int>(round_up(p.n, 16));
+    CUtensorMap hidden_map, weight_map;
+    if (!tile_map(&hidden_map, c.hidden.type, w.hidden, p.n_rows, p.cols, p.cols, few ? columns / 2 : 64) ||
+        !tile_map(&weight_map, c.hidden.type, w.weight, p.vocab, p.cols, w.weight_stride, 64))
+        return "a tensor map was refused";
+    if (few) {
+        Few f{};
+        f.shared = q.shared;
+        f.vocab = q.vocab;
+        f.width = q.width;
+        f.columns = columns;
+        f.n_rows = q.n_rows;
+        f.entry = q.entry;
+        f.exponent = q.exponent;
+        f.partial = q.partial;
+        f.entry_logits = q.entry_logits;
+        auto* kernel = bf16 ? few_kernel<true> : few_kernel<false>;
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+        if (e == cudaSuccess) e = launch(kernel, 2 * p.pairs, kThreads, kFewSmem, c.stream, weight_map, hidden_map, f);
+        if (e != cudaSuccess) return cuda_error(e);
+    } else if (cudaError_t e = launch_product<kForward>(bf16, p.pairs, hidden_map, weight_map, hidden_map, q, c.stream)) {
+        return cuda_error(e);
+    }
     JoinArgs j{};
     j.partial = q.partial;
     j.vocab = p.vocab;
     j.pairs = p.pairs;
+    j.few = few;
     j.n_rows = p.n_rows;
     j.shared = w.shared;
     j.rows = w.rows;

@@ -113,7 +113,7 @@ def make(seed, n, vocab, width, dtype, masked=0.25):
 
 
 SHAPES = [(1, 1, 1), (1, 2, 8), (2, 255, 7), (3, 256, 64), (127, 257, 65), (128, 1000, 200), (129, 300, 72), (255, 31, 130), (256, 513, 256), (257, 2049, 264), (513, 5003, 520),
-          (1000, 777, 1)]
+          (1000, 777, 1), (16, 40001, 136), (17, 19000, 64), (33, 18945, 200), (48, 300, 64), (63, 5000, 72), (64, 38000, 264), (65, 38000, 128)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
