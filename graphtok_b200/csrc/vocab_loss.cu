@@ -179,7 +179,7 @@ struct Ahead {
     __device__ __forceinline__ void step(const Product& p) {
         if (there) return;
         if (lo < hi) {
-            const int s = (hi - lo + 7) >> 3;
+            const int s = (hi - lo + 8) >> 3;          // hi - lo + 1 places are possible, and seven probes leave eight parts of them
             int c = 0;
 #pragma unroll
             for (int k = 1; k < 8; ++k) {

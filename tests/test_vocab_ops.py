@@ -152,12 +152,13 @@ def test_pieces_splits_and_few_active_rows(ops, n, vocab, width, kept):
     assert losses[others].eq(0).all() and lse[others].eq(0).all() and d_hidden[others].eq(0).all()
 
 
+@pytest.mark.parametrize("n", [20, 70])
 @pytest.mark.parametrize("dtype", [BF16, F16])
-def test_rows_that_are_all_masked(ops, dtype):
-    hidden, weight, targets, g = make(3, 70, 600, 96, dtype)
+def test_rows_that_are_all_masked(ops, dtype, n):
+    hidden, weight, targets, g = make(3, n, 600, 96, dtype)
     targets[:] = -100
     hidden[:] = float("nan")
-    for reduction, shape in (("none", (70,)), ("mean", ()), ("sum", ())):
+    for reduction, shape in (("none", (n,)), ("mean", ()), ("sum", ())):
         loss, lse = ops.cross_entropy_forward(hidden, weight, targets, reduction=reduction)
         assert loss.shape == shape and loss.eq(0).all()
         grads = ops.cross_entropy_grad(hidden, weight, targets, lse, torch.ones(shape, device="cuda"), reduction=reduction)
@@ -166,8 +167,9 @@ def test_rows_that_are_all_masked(ops, dtype):
     assert ops.cross_entropy_grad(hidden[:, :95].contiguous(), odd, targets, lse, g)[1].eq(0).all()
 
 
-def test_nothing_of_masked_rows_is_seen(ops):
-    hidden, weight, targets, g = make(4, 400, 900, 128, BF16, masked=0.4)
+@pytest.mark.parametrize("n", [50, 400])
+def test_nothing_of_masked_rows_is_seen(ops, n):
+    hidden, weight, targets, g = make(4, n, 900, 128, BF16, masked=0.4)
     masked = targets < 0
     losses, lse = ops.cross_entropy_forward(hidden, weight, targets)
     grads = ops.cross_entropy_grad(hidden, weight, targets, lse, g)
@@ -180,11 +182,12 @@ def test_nothing_of_masked_rows_is_seen(ops):
         assert all(torch.equal(a, b) for a, b in zip(ops.cross_entropy_grad(other, weight, targets, lse, og), grads))
 
 
-def test_nan_and_far_logits(ops):
-    hidden, weight, targets, g = make(6, 200, 700, 64, BF16, masked=0)
+@pytest.mark.parametrize("n", [30, 200])
+def test_nan_and_far_logits(ops, n):
+    hidden, weight, targets, g = make(6, n, 700, 64, BF16, masked=0)
     hidden[17] = float("nan")
     losses, lse = ops.cross_entropy_forward(hidden, weight, targets)
-    rest = torch.arange(200, device="cuda") != 17
+    rest = torch.arange(n, device="cuda") != 17
     assert losses[17].isnan() and lse[17].isnan() and losses[rest].isfinite().all()
     d_hidden, d_weight = ops.cross_entropy_grad(hidden, weight, targets, lse, g)
     assert d_hidden[17].isnan().all() and d_hidden[rest].isfinite().all() and d_weight.isnan().all()
@@ -195,7 +198,7 @@ def test_nan_and_far_logits(ops):
     losses, lse = ops.cross_entropy_forward(hidden, weight, targets)
     ref.check(losses, lse)
     # a table with a row of the lowest value and one of infinities that no hidden state reaches
-    hidden, weight, targets, g = make(7, 130, 513, 64, BF16, masked=0)
+    hidden, weight, targets, g = make(7, n, 513, 64, BF16, masked=0)
     hidden = hidden.abs()
     weight[512] = torch.finfo(BF16).min
     weight[7] = -float("inf")
@@ -209,17 +212,18 @@ def test_nan_and_far_logits(ops):
     assert (lse.double() - z.logsumexp(1)).abs().max() <= Reference(hidden, finite, *wanted_of_targets(targets, 513), g.double()).lse_tol.max()
 
 
-def test_targets_beyond_the_vocabulary(ops):
-    hidden, weight, targets, g = make(8, 100, 300, 64, BF16, masked=0)
+@pytest.mark.parametrize("n", [60, 100])
+def test_targets_beyond_the_vocabulary(ops, n):
+    hidden, weight, targets, g = make(8, n, 300, 64, BF16, masked=0)
     good, lse = ops.cross_entropy_forward(hidden, weight, targets)
     for bad in (300, 2 ** 31 - 1, 2 ** 40):
         wrong = targets.clone()
-        wrong[[3, 99]] = bad
+        wrong[[3, n - 1]] = bad
         losses, lse = ops.cross_entropy_forward(hidden, weight, wrong)
-        assert losses[[3, 99]].isnan().all() and torch.equal(losses[4:99], good[4:99])
+        assert losses[[3, n - 1]].isnan().all() and torch.equal(losses[4:n - 1], good[4:n - 1])
         assert ops.cross_entropy_forward(hidden, weight, wrong, reduction="mean")[0].isnan()
         wrong_grads = ops.cross_entropy_grad(hidden, weight, wrong, lse, g)
-        wrong[[3, 99]] = -100
+        wrong[[3, n - 1]] = -100
         assert all(torch.equal(a, b) for a, b in zip(wrong_grads, ops.cross_entropy_grad(hidden, weight, wrong, lse, g)))
     # an ignored id inside the vocabulary, and other negative ids
     targets[5], targets[6] = 7, -1
@@ -355,6 +359,21 @@ def test_distillation(ops, k, n, vocab, width, dtype):
         d_hidden, d_weight = ops.distill_grad(hidden, weight, ids, t, lse, g, temperature=temperature)
         ref.check(losses, lse, d_hidden, d_weight)
         assert losses[::7].eq(0).all() and d_hidden[::7].eq(0).all()
+
+
+@pytest.mark.parametrize("k", [1, 2, 7, 8, 9, 15, 16, 24, 63, 64, 65, 128, 511, 512, 1024])
+def test_rows_with_all_their_entries(ops, k):
+    """Every entry is one, all of them before, in or behind some tile of the vocabulary."""
+    n, vocab = 130, 5000
+    hidden, weight, _, g = make(33, n, vocab, 72, BF16)
+    first = torch.randint(0, vocab - k, (n, 1), generator=gen(k), device="cuda")
+    ids = first + torch.arange(k, device="cuda").flip(0)
+    spread = torch.rand(n // 2, vocab, generator=gen(k + 1), device="cuda").argsort(1)[:, :k]
+    ids[: n // 2] = spread
+    logits = randn(gen(k + 2), n, k)
+    ref = Reference(hidden, weight, *wanted_of_teacher(ids, logits, vocab, 1.0), g.double())
+    losses, lse = ops.distill_forward(hidden, weight, ids, logits)
+    ref.check(losses, lse, *ops.distill_grad(hidden, weight, ids, logits, lse, g))
 
 
 def test_a_teachers_masks(ops):
@@ -506,6 +525,47 @@ def test_embed_takes_part_in_autograd(ops):
         within(table.grad, want, tol)
     with torch.no_grad():
         assert not ops.embed(ids, table).requires_grad
+
+
+def test_offsets_beyond_32_bits(ops):
+    """Tables of more than 2^31 elements: rows at their end are looked up, summed and compared like others."""
+    vocab, width = 262209, 8200
+    table = torch.zeros(vocab, width, dtype=BF16, device="cuda")
+    g = gen(80)
+    some = torch.tensor([0, 1, 131071, 261900, 262207, 262208], device="cuda")
+    table[some] = randn(g, 6, width).to(BF16)
+    ids = some[torch.randint(0, 6, (70,), generator=g, device="cuda")]
+    assert torch.equal(ops.embed(ids, table), table[ids])
+    rows = randn(g, 70, width).to(BF16)
+    grad = ops.embed_grad(ids, rows, vocab)
+    want, tol = embed_grad_bound(torch.searchsorted(some, ids), rows, 6, 1.0, BF16)
+    within(grad[some], want, tol)
+    grad[some] = 0
+    assert not grad.any()
+    del grad
+    for n in (40, 70):                   # the form of few rows, and the other
+        hidden = (randn(g, n, width) / 32).to(BF16)
+        losses, lse = ops.cross_entropy_forward(hidden, table, ids[:n])
+        z = hidden.double() @ table[some].double().T
+        others = torch.full((n, 1), math.log(vocab - 6), dtype=torch.float64, device="cuda")       # logits of 0
+        full = torch.logsumexp(torch.cat([z, others], 1), 1)
+        at = torch.searchsorted(some, ids[:n])
+        size = ((width + 15) // 16 + 2) * 2.0 ** -23 * (hidden.double().abs() @ table[some].double().abs().T).max(1).values
+        # a quarter of a million equal terms are added in fp32, tile by tile and then one tile after the other
+        within(lse, full, size + 2000 * 2.0 ** -24 + 16 * 2.0 ** -24 * full.abs(), "lse")
+        within(losses, full - z.gather(1, at[:, None])[:, 0], 2 * size + 2000 * 2.0 ** -24 + 32 * 2.0 ** -24 * (full.abs() + z.abs().max(1).values), "losses")
+        d_hidden, d_weight = ops.cross_entropy_grad(hidden, table, ids[:n], lse, torch.ones(n, device="cuda"))
+        p = torch.exp(z - full[:, None])
+        d = p.clone()
+        d[torch.arange(n), at] -= 1
+        u = half_step(BF16)
+        slack = u * 1.1 + size.max() * 4 + 2.0 ** -12
+        within(d_hidden, d @ table[some].double(), slack * (d.abs() @ table[some].double().abs()) + (d @ table[some].double()).abs() * u * 1.01, "d_hidden")
+        want = d.T @ hidden.double()
+        within(d_weight[some], want, slack * (d.abs().T @ hidden.double().abs()) + want.abs() * u * 1.01, "d_weight")
+        rest = torch.tensor([2, 100000, 262000, 262206], device="cuda")
+        want = (torch.exp(-full)[:, None] * hidden.double()).sum(0)
+        within(d_weight[rest], want.expand(4, -1), (slack * (torch.exp(-full)[:, None] * hidden.double().abs()).sum(0) + want.abs() * u * 1.01).expand(4, -1), "d_weight")
 
 
 # ---- targets --------------------------------------------------------------------------
