@@ -105,7 +105,7 @@ const char* check_sizes(const gtok_x_vocab_loss* a) {
     if (h.cols != w.cols) return "hidden states and table have different widths";
     if (h.cols < 1 || h.cols > (1 << 16)) return "the width is out of range";
     // (a tile of the table's gradient sums over all rows, and is waited for in the kernel: 2^28 of them take a second)
-    if (h.rows < 0 || h.rows > (1ll << 28) || w.rows < 1 || w.rows > kMostRows) return "rows or vocabulary are out of range";
+    if (h.rows < 0 || h.rows > (1ll << 28) || w.rows < 1 || w.rows > (1ll << 30)) return "rows or vocabulary are out of range";
     if ((h.rows / 256 + 1) * (w.rows / 256 + 1) > (1 << 28)) return "rows times vocabulary are out of range";
     if (a->entries < 0 || a->entries > gtok::kMaxEntries) return "a teacher's row has 1 to 1024 entries";
     if (!(a->temperature > 0.f) || !std::isfinite(a->temperature) || !std::isfinite(1.f / a->temperature)) return "the temperature must be positive";
@@ -126,7 +126,7 @@ gtok::LossCall loss_call(const gtok_x_vocab_loss* a) {
     c.total = a->total;
     c.mean = a->mean != 0;
     c.grad = a->grad;
-    c.grad_stride = a->grad_stride;
+    c.grad_stride = a->mean ? 0 : a->grad_stride;
     c.kept = a->kept;
     c.d_hidden = matrix(a->d_hidden);
     c.d_weight = matrix(a->d_weight);

@@ -721,6 +721,12 @@ def test_refusals_of_the_c_entries(ops):
         return a
 
     assert lib.gtok_x_vocab_loss_forward(args()) == 0 and lib.gtok_x_vocab_loss_backward(args()) == 0
+    # the mean has one gradient, whatever the stride says
+    one, got = torch.full((), 0.5, device="cuda"), torch.empty_like(hidden)
+    a = args()
+    a.mean, a.grad, a.d_hidden = 1, one.data_ptr(), ops._matrix(got)
+    assert lib.gtok_x_vocab_loss_backward(a) == 0
+    assert torch.equal(got, ops.cross_entropy_grad(hidden, weight, targets, lse, one, reduction="mean")[0])
     need = lib.gtok_x_vocab_loss_workspace(args(), 0)
     changes = [("workspace_bytes", need - 1), ("workspace", None), ("workspace", work.data_ptr() + 16), ("workspace", host.data_ptr()), ("losses", None),
                ("losses", host.data_ptr()), ("lse", None), ("targets", host.data_ptr()), ("targets", None), ("targets", targets.data_ptr() + 4), ("target_bits", 16),

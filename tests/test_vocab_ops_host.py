@@ -46,7 +46,8 @@ def test_workspaces_hold_what_the_passes_keep(ops):
 
 @pytest.mark.parametrize("change", [dict(n=-1), dict(vocab=0), dict(width=0), dict(width=1 << 17), dict(entries=1025), dict(entries=-1), dict(kind=0), dict(kind=3),
                                     dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=math.inf), dict(temperature=math.nan),
-                                    dict(temperature=1e-40), dict(n=1 << 31), dict(n=(1 << 31) - 2048, vocab=1 << 20)])
+                                    dict(temperature=1e-40), dict(n=1 << 31), dict(n=(1 << 28) + 1), dict(vocab=(1 << 30) + 1),
+                                    dict(n=1 << 28, vocab=1 << 24)])
 def test_sizes_out_of_range_are_refused(ops, change):
     lib = ops._lib()
     assert lib.gtok_x_vocab_loss_workspace(loss_args(ops, **change), 1) == -1
