@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kSortThreads) count_kernel(const __grid_consta
 }
 
 // Many tiles: their counts of each bin become sums over the tiles before, and a row behind them the totals.  32 bins a block.
-constexpr int kFewTiles = 32;           // up to here each tile adds them up by itself; 4 steps of loads, as long as this launch
+constexpr int kFewTiles = 32;           // up to here each tile adds them up by itself: 32 tiles in all 47 us, with this launch 49; 64 tiles 65 and 64, 128 tiles 110 and 84
 __global__ void __launch_bounds__(1024) prefix_kernel(uint32_t* counts, int64_t tiles) {
     constexpr int kEach = 8;
     __shared__ uint32_t sums[32][33];
