@@ -246,7 +246,7 @@ int32_t gtok_x_next_targets(const int32_t* ids, int64_t n, const int32_t* doc_of
  *              with `mean`, their mean over the rows that have a loss (0 where none has)
  *   backward   reads lse, and grad: the gradient of each loss (grad_stride elements apart, 0 for one that all share), or with
  *              `mean` that of the mean.  Writes d_hidden and d_weight (either may have data = NULL).  dZ is rounded to the tables' type on its way
- *              into the two products (fp16: scaled by a power of two and the largest gradient)
+ *              into the two products (scaled, so that fp16's range does and a teacher's largest probabilities round well)
  * `kept` (may be NULL; gtok_x_vocab_loss_kept bytes, aligned to 256) is where a forward pass leaves its copy of the rows with a loss and their
  * targets; a backward pass that is given it does not look at `hidden`'s, `targets`' and `teacher_logits`' values again.  It must come from a
  * forward pass of the same sizes, `entries` and temperature, may be used any number of times, and is only read. */
