@@ -18,6 +18,7 @@ another one while they live fails.
 """
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -36,7 +37,11 @@ class _Loss(ctypes.Structure):
                 ("target_bits", ctypes.c_int32), ("entries", ctypes.c_int32), ("teacher_logits", _Matrix), ("ignore", ctypes.c_int64),
                 ("temperature", ctypes.c_float), ("mean", ctypes.c_int32), ("losses", ctypes.c_void_p), ("lse", ctypes.c_void_p),
                 ("total", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("grad_stride", ctypes.c_int64), ("d_hidden", _Matrix),
-                ("d_weight", _Matrix), ("kept", ctypes.c_void_p), ("kept_bytes", ctypes.c_uint64), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("cuda_stream", ctypes.c_void_p)]
+                ("d_weight", _Matrix), ("kept", ctypes.c_void_p), ("kept_bytes", ctypes.c_uint64), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64), ("cuda_stream", ctypes.c_void_p)]
+
+
+_HEAD = struct.Struct("@" + 2 * "Pqqqi" + "PqiiPqqqiqf")        # _Loss up to the temperature; what follows is 0 until it is set
 
 
 _bound = None
@@ -114,9 +119,13 @@ def _rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _matrix(t):
+def _parts(t):
     rows, cols = t.shape
-    return _Matrix(t.data_ptr(), rows, cols, t.stride(0) if rows > 1 else cols, _TYPES[t.dtype])
+    return t.data_ptr(), rows, cols, t.stride(0) if rows > 1 else cols, _TYPES[t.dtype]
+
+
+def _matrix(t):
+    return _Matrix(*_parts(t))
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)       # (a tenth of the time of the public way)
@@ -246,6 +255,12 @@ def _flat(hidden):
     return _rows(hidden if hidden.dim() == 2 else hidden.reshape(hidden.shape[:-1].numel(), hidden.shape[-1]))
 
 
+def _lines(weight):
+    """`weight` with rows that do not lie over one another."""
+    weight = _rows(weight)
+    return weight.contiguous() if weight.stride(0) < weight.shape[1] and weight.shape[0] > 1 else weight
+
+
 class _Call:
     """Arguments of one loss, checked, and what keeps their memory alive.  `teacher_logits` is None for cross entropy."""
 
@@ -269,72 +284,82 @@ class _Call:
         temperature = float(temperature)
         if not (temperature > 0.0 and math.isfinite(temperature)):
             raise ValueError("temperature must be positive and finite")
-        self.hidden, self.ids = _flat(hidden), _ids_of(what, ids)
-        a = self.args = _Loss()
-        a.hidden = _matrix(self.hidden)
-        self._take(weight)
-        a.targets, a.target_bits, a.ignore, a.temperature = self.ids.data_ptr(), _IDS[ids.dtype], ignore_index, temperature
+        # (kept until the kernels are queued: memory that is let go before may be handed out again to the same call)
+        self.hidden, self.weight, self.ids = h, w, i = _flat(hidden), _lines(weight), _ids_of(what, ids)
+        self.n, kind, bits = h.shape[0], _TYPES[h.dtype], _IDS[i.dtype]
+        k, logits = 0, (0, 0, 0, 0, 0)
         if teacher_logits is not None:
-            k = ids.shape[-1]
-            self.logits = _flat(teacher_logits)
-            a.entries, a.target_stride, a.teacher_logits = k, k, _matrix(self.logits)
-
-    def _take(self, weight):
-        self.weight = _rows(weight)
-        if self.weight.stride(0) < self.weight.shape[1] and self.weight.shape[0] > 1:
-            self.weight = self.weight.contiguous()
-        self.args.weight = _matrix(self.weight)
-
-    def _keep(self, kept):
-        self.kept = kept
-        self.args.kept, self.args.kept_bytes = kept.data_ptr(), kept.numel()
+            k, self.logits = ids.shape[-1], _flat(teacher_logits)
+            logits = _parts(self.logits)
+        memory = bytearray(ctypes.sizeof(_Loss))
+        _HEAD.pack_into(memory, 0, *_parts(h), *_parts(w), i.data_ptr(), k, bits, k, *logits, ignore_index, temperature)
+        self.args = _Loss.from_buffer(memory)
 
     def let_go(self):
         """Forgets the tensors, for a call that waits for its backward pass; `again` is that pass's."""
-        self.hidden = self.ids = self.logits = self.weight = self.kept = None
+        self.hidden = self.ids = self.logits = self.weight = self.kept = self.work = None
 
     def again(self, weight, kept):
         call = object.__new__(_Call)
-        call.index, call.args = self.index, _Loss.from_buffer_copy(self.args)
-        call._take(weight)
-        call._keep(kept)
+        call.index, call.n, call.args, call.weight, call.kept = self.index, self.n, _Loss.from_buffer_copy(self.args), _lines(weight), kept
+        a = call.args
+        a.weight, a.kept = _matrix(call.weight), kept.data_ptr()
+        a.lse = kept.data_ptr() + a.kept_bytes
         return call
 
-    def _run(self, entry, backward):
+    def _run(self, entry, backward, more=0):
+        """`more`: bytes behind the workspace, whose address is returned."""
         a = self.args
-        need = _done(_lib().gtok_x_vocab_loss_workspace(a, backward), "gtok_x_vocab_loss_workspace")
-        work = torch.empty(need, dtype=torch.uint8, device=self.weight.device)
-        a.workspace, a.workspace_bytes, a.cuda_stream = work.data_ptr(), need, _stream(self.index)
+        need = (_done(_lib().gtok_x_vocab_loss_workspace(a, backward), "gtok_x_vocab_loss_workspace") + 255) & ~255
+        self.work = torch.empty(need + more, dtype=torch.uint8, device=self.weight.device)
+        at = self.work.data_ptr()
+        a.workspace, a.workspace_bytes, a.cuda_stream = at, need, _stream(self.index)
+        if more:
+            if not a.losses:
+                a.losses = at + need
+            if not a.lse:
+                a.lse = at + need + more // 2
         _done(entry(a), entry.__name__)
 
-    def forward(self, reduction, keep=False):
-        return _there(self.index, self._forward, reduction, keep)
+    def forward(self, reduction, keep=False, want_lse=False):
+        return _there(self.index, self._forward, reduction, keep, want_lse)
 
-    def _forward(self, reduction, keep):
-        a, n, device = self.args, self.hidden.shape[0], self.hidden.device
-        losses, lse = torch.empty(n, dtype=torch.float32, device=device), torch.empty(n, dtype=torch.float32, device=device)
-        a.losses, a.lse = losses.data_ptr(), lse.data_ptr()
-        if reduction != "none":
-            total = torch.empty((), dtype=torch.float32, device=device)
-            a.total, a.mean, losses = total.data_ptr(), reduction == "mean", total
+    def _forward(self, reduction, keep, want_lse):
+        """(loss, lse or None).  With `keep`, what the backward pass takes is in `self.kept`, lse behind it; losses and lse that nobody asks for
+        lie behind the workspace."""
+        a, n, device, lse = self.args, self.n, self.weight.device, None
+        if reduction == "none":
+            result = torch.empty(n, dtype=torch.float32, device=device)
+            a.losses = result.data_ptr()
+        else:
+            result = torch.empty((), dtype=torch.float32, device=device)
+            a.total, a.mean = result.data_ptr(), reduction == "mean"
         if keep:
-            self._keep(torch.empty(_done(_lib().gtok_x_vocab_loss_kept(a), "gtok_x_vocab_loss_kept"), dtype=torch.uint8, device=device))
-        self._run(_lib().gtok_x_vocab_loss_forward, 0)
-        return losses, lse
+            size = (_done(_lib().gtok_x_vocab_loss_kept(a), "gtok_x_vocab_loss_kept") + 255) & ~255
+            self.kept = torch.empty(size + 4 * n, dtype=torch.uint8, device=device)
+            a.kept, a.kept_bytes, a.lse = self.kept.data_ptr(), size, self.kept.data_ptr() + size
+        elif want_lse:
+            lse = torch.empty(n, dtype=torch.float32, device=device)
+            a.lse = lse.data_ptr()
+        self._run(_lib().gtok_x_vocab_loss_forward, 0, 8 * n)
+        return result, lse
 
     def backward(self, lse, grad, reduction, want_hidden, want_weight):
+        """`lse`: None where it lies behind what was kept."""
         return _there(self.index, self._backward, lse, grad, reduction, want_hidden, want_weight)
 
     def _backward(self, lse, grad, reduction, want_hidden, want_weight):
         a = self.args
-        lse = lse.contiguous()
+        if lse is not None:
+            lse = lse.contiguous()
+            a.lse = lse.data_ptr()
         if reduction == "none":
             grad = grad if grad.dim() == 1 else grad.reshape(-1)
             a.grad_stride = grad.stride(0) if grad.numel() > 1 else 0
-        a.lse, a.grad, a.mean = lse.data_ptr(), grad.data_ptr(), reduction == "mean"
+        a.grad, a.mean = grad.data_ptr(), reduction == "mean"
         d_hidden = d_weight = None
         if want_hidden:
-            d_hidden = self.weight.new_empty((a.hidden.rows, a.hidden.cols))
+            d_hidden = self.weight.new_empty((self.n, self.weight.shape[1]))
             a.d_hidden = _matrix(d_hidden)
         if want_weight:
             d_weight = self.weight.new_empty(self.weight.shape)
@@ -362,8 +387,8 @@ class _LossFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, call, hidden, weight, reduction):
-        loss, lse = call.forward(reduction, keep=True)
-        ctx.save_for_backward(weight, lse, call.kept)
+        loss, _ = call.forward(reduction, keep=True)
+        ctx.save_for_backward(weight, call.kept)
         ctx.call, ctx.reduction, ctx.shape = call, reduction, hidden.shape
         call.let_go()
         return loss.view(hidden.shape[:-1]) if reduction == "none" else loss
@@ -371,9 +396,9 @@ class _LossFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        weight, lse, kept = ctx.saved_tensors
+        weight, kept = ctx.saved_tensors
         _, want_hidden, want_weight, _ = ctx.needs_input_grad
-        d_hidden, d_weight = ctx.call.again(weight, kept).backward(lse, grad, ctx.reduction, want_hidden, want_weight)
+        d_hidden, d_weight = ctx.call.again(weight, kept).backward(None, grad, ctx.reduction, want_hidden, want_weight)
         return None, d_hidden.view(ctx.shape) if want_hidden else None, d_weight, None
 
 
@@ -398,7 +423,7 @@ def cross_entropy(hidden, weight, targets, reduction="mean", ignore_index=-100, 
 def cross_entropy_forward(hidden, weight, targets, reduction="none", ignore_index=-100, temperature=1.0):
     """(loss, lse): what `cross_entropy` returns and the float32 logarithms of the rows' sums, which `cross_entropy_grad` takes."""
     _check_reduction(reduction)
-    loss, lse = _Call(hidden, weight, targets, None, ignore_index, temperature).forward(reduction)
+    loss, lse = _Call(hidden, weight, targets, None, ignore_index, temperature).forward(reduction, want_lse=True)
     return (loss.view(targets.shape) if reduction == "none" else loss), lse.view(targets.shape)
 
 
@@ -424,7 +449,7 @@ def distill_forward(hidden, weight, teacher_ids, teacher_logits, temperature=1.0
     """(loss, lse), as `cross_entropy_forward`."""
     _check_reduction(reduction)
     _on_gpu(hidden, teacher_logits=teacher_logits)
-    loss, lse = _Call(hidden, weight, teacher_ids, teacher_logits, -100, temperature).forward(reduction)
+    loss, lse = _Call(hidden, weight, teacher_ids, teacher_logits, -100, temperature).forward(reduction, want_lse=True)
     lead = hidden.shape[:-1]
     return (loss.view(lead) if reduction == "none" else loss), lse.view(lead)
 

@@ -263,6 +263,22 @@ def test_layouts_and_shapes(ops, width):
     assert torch.equal(ops.cross_entropy_forward(one, weight, targets)[0], ops.cross_entropy_forward(one.contiguous(), weight, targets)[0])
 
 
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("keep", [False, True])
+def test_a_calls_memory_is_apart(ops, reduction, keep):
+    """What a forward pass writes lies in tensors that live until it is queued, and none of it over another."""
+    for n in (1, 50, 700):
+        hidden, weight, targets, _ = make(13, n, 900, 64, BF16)
+        call = ops._Call(hidden, weight, targets, None, -100, 1.0)
+        result, lse = call.forward(reduction, keep=keep, want_lse=not keep)
+        a = call.args
+        spans = [(a.losses, 4 * n), (a.lse, 4 * n), (a.workspace, a.workspace_bytes)] + [(a.kept, a.kept_bytes)] * keep + [(a.total, 4)] * (reduction != "none")
+        spans.sort()
+        assert all(x + size <= y for (x, size), (y, _) in zip(spans, spans[1:]))
+        owners = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (result, lse, call.work, getattr(call, "kept", None)) if t is not None]
+        assert all(any(lo <= at and at + size <= hi for lo, hi in owners) for at, size in spans)
+
+
 def test_no_rows(ops):
     hidden, weight = torch.zeros(0, 64, dtype=BF16, device="cuda"), torch.ones(300, 64, dtype=BF16, device="cuda")
     targets = torch.zeros(0, dtype=torch.int64, device="cuda")
