@@ -1,0 +1,61 @@
+"""Cases at the borders of the operators between token ids and a model, on a B200: long running sums, exact logits, gradients that are not finite,
+results that another party looks at."""
+import math
+
+import pytest
+import torch
+
+from conftest import tiny_vocab
+from test_vocab_ops import BF16, F16, Reference, gen, make, ops, randn, wanted_of_targets, wanted_of_teacher, within     # noqa: F401  (ops is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def exact_logits(n, vocab):
+    """Rows whose products and sums of products are small whole numbers, exact in any order: a leading logit of 40 to 100 (of 0 in every eighth row) at an
+    id in the first tile that a pair of blocks takes (256 ids a tile, 74 pairs take them in turn), the others between -4 and 4."""
+    width = 64                                   # (a logit is scaled by 1 + 2^-24 for it, which is 1 in fp32)
+    g = gen(n)
+    weight = torch.zeros(vocab, width, device="cuda")
+    weight[:, 60:] = torch.randint(-1, 2, (vocab, 4), generator=g, device="cuda").float()
+    leads = torch.arange(60, device="cuda") * 256 + torch.randint(0, 256, (60,), generator=g, device="cuda")
+    weight[leads, 60:] = 0
+    weight[leads, torch.arange(60, device="cuda")] = 10
+    row = torch.arange(n, device="cuda")
+    hidden = torch.zeros(n, width, device="cuda")
+    hidden[row, row % 60] = (3 + row % 8).float() * (row % 8 > 0)
+    hidden[:, 60:] = torch.randint(0, 2, (n, 4), generator=g, device="cuda").float() * (row % 16 > 0)[:, None]
+    targets = leads[row % 60].clone()
+    targets[::5] = torch.randint(0, vocab, ((n + 4) // 5,), generator=g, device="cuda")
+    return hidden.to(BF16), weight.to(BF16), targets
+
+
+@pytest.mark.parametrize("n", [1, 37, 64, 65, 200, 256, 300])
+def test_long_running_sums(ops, n):  # noqa: F811
+    """A row's sum over 151,665 ids with its maximum at the front, whatever number of rows it is computed among.  The terms' sum S in units of
+    the largest is off by what its additions round, at most 2^-24 S each, and never by more than what they add; lse is maximum + log S.
+
+    Additions one after the other: 8 + 2 of a step of 32 columns, 36 steps, 8 + 5 to join them, and 43 in the form of few rows.  Where the maximum moves
+    (in whole numbers from -4 to 4, so at most 8 times) a power of 2 and a product, 2^-22 + 2^-24; three powers of 2 of each term and the sum."""
+    vocab = 151665
+    hidden, weight, targets = exact_logits(n, vocab)
+    losses, lse = ops.cross_entropy_forward(hidden, weight, targets)
+    z = hidden.double() @ weight.double().T
+    want = torch.logsumexp(z, 1)
+    rest = torch.exp(want - z.max(1).values) - 1                # beside the largest term, in its units
+    total = torch.minimum((59 + 8 * 5) * 2.0 ** -24 * (1 + rest), 2 * rest) + 3 * 2.0 ** -22 * (1 + rest)
+    step = 2.0 ** -24
+    # a term's exponent is rounded by half a step of 16 at most, log2(e) in it by half a step of its own
+    tol = total / (1 + rest) + 16 * step + 2 * step * torch.log1p(rest) + step * want.abs()
+    within(lse, want, tol, "lse")
+    at = z.gather(1, targets[:, None])[:, 0]
+    within(losses, want - at, tol + step * (want - at).abs(), "losses")
+
+
+@pytest.mark.parametrize("n", [9, 64])
+@pytest.mark.parametrize("temperature", [0.4, 2.5])
+def test_a_temperature_with_few_rows(ops, n, temperature):  # noqa: F811
+    hidden, weight, targets, g = make(90 + n, n, 40000, 136, BF16)
+    ref = Reference(hidden, weight, *wanted_of_targets(targets, 40000), g.double(), temperature)
+    losses, lse = ops.cross_entropy_forward(hidden, weight, targets, temperature=temperature)
+    ref.check(losses, lse, *ops.cross_entropy_grad(hidden, weight, targets, lse, g, temperature=temperature))
