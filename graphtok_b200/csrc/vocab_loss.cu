@@ -976,17 +976,18 @@ __global__ void __launch_bounds__(1024) scale_kernel(const __grid_constant__ Sca
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] = base + 1024 * i < active ? fabsf(a.grad[a.rows[base + 1024 * i] * a.grad_stride]) : 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max_nan(top, g[i]);
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, g[i] < INFINITY ? g[i] : 0.f);
     }
 #pragma unroll
-    for (int d = 16; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, d));
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
     if (lane == 0) warp_top[warp] = top;
     __syncthreads();
     top = warp_top[lane];
 #pragma unroll
-    for (int d = 16; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, d));
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
     // dZ is kept with the largest row gradient as 1 (bf16: its range is fp32's) or as 2^15 (and less than twice that, see below), so that fp16
-    // holds probabilities down to 2^-29 in full precision and nothing of 2^16 and more.
+    // holds probabilities down to 2^-29 in full precision and nothing of 2^16 and more.  The largest of the finite ones: one that is not finite
+    // is a matter of its own row, whose dZ it makes infinite or NaN.
     float unit = a.half ? 32768.f : 1.f;
     top = top < 0x1p-100f ? 0x1p-100f : top;
     if (a.entries) {
@@ -999,6 +1000,7 @@ __global__ void __launch_bounds__(1024) scale_kernel(const __grid_constant__ Sca
         for (int k = 0; k < 2; ++k) {
             const int i = tid + 1024 * k;
             x[k] = i < some ? fabsf(a.grad[a.grad_stride ? a.rows[i / a.entries] * a.grad_stride : 0]) / top * a.entry[i].share : 0.f;
+            x[k] = x[k] < INFINITY ? x[k] : 0.f;
         }
 #pragma unroll
         for (int j = 0; j < kScales; ++j) {

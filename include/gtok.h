@@ -246,7 +246,10 @@ int32_t gtok_x_next_targets(const int32_t* ids, int64_t n, const int32_t* doc_of
  *              with `mean`, their mean over the rows that have a loss (0 where none has)
  *   backward   reads lse, and grad: the gradient of each loss (grad_stride elements apart, 0 for one that all share), or with
  *              `mean` that of the mean.  Writes d_hidden and d_weight (either may have data = NULL).  dZ is rounded to the tables' type on its way
- *              into the two products (scaled, so that fp16's range does and a teacher's largest probabilities round well)
+ *              into the two products, in one scale for all rows: by the largest finite row gradient, so that fp16's range does, and in distillation
+ *              by what the teacher's probabilities in the call's first 2,048 entries round best at.  In fp16, rows whose gradient is far below the largest
+ *              keep fewer bits: dZ of less than 2^-29 of it lies among the numbers below the normal ones, of less than 2^-40 becomes 0.  A gradient that is
+ *              not finite makes its row of d_hidden, and all of d_weight, not finite, and leaves other rows of d_hidden as they are
  * `kept` (may be NULL; gtok_x_vocab_loss_kept bytes, aligned to 256) is where a forward pass leaves its copy of the rows with a loss and their
  * targets; a backward pass that is given it does not look at `hidden`'s, `targets`' and `teacher_logits`' values again.  It must come from a
  * forward pass of the same sizes, `entries` and temperature, may be used any number of times, and is only read. */

@@ -59,3 +59,36 @@ def test_a_temperature_with_few_rows(ops, n, temperature):  # noqa: F811
     ref = Reference(hidden, weight, *wanted_of_targets(targets, 40000), g.double(), temperature)
     losses, lse = ops.cross_entropy_forward(hidden, weight, targets, temperature=temperature)
     ref.check(losses, lse, *ops.cross_entropy_grad(hidden, weight, targets, lse, g, temperature=temperature))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("op", ["cross_entropy", "distill"])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_a_gradient_that_is_not_finite_stays_in_its_row(ops, value, op, dtype):  # noqa: F811
+    """dH_i = g_i dz_i W depends on its own row's gradient alone; dW takes part of every row."""
+    n, vocab = 300, 700
+    hidden, weight, targets, g = make(95, n, vocab, 64, dtype)
+    if op == "cross_entropy":
+        args, (q, entropy) = (targets,), wanted_of_targets(targets, vocab)
+    else:
+        ids, logits = torch.randint(0, vocab, (n, 6), generator=gen(96), device="cuda"), randn(gen(97), n, 6)
+        args, (q, entropy) = (ids, logits), wanted_of_teacher(ids, logits, vocab, 1.0)
+    forward, backward = getattr(ops, op + "_forward"), getattr(ops, op + "_grad")
+    _, lse = forward(hidden, weight, *args)
+    active = (q.sum(1) > 0).nonzero().squeeze(1)
+    wrong = active[[3, 100]]
+    bad = g.clone()
+    bad[wrong] = value
+    d_hidden, d_weight = backward(hidden, weight, *args, lse, bad)
+    assert not d_hidden[wrong].isfinite().any() and not d_weight.isfinite().any()
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[wrong] = False
+    g[wrong] = 0
+    ref = Reference(hidden, weight, q, entropy, g.double())
+    within(d_hidden[rest], ref.d_hidden[rest], ref.h_tol[rest], "d_hidden")
+    # all of them: nothing finite is made up
+    d_hidden, d_weight = backward(hidden, weight, *args, lse, torch.full_like(g, value))
+    assert not d_hidden[active].isfinite().any() and not d_weight.isfinite().any()
+    others = torch.ones(n, dtype=torch.bool, device="cuda")
+    others[active] = False
+    assert d_hidden[others].eq(0).all()
