@@ -47,7 +47,7 @@ inline float cut_off(int width) { return 1.f + static_cast<float>((width + 15) /
 struct Shared {
     int active;          // rows with a loss
     int error;           // a wait ran out
-    unsigned joined;     // blocks of join_kernel that are done
+    unsigned joined;     // blocks of join_kernel, or of the last product of a backward pass, that are done
     int splits;          // hidden gradient: parts of a piece's columns that are summed apart
     float unscale;       // gradients are the products times this
 };
@@ -87,7 +87,8 @@ struct Product {
     bool direct;               // weight gradient, where its rows are no lines of whole 16 bytes: written by the threads
     uint16_t* out;             // weight gradient
     int64_t out_stride;
-    HiddenOut hidden_out;      // weight gradient of the last piece: what its idle warps may finish meanwhile
+    bool last;                 // weight gradient: of the last piece
+    HiddenOut hidden_out;      // and what its idle warps may finish meanwhile
 };
 
 struct Place { int m, n, k0, k1, split; };     // tile of the output, blocks of the summed dimension
@@ -569,7 +570,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int64_t r = p.first + blockIdx.x; r < p.first + p.count; r += gridDim.x)
                 for (int i = threadIdx.x; i < p.width; i += kThreads) p.out[r * p.out_stride + i] = 0;
         }
-        if (threadIdx.x == 0 && *static_cast<volatile int*>(&p.shared->error)) p.out[0] = BF16 ? 0x7FC0 : 0x7E00;
+        // Behind everything else, a wait may have run out here or in any product before: then no gradient is left that looks like one.
+        if (p.last) {
+            bool behind = false;
+            if (threadIdx.x == 0) {
+                __threadfence();
+                behind = atomicAdd(&p.shared->joined, 1u) == gridDim.x - 1;
+                __threadfence();
+            }
+            if (__syncthreads_or(behind) && *static_cast<volatile int*>(&p.shared->error)) {
+                const uint16_t nan = BF16 ? 0x7FC0 : 0x7E00;
+                for (int64_t r = warp; r < p.vocab; r += kThreads / 32)
+                    for (int i = lane; i < p.width; i += 32) p.out[r * p.out_stride + i] = nan;
+                for (int j = warp; p.hidden_out.part && j < active; j += kThreads / 32)
+                    for (int i = lane; i < p.hidden_out.cols; i += 32) p.hidden_out.out[p.hidden_out.rows[j] * p.hidden_out.stride + i] = nan;
+            }
+        }
     }
     fence_before();
     cluster_sync();
@@ -1146,7 +1162,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Join
             for (int d = 16; d; d >>= 1) loss += __shfl_xor_sync(~0u, loss, d);
             if (x == 0) {
                 a.losses[row] = a.shared->error ? __int_as_float(0x7FC00000) : loss;
-                a.lse[row] = row_lse;
+                a.lse[row] = a.shared->error ? __int_as_float(0x7FC00000) : row_lse;
             }
         }
     }
@@ -1492,7 +1508,8 @@ const char* loss_backward(const LossCall& c) {
             q.out = d_weight;
             q.out_stride = c.d_weight.stride;
             q.width = p.width;
-            if (within && first + p.piece >= p.vocab) q.hidden_out = h;
+            q.last = first + p.piece >= p.vocab;
+            if (within && q.last) q.hidden_out = h;
             if (cudaError_t e = launch_product<kWeightGrad>(bf16, p.pairs, delta_map, hidden_map, weight_out, q, c.stream)) return cuda_error(e);
         }
     }

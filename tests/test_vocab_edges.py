@@ -92,3 +92,22 @@ def test_a_gradient_that_is_not_finite_stays_in_its_row(ops, value, op, dtype): 
     others = torch.ones(n, dtype=torch.bool, device="cuda")
     others[active] = False
     assert d_hidden[others].eq(0).all()
+
+
+@pytest.mark.parametrize("n,vocab,width", [(50, 3000, 64), (2100, 140000, 584), (300, 500, 65)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_an_error_makes_every_gradient_nan(ops, n, vocab, width, dtype):  # noqa: F811
+    """The flag that a kernel raises when a wait of its has run out, here set where a forward pass keeps it for the backward one; d_hidden finished by the
+    last product and by a launch of its own, the table's gradient in one piece and in several, by tiles and by threads."""
+    hidden, weight, targets, g = make(98, n, vocab, width, dtype)
+    call = ops._Call(hidden, weight, targets, None, -100, 1.0)
+    call.forward("none", keep=True)
+    good = call.again(weight, call.kept).backward(None, g, "none", True, True)
+    assert all(x.isfinite().all() for x in good)
+    call.kept[4:8].view(torch.int32).fill_(1)
+    for want_hidden, want_weight in ((True, True), (True, False), (False, True)):
+        d_hidden, d_weight = call.again(weight, call.kept).backward(None, g, "none", want_hidden, want_weight)
+        if want_hidden:
+            assert d_hidden[targets >= 0].isnan().all() and d_hidden[targets < 0].eq(0).all()
+        if want_weight:
+            assert d_weight.isnan().all()
