@@ -14,13 +14,15 @@ run on several streams at once.
 `embed`, `cross_entropy` and `distill` take part in autograd.  `embed_grad`, `cross_entropy_forward`, `cross_entropy_grad`,
 `distill_forward` and `distill_grad` are the same passes without autograd.  A step that is captured into a CUDA graph takes these: autograd's
 nodes for the gradients of leaves belong to the stream that first used them, and a backward pass of torch's that is captured on
-another one while they live fails.
+another one while they live fails.  There are no second and no forward-mode derivatives: the former raise in torch, and dual tensors are
+refused.
 """
 import ctypes
 import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import GTokError, load_lib
 from .ctypes_host import Matrix as _Matrix
@@ -98,6 +100,15 @@ def _on_gpu(first, **others):
         if t.device != device:
             raise ValueError("%s is on %s, other arguments on %s" % (name, t.device, device))
     raise ValueError("tensors must be on the GPU, not on %s" % device)
+
+
+def _no_tangents(*tensors):
+    """A result without the tangent that it should have would be taken for a constant."""
+    if getattr(forward_ad, "_current_level", 0) < 0:         # outside of all levels no tensor has one
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("the vocabulary operators have no forward-mode derivatives")
 
 
 def _there(index, f, *args):
@@ -181,6 +192,7 @@ def embed(ids, table, scale=1.0):
     """Rows of `table` [vocab, width] (float32, bfloat16 or float16) by id, times `scale`: a tensor of ids.shape + (width,).
 
     ids: int32 or int64, any shape.  A negative id gives a row of zeros, one beyond the table a row of NaN; neither has a gradient."""
+    _no_tangents(table)
     index = _on_gpu(table, table=table, ids=ids)
     _table("table", table)
     scale = _scale(scale)
@@ -195,6 +207,7 @@ def embed_grad(ids, grad, vocab, scale=1.0, out=None, accumulate=False):
 
     out: where to write it, of grad's type.  With `accumulate` it is added to what `out` holds, as for a table that is an
     output table too, and rows that are not asked for are not touched."""
+    _no_tangents(grad, out)
     index = _on_gpu(grad, grad=grad, ids=ids)
     if grad.dim() < 1 or grad.shape[:-1] != ids.shape:
         raise ValueError("grad must have the shape of ids and one dimension more")
@@ -265,6 +278,7 @@ class _Call:
     """Arguments of one loss, checked, and what keeps their memory alive.  `teacher_logits` is None for cross entropy."""
 
     def __init__(self, hidden, weight, ids, teacher_logits, ignore_index, temperature):
+        _no_tangents(hidden, weight)
         if teacher_logits is None:
             what, lead = "targets", getattr(ids, "shape", None)
             self.index = _on_gpu(hidden, hidden=hidden, weight=weight, targets=ids)
@@ -396,6 +410,7 @@ class _LossFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _no_tangents(grad)
         weight, kept = ctx.saved_tensors
         _, want_hidden, want_weight, _ = ctx.needs_input_grad
         d_hidden, d_weight = ctx.call.again(weight, kept).backward(None, grad, ctx.reduction, want_hidden, want_weight)
@@ -429,6 +444,7 @@ def cross_entropy_forward(hidden, weight, targets, reduction="none", ignore_inde
 
 def cross_entropy_grad(hidden, weight, targets, lse, grad, reduction="none", ignore_index=-100, temperature=1.0, want_hidden=True, want_weight=True):
     """(d_hidden, d_weight) for the gradient `grad` of the loss (float32, of its shape); None for what is not wanted."""
+    _no_tangents(lse, grad)
     call = _Call(hidden, weight, targets, None, ignore_index, temperature)
     _check_grad(lse, grad, targets.shape, reduction, hidden)
     d_hidden, d_weight = call.backward(lse, grad, reduction, want_hidden, want_weight)
@@ -441,6 +457,7 @@ def distill(hidden, weight, teacher_ids, teacher_logits, temperature=1.0, reduct
     hidden, weight: as in `cross_entropy`.  teacher_ids (int32 or int64) and teacher_logits: [..., k], k up to 1024, in any order;
     a negative id is no entry.  The teacher's probabilities are the softmax over a row's entries; a row without any carries no loss.
     The customary factor temperature ** 2 is not applied.  There is no gradient for the teacher."""
+    _no_tangents(hidden, weight)
     _on_gpu(hidden, teacher_logits=teacher_logits)
     return _loss(hidden, weight, teacher_ids, teacher_logits, reduction, -100, temperature)
 
@@ -448,6 +465,7 @@ def distill(hidden, weight, teacher_ids, teacher_logits, temperature=1.0, reduct
 def distill_forward(hidden, weight, teacher_ids, teacher_logits, temperature=1.0, reduction="none"):
     """(loss, lse), as `cross_entropy_forward`."""
     _check_reduction(reduction)
+    _no_tangents(hidden, weight)
     _on_gpu(hidden, teacher_logits=teacher_logits)
     loss, lse = _Call(hidden, weight, teacher_ids, teacher_logits, -100, temperature).forward(reduction, want_lse=True)
     lead = hidden.shape[:-1]
@@ -456,6 +474,7 @@ def distill_forward(hidden, weight, teacher_ids, teacher_logits, temperature=1.0
 
 def distill_grad(hidden, weight, teacher_ids, teacher_logits, lse, grad, temperature=1.0, reduction="none", want_hidden=True, want_weight=True):
     """(d_hidden, d_weight), as `cross_entropy_grad`."""
+    _no_tangents(hidden, weight, lse, grad)
     _on_gpu(hidden, teacher_logits=teacher_logits)
     call = _Call(hidden, weight, teacher_ids, teacher_logits, -100, temperature)
     _check_grad(lse, grad, hidden.shape[:-1], reduction, hidden)

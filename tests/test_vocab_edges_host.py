@@ -1,0 +1,26 @@
+"""What the vocabulary operators refuse, and what they say about memory and sources, without a GPU."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from test_vocab_ops_host import loss_args, ops     # noqa: F401  (ops is a fixture)
+
+
+def test_forward_mode_is_refused(ops):  # noqa: F811
+    """A result without a tangent would be taken for a constant."""
+    ids = torch.zeros(3, dtype=torch.int32)
+    table, rows = torch.zeros(5, 8), torch.zeros(3, 8)
+    hidden, weight, lse = torch.zeros(3, 8, dtype=torch.bfloat16), torch.zeros(5, 8, dtype=torch.bfloat16), torch.zeros(3)
+    teacher, logits = ids[:, None], torch.zeros(3, 1)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: ops.embed(ids, dual(table)), lambda: ops.embed_grad(ids, dual(rows), 5), lambda: ops.embed_grad(ids, rows, 5, out=dual(table)),
+                     lambda: ops.cross_entropy(dual(hidden), weight, ids), lambda: ops.cross_entropy(hidden, dual(weight), ids),
+                     lambda: ops.cross_entropy_forward(dual(hidden), weight, ids), lambda: ops.cross_entropy_grad(hidden, dual(weight), ids, lse, lse),
+                     lambda: ops.cross_entropy_grad(hidden, weight, ids, lse, dual(lse)), lambda: ops.cross_entropy_grad(hidden, weight, ids, dual(lse), lse),
+                     lambda: ops.distill(dual(hidden), weight, teacher, logits), lambda: ops.distill(hidden, dual(weight), teacher, logits),
+                     lambda: ops.distill_forward(hidden, dual(weight), teacher, logits), lambda: ops.distill_grad(dual(hidden), weight, teacher, logits, lse, lse)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(ValueError, match="must be on the GPU"):          # a level without dual tensors is no reason
+            ops.embed(ids, table)
