@@ -224,7 +224,10 @@ def embed_grad(ids, grad, vocab, scale=1.0, out=None, accumulate=False):
         _on_gpu(grad, out=out)
         if out.shape != (vocab, width) or out.dtype != grad.dtype or (width > 1 and out.stride(1) != 1):
             raise ValueError("out must be [vocab, width] of grad's type with the elements of a row next to one another")
-    return _there(index, _embed_grad, flat, rows, vocab, scale, out, accumulate, index)
+    result = _there(index, _embed_grad, flat, rows, vocab, scale, out, accumulate, index)
+    if out is not None:
+        torch.autograd.graph.increment_version(out)         # who has saved it for a backward pass is to notice
+    return result
 
 
 def _embed_grad(flat, rows, vocab, scale, out, accumulate, index):

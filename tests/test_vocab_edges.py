@@ -111,3 +111,16 @@ def test_an_error_makes_every_gradient_nan(ops, n, vocab, width, dtype):  # noqa
             assert d_hidden[targets >= 0].isnan().all() and d_hidden[targets < 0].eq(0).all()
         if want_weight:
             assert d_weight.isnan().all()
+
+
+def test_autograd_sees_what_embed_grad_writes(ops):  # noqa: F811
+    ids = torch.tensor([1, 3], device="cuda")
+    grad, out = torch.ones(2, 8, device="cuda"), torch.ones(5, 8, device="cuda")
+    x = torch.ones(5, 8, device="cuda", requires_grad=True)
+    product = x * out
+    ops.embed_grad(ids, grad, 5, out=out, accumulate=True)
+    assert out._version == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    with torch.inference_mode():
+        ops.embed_grad(ids, grad, 5, out=torch.zeros(5, 8, device="cuda"))
