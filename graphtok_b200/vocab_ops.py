@@ -201,11 +201,24 @@ def embed(ids, table, scale=1.0):
     return _there(index, _embed, ids, table, scale, index)
 
 
+def _overlap(a, b):
+    """Whether two matrices of one type may share an element: their memory does, and not as columns beside one another."""
+    size = a.element_size()
+    at = [t.data_ptr() for t in (a, b)]
+    end = [x + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * size for x, t in zip(at, (a, b))]
+    if not (a.numel() and b.numel() and at[0] < end[1] and at[1] < end[0]):
+        return False
+    line = (a if a.shape[0] > 1 else b).stride(0) * size
+    apart = (at[1] - at[0]) % line if line else 0
+    alike = a.shape[0] == 1 or b.shape[0] == 1 or a.stride(0) == b.stride(0)
+    return not (alike and a.shape[1] * size <= apart <= line - b.shape[1] * size)
+
+
 def embed_grad(ids, grad, vocab, scale=1.0, out=None, accumulate=False):
     """Gradient of `embed`: [vocab, width] with, for each id, `scale` times the sum of the rows of `grad` (ids.shape + (width,)) that were
     looked up from it, 0 for ids that were not.  The sum is in float32 and in the order of the ids, whatever they are.
 
-    out: where to write it, of grad's type.  With `accumulate` it is added to what `out` holds, as for a table that is an
+    out: where to write it, of grad's type and apart from grad's memory.  With `accumulate` it is added to what `out` holds, as for a table that is an
     output table too, and rows that are not asked for are not touched."""
     _no_tangents(grad, out)
     index = _on_gpu(grad, grad=grad, ids=ids)
@@ -224,6 +237,8 @@ def embed_grad(ids, grad, vocab, scale=1.0, out=None, accumulate=False):
         _on_gpu(grad, out=out)
         if out.shape != (vocab, width) or out.dtype != grad.dtype or (width > 1 and out.stride(1) != 1):
             raise ValueError("out must be [vocab, width] of grad's type with the elements of a row next to one another")
+        if _overlap(rows, out):
+            raise ValueError("out and grad overlap")
     result = _there(index, _embed_grad, flat, rows, vocab, scale, out, accumulate, index)
     if out is not None:
         torch.autograd.graph.increment_version(out)         # who has saved it for a backward pass is to notice

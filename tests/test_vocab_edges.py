@@ -124,3 +124,18 @@ def test_autograd_sees_what_embed_grad_writes(ops):  # noqa: F811
         product.sum().backward()
     with torch.inference_mode():
         ops.embed_grad(ids, grad, 5, out=torch.zeros(5, 8, device="cuda"))
+
+
+def test_embed_grad_onto_its_own_input_is_refused(ops):  # noqa: F811
+    ids = torch.arange(5, device="cuda")
+    both = torch.ones(6, 16, device="cuda")
+    for out in (both[:5], both[1:], both[:5, :16]):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.embed_grad(ids, both[:5], 5, out=out)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.embed_grad(ids, both[:5, :8], 5, out=both[:5, 4:12])
+    # columns beside one another are apart, and so are rows behind one another
+    got = ops.embed_grad(ids, both[:5, :8], 5, out=both[:5, 8:])
+    assert got.eq(1).all()
+    two = torch.ones(10, 16, device="cuda")
+    assert ops.embed_grad(ids, two[:5], 5, out=two[5:], accumulate=True).eq(2).all() and two[:5].eq(1).all()
