@@ -107,9 +107,12 @@ class Tokenizer:
     def encode_batch_for_model(self, texts, table, scale=1.0, loss_mask=None):
         """What a training or scoring step takes of a batch, all on the GPU: (rows of `table` for the ids times `scale`, int32 ids, int32 n+1 token
         offsets, int32 targets).  A target is the id that follows in the same document, -100 at its last one and where `loss_mask`
-        is false; `graphtok_b200.vocab_ops` has the losses that take them.  The rows take part in autograd."""
+        is false: a function of ids and offsets that returns a boolean tensor as long as the ids, or such a tensor.
+        `graphtok_b200.vocab_ops` has the losses that take them.  The rows take part in autograd."""
         from .. import vocab_ops
         ids, offsets = self.encode_batch_to_device(texts)
+        if callable(loss_mask):
+            loss_mask = loss_mask(ids, offsets)
         return vocab_ops.embed(ids, table, scale=scale), ids, offsets, vocab_ops.next_targets(ids, offsets, loss_mask=loss_mask)
 
     # ---- decode (on the device: ids -> the tokens' bytes, gtok_x_decode) ---------

@@ -139,3 +139,48 @@ def test_embed_grad_onto_its_own_input_is_refused(ops):  # noqa: F811
     assert got.eq(1).all()
     two = torch.ones(10, 16, device="cuda")
     assert ops.embed_grad(ids, two[:5], 5, out=two[5:], accumulate=True).eq(2).all() and two[:5].eq(1).all()
+
+
+@pytest.mark.parametrize("family", ["llama3", "gemma"])
+def test_texts_with_a_mask(ops, family):  # noqa: F811
+    """A mask is made of the ids that the call makes: here prompts whose positions carry no loss, by their lengths in ids."""
+    from graphtok_b200.gpu_bpe_tokenizer import Tokenizer
+    tok = Tokenizer(tiny_vocab(family))
+    prompts, answers = ["A question? ", "", "Another, longer question:\n"], ["An answer.", "No prompt.", "42"]
+    table = randn(gen(72), tok.vocab_size, 64).to(BF16)
+    lengths = torch.tensor([len(tok.encode(p)) for p in prompts], device="cuda")
+    seen = []
+
+    def answers_only(ids, offsets):
+        seen.append((ids, offsets))
+        at = torch.arange(ids.numel(), device="cuda")
+        doc = torch.searchsorted(offsets[1:].contiguous(), at.int(), right=True)
+        return at - offsets[doc] + 1 >= lengths[doc]
+
+    rows, ids, offsets, targets = tok.encode_batch_for_model([p + a for p, a in zip(prompts, answers)], table, loss_mask=answers_only)
+    assert len(seen) == 1 and seen[0][0] is ids and seen[0][1] is offsets
+    want = [-100] * ids.numel()
+    o = offsets.tolist()
+    for d in range(3):
+        for i in range(o[d], o[d + 1] - 1):
+            if i - o[d] + 1 >= lengths[d]:
+                want[i] = int(ids[i + 1])
+    assert targets.tolist() == want and 0 < sum(t >= 0 for t in want) < len(want) - 3
+    assert torch.equal(rows, table[ids.long()])
+    mask = answers_only(ids, offsets)                    # one that is there already is taken as it is
+    assert torch.equal(tok.encode_batch_for_model([p + a for p, a in zip(prompts, answers)], table, loss_mask=mask)[3], targets)
+    with pytest.raises(ValueError, match="loss_mask"):
+        tok.encode_batch_for_model(prompts, table, loss_mask=lambda ids, offsets: torch.ones(1, dtype=torch.bool, device="cuda"))
+
+
+def test_no_texts(ops):  # noqa: F811
+    from graphtok_b200.gpu_bpe_tokenizer import Tokenizer
+    tok = Tokenizer(tiny_vocab("llama3"))
+    table = torch.ones(tok.vocab_size, 64, dtype=BF16, device="cuda", requires_grad=True)
+    for texts in ([], [""], ["", ""]):
+        rows, ids, offsets, targets = tok.encode_batch_for_model(texts, table)
+        assert rows.shape == (0, 64) and ids.numel() == targets.numel() == 0 and offsets.tolist() == [0] * (len(texts) + 1)
+        table.grad = None
+        loss = ops.cross_entropy(rows, table, targets)
+        loss.backward()
+        assert loss == 0 and table.grad.eq(0).all()
