@@ -53,6 +53,8 @@ bool usable(const void* at, int d) {
     return (a.type == cudaMemoryTypeDevice && a.device == d) || a.type == cudaMemoryTypeManaged;
 }
 
+bool floats(const void* at, int d) { return at && reinterpret_cast<uintptr_t>(at) % 4 == 0 && usable(at, d); }
+
 const char* check(const gtok_x_matrix* m, int d) {
     if (!m) return "a matrix is missing";
     if (m->type != gtok::kF32 && m->type != gtok::kBF16 && m->type != gtok::kF16) return "a matrix's type is none of fp32, bf16, fp16";
@@ -231,9 +233,9 @@ int32_t gtok_x_vocab_loss_forward(const gtok_x_vocab_loss* args) {
         if (d < 0) return -1;
         if (!args) return refuse("arguments are missing");
         if (const char* e = check_loss(args, d, true)) return refuse(e);
-        if (args->hidden.rows && (!args->losses || !args->lse || !usable(args->losses, d) || !usable(args->lse, d)))
-            return refuse("losses or lse are missing or not in the current device's memory");
-        if (args->total && !usable(args->total, d)) return refuse("the total is not in the current device's memory");
+        if (args->hidden.rows && (!floats(args->losses, d) || !floats(args->lse, d)))
+            return refuse("losses or lse are missing, not aligned, or not in the current device's memory");
+        if (args->total && !floats(args->total, d)) return refuse("the total is not aligned or not in the current device's memory");
         const gtok::LossCall c = loss_call(args);
         if (const char* e = check_workspace(args->workspace, args->workspace_bytes, gtok::loss_workspace(c, false), d)) return refuse(e);
         return done(gtok::loss_forward(c));
@@ -247,8 +249,8 @@ int32_t gtok_x_vocab_loss_backward(const gtok_x_vocab_loss* args) {
         if (!args) return refuse("arguments are missing");
         if (const char* e = check_loss(args, d, !args->kept)) return refuse(e);
         if (!args->d_hidden.data && !args->d_weight.data) return 0;
-        if (args->hidden.rows && (!args->lse || !args->grad || !usable(args->lse, d) || !usable(args->grad, d)))
-            return refuse("lse or the losses' gradient are missing or not in the current device's memory");
+        if (args->hidden.rows && (!floats(args->lse, d) || !floats(args->grad, d)))
+            return refuse("lse or the losses' gradient are missing, not aligned, or not in the current device's memory");
         if (args->grad_stride < 0) return refuse("the stride of the losses' gradient is out of range");
         if (const char* e = check_gradient(&args->d_hidden, args->hidden, d)) return refuse(e);
         if (const char* e = check_gradient(&args->d_weight, args->weight, d)) return refuse(e);

@@ -184,3 +184,26 @@ def test_no_texts(ops):  # noqa: F811
         loss = ops.cross_entropy(rows, table, targets)
         loss.backward()
         assert loss == 0 and table.grad.eq(0).all()
+
+
+def test_numbers_at_odd_addresses_are_refused(ops):  # noqa: F811
+    """Losses, lse, their total and their gradient are whole fp32 numbers to the kernels: a message in place of a misaligned access."""
+    hidden, weight, targets, g = make(99, 10, 300, 64, BF16)
+    lib, room = ops._lib(), torch.zeros(64, device="cuda")
+    work = torch.empty(1 << 26, dtype=torch.uint8, device="cuda")
+
+    def args():
+        a = ops._Call(hidden, weight, targets, None, -100, 1.0).args
+        a.losses, a.lse, a.total, a.workspace, a.workspace_bytes = room.data_ptr(), room.data_ptr() + 64, room.data_ptr() + 128, work.data_ptr(), work.numel()
+        a.grad, a.grad_stride, a.cuda_stream = g.data_ptr(), 1, torch.cuda.current_stream().cuda_stream
+        a.d_weight = ops._matrix(torch.empty_like(weight))
+        return a
+
+    assert lib.gtok_x_vocab_loss_forward(args()) == 0 and lib.gtok_x_vocab_loss_backward(args()) == 0
+    for entry, names in ((lib.gtok_x_vocab_loss_forward, ("losses", "lse", "total")), (lib.gtok_x_vocab_loss_backward, ("lse", "grad"))):
+        for name in names:
+            for odd in (1, 2, 3):
+                a = args()
+                setattr(a, name, getattr(a, name) + odd)
+                assert entry(a) == -1 and b"aligned" in lib.gtok_x_last_error(), name
+    torch.cuda.synchronize()
