@@ -110,7 +110,8 @@ const char* check_sizes(const gtok_x_vocab_loss* a) {
     if (h.rows < 0 || h.rows > (1ll << 28) || w.rows < 1 || w.rows > (1ll << 30)) return "rows or vocabulary are out of range";
     if ((h.rows / 256 + 1) * (w.rows / 256 + 1) > (1 << 28)) return "rows times vocabulary are out of range";
     if (a->entries < 0 || a->entries > gtok::kMaxEntries) return "a teacher's row has 1 to 1024 entries";
-    if (!(a->temperature > 0.f) || !std::isfinite(a->temperature) || !std::isfinite(1.f / a->temperature)) return "the temperature must be positive";
+    // (log2(e) / T is a number of fp32 for every normal one)
+    if (!(a->temperature > 0.f) || !std::isnormal(a->temperature)) return "the temperature must be positive, finite and at least 2^-126";
     return nullptr;
 }
 

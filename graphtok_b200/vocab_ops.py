@@ -32,6 +32,7 @@ __all__ = ["embed", "embed_grad", "next_targets", "cross_entropy", "cross_entrop
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _IDS = {torch.int32: 32, torch.int64: 64}
 MAX_ENTRIES = 1024
+_LEAST, _MOST = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 
 
 class _Loss(ctypes.Structure):
@@ -314,8 +315,8 @@ class _Call:
         if hidden.shape[:-1] != lead:
             raise ValueError("hidden and %s differ in their leading dimensions" % what)
         temperature = float(temperature)
-        if not (temperature > 0.0 and math.isfinite(temperature)):
-            raise ValueError("temperature must be positive and finite")
+        if not _LEAST <= temperature <= _MOST:
+            raise ValueError("temperature must be positive and finite, as a normal number of float32")
         # (kept until the kernels are queued: memory that is let go before may be handed out again to the same call)
         self.hidden, self.weight, self.ids = h, w, i = _flat(hidden), _lines(weight), _ids_of(what, ids)
         self.n, kind, bits = h.shape[0], _TYPES[h.dtype], _IDS[i.dtype]

@@ -261,7 +261,7 @@ typedef struct {
     int32_t entries;
     gtok_x_matrix teacher_logits;
     int64_t ignore;
-    float temperature;
+    float temperature;       /* T: at least 2^-126 */
     int32_t mean;
     float* losses;
     float* lse;

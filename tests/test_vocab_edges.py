@@ -207,3 +207,12 @@ def test_numbers_at_odd_addresses_are_refused(ops):  # noqa: F811
                 setattr(a, name, getattr(a, name) + odd)
                 assert entry(a) == -1 and b"aligned" in lib.gtok_x_last_error(), name
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("temperature", [1e-40, 1.1e-38, 1e39, 0.0, -1.0, math.inf, math.nan])
+def test_temperatures_that_float32_does_not_hold(ops, temperature):  # noqa: F811
+    hidden, weight, targets, _ = make(100, 10, 300, 64, BF16)
+    with pytest.raises(ValueError, match="temperature"):
+        ops.cross_entropy(hidden, weight, targets, temperature=temperature)
+    least = 2.0 ** -126
+    assert ops.cross_entropy(torch.zeros_like(hidden), weight, targets, temperature=least, reduction="none")[targets >= 0].sub(math.log(300)).abs().max() < 1e-5

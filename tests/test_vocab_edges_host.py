@@ -24,3 +24,11 @@ def test_forward_mode_is_refused(ops):  # noqa: F811
                 call()
         with pytest.raises(ValueError, match="must be on the GPU"):          # a level without dual tensors is no reason
             ops.embed(ids, table)
+
+
+@pytest.mark.parametrize("temperature", [3e-39, 4.2e-39, 1.1e-38])
+def test_temperatures_below_the_normal_numbers_are_refused(ops, temperature):  # noqa: F811
+    """log2(e) / T has to be a number of fp32: at 4.2e-39 1 / T still is and it is not."""
+    assert ops._lib().gtok_x_vocab_loss_workspace(loss_args(ops, temperature=temperature), 0) == -1
+    assert b"temperature" in ops._lib().gtok_x_last_error()
+    assert ops._lib().gtok_x_vocab_loss_workspace(loss_args(ops, temperature=2.0 ** -126), 0) > 0
