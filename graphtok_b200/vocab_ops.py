@@ -18,7 +18,6 @@ another one while they live fails.  There are no second and no forward-mode deri
 refused.
 """
 import ctypes
-import math
 import struct
 
 import torch
@@ -149,8 +148,8 @@ def _stream(index):
 
 def _scale(scale):
     scale = float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    if not -_MOST <= scale <= _MOST:
+        raise ValueError("scale must be finite, in float32")
     return scale
 
 

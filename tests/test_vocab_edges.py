@@ -216,3 +216,12 @@ def test_temperatures_that_float32_does_not_hold(ops, temperature):  # noqa: F81
         ops.cross_entropy(hidden, weight, targets, temperature=temperature)
     least = 2.0 ** -126
     assert ops.cross_entropy(torch.zeros_like(hidden), weight, targets, temperature=least, reduction="none")[targets >= 0].sub(math.log(300)).abs().max() < 1e-5
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, 3.5e38, math.inf, math.nan])
+def test_scales_that_float32_does_not_hold(ops, scale):  # noqa: F811
+    ids, table = torch.tensor([1, 2], device="cuda"), torch.zeros(5, 8, device="cuda")
+    for call in (lambda: ops.embed(ids, table, scale=scale), lambda: ops.embed_grad(ids, table[:2], 5, scale=scale)):
+        with pytest.raises(ValueError, match="scale"):
+            call()
+    assert ops.embed(ids, table, scale=torch.finfo(torch.float32).max).eq(0).all()
