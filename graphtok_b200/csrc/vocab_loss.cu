@@ -10,7 +10,8 @@
 // Forward: one matrix product whose epilogue reduces each 256 x 256 tile of Z, as it leaves the accumulators, to a running maximum and
 // sum per row (and takes the entries' logits out); a small kernel joins the tiles' pairs.  Up to 64 rows have a form of their own (few_kernel).  Backward: per piece of the vocabulary, the
 // tile of Z is computed again and becomes dZ in 16 bits, from which two more products give the piece's part of dH and its rows of dW.
-// A piece's dZ is the only thing in memory that grows with n x vocab.
+// Nothing in memory grows with n x vocab as the logits do: of dZ there is a piece at a time, 512 MiB or one tile of the vocabulary, and the
+// forward pass keeps a maximum and a sum for each row and 128 ids, 8 bytes, a 32nd of the logits in 16 bits (65 MB for 8,192 rows of 128,256).
 //
 // Rows without a loss (ignored targets, no teacher entries) are left out before the products: the others are copied together, so
 // neither time nor NaN of masked positions is carried along.
@@ -40,7 +41,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // The matrix instruction's sums are cut off, not rounded: each step of 16 elements takes the logit towards 0, by 2^-26 of its final
 // value on average (measured on random and on coherent rows alike: 1.9e-6 to 2.1e-6 of it at a width of 2048, 4.0e-6 to 4.2e-6 at
-// 4096).  Logits are scaled up by that much.
+// 4096).  Logits are scaled up by that much.  Where nothing is cut off, as in rows of one element or of small whole numbers, they are too large
+// by it instead: the error of such rows is what that of all others would be without (losses of 4,093 rows of width 4096 against 64 bits: 6e-7 with, 2.6e-6 without).
 inline float cut_off(int width) { return 1.f + static_cast<float>((width + 15) / 16) * 0x1p-26f; }
 
 // Scalars in device memory that the kernels hand to one another.

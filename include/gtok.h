@@ -234,7 +234,10 @@ int32_t gtok_x_next_targets(const int32_t* ids, int64_t n, const int32_t* doc_of
                             void* cuda_stream);
 
 /* Losses over the vocabulary from hidden states H [n, width] and an output table W [vocab, width] (both bf16 or both fp16),
- * with logits Z = H W^T that are never held as a whole:
+ * with logits Z = H W^T that are never held as a whole.  Beside copies of the rows (and of a table whose rows are no whole 16 bytes) a forward pass
+ * takes a workspace of 8 bytes for each of the n rows and 128 ids of the vocabulary (4.7 KB a row at least), a backward pass one of at most 512 MiB (or 512
+ * bytes a row, where that is more) and the fp32 sums of d_hidden (for few rows in several parts, up to 155 MB).  Tensor-core sums are cut off rather than rounded; logits are scaled by 1 + 2^-26 for each 16 elements of the width, what that
+ * takes from them on average, which is also how far they are off where nothing is cut off.
  *   entries == 0   cross entropy: losses[i] = lse(z_i / T) - z_i[targets[i]] / T.  A negative target and `ignore` are no loss
  *   entries > 0    distillation from a teacher's `entries` (at most 1024) top logits a row: ids in `targets` (rows
  *                  `target_stride` apart; a negative id is no entry), logits of any type in teacher_logits.  With q the softmax of a row's

@@ -61,6 +61,26 @@ def test_a_temperature_with_few_rows(ops, n, temperature):  # noqa: F811
     ref.check(losses, lse, *ops.cross_entropy_grad(hidden, weight, targets, lse, g, temperature=temperature))
 
 
+@pytest.mark.parametrize("n", [20, 300])
+@pytest.mark.parametrize("width", [64, 4096])
+def test_exact_logits(ops, n, width):  # noqa: F811
+    """Hidden states with one element: every logit is one product.  It is taken 2^-26 a step of 16 elements too large, and no more."""
+    g = gen(n + width)
+    weight = randn(g, 500, width).to(BF16)
+    column = torch.randint(0, width, (n,), generator=g, device="cuda")
+    hidden = torch.zeros(n, width, dtype=BF16, device="cuda")
+    hidden[torch.arange(n, device="cuda"), column] = (randn(g, n) * 4).to(BF16)
+    targets = torch.randint(0, 500, (n,), generator=g, device="cuda")
+    losses, lse = ops.cross_entropy_forward(hidden, weight, targets)
+    z = hidden.double() @ weight.double().T
+    dz = z.abs().max(1).values * (width / 16 * 2.0 ** -26 + 2.0 ** -24)
+    want = torch.logsumexp(z, 1)
+    # sums of 500 terms: 12 powers of 2 and 60 additions at most, logarithm and last sum
+    tol = dz + (12 * 4 + 60) * 2.0 ** -24 + 2.0 ** -22 * (want.abs() + z.abs().max(1).values)
+    within(lse, want, tol, "lse")
+    within(losses, want - z.gather(1, targets[:, None])[:, 0], tol + dz, "losses")
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("op", ["cross_entropy", "distill"])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])

@@ -32,3 +32,13 @@ def test_temperatures_below_the_normal_numbers_are_refused(ops, temperature):  #
     assert ops._lib().gtok_x_vocab_loss_workspace(loss_args(ops, temperature=temperature), 0) == -1
     assert b"temperature" in ops._lib().gtok_x_last_error()
     assert ops._lib().gtok_x_vocab_loss_workspace(loss_args(ops, temperature=2.0 ** -126), 0) > 0
+
+
+@pytest.mark.parametrize("n,vocab,width,entries", [(1, 1, 8, 0), (37, 151665, 2048, 0), (300, 50256, 100, 0), (8192, 128256, 2048, 0), (131072, 151665, 1024, 0), (2048, 151665, 2048, 64)])
+def test_memory_of_the_forward_pass(ops, n, vocab, width, entries):  # noqa: F811
+    """A copy of the rows, their lists, and a maximum and a sum of each row for every 128 ids: not the logits, a 32nd of them."""
+    got = ops._lib().gtok_x_vocab_loss_workspace(loss_args(ops, n, vocab, width, entries), 0)
+    rows, k = -(-n // 256) * 256, max(1, entries)
+    copies = 2 * (rows + (vocab if width % 8 else 0)) * (-(-width // 8) * 8)
+    sums = 8 * rows * max(2 * -(-vocab // 256), 8 * 132)
+    assert got <= copies + sums + n * (8 + 20 * k) + 16 * 1024
