@@ -35,20 +35,29 @@ def _newer(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-# What the profiles of the encode and decode kernels do not depend on: the C boundary and the operators on a model's tables.
-NOT_HASHED = ("gtok_abi.cc", "vocab_abi.cc", "vocab_loss.cu", "vocab_ops.h", "vocab_rows.cu")
+# The C boundary, on which no profile depends, and the operators on a model's tables, whose profiles have a hash of their own.
+ABI_SOURCES = ("gtok_abi.cc", "vocab_abi.cc")
+VOCAB_SOURCES = ("sm100.cuh", "vocab_launch.cuh", "vocab_loss.cu", "vocab_ops.h", "vocab_rows.cu")
+
+
+def _hash_of(names):
+    import hashlib
+    h = hashlib.sha256()
+    for name in sorted(names):
+        with open(os.path.join(CSRC, name), "rb") as f:
+            h.update(name.encode() + b"\0" + f.read())
+    return h.hexdigest()[:16]
 
 
 def source_hash():
-    """Short hash of the native sources of the encode and decode paths (csrc/ without the C boundary and the operators of
-    vocab_ops.h): identifies the build a measurement or a profile summary was taken from."""
-    import hashlib
-    h = hashlib.sha256()
-    for name in sorted(os.listdir(CSRC)):
-        if name.endswith((".h", ".cu", ".cc", ".map")) and name not in NOT_HASHED:
-            with open(os.path.join(CSRC, name), "rb") as f:
-                h.update(name.encode() + b"\0" + f.read())
-    return h.hexdigest()[:16]
+    """Short hash of the native sources of the encode and decode paths: all of csrc/ but the C boundary and the operators on a model's
+    tables.  Identifies the build that a measurement or a profile summary was taken from."""
+    return _hash_of(n for n in os.listdir(CSRC) if n.endswith((".h", ".cuh", ".cu", ".cc", ".map")) and n not in ABI_SOURCES + VOCAB_SOURCES)
+
+
+def vocab_source_hash():
+    """The same of the operators on a model's tables (profiles/embed_kernels.md, profiles/vocab_products.md)."""
+    return _hash_of(VOCAB_SOURCES)
 
 
 def _nvcc():

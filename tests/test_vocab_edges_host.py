@@ -42,3 +42,35 @@ def test_memory_of_the_forward_pass(ops, n, vocab, width, entries):  # noqa: F81
     copies = 2 * (rows + (vocab if width % 8 else 0)) * (-(-width // 8) * 8)
     sums = 8 * rows * max(2 * -(-vocab // 256), 8 * 132)
     assert got <= copies + sums + n * (8 + 20 * k) + 16 * 1024
+
+
+def test_profiles_are_matched_by_all_that_their_kernels_are_made_of(tmp_path, monkeypatch):
+    """A change of any source that a kernel includes, directly or not, changes the hash of its profiles and not the other."""
+    import re
+    import shutil
+
+    from graphtok_b200 import build
+    copy = tmp_path / "csrc"
+    shutil.copytree(build.CSRC, copy)
+    monkeypatch.setattr(build, "CSRC", str(copy))
+
+    def made_of(name, seen):
+        if name not in seen and (copy / name).exists():
+            seen.add(name)
+            for other in re.findall(r'#include "([^"/]+)"', (copy / name).read_text()):
+                made_of(other, seen)
+        return seen
+
+    hashes = (build.source_hash, build.vocab_source_hash)
+    encode, vocab = set(), set()
+    for name in build.SOURCES:
+        if name.endswith(".cu"):
+            made_of(name, vocab if name.startswith("vocab_") else encode)
+    assert "gpu_block.cuh" in encode and "sm100.cuh" in vocab and not encode & vocab
+    for names, which in ((encode, 0), (vocab, 1)):
+        for name in names:
+            before = [h() for h in hashes]
+            with open(copy / name, "a") as f:
+                f.write("\n")
+            after = [h() for h in hashes]
+            assert (before[which] != after[which]) and before[1 - which] == after[1 - which], name
