@@ -15,7 +15,8 @@ run on several streams at once.
 `distill_forward` and `distill_grad` are the same passes without autograd.  A step that is captured into a CUDA graph takes these: autograd's
 nodes for the gradients of leaves belong to the stream that first used them, and a backward pass of torch's that is captured on
 another one while they live fails.  There are no second and no forward-mode derivatives: the former raise in torch, and dual tensors are
-refused.
+refused.  torch.compile and torch.export do not look into the operators: compiled code calls them through torch.compiler.disable, between its
+graphs.
 """
 import ctypes
 import struct

@@ -245,3 +245,53 @@ def test_scales_that_float32_does_not_hold(ops, scale):  # noqa: F811
         with pytest.raises(ValueError, match="scale"):
             call()
     assert ops.embed(ids, table, scale=torch.finfo(torch.float32).max).eq(0).all()
+
+
+def test_captured_behind_copies_and_on_forked_streams(ops):  # noqa: F811
+    """In a graph whose nodes in front of the kernels are copies and fills, and with two passes side by side."""
+    hidden, weight, targets, g = make(101, 300, 3000, 128, BF16)
+    ids, rows = torch.randint(0, 3000, (2500,), generator=gen(102), device="cuda"), randn(gen(103), 2500, 128).to(BF16)
+
+    def step(h, w):
+        losses, lse = ops.cross_entropy_forward(h, w, targets)
+        return [losses, lse, *ops.cross_entropy_grad(h, w, targets, lse, g), ops.embed(ids, w), ops.embed_grad(ids, rows, 3000)]
+
+    want = [x.clone() for x in step(hidden, weight)]
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        h, w = torch.empty_like(hidden).copy_(hidden), torch.zeros_like(weight).copy_(weight)
+        first = ops.embed(ids, w)
+        other.wait_stream(side)
+        with torch.cuda.stream(other):
+            there = step(h, w)
+        here = step(h, w)
+        side.wait_stream(other)
+        joined = ops.embed(ids, w)
+        onto = ops.embed_grad(ids, rows, 3000, out=torch.zeros_like(weight), accumulate=True)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for outs in (here, there) for a, b in zip(outs, want))
+        assert torch.equal(first, want[4]) and torch.equal(joined, want[4]) and torch.equal(onto, want[5])
+
+
+def test_from_compiled_code(ops):  # noqa: F811
+    """torch.compile does not look into the operators; called through torch.compiler.disable they run between its graphs."""
+    hidden, weight, targets, _ = make(104, 70, 900, 64, BF16)
+    embed, loss_of = torch.compiler.disable(ops.embed), torch.compiler.disable(ops.cross_entropy)
+
+    @torch.compile(backend="eager")
+    def step(ids, table, layer):
+        return loss_of(embed(ids, table) @ layer, table, targets) * 2
+
+    ids = torch.randint(0, 900, (70,), generator=gen(105), device="cuda")
+    layer = (randn(gen(106), 64, 64) / 8).to(BF16)
+    got, want = [], []
+    for outs, f in ((got, step), (want, lambda i, t, m: ops.cross_entropy(ops.embed(i, t) @ m, t, targets) * 2)):
+        t, m = weight.clone().requires_grad_(), layer.clone().requires_grad_()
+        loss = f(ids, t, m)
+        loss.backward()
+        outs += [loss.detach(), t.grad, m.grad]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
