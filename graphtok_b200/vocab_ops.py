@@ -127,7 +127,9 @@ def _ids_of(name, t):
 
 
 def _rows(t):
-    """`t` with its rows' elements next to one another (a copy only where they are not)."""
+    """`t` with its rows' elements next to one another and in memory as they are (a copy only where they are not)."""
+    if t.is_neg():
+        t = t.resolve_neg()
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
@@ -236,8 +238,8 @@ def embed_grad(ids, grad, vocab, scale=1.0, out=None, accumulate=False):
     scale = _scale(scale)
     if out is not None:
         _on_gpu(grad, out=out)
-        if out.shape != (vocab, width) or out.dtype != grad.dtype or (width > 1 and out.stride(1) != 1):
-            raise ValueError("out must be [vocab, width] of grad's type with the elements of a row next to one another")
+        if out.shape != (vocab, width) or out.dtype != grad.dtype or (width > 1 and out.stride(1) != 1) or out.is_neg():
+            raise ValueError("out must be [vocab, width] of grad's type with the elements of a row next to one another, no view of negated ones")
         if _overlap(rows, out):
             raise ValueError("out and grad overlap")
     result = _there(index, _embed_grad, flat, rows, vocab, scale, out, accumulate, index)
@@ -384,8 +386,9 @@ class _Call:
     def _backward(self, lse, grad, reduction, want_hidden, want_weight):
         a = self.args
         if lse is not None:
-            lse = lse.contiguous()
+            lse = lse.resolve_neg().contiguous()
             a.lse = lse.data_ptr()
+        grad = grad.resolve_neg()
         if reduction == "none":
             grad = grad if grad.dim() == 1 else grad.reshape(-1)
             a.grad_stride = grad.stride(0) if grad.numel() > 1 else 0

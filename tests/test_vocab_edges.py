@@ -295,3 +295,35 @@ def test_from_compiled_code(ops):  # noqa: F811
         loss.backward()
         outs += [loss.detach(), t.grad, m.grad]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def negated(*shape):
+    """(values as a view whose memory holds their negatives, as torch gives for parts of complex gradients; the same in memory of their own)"""
+    x = torch.complex(torch.zeros(shape, device="cuda"), torch.randn(shape, generator=gen(107), device="cuda")).conj().imag
+    assert x.is_neg()
+    return x, x.clone()
+
+
+def test_views_of_negated_values(ops):  # noqa: F811
+    hidden, weight, targets, _ = make(108, 300, 700, 64, BF16)
+    _, lse = ops.cross_entropy_forward(hidden, weight, targets)
+    view, plain = negated(300)
+    assert all(torch.equal(a, b) for a, b in zip(ops.cross_entropy_grad(hidden, weight, targets, lse, view), ops.cross_entropy_grad(hidden, weight, targets, lse, plain)))
+    view, plain = negated()
+    assert all(torch.equal(a, b) for a, b in zip(ops.cross_entropy_grad(hidden, weight, targets, lse, view, reduction="sum"),
+                                                 ops.cross_entropy_grad(hidden, weight, targets, lse, plain, reduction="sum")))
+    # through autograd: the losses as the imaginary part of a complex number
+    grads = []
+    for part in (lambda x: torch.complex(torch.zeros_like(x), x).conj().imag, lambda x: -x):
+        h = hidden.clone().requires_grad_()
+        part(ops.cross_entropy(h, weight, targets, reduction="none")).sum().backward()
+        grads.append(h.grad)
+    assert torch.equal(*grads)
+    ids = torch.randint(0, 300, (50,), generator=gen(109), device="cuda")
+    for width in (1, 8):
+        view, plain = negated(300, width)
+        assert torch.equal(ops.embed(ids, view), ops.embed(ids, plain))
+        assert torch.equal(ops.embed_grad(ids, view[:50], 300), ops.embed_grad(ids, plain[:50], 300))
+    view, plain = negated(300, 1)
+    with pytest.raises(ValueError, match="negated"):
+        ops.embed_grad(ids, plain[:50], 300, out=view)
