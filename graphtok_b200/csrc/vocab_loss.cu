@@ -286,7 +286,7 @@ __device__ __forceinline__ void finish_hidden(const HiddenOut& h, const Shared* 
 // Bound by the tensor cores, and in long calls by the power that they may take.  256 x 256 a pair, because a tile then takes 64 KB of operands from
 // L2 for each 8.4 MFLOP, which L2 just gives at the full rate (13 TB/s); both operands come through TMA in 128-byte lines, whichever way they
 // run, so nothing is ever transposed in memory.  Epilogues work from registers: 32 columns of a row a thread and step, the next 32 on their way.
-// Tensor pipe in use (2,048 rows, 128,256 x 1024): forward 97 %, delta 94, hidden gradient 95, weight gradient 93.  Forward of 4,093 rows against
+// Tensor pipe in use (2,048 rows, 128,256 x 1024): forward 97 %, the others 93 to 96.  Forward of 4,093 rows against
 // 128,256 x 4096 in 2.5 to 2.6 ms: 1.6 to 1.7 PFLOP/s, 1.00 to 1.04 of what a library product of 8192^3 measured.
 template <int MODE, bool BF16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
