@@ -52,6 +52,31 @@ def test_long_running_sums(ops, n):  # noqa: F811
     within(losses, want - at, tol + step * (want - at).abs(), "losses")
 
 
+@pytest.mark.parametrize("n", [37, 200, 300])
+def test_gradients_of_confident_rows(ops, n):  # noqa: F811
+    """Where a row's target is its far logit, p - 1 is next to nothing, and what lse is off by would be all of it.  With the logits exact, the exponent of p
+    is off by half a step each of lse, of its power of 2 and of their difference, log2(e) in the difference by half a step more; then a power of 2."""
+    vocab = 151665
+    hidden, weight, targets = exact_logits(n, vocab)
+    _, lse = ops.cross_entropy_forward(hidden, weight, targets)
+    d_hidden, d_weight = ops.cross_entropy_grad(hidden, weight, targets, lse, torch.ones(n, device="cuda"))
+    h, w = hidden.double(), weight.double()
+    z = h @ w.T
+    want = torch.logsumexp(z, 1, keepdim=True)
+    rest = torch.exp(want - z.max(1, keepdim=True).values) - 1
+    step, u = 2.0 ** -24, torch.finfo(BF16).eps / 2
+    lse_off = torch.minimum((59 + 8 * 5) * step * (1 + rest), 2 * rest) / (1 + rest) + 3 * 2.0 ** -22 + 16 * step + 2 * step * torch.log1p(rest) + step * want.abs()
+    p = torch.exp(z - want)
+    q = torch.zeros_like(p).scatter_(1, targets[:, None], 1.0)
+    d = p - q
+    # three products and a difference in fp32, 16 bits, and the sums of the two products (a step every 16 elements, 40 more for pieces and splits)
+    least = 2.0 ** -126                    # powers of 2 below the least normal number are 0, and a product or a sum may lose as much
+    off = p * (lse_off + step * (want.abs() + 2 * (z - want).abs()) + 2.0 ** -22) + 4 * step * (p + q) + d.abs() * u + least
+    for got, a, b, o, m in ((d_hidden, d, w, off, vocab), (d_weight, d.T, h, off.T, n)):
+        size = a.abs() @ b.abs()
+        within(got, a @ b, o @ b.abs() + size * (m / 16 + 40) * 2.0 ** -23 + (a @ b).abs() * u * 1.01 + least)
+
+
 @pytest.mark.parametrize("n", [9, 64])
 @pytest.mark.parametrize("temperature", [0.4, 2.5])
 def test_a_temperature_with_few_rows(ops, n, temperature):  # noqa: F811
