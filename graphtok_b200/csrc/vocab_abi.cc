@@ -5,6 +5,7 @@
 
 #include <cmath>
 
+#include "vocab_next.h"
 #include "vocab_ops.h"
 
 namespace gtok {
@@ -166,9 +167,172 @@ const char* check_gradient(const gtok_x_matrix* m, const gtok_x_matrix& of, int 
     return check_out(m, d);
 }
 
+const char* check_table4_sizes(int64_t vocab, int64_t width, int64_t group) {
+    if (vocab < 1 || vocab > (1 << 24) || width < 1 || width > (1 << 16)) return "a table's rows or columns are out of range";
+    if (group != 32 && (group < 64 || group > (1 << 16) || group % 64)) return "a group has 32 columns or a multiple of 64";
+    return nullptr;
+}
+const char* check_table4(const gtok_x_table4* t, int d) {
+    if (!t) return "a table is missing";
+    if (t->type != gtok::kBF16 && t->type != gtok::kF16) return "a table's scales are bf16 or fp16";
+    if (const char* e = check_table4_sizes(t->vocab, t->width, t->group)) return e;
+    if (t->zeros != 0 && t->zeros != 1) return "zeros is 0 or 1";
+    if (t->bytes < gtok::table4_plan(t->vocab, t->width, t->group, t->zeros != 0).bytes) return "the table's memory is too small";
+    if (!t->data || reinterpret_cast<uintptr_t>(t->data) % 256 || !usable(t->data, d)) return "the table's memory is missing, not aligned to 256 bytes, or not in the current device's memory";
+    return nullptr;
+}
+gtok::Table4 table4(const gtok_x_table4& t) {
+    gtok::Table4 r;
+    r.data = t.data;
+    r.vocab = t.vocab;
+    r.width = t.width;
+    r.group = t.group;
+    r.type = t.type;
+    r.zeros = t.zeros != 0;
+    return r;
+}
+
+// Logits: rows as wide as a vocabulary.
+const char* check_logits(const gtok_x_matrix* m, int d) {
+    if (m->cols < 1 || m->cols > (1 << 24)) return "a vocabulary has 1 to 2^24 ids";
+    if (m->rows > (1 << 20)) return "the number of rows is out of range";
+    gtok_x_matrix shape = *m;
+    shape.cols = 1;                            // (a matrix of fewer columns than a vocabulary may have ids is meant elsewhere)
+    return check(&shape, d);
+}
+// An optional list of numbers of 4 bytes.
+bool words(const void* at, int d) { return !at || floats(at, d); }
+
 }  // namespace
 
 extern "C" {
+
+int64_t gtok_x_table4_bytes(int64_t vocab, int64_t width, int64_t group, int32_t zeros) {
+    if (const char* e = check_table4_sizes(vocab, width, group)) return refuse(e);
+    return static_cast<int64_t>(gtok::table4_plan(vocab, width, group, zeros != 0).bytes);
+}
+
+int32_t gtok_x_table4_pack(const gtok_x_table4* table, const uint8_t* codes, int64_t codes_stride, const gtok_x_matrix* scales, const uint8_t* zeros, int64_t zeros_stride,
+                           void* cuda_stream) {
+    try {
+        const int d = device();
+        if (d < 0) return -1;
+        if (const char* e = check_table4(table, d)) return refuse(e);
+        if (!codes || !usable(codes, d)) return refuse("the codes are missing or not in the current device's memory");
+        if (codes_stride < 0 || codes_stride > (1ll << 35) || zeros_stride < 0 || zeros_stride > (1ll << 35)) return refuse("the stride of the codes or zeros is out of range");
+        if (const char* e = check(scales, d)) return refuse(e);
+        if (scales->type != table->type || scales->rows != table->vocab || scales->cols != (table->width + table->group - 1) / table->group)
+            return refuse("the scales have another shape or type than the table's");
+        if (table->zeros && (!zeros || !usable(zeros, d))) return refuse("the zeros are missing or not in the current device's memory");
+        return done(gtok::pack_table(table4(*table), codes, codes_stride, matrix(*scales), zeros, zeros_stride, static_cast<cudaStream_t>(cuda_stream)));
+    } catch (...) { return refuse("an internal error"); }
+}
+
+int32_t gtok_x_table4_quantize(const gtok_x_table4* table, const gtok_x_matrix* weight, void* cuda_stream) {
+    try {
+        const int d = device();
+        if (d < 0) return -1;
+        if (const char* e = check_table4(table, d)) return refuse(e);
+        if (const char* e = check(weight, d)) return refuse(e);
+        if (weight->rows != table->vocab || weight->cols != table->width) return refuse("the weights have another shape than the table");
+        return done(gtok::quantize_table(table4(*table), matrix(*weight), static_cast<cudaStream_t>(cuda_stream)));
+    } catch (...) { return refuse("an internal error"); }
+}
+
+int32_t gtok_x_table4_logits(const gtok_x_matrix* hidden, const gtok_x_table4* table, const gtok_x_matrix* out, void* cuda_stream) {
+    try {
+        const int d = device();
+        if (d < 0) return -1;
+        if (const char* e = check_table4(table, d)) return refuse(e);
+        if (const char* e = check(hidden, d)) return refuse(e);
+        if (hidden->cols != table->width || hidden->type != table->type) return refuse("the hidden states have another width or type than the table");
+        if (!out || out->cols != table->vocab || out->rows != hidden->rows) return refuse("the logits have another shape than hidden states and table");
+        if (out->type != gtok::kF32 && out->type != table->type) return refuse("logits are fp32 or of the table's type");
+        if (const char* e = check_logits(out, d)) return refuse(e);
+        if (out->rows > 1 && out->stride < out->cols) return refuse("rows of an output lie over one another");
+        return done(gtok::table_logits(matrix(*hidden), table4(*table), matrix(*out), static_cast<cudaStream_t>(cuda_stream)));
+    } catch (...) { return refuse("an internal error"); }
+}
+
+int32_t gtok_x_adjust_logits(const gtok_x_adjustment* a) {
+    try {
+        const int d = device();
+        if (d < 0) return -1;
+        if (!a) return refuse("arguments are missing");
+        const int64_t n = a->logits.rows, vocab = a->logits.cols;
+        if (const char* e = check_logits(&a->logits, d)) return refuse(e);
+        if (const char* e = check_logits(&a->out, d)) return refuse(e);
+        if (a->out.rows != n || a->out.cols != vocab || a->out.type != a->logits.type) return refuse("the output has another shape or type than the logits");
+        if (n > 1 && a->out.stride < vocab) return refuse("rows of an output lie over one another");
+        if (n > 1 && a->out.data == a->logits.data && a->out.stride != a->logits.stride) return refuse("logits that are changed in place have one stride");
+        if (a->offsets) {
+            if (const char* e = check_ids(a->ids, a->id_bits, a->n_ids, d)) return refuse(e);
+            if (const char* e = check_ids(a->offsets, 32, n + 1, d)) return refuse(e);
+        }
+        if (!words(a->prompt_lengths, d) || !words(a->repetition, d) || !words(a->presence, d) || !words(a->frequency, d))
+            return refuse("prompt lengths or penalties are not aligned or not in the current device's memory");
+        if (a->entries < 0 || a->entries > gtok::kMaxBiases) return refuse("a row has at most 1024 biases");
+        if (a->bias_stride < 0 || a->bias_stride > (1ll << 35)) return refuse("the stride of the biases is out of range");
+        if (n && a->entries && (!floats(a->bias_ids, d) || !floats(a->bias, d))) return refuse("biases are missing, not aligned, or not in the current device's memory");
+        if (!words(a->allowed, d) || !words(a->allowed_rows, d)) return refuse("masks are not aligned or not in the current device's memory");
+        if (a->allowed && (a->allowed_count < 0 || a->allowed_stride < 0 || a->allowed_stride > (1ll << 35))) return refuse("number or stride of the masks are out of range");
+        gtok::AdjustCall c;
+        c.logits = matrix(a->logits);
+        c.out = matrix(a->out);
+        c.ids = make_ids(a->ids, a->id_bits, 1);
+        c.n_ids = a->n_ids;
+        c.offsets = a->offsets;
+        c.prompt_lengths = a->prompt_lengths;
+        c.repetition = a->repetition;
+        c.presence = a->presence;
+        c.frequency = a->frequency;
+        c.one_repetition = a->one_repetition;
+        c.one_presence = a->one_presence;
+        c.one_frequency = a->one_frequency;
+        c.entries = a->entries;
+        c.bias_ids = a->bias_ids;
+        c.bias = a->bias;
+        c.bias_stride = a->bias_stride;
+        c.allowed = a->allowed;
+        c.allowed_rows = a->allowed_rows;
+        c.allowed_count = a->allowed_count;
+        c.allowed_stride = a->allowed_stride;
+        c.stream = static_cast<cudaStream_t>(a->cuda_stream);
+        return done(gtok::adjust_logits(c));
+    } catch (...) { return refuse("an internal error"); }
+}
+
+int32_t gtok_x_sample(const gtok_x_draw* a) {
+    try {
+        const int d = device();
+        if (d < 0) return -1;
+        if (!a) return refuse("arguments are missing");
+        if (const char* e = check_logits(&a->logits, d)) return refuse(e);
+        if (a->u_bits != 32 && a->u_bits != 64) return refuse("random numbers have 32 or 64 bits");
+        if (a->logits.rows) {
+            if (!a->u || reinterpret_cast<uintptr_t>(a->u) % (a->u_bits / 8) || !usable(a->u, d)) return refuse("random numbers are missing, not aligned, or not in the current device's memory");
+            if (!floats(a->ids, d) || !floats(a->logprobs, d)) return refuse("ids or logprobs are missing, not aligned, or not in the current device's memory");
+        }
+        if (!words(a->temperature, d) || !words(a->top_k, d) || !words(a->top_p, d) || !words(a->min_p, d))
+            return refuse("temperature, top_k, top_p or min_p are not aligned or not in the current device's memory");
+        gtok::SampleCall c;
+        c.logits = matrix(a->logits);
+        c.u = a->u;
+        c.wide_u = a->u_bits == 64;
+        c.temperature = a->temperature;
+        c.top_k = a->top_k;
+        c.top_p = a->top_p;
+        c.min_p = a->min_p;
+        c.one_temperature = a->one_temperature;
+        c.one_top_k = a->one_top_k;
+        c.one_top_p = a->one_top_p;
+        c.one_min_p = a->one_min_p;
+        c.ids = a->ids;
+        c.logprobs = a->logprobs;
+        c.stream = static_cast<cudaStream_t>(a->cuda_stream);
+        return done(gtok::sample(c));
+    } catch (...) { return refuse("an internal error"); }
+}
 
 int32_t gtok_x_embed(const void* ids, int32_t id_bits, int64_t n, const gtok_x_matrix* table, float scale, const gtok_x_matrix* out, void* cuda_stream) {
     try {

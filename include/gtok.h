@@ -283,6 +283,83 @@ int64_t gtok_x_vocab_loss_kept(const gtok_x_vocab_loss* args);
 int32_t gtok_x_vocab_loss_forward(const gtok_x_vocab_loss* args);
 int32_t gtok_x_vocab_loss_backward(const gtok_x_vocab_loss* args);
 
+/* ---- from hidden states to the next ids ---------------------------------------------
+ * No counterpart in the reference.  The last steps of a model that answers: products of some hidden states with an output table that is
+ * held in 4 bits, changes to the logits, and the draw of an id for each row.  As for the entries above: device memory only, no handle, nothing is allocated or
+ * waited for, calls on different streams may overlap and may be captured.  They need no workspace.
+ *
+ * A table of `vocab` rows and `width` columns: codes q of 4 bits, and for every `group` columns of a row (32, or a multiple of 64; the last group may be shorter) a scale s
+ * in 16 bits and, with `zeros`, a zero b of 4 bits (8 for all where there are none).  The value of an element is s * (q - b).  It lies in one piece of memory of
+ * gtok_x_table4_bytes, aligned to 256 bytes, in an order of its own.
+ *   pack       from codes (a byte each, of which the low four bits count; rows `codes_stride` apart), scales [vocab, groups of a row] of the table's type, and zeros likewise
+ *   quantize   from weights of any type: without zeros s = max |w| / 7, q = round(w / s) + 8; with zeros s = (max(w, 0) - min(w, 0)) / 15, b = round(-min(w, 0) / s),
+ *              q = round(w / s) + b; s is rounded to the table's type first, ties go to even, q is held to 0 to 15.  A group with a NaN or an infinity has NaN for a scale
+ *   logits     out[i, v] = sum over the groups of s * (sum over the group's columns of (q - b) * hidden[i, k]), for hidden states of the table's type; out is fp32 or of
+ *              that type.  Products are exact and summed in fp32, in an order that depends on the sizes alone.  A row's hidden states touch no other row */
+typedef struct {
+    void* data;
+    uint64_t bytes;
+    int64_t vocab, width, group;
+    int32_t type;            /* of scales and hidden states: 1 bf16, 2 fp16 */
+    int32_t zeros;           /* 0 or 1 */
+} gtok_x_table4;
+int64_t gtok_x_table4_bytes(int64_t vocab, int64_t width, int64_t group, int32_t zeros);
+int32_t gtok_x_table4_pack(const gtok_x_table4* table, const uint8_t* codes, int64_t codes_stride, const gtok_x_matrix* scales, const uint8_t* zeros, int64_t zeros_stride,
+                           void* cuda_stream);
+int32_t gtok_x_table4_quantize(const gtok_x_table4* table, const gtok_x_matrix* weight, void* cuda_stream);
+int32_t gtok_x_table4_logits(const gtok_x_matrix* hidden, const gtok_x_table4* table, const gtok_x_matrix* out, void* cuda_stream);
+
+/* Changes to logits [n, vocab], in fp32 and rounded once; `out` has their type and is their memory, with the same stride, or apart from it.  In this order:
+ *   ids of the row's history: l > 0 becomes l / repetition, others l * repetition; then, for ids that come `count` > 0 times behind the row's first
+ *     prompt_lengths (all of them without it), l - frequency * count - presence.  Row i's history is ids[offsets[i]] to ids[offsets[i + 1] - 1] (of `n_ids` in all; `offsets` NULL: none); ids
+ *     outside the vocabulary are left out
+ *   l + the sum, in the order of the list, of the row's biases for that id: `entries` (at most 1024) ids and values a row, `bias_stride` apart (0: one list for all).  A negative id is no entry
+ *   -infinity, whatever stood there, where bit id % 32 of word id / 32 of the row's mask is 0.  Masks are `allowed_stride` words apart; row i has mask allowed_rows[i], or
+ *     mask i without it.  A negative number is no mask, one of allowed_count or more allows nothing
+ * repetition, presence and frequency: a value for each row or, where NULL, the one_ value for all. */
+typedef struct {
+    gtok_x_matrix logits, out;
+    const void* ids;
+    int64_t n_ids;
+    int32_t id_bits;         /* 32 or 64 */
+    int32_t entries;
+    const int32_t* offsets;
+    const int32_t* prompt_lengths;
+    const float *repetition, *presence, *frequency;
+    float one_repetition, one_presence, one_frequency;
+    int32_t reserved;
+    const int32_t* bias_ids;
+    const float* bias;
+    int64_t bias_stride;
+    const int32_t* allowed;
+    const int32_t* allowed_rows;
+    int64_t allowed_count, allowed_stride;
+    void* cuda_stream;
+} gtok_x_adjustment;
+int32_t gtok_x_adjust_logits(const gtok_x_adjustment* args);
+
+/* An id for each row of logits [n, vocab] (vocab at most 2^24).  With m = exp((l - max) / temperature), ids go in order of falling logits, equal ones in order of rising ids.  The first top_k
+ * are kept (all, where it is 0 or less); of these the fewest whose m make up at least top_p of theirs (all, where it is 1 or more; one, where it is 0 or less); of these the ones with m >= min_p;
+ * the first in any case.  ids[i] is the first id, in the order of ids, at which the running sum of the kept m exceeds u[i] times their sum (u from 0, below 1); logprobs[i] is
+ * the logarithm of its share of all m, kept or not.  Temperature 0 gives the first id and logprob 0.  Masses and their sums have 64 bits and do not depend on the order of summation.
+ * -infinity is never drawn; a row of nothing else gives id -1 and logprob -infinity.  A row with a NaN, or whose temperature is negative or not finite, whose u is outside its range
+ * or whose top_p or min_p is NaN gives id -1 and logprob NaN.  Parameters: a value for each row or, where NULL, the one_ value for all. */
+typedef struct {
+    gtok_x_matrix logits;
+    const void* u;           /* n numbers */
+    int32_t u_bits;          /* fp32 or fp64: 32 or 64 */
+    int32_t one_top_k;
+    const float* temperature;
+    const int32_t* top_k;
+    const float *top_p, *min_p;
+    float one_temperature, one_top_p, one_min_p;
+    int32_t reserved;
+    int32_t* ids;
+    float* logprobs;
+    void* cuda_stream;
+} gtok_x_draw;
+int32_t gtok_x_sample(const gtok_x_draw* args);
+
 #ifdef __cplusplus
 }
 #endif
