@@ -37,7 +37,7 @@ def _newer(target, deps):
 
 # The C boundary, on which no profile depends, and the operators on a model's tables, whose profiles have a hash of their own.
 ABI_SOURCES = ("gtok_abi.cc", "vocab_abi.cc")
-VOCAB_SOURCES = ("sm100.cuh", "vocab_launch.cuh", "vocab_loss.cu", "vocab_next.cu", "vocab_next.h", "vocab_ops.h", "vocab_quant.cu", "vocab_rows.cu")
+VOCAB_SOURCES = ("sm100.cuh", "vocab_launch.cuh", "vocab_loss.cu", "vocab_maps.h", "vocab_next.cu", "vocab_next.h", "vocab_ops.h", "vocab_quant.cu", "vocab_rows.cu")
 
 
 def _hash_of(names):

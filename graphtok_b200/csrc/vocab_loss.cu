@@ -17,6 +17,7 @@
 // neither time nor NaN of masked positions is carried along.
 #include "sm100.cuh"
 #include "vocab_launch.cuh"
+#include "vocab_maps.h"
 #include "vocab_ops.h"
 
 #include <algorithm>
@@ -1267,28 +1268,6 @@ Plan make_plan(const LossCall& c, bool backward) {
     }
     p.bytes = at;
     return p;
-}
-
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                              CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encode_fn() {
-    static const EncodeFn fn = [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult got;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &got) != cudaSuccess || got != cudaDriverEntryPointSuccess) f = nullptr;
-        return reinterpret_cast<EncodeFn>(f);
-    }();
-    return fn;
-}
-
-// Lines of 128 bytes, `height` of them a box, swizzled.
-bool tile_map(CUtensorMap* map, int type, const void* data, int64_t rows, int64_t cols, int64_t stride, int height) {
-    const int size = type == kF32 ? 4 : 2;
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(stride * size)};
-    const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size), static_cast<cuuint32_t>(height)}, steps[2] = {1, 1};
-    const CUtensorMapDataType kind = type == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    return encode_fn()(map, kind, 2, const_cast<void*>(data), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int MODE>

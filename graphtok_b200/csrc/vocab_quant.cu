@@ -3,7 +3,9 @@
 // z[i, v] = sum over groups g of s[v, g] * sum over k in g of (q[v, k] - b[v, g]) * h[i, k], with codes q of 0 to 15, a scale s and a zero b
 // (8 where there are none) for each group of a row.  q - b is a whole number of at most 15 and exact in bf16 and fp16, so the inner sums are
 // matrix products of what is stored, in fp32, and only they are scaled: no weight is rounded on the way.
+#include "sm100.cuh"
 #include "vocab_launch.cuh"
+#include "vocab_maps.h"
 #include "vocab_next.h"
 
 #include <cuda_bf16.h>
@@ -161,8 +163,8 @@ __global__ void __launch_bounds__(256) quantize_kernel(const __grid_constant__ Q
 }
 
 // ---- products -------------------------------------------------------------------------
-constexpr int kWarps = 16, kThreads = kWarps * 32, kAhead = 4;
-constexpr int kPartLine = 36;              // floats from a row of hidden states to the next among partial sums: lanes of a fragment meet no bank twice
+constexpr int kWarps = 16, kThreads = kWarps * 32, kAhead = 2;
+constexpr int kPartLine = 68;              // floats from a row of hidden states to the next among partial sums: lanes of a fragment meet no bank twice
 
 struct LogitsArgs {
     const uint4* codes;
@@ -172,24 +174,28 @@ struct LogitsArgs {
     int64_t hidden_stride;
     void* out;
     int64_t out_stride, vocab, width;
-    int64_t tiles, groups;
-    int units, group_units;        // of 64 columns; how many share a group (0: each has two)
+    int tiles, groups;             // (no more than 2^19 tiles of 2^10 units or 2^11 groups)
+    int units;                     // of 64 columns
+    uint32_t per_group;            // 2^20 / how many of them share a group, rounded up; 0: each has two groups
     int rows;                      // of hidden states, at most 8 NT
     int split, split_log;          // warps that share a tile
     bool staged;                   // hidden states fit into shared memory
+    int buffers;                   // of partial sums
 };
 
 template <bool BF16> struct Half16;
 template <> struct Half16<true> {
     using type = __nv_bfloat16;
     static constexpr uint32_t kBase = 0x43004300u;             // 128 + code, twice
+    static __device__ __forceinline__ float lower_half(uint32_t w) { return __uint_as_float(w << 16); }
+    static __device__ __forceinline__ float upper_half(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
     static __device__ __forceinline__ uint32_t pair(uint32_t zero) { return kBase + (zero << 16 | zero); }
     static __device__ __forceinline__ uint32_t minus(uint32_t a, uint32_t b) {
         const __nv_bfloat162 r = __hsub2(reinterpret_cast<const __nv_bfloat162&>(a), reinterpret_cast<const __nv_bfloat162&>(b));
         return reinterpret_cast<const uint32_t&>(r);
     }
     static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint2 b) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
     }
@@ -197,13 +203,15 @@ template <> struct Half16<true> {
 template <> struct Half16<false> {
     using type = __half;
     static constexpr uint32_t kBase = 0x64006400u;             // 1024 + code, twice
+    static __device__ __forceinline__ float lower_half(uint32_t w) { return __low2float(reinterpret_cast<const __half2&>(w)); }
+    static __device__ __forceinline__ float upper_half(uint32_t w) { return __high2float(reinterpret_cast<const __half2&>(w)); }
     static __device__ __forceinline__ uint32_t pair(uint32_t zero) { return kBase + (zero << 16 | zero); }
     static __device__ __forceinline__ uint32_t minus(uint32_t a, uint32_t b) {
         const __half2 r = __hsub2(reinterpret_cast<const __half2&>(a), reinterpret_cast<const __half2&>(b));
         return reinterpret_cast<const uint32_t&>(r);
     }
     static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint2 b) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
     }
@@ -217,12 +225,13 @@ __device__ __forceinline__ uint32_t hidden_pair(const LogitsArgs& a, int n, int6
     return high << 16 | low;
 }
 
-// What a lane has under way of one unit pair: 32 rows x 64 columns.
+// What a lane has under way: 64 rows x 64 columns, two tiles' units.
+constexpr int kHalves = 4;                 // of 16 rows
 template <int SUBS, bool ZEROS>
 struct Lot {
-    uint4 code[2];
-    uint2 scale[SUBS];             // of the lane's four rows, 16 bits each
-    uint32_t zero[ZEROS ? SUBS : 1];
+    uint4 code[kHalves];
+    uint2 scale[2][SUBS];          // of a tile's four rows that are the lane's, 16 bits each
+    uint32_t zero[2][ZEROS ? SUBS : 1];
 };
 
 __device__ __forceinline__ uint4 load_once(const uint4* p) {
@@ -231,44 +240,62 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
     return v;
 }
 
+// Up to 8 NT rows of hidden states.  Warps take 64 rows of the table and every `split`th unit of the width; those that share rows add up through
+// shared memory when they are done with them.  Codes come from memory straight into the lanes that multiply with them, kAhead steps before they are
+// needed, across the ends of rows; hidden states lie in shared memory in the order of operands.  What bounds it: memory, and not far below the integer units, which make
+// two codes of a word in 3.5 operations (shift, and-or twice; the subtraction is another unit's) at half of an SM's rate.
 template <bool BF16, int NT, int SUBS, bool ZEROS, typename Out>
 __global__ void __launch_bounds__(kThreads, 1) few_rows_kernel(const __grid_constant__ LogitsArgs a) {
     using H = Half16<BF16>;
+    using T = typename H::type;
     extern __shared__ uint4 smem[];
     constexpr int kPart = 8 * NT * kPartLine;                  // floats of a warp's partial sums
-    float* parts = reinterpret_cast<float*>(smem);             // [2][kWarps][kPart]
-    uint2* staged = reinterpret_cast<uint2*>(parts + 2 * kWarps * kPart);      // [units * 4][NT][32]
+    float* parts = reinterpret_cast<float*>(smem);             // [buffers][kWarps][kPart]
+    uint2* staged = reinterpret_cast<uint2*>(parts + a.buffers * kWarps * kPart);      // [units * 4][NT][32]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     after_previous();
     let_next_begin();
-    const int64_t first = a.tiles * blockIdx.x / gridDim.x, last = a.tiles * (blockIdx.x + 1) / gridDim.x;
+    // of pairs of tiles
+    const int pairs = (a.tiles + 1) / 2, first = static_cast<int>(static_cast<int64_t>(pairs) * blockIdx.x / gridDim.x),
+              last = static_cast<int>(static_cast<int64_t>(pairs) * (blockIdx.x + 1) / gridDim.x);
     const int at_once = kWarps >> a.split_log, part = warp & (a.split - 1), slot = warp >> a.split_log;
-    const int64_t rounds = (last - first + at_once - 1) >> (4 - a.split_log);
-    const int count = (a.units - part + a.split - 1) >> a.split_log;           // units of a tile that are this warp's; one at least
+    const int rounds = (last - first + at_once - 1) >> (4 - a.split_log);
+    const int count = (a.units - part + a.split - 1) >> a.split_log;           // units of a row that are this warp's; one at least
 
-    // Units are fetched kAhead before they are needed, across the ends of tiles.
     Lot<SUBS, ZEROS> lot[kAhead];
-    int64_t fetch_round = 0;
-    int fetch_i = 0;
-    const auto fetch = [&](Lot<SUBS, ZEROS>& l) {
-        if (fetch_round >= rounds) return;
-        int64_t tile = first + fetch_round * at_once + slot;
-        if (tile >= last) tile = last - 1;                     // (its sums are left out)
-        const int u = part + (fetch_i << a.split_log);
-        const uint4* p = a.codes + (tile * a.units + u) * 64 + lane;
-        l.code[0] = load_once(p);
-        l.code[1] = load_once(p + 32);
+    int fetch_round = 0, fetch_u = part;
+    const uint4* fetch_at[2];
+    int fetch_tile[2];
+    const auto start = [&] {
+        const int pair = min(first + fetch_round * at_once + slot, last - 1);  // (behind the last: its sums are left out)
 #pragma unroll
-        for (int s = 0; s < SUBS; ++s) {
-            const int64_t g = tile * a.groups + (SUBS == 2 ? u * 2 + s : u / a.group_units);
-            l.scale[s] = __ldg(reinterpret_cast<const uint2*>(a.scales + g * 32) + lane / 4);
-            if constexpr (ZEROS) l.zero[s] = __ldg(reinterpret_cast<const uint32_t*>(a.zeros + g * 32) + lane / 4);
-        }
-        if (++fetch_i == count) {
-            fetch_i = 0;
-            ++fetch_round;
+        for (int t = 0; t < 2; ++t) {
+            fetch_tile[t] = min(2 * pair + t, a.tiles - 1);
+            fetch_at[t] = a.codes + static_cast<int64_t>(fetch_tile[t] * a.units + part) * 64 + lane;
         }
     };
+    const auto fetch = [&](Lot<SUBS, ZEROS>& l) {
+        if (fetch_round >= rounds) return;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            l.code[2 * t] = load_once(fetch_at[t]);
+            l.code[2 * t + 1] = load_once(fetch_at[t] + 32);
+            fetch_at[t] += a.split * 64;
+#pragma unroll
+            for (int s = 0; s < SUBS; ++s) {
+                const uint32_t g = fetch_tile[t] * a.groups + (SUBS == 2 ? fetch_u * 2 + s : fetch_u * a.per_group >> 20);
+                l.scale[t][s] = __ldg(reinterpret_cast<const uint2*>(a.scales) + static_cast<uint64_t>(g) * 8 + lane / 4);
+                if constexpr (ZEROS) l.zero[t][s] = __ldg(reinterpret_cast<const uint32_t*>(a.zeros) + static_cast<uint64_t>(g) * 8 + lane / 4);
+            }
+        }
+        fetch_u += a.split;
+        if (fetch_u >= a.units) {
+            fetch_u = part;
+            ++fetch_round;
+            start();
+        }
+    };
+    start();
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) fetch(lot[s]);
     if (a.staged) {
@@ -280,63 +307,63 @@ __global__ void __launch_bounds__(kThreads, 1) few_rows_kernel(const __grid_cons
         __syncthreads();
     }
 
-    float acc[2][NT][4] = {};
-    int i = 0, buffer = 0;
-    int64_t round = 0;
+    float acc[kHalves][NT][4] = {};
+    int i = 0, buffer = 0, round = 0;
     while (round < rounds) {
 #pragma unroll
         for (int s = 0; s < kAhead; ++s) {
             if (round >= rounds) break;
             const Lot<SUBS, ZEROS>& l = lot[s];
             const int u = part + (i << a.split_log);
+            constexpr int kSteps = 4 / SUBS;                   // of 16 columns in a group's part
 #pragma unroll
             for (int sub = 0; sub < SUBS; ++sub) {
-                float sum[2][NT][4] = {};
-                uint32_t base[4];
+                uint2 b[kSteps][NT];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) base[r] = H::pair(ZEROS ? l.zero[ZEROS ? sub : 0] >> (8 * r) & 15 : 8);
-#pragma unroll
-                for (int k = 4 / SUBS * sub; k < 4 / SUBS * (sub + 1); ++k) {
-                    uint2 b[NT];
+                for (int k = 0; k < kSteps; ++k)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        if (a.staged) b[nt] = staged[((u * 4 + k) * NT + nt) * 32 + lane];
+                        const int step = u * 4 + sub * kSteps + k;
+                        if (a.staged) b[k][nt] = staged[(step * NT + nt) * 32 + lane];
                         else {
-                            const int64_t col = (u * 4 + k) * 16 + 2 * (lane & 3);
-                            b[nt] = make_uint2(hidden_pair(a, nt * 8 + lane / 4, col), hidden_pair(a, nt * 8 + lane / 4, col + 8));
+                            const int64_t col = step * 16 + 2 * (lane & 3);
+                            b[k][nt] = make_uint2(hidden_pair(a, nt * 8 + lane / 4, col), hidden_pair(a, nt * 8 + lane / 4, col + 8));
                         }
                     }
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const uint32_t w = k == 0 ? l.code[half].x : k == 1 ? l.code[half].y : k == 2 ? l.code[half].z : l.code[half].w;
+                for (int half = 0; half < kHalves; ++half) {
+                    float sum[NT][4] = {};
+                    uint32_t base[2];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) base[r] = H::pair(ZEROS ? l.zero[half / 2][ZEROS ? sub : 0] >> (16 * (half & 1) + 8 * r) & 15 : 8);
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k) {
+                        const int word = sub * kSteps + k;
+                        const uint32_t w = word == 0 ? l.code[half].x : word == 1 ? l.code[half].y : word == 2 ? l.code[half].z : l.code[half].w;
                         uint32_t q[4];
 #pragma unroll
-                        for (int p = 0; p < 4; ++p) q[p] = H::minus((w >> (4 * p) & 0x000F000Fu) | H::kBase, base[half * 2 + (p & 1)]);
+                        for (int p = 0; p < 4; ++p) q[p] = H::minus((w >> (4 * p) & 0x000F000Fu) | H::kBase, base[p & 1]);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) H::mma(sum[half][nt], q, b[nt]);
+                        for (int nt = 0; nt < NT; ++nt) H::mma(sum[nt], q, b[k][nt]);
                     }
-                }
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    using T = typename H::type;
-                    const uint32_t w = half ? l.scale[sub].y : l.scale[sub].x;
-                    const float upper = to_float<T>(reinterpret_cast<const T*>(&w)[0]), lower = to_float<T>(reinterpret_cast<const T*>(&w)[1]);
+                    const uint32_t w = half & 1 ? l.scale[half / 2][sub].y : l.scale[half / 2][sub].x;
+                    const float upper = H::lower_half(w), lower = H::upper_half(w);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        acc[half][nt][0] = fmaf(upper, sum[half][nt][0], acc[half][nt][0]);
-                        acc[half][nt][1] = fmaf(upper, sum[half][nt][1], acc[half][nt][1]);
-                        acc[half][nt][2] = fmaf(lower, sum[half][nt][2], acc[half][nt][2]);
-                        acc[half][nt][3] = fmaf(lower, sum[half][nt][3], acc[half][nt][3]);
+                        acc[half][nt][0] = fmaf(upper, sum[nt][0], acc[half][nt][0]);
+                        acc[half][nt][1] = fmaf(upper, sum[nt][1], acc[half][nt][1]);
+                        acc[half][nt][2] = fmaf(lower, sum[nt][2], acc[half][nt][2]);
+                        acc[half][nt][3] = fmaf(lower, sum[nt][3], acc[half][nt][3]);
                     }
                 }
             }
             fetch(lot[s]);
             if (++i < count) continue;
-            // The tiles of a round are done: partial sums of the warps that share one are added in their order.
+            // The rows of a round are done: partial sums of the warps that share some are added in their order.
             i = 0;
             float* mine = parts + (buffer * kWarps + warp) * kPart;
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int half = 0; half < kHalves; ++half)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -345,39 +372,384 @@ __global__ void __launch_bounds__(kThreads, 1) few_rows_kernel(const __grid_cons
                         acc[half][nt][e] = 0.f;
                     }
             asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");        // (warps come here from different places of the unrolled loop)
-            for (int o = tid; o < at_once * a.rows * 32; o += kThreads) {
-                const int r = o & 31, n = (o >> 5) % a.rows, t = (o >> 5) / a.rows;
-                const int64_t tile = first + round * at_once + t, v = tile * 32 + r;
-                if (tile >= last || v >= a.vocab) continue;
+            for (int o = tid; o < at_once * a.rows * 64; o += kThreads) {
+                const int r = o & 63, n = (o >> 6) % a.rows, t = (o >> 6) / a.rows;
+                const int pair = first + round * at_once + t;
+                const int64_t v = static_cast<int64_t>(pair) * 64 + r;
+                if (pair >= last || v >= a.vocab) continue;
                 const float* from = parts + (buffer * kWarps + (t << a.split_log)) * kPart + n * kPartLine + r;
                 float total = from[0];
                 for (int p = 1; p < a.split; ++p) total += from[p * kPart];
                 static_cast<Out*>(a.out)[n * a.out_stride + v] = from_float<Out>(total);
             }
-            buffer ^= 1;
+            if (a.buffers > 1) buffer ^= 1;
+            else asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
             ++round;
         }
     }
 }
 
-int few_smem(int nt, int units, bool staged) { return 2 * kWarps * 8 * nt * kPartLine * 4 + (staged ? units * 4 * nt * 32 * 8 : 0); }
+int few_smem(int nt, int units, bool staged, int buffers) { return buffers * kWarps * 8 * nt * kPartLine * 4 + (staged ? units * 4 * nt * 32 * 8 : 0); }
 constexpr int kMostSmem = 227 * 1024;
+// Above them the kernel for more (13 rows of 151,665 x 2560: 95 us here and 131 there; 17 would be two passes here).
+constexpr int kFewRows = 16;
 
 template <bool BF16, int NT, int SUBS, bool ZEROS, typename Out>
 cudaError_t few_rows(const LogitsArgs& a, int blocks, cudaStream_t stream) {
     auto* kernel = few_rows_kernel<BF16, NT, SUBS, ZEROS, Out>;
-    const int smem = few_smem(NT, a.units, a.staged);
+    const int smem = few_smem(NT, a.units, a.staged, a.buffers);
     if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem)) return e;
     return launch(kernel, blocks, kThreads, smem, stream, a);
 }
 template <bool BF16, int NT, typename Out>
 cudaError_t few_rows(const LogitsArgs& a, int blocks, cudaStream_t stream) {
-    if (a.group_units == 0) return a.zeros ? few_rows<BF16, NT, 2, true, Out>(a, blocks, stream) : few_rows<BF16, NT, 2, false, Out>(a, blocks, stream);
+    if (a.per_group == 0) return a.zeros ? few_rows<BF16, NT, 2, true, Out>(a, blocks, stream) : few_rows<BF16, NT, 2, false, Out>(a, blocks, stream);
     return a.zeros ? few_rows<BF16, NT, 1, true, Out>(a, blocks, stream) : few_rows<BF16, NT, 1, false, Out>(a, blocks, stream);
 }
 template <bool BF16, typename Out>
 cudaError_t few_rows(const LogitsArgs& a, int nt, int blocks, cudaStream_t stream) {
     return nt == 1 ? few_rows<BF16, 1, Out>(a, blocks, stream) : few_rows<BF16, 2, Out>(a, blocks, stream);
+}
+
+// ---- products with more rows --------------------------------------------------------------
+// As for few rows, with the matrix instruction that takes 256 of the table's rows at a time, two blocks of a cluster half of them each, and all hidden states as columns.
+// Eight warps of a block make 16-bit operands of codes, in registers, and put them into tensor memory, from where the instruction takes them: a stage holds 128 rows x 64 columns.
+// Hidden states come to shared memory by tiled copies, each block half of the rows.  A group's product is taken out of tensor memory by eight more warps and added, with its
+// scale, to sums in registers, while the next group's goes to the other half of the accumulators.
+//
+// Bound by reading the codes up to some 60 rows, and beyond by this taking out: a row of hidden states costs an addition for each row of the table and group.
+constexpr int kManyStages = 4, kTakers = 8, kCodeStages = 10, kAheadMeta = 8;
+// Warps that make operands.  In groups of 32 columns the taking out is what is slow, and more of them are in its way: 125 rows of 151,665 x 2048 236 us with eight,
+// 212 with four; in groups of 128, 47 rows of 128,256 x 4096, 128 and 171.
+__host__ __device__ constexpr int makers(bool two) { return two ? 4 : 8; }
+__host__ __device__ constexpr int many_threads(bool two) { return 32 * (makers(two) + kTakers + 3); }
+constexpr int kMostColumns = 128;          // of hidden states
+constexpr int kManySmem = 1024 + kManyStages * (kMostColumns / 2) * 256 + kCodeStages * 8192 + 1024;
+
+struct ManyArgs {
+    const uint4* codes;
+    const uint16_t* scales;
+    const uint32_t* zeros;         // of eight times four rows; NULL: 8 everywhere
+    void* out;
+    int64_t out_stride, vocab;
+    int tiles, groups;             // of 32 rows; of a row
+    int units, group_units;        // of 64 columns; how many share a group (0: each has two)
+    uint32_t per_group;
+    int rows;
+    bool wide;                     // logits are fp32
+};
+
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void load_line(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ uint4 shared_uint4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+// 16 lanes x 32 columns: register 2 i + r of lane l goes to lane l / 4 + 8 r, column 4 i + l % 4.
+__device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <int NC>
+__device__ __forceinline__ void tmem_take(uint32_t at, float (&v)[NC]) {       // on their way
+#pragma unroll
+    for (int c = 0; c < NC; c += 8)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=f"(v[c]), "=f"(v[c + 1]), "=f"(v[c + 2]), "=f"(v[c + 3]), "=f"(v[c + 4]), "=f"(v[c + 5]), "=f"(v[c + 6]), "=f"(v[c + 7])
+                     : "r"(at + c));
+}
+template <int NC>
+__device__ __forceinline__ void tmem_taken(float (&v)[NC]) {                   // there
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < NC; c += 8)
+        asm volatile("" : "+f"(v[c]), "+f"(v[c + 1]), "+f"(v[c + 2]), "+f"(v[c + 3]), "+f"(v[c + 4]), "+f"(v[c + 5]), "+f"(v[c + 6]), "+f"(v[c + 7]));
+}
+// s += scale * v, two at a time
+__device__ __forceinline__ void add_scaled(float& s0, float& s1, float scale, float v0, float v1) {
+    asm("{\n.reg .b64 s, f, v;\nmov.b64 s, {%0, %1};\nmov.b64 f, {%2, %2};\nmov.b64 v, {%3, %4};\nfma.rn.f32x2 s, f, v, s;\nmov.b64 {%0, %1}, s;\n}"
+        : "+f"(s0), "+f"(s1)
+        : "f"(scale), "f"(v0), "f"(v1));
+}
+// The left operand lies in tensor memory: a lane a row, two elements to a column.
+__device__ __forceinline__ void mma_from_tmem(uint32_t acc, uint32_t a, uint64_t b, uint32_t kind, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(acc), "r"(a), "l"(b), "r"(kind),
+                 "r"(static_cast<uint32_t>(add))
+                 : "memory");
+}
+
+// NC: columns of a taking warp, half of all.  TWO: a unit has two groups, else a group has one or more units.
+template <bool BF16, int NC, bool TWO>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(many_threads(TWO), 1) many_rows_kernel(const __grid_constant__ CUtensorMap map_hidden, const __grid_constant__ ManyArgs a) {
+    using namespace sm100;
+    using H = Half16<BF16>;
+    constexpr int kMakers = makers(TWO), kTurns = kMakers / 4, kStageBytes = NC * 256, kAcc = kManyStages * 64;             // accumulators lie behind the stages
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_addr(smem_raw) + 1023) & ~1023u;
+    const uint32_t codes = base + kManyStages * kStageBytes, full = codes + kCodeStages * 8192, empty = full + 8 * kManyStages, acc_full = empty + 8 * kManyStages,
+                   acc_empty = acc_full + 16, code_full = acc_empty + 16, code_empty = code_full + 8 * kCodeStages, tmem_at = code_empty + 8 * kCodeStages;
+    const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;           // (of which the compiler knows that it is one for all)
+    const uint32_t rank = cluster_rank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kManyStages; ++s) {
+            bar_init(full + 8 * s, 2 * 4 + 1);                 // four warps of each block, and the copies
+            bar_init(empty + 8 * s, 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            bar_init(acc_full + 8 * s, 1);
+            bar_init(acc_empty + 8 * s, 2 * kTakers);
+        }
+        for (int s = 0; s < kCodeStages; ++s) {
+            bar_init(code_full + 8 * s, 1);
+            bar_init(code_empty + 8 * s, 4);
+        }
+        bar_init_fence();
+    }
+    if (warp == 0) tmem_alloc(tmem_at, 512);
+    __syncthreads();
+    fence_before();
+    cluster_sync();
+    fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
+    after_previous();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, blocks = (a.tiles + 7) / 8;        // of 256 rows
+    const int stages = (a.units + 1) / 2;      // of two units; the last one of a tile may have one
+    bool ok = true;
+
+    if (warp < kMakers) {
+        // Codes to operands: a warp every other unit of its 32 rows, which are its quarter of tensor memory.
+        const int quarter = warp & 3, turn = warp >> 2;
+        const uint32_t to = tmem + (static_cast<uint32_t>(quarter * 32) << 16), full_of_pair = in_block(full, 0);
+        const int steps = (blocks - pair + pairs - 1) / pairs * stages;
+        uint32_t handed = 0;                   // the barrier of a stage that is on its way to tensor memory
+        const auto hand_over = [&] {
+            tmem_stored();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive_cluster(handed);         // (what is handed over is in tensor memory, and there)
+        };
+        int step = turn % stages, block = pair + turn / stages * pairs;
+        for (int it = turn; it < steps && ok; it += kTurns) {
+            const uint32_t cs = it % kCodeStages, s = it % kManyStages;
+            const int u = 2 * step, many = min(2, a.units - u);
+            uint32_t z[2][2] = {{0x08080808u, 0x08080808u}, {0x08080808u, 0x08080808u}};
+            if (a.zeros) {
+                const int tile = min(block * 8 + static_cast<int>(rank) * 4 + quarter, a.tiles - 1);
+                const uint32_t* of_tile = a.zeros + static_cast<uint64_t>(tile * a.groups) * 8 + lane / 4;
+                const auto group = [&](int unit) { return TWO ? unit * 2 : static_cast<int>(unit * a.per_group >> 20); };
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (h < many) {
+                        z[h][0] = __ldg(of_tile + group(u + h) * 8);
+                        if (TWO) z[h][1] = __ldg(of_tile + group(u + h) * 8 + 8);
+                    }
+                if (u + kAheadMeta < a.units) prefetch(of_tile + group(u + kAheadMeta) * 8);
+            }
+            for (step += kTurns; step >= stages; step -= stages) block += pairs;
+            ok = __all_sync(~0u, bar_wait(code_full + 8 * cs, (it / kCodeStages) & 1));
+            if (!ok) break;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (h >= many) break;
+                const uint32_t at = codes + cs * 8192 + quarter * 2048 + h * 1024 + lane * 16;
+                const uint4 code[2] = {shared_uint4(at), shared_uint4(at + 512)};
+                uint32_t q[2][16];
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t w = k == 0 ? code[half].x : k == 1 ? code[half].y : k == 2 ? code[half].z : code[half].w;
+#pragma unroll
+                        for (int p = 0; p < 4; ++p)
+                            q[half][4 * k + p] = H::minus((w >> (4 * p) & 0x000F000Fu) | H::kBase, H::pair(z[h][TWO ? k >> 1 : 0] >> (16 * half + 8 * (p & 1)) & 15));
+                    }
+                if (h == 0) {
+                    if (handed) hand_over();
+                    ok = __all_sync(~0u, bar_wait(empty + 8 * s, ((it / kManyStages) & 1) ^ 1));
+                    if (!ok) break;
+                    fence_after();
+                }
+                tmem_store(to + s * 64 + h * 32, q[0]);
+                tmem_store(to + (16u << 16) + s * 64 + h * 32, q[1]);
+            }
+            __syncwarp();
+            if (lane == 0) bar_arrive(code_empty + 8 * cs);
+            handed = full_of_pair + 8 * s;
+        }
+        if (handed && ok) hand_over();
+    } else if (warp < kMakers + kTakers) {
+        // Products to sums: a warp 32 rows and half of the columns.
+        const int quarter = warp & 3, half = (warp - kMakers) >> 2;
+        const int place = (lane & 7) * 4 + (lane >> 3);
+        uint32_t acc = 0;
+        for (int t = pair; t < blocks; t += pairs) {
+            const int tile = min(t * 8 + static_cast<int>(rank) * 4 + quarter, a.tiles - 1);
+            const uint16_t* scales = a.scales + static_cast<int64_t>(tile) * a.groups * 32 + place;
+            float sum[NC];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) sum[c] = 0.f;
+            uint32_t next = __ldg(scales);
+            for (int g = 2; g < 2 + kAheadMeta && g < a.groups; g += 2) prefetch(scales + g * 32);
+            for (int g = 0; g < a.groups && ok; ++g, ++acc) {
+                const float scale = H::lower_half(next);
+                if (g + 1 < a.groups) next = __ldg(scales + (g + 1) * 32);
+                if (g + 2 + kAheadMeta < a.groups) prefetch(scales + (g + 2 + kAheadMeta) * 32);
+                ok = __all_sync(~0u, bar_wait(acc_full + 8 * (acc & 1), (acc >> 1) & 1));
+                if (!ok) break;
+                fence_after();
+                // in parts, as registers allow; the next one comes while one is added
+                constexpr int kOnce = NC <= 32 ? NC : 16, kParts = NC / kOnce;
+                const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + kAcc + (acc & 1) * 2 * NC + half * NC;
+                float v[kParts > 1 ? 2 : 1][kOnce];
+                tmem_take<kOnce>(at, v[0]);
+#pragma unroll
+                for (int part = 0; part < kParts; ++part) {
+                    float (&w)[kOnce] = v[kParts > 1 ? part & 1 : 0];
+                    tmem_taken<kOnce>(w);
+                    if (part + 1 < kParts) tmem_take<kOnce>(at + (part + 1) * kOnce, v[kParts > 1 ? part + 1 & 1 : 0]);
+                    else {
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive_cluster(in_block(acc_empty + 8 * (acc & 1), 0));
+                    }
+#pragma unroll
+                    for (int c = 0; c < kOnce; c += 2) add_scaled(sum[part * kOnce + c], sum[part * kOnce + c + 1], scale, w[c], w[c + 1]);
+                }
+            }
+            const int64_t row = static_cast<int64_t>(t) * 256 + rank * 128 + quarter * 32 + lane;
+            if (row >= a.vocab) continue;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int n = half * NC + c;
+                if (n >= a.rows) break;
+                const float x = ok ? sum[c] : __int_as_float(0x7FC00000);      // (a wait that ran out: nothing that could be taken for logits)
+                if (a.wide) static_cast<float*>(a.out)[n * a.out_stride + row] = x;
+                else static_cast<typename H::type*>(a.out)[n * a.out_stride + row] = from_float<typename H::type>(x);
+            }
+        }
+    } else if (warp == kMakers + kTakers) {
+        // Hidden states.
+        const uint32_t full_of_pair = in_block(full, 0);
+        uint32_t it = 0;
+        for (int t = pair; t < blocks && ok; t += pairs)
+            for (int step = 0; step < stages; ++step, ++it) {
+                const uint32_t s = it % kManyStages;
+                ok = __all_sync(~0u, bar_wait(empty + 8 * s, ((it / kManyStages) & 1) ^ 1));
+                if (!ok) break;
+                const bool two = 2 * step + 1 < a.units;
+                if (elect()) {
+                    if (rank == 0) bar_expect(full + 8 * s, two ? 2 * kStageBytes : kStageBytes);
+                    load_tile(base + s * kStageBytes, &map_hidden, step * 128, rank * NC, full_of_pair + 8 * s);
+                    if (two) load_tile(base + s * kStageBytes + NC * 128, &map_hidden, step * 128 + 64, rank * NC, full_of_pair + 8 * s);
+                }
+                __syncwarp();
+            }
+        for (uint32_t i = it < kManyStages ? 0 : it - kManyStages; i < it && ok; ++i) ok = __all_sync(~0u, bar_wait(empty + 8 * (i % kManyStages), (i / kManyStages) & 1));
+        if (!ok) {                             // (copies that are under way end before the block does)
+            const uint64_t from = nanoseconds();
+            while (nanoseconds() - from < 2000000ull) __nanosleep(1000);
+        }
+    } else if (warp == kMakers + kTakers + 1) {
+        // Codes.
+        uint32_t it = 0;
+        for (int t = pair; t < blocks && ok; t += pairs) {
+            const uint4* from[4];
+#pragma unroll
+            for (int quarter = 0; quarter < 4; ++quarter)
+                from[quarter] = a.codes + static_cast<int64_t>(min(t * 8 + static_cast<int>(rank) * 4 + quarter, a.tiles - 1)) * a.units * 64;
+            for (int step = 0; step < stages; ++step, ++it) {
+                const uint32_t s = it % kCodeStages, bytes = 2 * step + 1 < a.units ? 2048 : 1024;
+                ok = __all_sync(~0u, bar_wait(code_empty + 8 * s, ((it / kCodeStages) & 1) ^ 1));
+                if (!ok) break;
+                if (elect()) {
+                    bar_expect(code_full + 8 * s, 4 * bytes);
+#pragma unroll
+                    for (int quarter = 0; quarter < 4; ++quarter) load_line(codes + s * 8192 + quarter * 2048, from[quarter] + step * 128, bytes, code_full + 8 * s);
+                }
+                __syncwarp();
+            }
+        }
+        for (uint32_t i = it < kCodeStages ? 0 : it - kCodeStages; i < it && ok; ++i) ok = __all_sync(~0u, bar_wait(code_empty + 8 * (i % kCodeStages), (i / kCodeStages) & 1));
+        if (!ok) {
+            const uint64_t from = nanoseconds();
+            while (nanoseconds() - from < 2000000ull) __nanosleep(1000);
+        }
+    } else if (rank == 0 && elect()) {
+        // Products.
+        const uint32_t kind = mma_kind(BF16, false, false, 2 * NC);
+        uint32_t it = 0, acc = 0;
+        int in_group = 0;
+        // One unit, in one thread and without more branches than there have to be: each costs the others' way through the instruction cache.
+        const auto unit = [&](uint32_t b, uint32_t from, bool last) {
+            if (in_group == 0) {
+                if (!bar_wait(acc_empty + 8 * (acc & 1), ((acc >> 1) & 1) ^ 1)) return false;
+                fence_after();
+            }
+            const uint64_t b0 = operand(b, false);                     // (32 bytes on: 2 more)
+            const uint32_t to = tmem + kAcc + (acc & 1) * 2 * NC;
+            mma_from_tmem(to, from, b0, kind, in_group > 0);
+            mma_from_tmem(to, from + 8, b0 + 2, kind, true);
+            uint32_t second = to;
+            if (TWO) {                         // (the unit's second group)
+                mma_commit(acc_full + 8 * (acc & 1));
+                ++acc;
+                if (!bar_wait(acc_empty + 8 * (acc & 1), ((acc >> 1) & 1) ^ 1)) return false;
+                fence_after();
+                second = tmem + kAcc + (acc & 1) * 2 * NC;
+            }
+            mma_from_tmem(second, from + 16, b0 + 4, kind, !TWO);
+            mma_from_tmem(second, from + 24, b0 + 6, kind, true);
+            if (TWO || ++in_group == a.group_units || last) {
+                in_group = 0;
+                mma_commit(acc_full + 8 * (acc & 1));
+                ++acc;
+            }
+            return true;
+        };
+        for (int t = pair; t < blocks && ok; t += pairs)
+            for (int step = 0; step < stages; ++step, ++it) {
+                const uint32_t s = it % kManyStages, b = base + s * kStageBytes, from = tmem + s * 64;
+                if (!bar_wait(full + 8 * s, (it / kManyStages) & 1)) { ok = false; break; }
+                fence_after();
+                const bool two = 2 * step + 1 < a.units, last = step + 1 == stages;
+                ok = unit(b, from, last && !two);
+                if (ok && two) ok = unit(b + NC * 128, from + 32, last);
+                if (!ok) break;
+                mma_commit(empty + 8 * s);
+            }
+    }
+    __syncwarp();
+    let_next_begin();
+    __syncthreads();
+    fence_before();
+    cluster_sync();
+    fence_after();
+    if (warp == 0) tmem_free(tmem, 512);
+}
+
+template <bool BF16, int NC>
+cudaError_t many_rows(const CUtensorMap& map, const ManyArgs& a, int blocks, cudaStream_t stream) {
+    auto* kernel = a.group_units ? many_rows_kernel<BF16, NC, false> : many_rows_kernel<BF16, NC, true>;
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem)) return e;
+    return launch(kernel, blocks, many_threads(!a.group_units), kManySmem, stream, map, a);
+}
+template <bool BF16>
+cudaError_t many_rows(const CUtensorMap& map, const ManyArgs& a, int columns, int blocks, cudaStream_t stream) {
+    switch (columns) {
+        case 8: return many_rows<BF16, 8>(map, a, blocks, stream);
+        case 16: return many_rows<BF16, 16>(map, a, blocks, stream);
+        case 24: return many_rows<BF16, 24>(map, a, blocks, stream);
+        case 32: return many_rows<BF16, 32>(map, a, blocks, stream);
+        case 48: return many_rows<BF16, 48>(map, a, blocks, stream);
+        default: return many_rows<BF16, 64>(map, a, blocks, stream);
+    }
 }
 
 const char* said(cudaError_t e) { return e == cudaSuccess ? nullptr : cudaGetErrorString(e); }
@@ -435,20 +807,56 @@ const char* table_logits(const Matrix& hidden, const Table4& t, const Matrix& ou
     a.out_stride = out.stride;
     a.vocab = t.vocab;
     a.width = t.width;
-    a.tiles = p.tiles;
-    a.groups = p.groups;
+    a.tiles = static_cast<int>(p.tiles);
+    a.groups = static_cast<int>(p.groups);
     a.units = static_cast<int>(p.units);
-    a.group_units = t.group == 32 ? 0 : static_cast<int>(t.group / 64);
-    const int blocks = static_cast<int>(std::min<int64_t>(148, p.tiles));
-    // warps that share a tile: all, or as many as there are units
-    a.split_log = 4;
-    while ((1 << a.split_log) > a.units) --a.split_log;
+    // (u / d for u and d up to 1024: u times the rounding is less than 1 / d of 2^20)
+    a.per_group = t.group == 32 ? 0 : static_cast<uint32_t>(div_up(1 << 20, t.group / 64));
+    const int64_t pairs = div_up(p.tiles, 2);
+    const int blocks = static_cast<int>(std::min<int64_t>(148, pairs));
+    // Warps that share rows: so many that the slowest warp of the fullest block takes the fewest steps, of which adding up at the end of its rows is about one.
+    const auto steps = [&](int log) { return div_up(div_up(pairs, blocks), kWarps >> log) * (div_up(a.units, 1 << log) + 1); };
+    a.split_log = 0;
+    for (int log = 1; log <= 4 && (1 << log) <= a.units; ++log)
+        if (steps(log) <= steps(a.split_log)) a.split_log = log;
     a.split = 1 << a.split_log;
     const int size = out.type == kF32 ? 4 : 2;
+    // Tiled copies of hidden states take lines of whole 16 bytes.
+    const bool whole = reinterpret_cast<uintptr_t>(hidden.data) % 16 == 0 && hidden.stride % 8 == 0 && hidden.stride >= hidden.cols;
+    ManyArgs m{};
+    m.codes = a.codes;
+    m.scales = a.scales;
+    m.zeros = reinterpret_cast<const uint32_t*>(a.zeros);
+    m.out_stride = out.stride;
+    m.vocab = t.vocab;
+    m.tiles = a.tiles;
+    m.groups = a.groups;
+    m.units = a.units;
+    m.group_units = t.group == 32 ? 0 : static_cast<int>(t.group / 64);
+    m.per_group = a.per_group;
+    m.wide = out.type == kF32;
     for (int64_t row = 0; row < hidden.rows;) {
         const int64_t left = hidden.rows - row;
-        const int nt = left > 8 && few_smem(2, a.units, true) <= kMostSmem ? 2 : 1;
-        a.staged = few_smem(nt, a.units, true) <= kMostSmem;
+        const bool few = few_smem(2, a.units, true, 1) <= kMostSmem;           // two tiles of eight rows are at hand
+        if (left > (few ? kFewRows : 8) && whole) {
+            // Rows in equal parts, as a part of few rows costs about what one of many does.
+            const int rows = static_cast<int>(div_up(left, div_up(left, kMostColumns))), needed = (rows + 15) / 16 * 8;
+            const int columns = needed <= 32 ? needed : needed <= 48 ? 48 : 64;
+            CUtensorMap map;
+            if (!encode_fn()) return "the driver has no tiled copies";
+            if (!tile_map(&map, hidden.type, static_cast<const uint16_t*>(hidden.data) + row * hidden.stride, rows, hidden.cols, hidden.stride, columns))
+                return "a tensor map was refused";
+            m.out = static_cast<char*>(const_cast<void*>(out.data)) + row * out.stride * size;
+            m.rows = rows;
+            const cudaError_t e = hidden.type == kBF16 ? many_rows<true>(map, m, columns, 2 * static_cast<int>(std::min<int64_t>(74, div_up(p.tiles, 8))), stream)
+                                                       : many_rows<false>(map, m, columns, 2 * static_cast<int>(std::min<int64_t>(74, div_up(p.tiles, 8))), stream);
+            if (e != cudaSuccess) return cudaGetErrorString(e);
+            row += rows;
+            continue;
+        }
+        const int nt = left > 8 && few ? 2 : 1;
+        a.staged = few_smem(nt, a.units, true, 1) <= kMostSmem;
+        a.buffers = few_smem(nt, a.units, a.staged, 2) <= kMostSmem ? 2 : 1;
         a.rows = static_cast<int>(std::min<int64_t>(left, 8 * nt));
         a.hidden = static_cast<const uint16_t*>(hidden.data) + row * hidden.stride;
         a.out = static_cast<char*>(const_cast<void*>(out.data)) + row * out.stride * size;
