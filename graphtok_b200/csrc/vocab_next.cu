@@ -32,16 +32,18 @@ struct alignas(sizeof(T) * N) Lump {
 
 // ---- penalties, biases, masks -------------------------------------------------------
 // A block takes a slice of a row.  It counts the row's history into shared memory, as far as it lies in the slice, and then passes over
-// the slice once.  Bound by memory: a logit read and written, a bit of a mask; in place, only what changes.
-constexpr int kAdjustThreads = 512;
+// the slice once, the logits of which are on their way meanwhile.  Bound by memory: a logit read and written, a bit of a mask; in place, only what changes.
+// A cluster that goes over a history once, each block a part, and counts into one another's shared memory, waits for the block with the frequent ids: 251 rows of 128,256
+// with 12,500 ids each TIMES.
+constexpr int kAdjustThreads = 512, kMostSlice = 16384;
 constexpr int kSpare = 8;                        // ids of the lump in front of a slice
 constexpr uint32_t kSaid = 0x80000000u;          // of a count: the id is in the prompt
 
 struct AdjustArgs {
     const void* logits;
     void* out;
-    int64_t stride, out_stride, vocab, slices;
-    int slice;
+    int64_t stride, out_stride;
+    int vocab, slice, slices;
     bool in_place, history;
     const void* ids;
     int id_bits;
@@ -58,12 +60,13 @@ struct AdjustArgs {
 };
 
 template <typename T, int N>
-__global__ void __launch_bounds__(kAdjustThreads) adjust_kernel(const __grid_constant__ AdjustArgs a) {
+__global__ void __launch_bounds__(kAdjustThreads, 3) adjust_kernel(const __grid_constant__ AdjustArgs a) {
     extern __shared__ uint4 smem[];
     uint32_t* count = reinterpret_cast<uint32_t*>(smem);                       // [slice + kSpare]
-    uint16_t* entry = reinterpret_cast<uint16_t*>(count + a.slice + kSpare);   // [slice + kSpare]: place in the list of biases and 1, where there are any
-    float* sums = reinterpret_cast<float*>(entry + a.slice + kSpare);          // [entries]
-    int32_t* listed = reinterpret_cast<int32_t*>(sums + a.entries);
+    uint32_t* biased = count + a.slice + kSpare;                               // [kMostSlice / 32 + 1]: a bit for each id that has a bias
+    float* bias = reinterpret_cast<float*>(biased + kMostSlice / 32 + 1);      // [entries]
+    int32_t* listed = reinterpret_cast<int32_t*>(bias + a.entries);            // [entries]
+    __shared__ int twice;                                                      // an id comes more than once
     const int tid = threadIdx.x;
     after_previous();
     let_next_begin();
@@ -72,43 +75,10 @@ __global__ void __launch_bounds__(kAdjustThreads) adjust_kernel(const __grid_con
     const T* in = static_cast<const T*>(a.logits) + row * a.stride;
     T* out = static_cast<T*>(a.out) + row * a.out_stride;
     // Lumps lie on 16 bytes of the input, whatever the row begins at; the first one of the row is no whole one.
-    const int64_t off = N == 1 ? 0 : static_cast<int64_t>((16 - reinterpret_cast<uintptr_t>(in) % 16) % 16 / sizeof(T));
-    const int64_t base = off + static_cast<int64_t>(s) * a.slice - N;          // id of count[0]
-    const int64_t begin = s == 0 ? 0 : base + N, end = base + N + a.slice < a.vocab ? base + N + a.slice : a.vocab;
-
-    for (int i = tid; i < (a.slice + kSpare) / 4; i += kAdjustThreads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0, 0, 0, 0);
-    if (a.entries) {
-        for (int i = tid; i < (a.slice + kSpare) / 8; i += kAdjustThreads) reinterpret_cast<uint4*>(entry)[i] = make_uint4(0, 0, 0, 0);
-        for (int i = tid; i < a.entries; i += kAdjustThreads) listed[i] = a.bias_ids[row * a.bias_stride + i];
-    }
-    __syncthreads();
-    if (a.history) {
-        int64_t from = a.offsets[row], to = a.offsets[row + 1];
-        from = from < 0 ? 0 : from;
-        to = to > a.n_ids ? a.n_ids : to;
-        const int64_t behind = from + (a.prompt_lengths ? a.prompt_lengths[row] : 0);
-#pragma unroll 4
-        for (int64_t i = from + tid; i < to; i += kAdjustThreads) {
-            const int64_t id = a.id_bits == 64 ? static_cast<const int64_t*>(a.ids)[i] : static_cast<const int32_t*>(a.ids)[i];
-            if (id < begin || id >= end) continue;
-            if (i < behind) atomicOr(&count[id - base], kSaid);
-            else atomicAdd(&count[id - base], 1u);
-        }
-    }
-    // An id's biases are added up in the order of the list, at its first entry.
-    for (int i = tid; i < a.entries; i += kAdjustThreads) {
-        const int64_t id = listed[i];
-        if (id < begin || id >= end) continue;
-        bool first = true;
-        for (int j = 0; j < i && first; ++j) first = listed[j] != id;
-        if (!first) continue;
-        float sum = 0.f;
-        for (int j = i; j < a.entries; ++j)
-            if (listed[j] == id) sum += a.bias[row * a.bias_stride + j];
-        sums[i] = sum;
-        entry[id - base] = static_cast<uint16_t>(i + 1);
-    }
-    __syncthreads();
+    const int off = N == 1 ? 0 : static_cast<int>((16 - reinterpret_cast<uintptr_t>(in) % 16) % 16 / sizeof(T));
+    const int base = off + s * a.slice - N;                                    // id of count[0]
+    const int begin = s == 0 ? 0 : base + N, end = min(base + N + a.slice, a.vocab);
+    const int v_first = base + (s == 0 ? 0 : N) + tid * N;                     // this thread's first lump
 
     const float rho = a.repetition ? a.repetition[row] : a.one_repetition, presence = a.presence ? a.presence[row] : a.one_presence,
                 frequency = a.frequency ? a.frequency[row] : a.one_frequency;
@@ -119,59 +89,142 @@ __global__ void __launch_bounds__(kAdjustThreads) adjust_kernel(const __grid_con
         if (which >= a.allowed_count) nothing = true;
         else if (which >= 0) words = reinterpret_cast<const uint32_t*>(a.allowed) + which * a.allowed_stride;
     }
-    const auto changed = [&](float x, uint32_t c, int e, bool allowed) {
+    // The first logits and their bits of the mask are fetched while ids are counted; in place most logits are not needed.
+    constexpr int kFetch = 2;
+    Lump<T, N> ahead[kFetch];
+    uint32_t bits[kFetch];
+    const auto whole = [&](int v) { return v >= 0 && v < end && v + N <= a.vocab; };
+    const auto allowed_at = [&](int v) {
+        uint32_t b = nothing ? 0 : ~0u;
+        if (words) b = __funnelshift_r(words[v >> 5], words[(v + N - 1) >> 5], v & 31);
+        return b | ~((1u << N) - 1);
+    };
+#pragma unroll
+    for (int q = 0; q < kFetch; ++q) {
+        const int v = v_first + q * kAdjustThreads * N;
+        if (!whole(v)) continue;
+        if (!a.in_place) ahead[q] = *reinterpret_cast<const Lump<T, N>*>(in + v);
+        bits[q] = allowed_at(v);
+    }
+
+    for (int i = tid; i < (a.slice + kSpare) / 4; i += kAdjustThreads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0, 0, 0, 0);
+    if (a.entries) {
+        for (int i = tid; i < kMostSlice / 32 + 1; i += kAdjustThreads) biased[i] = 0;
+        for (int i = tid; i < a.entries; i += kAdjustThreads) {
+            listed[i] = a.bias_ids[row * a.bias_stride + i];
+            bias[i] = a.bias[row * a.bias_stride + i];
+        }
+        if (tid == 0) twice = 0;
+    }
+    __syncthreads();
+    if (a.history) {
+        int64_t from = a.offsets[row], to = a.offsets[row + 1];
+        from = from < 0 ? 0 : from;
+        to = to > a.n_ids ? a.n_ids : to;
+        const int64_t behind = from + (a.prompt_lengths ? a.prompt_lengths[row] : 0);
+        constexpr int kIds = 4;                // under way a thread
+        for (int64_t i = from + tid; i < to; i += kAdjustThreads * kIds) {
+            int64_t id[kIds];
+#pragma unroll
+            for (int q = 0; q < kIds; ++q) {
+                const int64_t at = i + q * kAdjustThreads;
+                id[q] = at >= to ? -1 : a.id_bits == 64 ? static_cast<const int64_t*>(a.ids)[at] : static_cast<const int32_t*>(a.ids)[at];
+            }
+#pragma unroll
+            for (int q = 0; q < kIds; ++q) {
+                if (id[q] < begin || id[q] >= end) continue;
+                if (i + q * kAdjustThreads < behind) atomicOr(&count[id[q] - base], kSaid);
+                else atomicAdd(&count[id[q] - base], 1u);
+            }
+        }
+    }
+    // Ids with a bias are changed by themselves in the end, by the thread of their first entry to come, which takes their logit before it is written.
+    constexpr int kBiases = (kMaxBiases + kAdjustThreads - 1) / kAdjustThreads;
+    T biased_logit[kBiases];
+    bool mine[kBiases];
+#pragma unroll
+    for (int q = 0; q < kBiases; ++q) {
+        const int i = tid + q * kAdjustThreads, id = i < a.entries ? listed[i] : -1;
+        mine[q] = false;
+        if (id < begin || id >= end) continue;
+        const uint32_t bit = 1u << (id & 31);
+        mine[q] = !(atomicOr(&biased[(id >> 5) - (begin >> 5)], bit) & bit);
+        if (mine[q]) biased_logit[q] = in[id];
+        else twice = 1;
+    }
+    __syncthreads();
+
+    const auto changed = [&](float x, uint32_t c, float b, bool allowed) {
         if (c) {
             x = x > 0.f ? x / rho : x * rho;
             const uint32_t times = c & ~kSaid;
             if (times) x = x - frequency * static_cast<float>(times) - presence;
         }
-        if (e) x += sums[e - 1];
-        return allowed ? x : -INFINITY;
+        return allowed ? x + b : -INFINITY;
     };
-    for (int64_t v0 = base + (s == 0 ? 0 : N) + static_cast<int64_t>(tid) * N; v0 < end; v0 += kAdjustThreads * N) {
-        if (N == 1 || (v0 >= 0 && v0 + N <= a.vocab)) {
-            if (v0 < 0) continue;                      // (single elements: the one before the row)
-            uint32_t allowed = nothing ? ~((1u << N) - 1) : ~0u;
-            if (words) {
-                const uint32_t low = words[v0 >> 5], high = words[(v0 + N - 1) >> 5];
-                allowed = __funnelshift_r(low, high, v0 & 31) | ~((1u << N) - 1);
-            }
-            uint32_t c[N], e[N], any = 0;
+    const auto allowed_one = [&](int v) { return !nothing && (!words || (words[v >> 5] >> (v & 31) & 1)); };
+    const auto lump = [&](int v0, bool fetched, Lump<T, N> x, uint32_t allowed) {
+        if (whole(v0)) {
+            if (!fetched) allowed = allowed_at(v0);
+            uint32_t c[N], any = 0;
+            if constexpr (N == 1) {
+                c[0] = count[v0 - base];
+            } else {                           // 16 bytes at a time
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                c[i] = count[v0 - base + i];
-                e[i] = a.entries ? entry[v0 - base + i] : 0;
-                any |= c[i] | e[i];
+                for (int i = 0; i < N; i += 4) {
+                    const uint4 four = *reinterpret_cast<const uint4*>(count + (v0 - base) + i);
+                    c[i] = four.x; c[i + 1] = four.y; c[i + 2] = four.z; c[i + 3] = four.w;
+                }
             }
-            if (a.in_place && !any && allowed == ~0u) continue;
-            Lump<T, N> x = *reinterpret_cast<const Lump<T, N>*>(in + v0);
+#pragma unroll
+            for (int i = 0; i < N; ++i) any |= c[i];
+            if (a.in_place && !any && allowed == ~0u) return;
+            if (!fetched || a.in_place) x = *reinterpret_cast<const Lump<T, N>*>(in + v0);
             if (any || allowed != ~0u)
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (c[i] || e[i] || !(allowed >> i & 1)) x.v[i] = from_float<T>(changed(to_float<T>(x.v[i]), c[i], static_cast<int>(e[i]), allowed >> i & 1));
+                    if (c[i] || !(allowed >> i & 1)) x.v[i] = from_float<T>(changed(to_float<T>(x.v[i]), c[i], -0.f, allowed >> i & 1));
             *reinterpret_cast<Lump<T, N>*>(out + v0) = x;
-        } else {
+        } else if (N > 1) {
             for (int i = 0; i < N; ++i) {
-                const int64_t v = v0 + i;
-                if (v < 0 || v >= a.vocab) continue;
-                const bool allowed = !nothing && (!words || (words[v >> 5] >> (v & 31) & 1));
+                const int v = v0 + i;
+                if (v < 0 || v >= end) continue;
+                const bool allowed = allowed_one(v);
                 const uint32_t c = count[v - base];
-                const int e = a.entries ? entry[v - base] : 0;
-                T x = in[v];
-                if (c || e || !allowed) x = from_float<T>(changed(to_float<T>(x), c, e, allowed));
-                out[v] = x;
+                T one = in[v];
+                if (c || !allowed) one = from_float<T>(changed(to_float<T>(one), c, -0.f, allowed));
+                out[v] = one;
             }
         }
+    };
+#pragma unroll
+    for (int q = 0; q < kFetch; ++q)
+        if (v_first + q * kAdjustThreads * N < end) lump(v_first + q * kAdjustThreads * N, true, ahead[q], bits[q]);
+    for (int v = v_first + kFetch * kAdjustThreads * N; v < end; v += kAdjustThreads * N) lump(v, false, ahead[0], 0);
+    if (!a.entries) return;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kBiases; ++q) {
+        if (!mine[q]) continue;
+        const int i = tid + q * kAdjustThreads, id = listed[i];
+        float sum = bias[i];
+        if (twice) {                           // in the order of the list, whichever entry this is
+            sum = 0.f;
+            for (int j = 0; j < a.entries; ++j)
+                if (listed[j] == id) sum += bias[j];
+        }
+        out[id] = from_float<T>(changed(to_float<T>(biased_logit[q]), count[id - base], sum, allowed_one(id)));
     }
 }
 
 template <typename T, int N>
 cudaError_t adjust(AdjustArgs a, int64_t rows, cudaStream_t stream) {
     // Slices of 16,384 ids count a long history least often; of fewer where that leaves SMs without work.
-    a.slice = 16384;
+    a.slice = kMostSlice;
     while (a.slice > 2048 && rows * div_up(a.vocab, a.slice) < 148) a.slice /= 2;
-    a.slices = div_up(a.vocab, a.slice);
-    const int smem = (a.slice + kSpare) * (a.entries ? 6 : 4) + a.entries * 8;
+    a.slices = static_cast<int>(div_up(a.vocab, a.slice));
+    a.slice = static_cast<int>(round_up(div_up(a.vocab, a.slices), 64));
+    const int smem = (a.slice + kSpare) * 4 + (a.entries ? (kMostSlice / 32 + 1) * 4 + a.entries * 8 : 0);
     auto* kernel = adjust_kernel<T, N>;
     if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024)) return e;
     return launch(kernel, rows * a.slices, kAdjustThreads, smem, stream, a);
@@ -1188,7 +1241,7 @@ const char* adjust_logits(const AdjustCall& c) {
     a.out = const_cast<void*>(c.out.data);
     a.stride = c.logits.stride;
     a.out_stride = c.out.stride;
-    a.vocab = c.logits.cols;
+    a.vocab = static_cast<int>(c.logits.cols);
     a.in_place = a.logits == a.out;
     a.history = c.offsets != nullptr;
     a.ids = c.ids.data;

@@ -179,6 +179,9 @@ def _logits(hidden, table, dtype, index):
     flat = _rows(hidden if hidden.dim() == 2 else hidden.reshape(hidden.shape[:-1].numel(), hidden.shape[-1]))
     out = torch.empty((*hidden.shape[:-1], table.vocab), dtype=dtype, device=hidden.device)
     n = flat.shape[0]
+    if n > 8 and (flat.data_ptr() % 16 or flat.stride(0) % 8):       # more rows are copied by whole 16 bytes
+        width = flat.shape[1]
+        flat = torch.empty((n, -(-width // 8) * 8), dtype=flat.dtype, device=flat.device)[:, :width].copy_(flat)
     if n:
         code = _lib().gtok_x_table4_logits(_matrix(flat), table._args, _Matrix(out.data_ptr(), n, table.vocab, table.vocab, _TYPES[dtype]), _stream(index))
         if code:
