@@ -861,12 +861,12 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
             }
             v = join(v, a.blocks);
             const float mean = v.y / v.w;
-            if (lane == 0) s.seen[0] = make_float4(v.x, mean, sqrtf(fmaxf(v.z / v.w - mean * mean, 0.f)), 0.f);
+            if (lane == 0) s.seen[0] = make_float4(v.x, mean, sqrtf(fmaxf(v.z / v.w - mean * mean, 0.f)), v.w * (16 / sizeof(T)));
         }
         __syncthreads();
     }
     row.top = __float_as_uint(s.seen[0].x);
-    const float mean = s.seen[0].y, deviation = s.seen[0].z;
+    const float mean = s.seen[0].y, deviation = s.seen[0].z, finite_ids = s.seen[0].w;
     const bool bad = row.top == kNone || !(heat >= 0.f && heat <= 3.402823466e38f) || !(u >= 0.0 && u < 1.0) || top_p != top_p || min_p != min_p;
     if (bad || row.top <= kLowest) {
         if (block == 0 && tid == 0) {
@@ -913,8 +913,11 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         while (min_key > kLowest + 1 && in(min_key - 1)) --min_key;
         while (min_key < row.top && !in(min_key)) ++min_key;
     }
-    // What is near: two and a half deviations above the mean, and no more than 12 below the largest.
-    uint32_t near = row.top < kHighest ? key_of(fminf(fmaxf(mean + 2.5f * deviation, most_value - 12.f), most_value)) : row.top;
+    // What is near: some 400 ids, more than top_k in any case, if logits were distributed normally (the quantile by Abramowitz and Stegun's 26.2.22), and nothing that is
+    // more than 12 below the largest where that may leave out no id of the top_k.
+    const float part = fminf(fmaxf(by_k ? 1.5f * top_k + 100.f : 400.f, 1.f) / fmaxf(finite_ids, 1.f), 0.5f), t = sqrtf(-2.f * logf(part));
+    const float above_mean = part < 0.5f ? t - (2.30753f + 0.27061f * t) / (1.f + t * (0.99229f + 0.04481f * t)) : -8.f;
+    uint32_t near = row.top < kHighest ? key_of(fminf(fmaxf(mean + above_mean * deviation, by_k ? -INFINITY : most_value - 12.f), most_value)) : row.top;
     if (near > row.top || near <= kLowest) near = row.top;
     const float near_value = value_of(near);
     float rest_end = fmaxf(mean - 3.f * deviation, near_value - 64.f * fmaxf(1.f, heat));
@@ -1003,22 +1006,22 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     };
     bool summed = true;                        // warp_mass and `before` hold what is kept
     if (cuts) {
-        // The bin of what is near in which the first cut lies, and how many ids there are down to its end.
+        // The bin of what is near in which the first cut lies, kBins if it lies lower.
         uint64_t above = 0, target = 0;
-        int bin = 0;
+        int bin = kBins;
         if (by_k || by_p) {
             target = by_k ? static_cast<uint64_t>(top_k) : p_target();
             bin = locate(s, !by_k, target, above);
-        } else {
-            bin = min_key >= near ? near_bins(value_of(min_key)) : kBins;
         }
+        // The last bin of which ids may be kept, and how many there are down to its end.  (Of both top_k and top_p it takes all of the top_k to say where the latter cuts.)
+        const int end_bin = by_min && min_key >= near && !(by_k && by_p) ? min(bin, near_bins(value_of(min_key))) : bin;
         uint32_t ids = 0;
         for (int b = lane; b < kBins; b += 32)
-            if (b <= bin) ids += s.all_count[b];
+            if (b <= end_bin) ids += s.all_count[b];
         ids = __reduce_add_sync(~0u, ids);
-        if (bin < kBins && ids <= kRanked) {
+        if (end_bin < kBins && ids <= kRanked) {
             // ---- Few candidates: the first block ranks them, cuts and draws.
-            pick_ids(row, near_bins.least(bin), row.top, all, false);
+            pick_ids(row, near_bins.least(end_bin), row.top, all, false);
             sm100::cluster_sync();
             if (block == 0) {
                 gather_picked(row);
@@ -1206,11 +1209,14 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     sm100::cluster_sync();                                     // (no block leaves while another may read from it)
 }
 
+// Blocks that find an SM each, in clusters of so many: the SMs of a processing cluster (18 or so) that are left over when they are more than two stay idle.
+constexpr int alone(int blocks) { return blocks > 2 ? 128 : 148; }
+
 template <typename T>
 cudaError_t draw(const DrawArgs& a, int64_t rows, cudaStream_t stream) {
     // Blocks that find an SM each are to have one: no two of them fit.
     int smem = static_cast<int>(sizeof(DrawShared)) + a.listed * 8 + (a.held ? a.segment * kDrawWarps * 4 : 0);
-    if (rows * a.blocks <= 148) smem = std::max(smem, 116 * 1024);
+    if (rows * a.blocks <= alone(a.blocks)) smem = std::max(smem, 116 * 1024);
     auto* kernel = draw_kernel<T>;
     if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024)) return e;
     cudaLaunchConfig_t config{};
@@ -1280,9 +1286,14 @@ const char* sample(const SampleCall& c) {
     a.logits = c.logits.data;
     a.stride = c.logits.stride;
     a.vocab = static_cast<int>(c.logits.cols);
-    // Blocks of a row: the fewer, the less they wait for one another; the more, the more of the GPU works on few rows.
+    // Blocks of a row, by what was measured for 128,256 ids in fp32 without cuts: 8 us and 35 over the blocks where each block has an SM to itself, 1.5 times that where two share
+    // one (1.75 for rows in one block), in as many rounds as it takes.  (47 rows with top-k, top-p and min-p: 76, 49, 42 and 55 us in 1, 2, 4 and 8 blocks; 1 row 75, 45, 31
+    // and 24; 251 rows 134, 131, 156 and 221.)
     a.blocks = 1;
-    const auto cost = [&](int blocks) { return static_cast<double>(div_up(c.logits.rows * blocks, 148)) * (0.8 * a.vocab / blocks + 12000); };
+    const auto cost = [&](int blocks) {
+        const int64_t all = c.logits.rows * blocks;
+        return (8 + 35 * (a.vocab / 128256.0) / blocks) * (all <= alone(blocks) ? 1 : (blocks == 1 ? 1.75 : 1.5) * div_up(all, 296));
+    };
     for (int blocks = 2; blocks <= kMostBlocks; blocks *= 2)
         if (cost(blocks) < cost(a.blocks)) a.blocks = blocks;
     a.segment = static_cast<int>(round_up(div_up(a.vocab, a.blocks * kDrawWarps), 32));
