@@ -403,18 +403,31 @@ struct Row {                       // a block's share of a row
         }
     }
 
-    // f(logits, place) for this thread's share, in which a warp's ids follow one another, kAtOnce of them at a time, 32 apart; NaN behind the last.
+    // f(logits, place of the first) for this thread's share, in which a warp's ids follow one another, kAtOnce of them at a time; NaN behind the last.
     static constexpr int kAtOnce = 4;
     template <typename F>
     __device__ __forceinline__ void some(F f) const {
         const int from = (threadIdx.x >> 5) * segment, to = from + segment < count ? from + segment : count;
+        const bool together = held || reinterpret_cast<uintptr_t>(in) % (kAtOnce * sizeof(T)) == 0;    // (segments are whole lots)
         float next[kAtOnce];                   // a step ahead: from memory they take longer than a step
         const auto fetch = [&](int i) {
+            if (together && i + kAtOnce <= to) {
+                if (held) {
+                    const float4 v = *reinterpret_cast<const float4*>(held + i);
+                    next[0] = v.x; next[1] = v.y; next[2] = v.z; next[3] = v.w;
+                } else {
+                    const Lump<T, kAtOnce> v = *reinterpret_cast<const Lump<T, kAtOnce>*>(in + i);
 #pragma unroll
-            for (int q = 0; q < kAtOnce; ++q) next[q] = i + 32 * q < to ? value(i + 32 * q) : __int_as_float(0x7FC00000);
+                    for (int q = 0; q < kAtOnce; ++q) next[q] = to_float<T>(v.v[q]);
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < kAtOnce; ++q) next[q] = i + q < to ? value(i + q) : __int_as_float(0x7FC00000);
+            }
         };
-        fetch(from + (threadIdx.x & 31));
-        for (int i = from + (threadIdx.x & 31); i < to; i += 32 * kAtOnce) {
+        const int first_place = from + (threadIdx.x & 31) * kAtOnce;
+        fetch(first_place);
+        for (int i = first_place; i < to; i += 32 * kAtOnce) {
             float x[kAtOnce];
 #pragma unroll
             for (int q = 0; q < kAtOnce; ++q) x[q] = next[q];
@@ -427,7 +440,7 @@ struct Row {                       // a block's share of a row
     __device__ __forceinline__ void each(F f) const {
         some([&](const float (&x)[kAtOnce], int i) {
 #pragma unroll
-            for (int q = 0; q < kAtOnce; ++q) f(x[q], i + 32 * q);
+            for (int q = 0; q < kAtOnce; ++q) f(x[q], i + q);
         });
     }
     // The sum of the masses of what f(logit, place) holds for.
@@ -437,7 +450,7 @@ struct Row {                       // a block's share of a row
         some([&](const float (&x)[kAtOnce], int i) {
             bool in[kAtOnce], any = false;
 #pragma unroll
-            for (int q = 0; q < kAtOnce; ++q) any |= in[q] = f(x[q], i + 32 * q);
+            for (int q = 0; q < kAtOnce; ++q) any |= in[q] = f(x[q], i + q);
             if (!__any_sync(__activemask(), any)) return;
             int64_t m[kAtOnce];
             masses(x, m);
