@@ -537,6 +537,20 @@ struct Row {                       // a block's share of a row
     }
 };
 
+// The least key from lo to hi for which in(key) holds, which does for hi and for all keys above one for which it does; asked by whole warps.
+template <typename F>
+__device__ __forceinline__ uint32_t least_key(uint32_t lo, uint32_t hi, F in) {
+    while (lo < hi) {                                          // a lane a place: a 32nd of what is left
+        const uint32_t step = ((hi - lo) >> 5) + 1, mine = static_cast<uint32_t>(min(static_cast<uint64_t>(hi), lo + static_cast<uint64_t>(threadIdx.x & 31) * step));
+        const uint32_t found = __ballot_sync(~0u, in(mine));
+        const int at = found ? __ffs(found) - 1 : 32;          // the first of the lanes; `hi` if there is none
+        const uint32_t up = at < 32 ? __shfl_sync(~0u, mine, at & 31) : hi, down = at ? __shfl_sync(~0u, mine, (at - 1) & 31) + 1 : lo;
+        hi = up;
+        lo = at ? down : up;
+    }
+    return lo;
+}
+
 // Bins of an interval of keys [low, high], the highest first.  Even in the logits where it is wide, in the keys where it is not or `by_key` says so.
 template <int N>
 struct Bins {
@@ -567,16 +581,7 @@ struct Bins {
             const uint64_t down = (static_cast<uint64_t>(b + 1) << shift) - 1;
             return down >= high - low ? low : high - static_cast<uint32_t>(down);
         }
-        uint32_t lo = low, hi = high;                          // hi: in the bin or higher
-        while (lo < hi) {                                      // a lane a place: a 32nd of what is left
-            const uint32_t step = ((hi - lo) >> 5) + 1, mine = static_cast<uint32_t>(min(static_cast<uint64_t>(hi), lo + static_cast<uint64_t>(threadIdx.x & 31) * step));
-            const uint32_t in = __ballot_sync(~0u, (*this)(value_of(mine)) <= b);
-            const int at = in ? __ffs(in) - 1 : 32;            // the first that is in; `hi` if no lane's is
-            const uint32_t up = at < 32 ? __shfl_sync(~0u, mine, at & 31) : hi, down = at ? __shfl_sync(~0u, mine, (at - 1) & 31) + 1 : lo;
-            hi = up;
-            lo = at ? down : up;
-        }
-        return lo;
+        return least_key(low, high, [&](uint32_t k) { return (*this)(value_of(k)) <= b; });      // `high` is in bin 0
     }
 };
 
@@ -917,14 +922,11 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     const bool by_k = !one && top_k > 0 && top_k < a.vocab, by_p = !one && top_p < 1.f, by_min = !one && min_p > 0.f && row.top < kHighest;
     const Cut all{kLowest + 1, 0x7FFFFFFF};
     Cut cut = all;
-    // the least key with d / T >= log(min_p): next to that logit rounded to fp32
+    // the least key with d / T >= log(min_p)
     uint32_t min_key = kLowest + 1;
     if (by_min) {
         const double depth = log(static_cast<double>(min_p)) * static_cast<double>(heat);
-        const auto in = [&](uint32_t k) { return static_cast<double>(value_of(k)) - row.top_value >= depth; };
-        min_key = min(row.top, max(min_key, key_of(static_cast<float>(fmax(row.top_value + depth, -3.402823466e38)))));
-        while (min_key > kLowest + 1 && in(min_key - 1)) --min_key;
-        while (min_key < row.top && !in(min_key)) ++min_key;
+        min_key = least_key(min_key, row.top, [&](uint32_t k) { return static_cast<double>(value_of(k)) - row.top_value >= depth; });
     }
     // What is near: some 400 ids, more than top_k in any case, if logits were distributed normally (the quantile by Abramowitz and Stegun's 26.2.22), and nothing that is
     // more than 12 below the largest where that may leave out no id of the top_k.

@@ -90,14 +90,36 @@ def _no_gradient(what, *tensors):
 # ---- tables in 4 bits -------------------------------------------------------------
 class QuantizedTable:
     """A table [vocab, width] in 4 bits, as `quantize_table` and `pack_table` make it: a scale in `dtype` (bfloat16 or float16), and with `zeros` a
-    zero, for every `group` columns of a row.  It lies in `data`, one uint8 tensor, in an order of its own."""
+    zero, for every `group` columns of a row.  It lies in `data`, one uint8 tensor, in an order of its own; `to`, copy.deepcopy and torch.save work as on tensors."""
 
-    def __init__(self, vocab, width, group, dtype, zeros, device):
-        self.vocab, self.width, self.group, self.dtype, self.zeros, self.device = vocab, width, group, dtype, zeros, device
+    def __init__(self, vocab, width, group, dtype, zeros, device, data=None):
+        self.vocab, self.width, self.group, self.dtype, self.zeros = vocab, width, group, dtype, zeros
         need = _done(_lib().gtok_x_table4_bytes(vocab, width, group, zeros), "gtok_x_table4_bytes")
-        self.data = torch.empty(need, dtype=torch.uint8, device=device)
-        self._index = self.data.get_device()
-        self._args = _Table4(self.data.data_ptr(), need, vocab, width, group, _TYPES[dtype], zeros)
+        if data is None:
+            data = torch.empty(need, dtype=torch.uint8, device=device)
+        elif data.shape != (need,) or data.dtype != torch.uint8 or not data.is_contiguous():
+            raise ValueError("data must be uint8 [%d]" % need)
+        self._data = data
+        self._args = _Table4(data.data_ptr(), need, vocab, width, group, _TYPES[dtype], zeros)
+
+    @property
+    def data(self):
+        return self._data
+
+    @property
+    def device(self):
+        return self._data.device
+
+    def to(self, device):
+        """The same table on another device."""
+        data = self._data.to(device)
+        return self if data is self._data else QuantizedTable(self.vocab, self.width, self.group, self.dtype, self.zeros, data.device, data)
+
+    def __reduce__(self):                  # (copies and files: the address is not part of it)
+        return QuantizedTable, (self.vocab, self.width, self.group, self.dtype, self.zeros, None, self._data)
+
+    def __deepcopy__(self, memo):
+        return QuantizedTable(self.vocab, self.width, self.group, self.dtype, self.zeros, None, self._data.clone())
 
     @property
     def shape(self):
@@ -170,7 +192,7 @@ def table_logits(hidden, table, dtype=torch.float32):
     if table.__class__ is not QuantizedTable and not isinstance(table, QuantizedTable):
         raise TypeError("table must be a QuantizedTable, as quantize_table and pack_table make it")
     _no_gradient("table_logits", hidden)
-    index = _on_gpu(hidden, hidden=hidden, table=table.data)
+    index = _on_gpu(hidden, hidden=hidden, table=table._data)
     if hidden.dtype != table.dtype:
         raise TypeError("hidden must be %s, as the table's scales are, not %s" % (table.dtype, hidden.dtype))
     if hidden.dim() < 1 or hidden.shape[-1] != table.width:

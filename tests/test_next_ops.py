@@ -633,6 +633,137 @@ def test_refusals(ops):
             ops.sample(*args, **named)
 
 
+def test_a_least_share_far_below_a_huge_logit(ops):
+    """The border of min_p among logits next to 0, where floating numbers lie so dense that their distance to the largest is the same for millions of them."""
+    logits = torch.cat([torch.tensor([1e10, 0.0, 1e-38, -1e-7, -1e-5, -1.0, -10.0]), torch.linspace(-3e-6, 3e-6, 2000)]).cuda().repeat(6, 1)
+    u = torch.tensor([0.0, 0.3, 0.6, 0.9, 0.99, 0.9999], device="cuda")
+    for heat in (1e10 / math.log(10), 1e10 / math.log(10) * (1 + 2.0 ** -23), 5e9):
+        check_draw(ops, logits, u, heat, 0, 1.0, 0.1)
+
+
+def test_tables_are_copied_and_kept(ops, tmp_path):
+    import copy
+    table = ops.quantize_table(randn(gen(60), 300, 200), zeros=True, dtype=F16)
+    hidden = randn(gen(61), 3, 200).to(F16)
+    want = ops.table_logits(hidden, table)
+    other = copy.deepcopy(table)
+    assert other.data.data_ptr() != table.data.data_ptr() and torch.equal(ops.table_logits(hidden, other), want)
+    torch.save(table, tmp_path / "table")
+    kept = torch.load(tmp_path / "table", weights_only=False, map_location="cpu")
+    with pytest.raises(ValueError, match="is on"):
+        ops.table_logits(hidden, kept)
+    assert torch.equal(ops.table_logits(hidden, kept.to("cuda")), want) and table.to("cuda") is table
+    with pytest.raises(AttributeError):
+        table.data = kept.data
+
+
+def test_in_inference_mode(ops):
+    with torch.inference_mode():
+        table = ops.quantize_table(randn(gen(70), 5000, 64))
+        logits = ops.table_logits(randn(gen(71), 4, 64).to(BF16), table)
+        assert ops.adjust_logits(logits, bias_ids=torch.tensor([7], dtype=torch.int32, device="cuda"), bias=torch.tensor([99.0], device="cuda"), out=logits) is logits
+        assert ops.sample(logits, torch.rand(4, generator=gen(72), device="cuda"), temperature=0.0)[0].tolist() == [7] * 4
+
+
+@pytest.mark.parametrize("n", [9, 16, 17, 33, 64, 65, 97, 128, 129, 200])
+def test_table_logits_of_more_rows_and_odd_lines(ops, n):
+    """Rows of hidden states that begin at odd addresses, for every number of columns that the kernels are made for."""
+    for width, group in ((130, 32), (191, 64), (320, 192)):
+        codes, scales, z, values = make_table(n + width, 601, width, group, BF16, True)
+        table = ops.pack_table(codes, scales, z, group=group)
+        room = randn(gen(n), n, width + 3).to(BF16)
+        for hidden in (room[:, 1:1 + width], room[:, :width].contiguous(), room[:1, :width].expand(n, width)):
+            check_logits(ops.table_logits(hidden, table), hidden, values, group)
+
+
+def test_c_entries_take_hidden_states_at_any_address(ops):
+    """Through the C entry, which makes no copies: more rows than a pass, odd addresses and strides, rows of the output apart."""
+    codes, scales, z, values = make_table(5, 333, 100, 64, F16, True)
+    table = ops.pack_table(codes, scales, z, group=64)
+    room = randn(gen(6), 70, 103).to(F16)
+    hidden = room[:, 2:102]
+    out = torch.full((70, 340), 5.0, device="cuda")
+    lib = ops._lib()
+    assert lib.gtok_x_table4_logits(ops._Matrix(hidden.data_ptr(), 70, 100, 103, 2), table._args, ops._Matrix(out.data_ptr() + 4, 70, 333, 340, 0), torch.cuda.current_stream().cuda_stream) == 0
+    check_logits(out[:, 1:334], hidden, values, 64)
+    assert (out[:, 0] == 5).all() and (out[:, 334:] == 5).all()
+    # and what they refuse
+    good = ops._Matrix(hidden.data_ptr(), 70, 100, 103, 2)
+    for m, o in ((ops._Matrix(hidden.data_ptr() + 1, 70, 100, 103, 2), ops._Matrix(out.data_ptr(), 70, 333, 340, 0)), (ops._Matrix(hidden.data_ptr(), 70, 99, 103, 2), ops._Matrix(out.data_ptr(), 70, 333, 340, 0)),
+                 (ops._Matrix(hidden.data_ptr(), 70, 100, 103, 1), ops._Matrix(out.data_ptr(), 70, 333, 340, 0)), (good, ops._Matrix(out.data_ptr(), 70, 333, 332, 0)),
+                 (good, ops._Matrix(out.data_ptr(), 70, 333, 340, 1)), (good, ops._Matrix(out.data_ptr() + 2, 70, 333, 340, 0)), (good, ops._Matrix(0, 70, 333, 340, 0)),
+                 (good, ops._Matrix(out.data_ptr(), 69, 333, 340, 0))):
+        assert lib.gtok_x_table4_logits(m, table._args, o, None) == -1
+    for change in (dict(data=table.data.data_ptr() + 16), dict(bytes=table.data.numel() - 1), dict(group=48), dict(type=0), dict(zeros=2), dict(data=0)):
+        bad = ops._Table4(table.data.data_ptr(), table.data.numel(), 333, 100, 64, 2, 1)
+        for k, v in change.items():
+            setattr(bad, k, v)
+        assert lib.gtok_x_table4_logits(good, bad, ops._Matrix(out.data_ptr(), 70, 333, 340, 0), None) == -1
+    logits = torch.zeros(3, 50, device="cuda")
+    a = ops._Adjustment()
+    a.logits, a.out, a.offsets, a.ids, a.id_bits, a.n_ids = ops._Matrix(logits.data_ptr(), 3, 50, 50, 0), ops._Matrix(logits.data_ptr(), 3, 50, 50, 0), 0, 0, 32, 0
+    assert lib.gtok_x_adjust_logits(a) == 0
+    for change in (dict(entries=1025), dict(entries=3), dict(offsets=logits.data_ptr() + 2), dict(repetition=logits.data_ptr() + 1), dict(allowed=12), dict(id_bits=16, offsets=logits.data_ptr()),
+                   dict(out=ops._Matrix(logits.data_ptr(), 3, 50, 60, 0)), dict(out=ops._Matrix(logits.data_ptr(), 3, 50, 50, 1)), dict(logits=ops._Matrix(logits.data_ptr(), 3, 0, 50, 0))):
+        b = ops._Adjustment()
+        b.logits, b.out, b.id_bits = a.logits, a.out, 32
+        for k, v in change.items():
+            setattr(b, k, v)
+        assert lib.gtok_x_adjust_logits(b) == -1, change
+    u, ids, logprobs = torch.zeros(3, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(3, device="cuda")
+    d = dict(logits=a.logits, u=u.data_ptr(), u_bits=32, one_temperature=1.0, one_top_p=1.0, ids=ids.data_ptr(), logprobs=logprobs.data_ptr())
+    for change, code in (({}, 0), (dict(u_bits=16), -1), (dict(u=0), -1), (dict(u=u.data_ptr() + 4, u_bits=64), -1), (dict(ids=0), -1), (dict(logprobs=logprobs.data_ptr() + 1), -1),
+                         (dict(temperature=u.data_ptr() + 2), -1), (dict(logits=ops._Matrix(logits.data_ptr(), 3, (1 << 24) + 1, 50, 0)), -1), (dict(logits=ops._Matrix(logits.data_ptr(), -1, 50, 50, 0)), -1)):
+        c = ops._Draw()
+        for k, v in (d | change).items():
+            setattr(c, k, v)
+        assert lib.gtok_x_sample(c) == code, change
+
+
+@pytest.mark.parametrize("n,vocab", [(1, 128256), (16, 20000), (17, 20000), (40, 9000), (70, 9000), (150, 5000), (300, 3000)])
+def test_every_share_of_a_row(ops, n, vocab):
+    """As many rows as make one to eight blocks of a row, held in shared memory or not."""
+    for i, wish in enumerate(((1.0, 0, 1.0, 0.0), (0.9, 30, 0.9, 0.0), (1.5, 0, 0.95, 0.0), (1.0, 900, 0.97, 0.0))):
+        check_draw(ops, model_logits(7 * n + i, n, vocab, BF16 if i % 2 else F32), torch.rand(n, generator=gen(i + n), device="cuda"), *wish)
+
+
+def test_rows_with_few_logits_left(ops):
+    """Masks that leave a few ids, fewer than top_k or hardly more, and lowest finite values in place of -inf."""
+    g = gen(80)
+    logits = randn(g, 40, 30000) * 2
+    lowest = torch.finfo(F32).min
+    for i in range(40):
+        keep = torch.randint(0, 30000, ((1, 2, 5, 39, 40, 41, 500, 2500)[i % 8],), generator=g, device="cuda")
+        masked = torch.full((30000,), -math.inf if i % 3 else lowest, device="cuda")
+        masked[keep] = logits[i, keep]
+        logits[i] = masked
+    u = torch.rand(40, generator=g, device="cuda")
+    for wish in ((1.0, 0, 1.0, 0.0), (0.8, 40, 1.0, 0.0), (0.8, 40, 0.9, 0.0), (1.0, 0, 0.5, 0.0), (1.0, 0, 0.999, 0.0), (1.0, 0, 0.9, 0.2), (1e38, 0, 0.9, 0.0)):
+        check_draw(ops, logits, u, *wish)
+
+
+@pytest.mark.parametrize("n", [1, 3, 60])
+def test_long_histories_of_every_kind(ops, n):
+    """Histories that pass a block's steps, with the ids that come most often at the beginning of the vocabulary, at its end, and all the same."""
+    g = gen(90 + n)
+    vocab = 50257
+    logits = randn(g, n, vocab)
+    parts = [torch.randint(0, 40, (4000,), generator=g, device="cuda"), vocab - 1 - torch.randint(0, 40, (4000,), generator=g, device="cuda"), torch.full((4001,), 7, device="cuda"),
+             torch.randint(0, vocab, (9000,), generator=g, device="cuda")]
+    row = torch.cat(parts)
+    ids = row.repeat(n)
+    offsets = (torch.arange(n + 1, device="cuda") * row.numel()).int()
+    prompts = torch.randint(0, row.numel() + 1, (n,), generator=g, device="cuda").int()
+    got = ops.adjust_logits(logits, ids, offsets, prompt_lengths=prompts, repetition=1.25, frequency=0.5, presence=2.0)
+    for i in range(n):
+        said = torch.zeros(vocab, dtype=torch.bool, device="cuda")
+        said[row] = True
+        times = torch.bincount(row[prompts[i]:], minlength=vocab).double()
+        x = logits[i].double()
+        want = torch.where(said, torch.where(x > 0, x / 1.25, x * 1.25), x) - 0.5 * times - 2.0 * (times > 0)
+        within(got[i], want, 4 * 2.0 ** -24 * (x.abs() * 1.25 + 0.5 * times + 2) * said, "logits")
+
+
 def test_the_version_of_what_is_written(ops):
     logits = randn(gen(1), 2, 100)
     before = logits._version
