@@ -322,12 +322,12 @@ __device__ __forceinline__ float upper_value(uint32_t key) { return value_of(key
 
 __device__ __forceinline__ uint64_t peer_u64(const uint64_t* p, int block) {
     uint64_t v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(sm100::in_block(sm100::smem_addr(p), block)) : "memory");
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(sm100::in_block(sm100::smem_addr(p), block)));
     return v;
 }
 __device__ __forceinline__ uint32_t peer_u32(const void* p, int block) {
     uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(sm100::in_block(sm100::smem_addr(p), block)) : "memory");
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(sm100::in_block(sm100::smem_addr(p), block)));
     return v;
 }
 
@@ -498,6 +498,24 @@ struct Row {                       // a block's share of a row
         }
     }
 
+    // The sum of a variable of all blocks, all of them fetched at once.
+    __device__ __forceinline__ uint64_t over_blocks(const uint64_t* p) const {
+        uint64_t v[kMostBlocks], sum = 0;
+#pragma unroll
+        for (int o = 0; o < kMostBlocks; ++o) v[o] = o < blocks ? peer_u64(p, o) : 0;
+#pragma unroll
+        for (int o = 0; o < kMostBlocks; ++o) sum += v[o];
+        return sum;
+    }
+    __device__ __forceinline__ uint32_t over_blocks(const uint32_t* p) const {
+        uint32_t v[kMostBlocks], sum = 0;
+#pragma unroll
+        for (int o = 0; o < kMostBlocks; ++o) v[o] = o < blocks ? peer_u32(p, o) : 0;
+#pragma unroll
+        for (int o = 0; o < kMostBlocks; ++o) sum += v[o];
+        return sum;
+    }
+
     // ---- bins: cleared, added to, told to the cluster, gathered
     __device__ void clear_bins() {
         for (int b = threadIdx.x; b < kBins; b += kDrawThreads) {
@@ -524,13 +542,9 @@ struct Row {                       // a block's share of a row
     __device__ void gather_bins(int buffer) {
         for (int b = threadIdx.x; b < 2 * kBins; b += kDrawThreads) {
             if (b < kBins) {
-                uint64_t m = 0;
-                for (int o = 0; o < blocks; ++o) m += peer_u64(&s.bin_mass[buffer][b], o);
-                s.all_mass[b] = m;
+                s.all_mass[b] = over_blocks(&s.bin_mass[buffer][b]);
             } else {
-                uint32_t c = 0;
-                for (int o = 0; o < blocks; ++o) c += peer_u32(&s.bin_count[buffer][b - kBins], o);
-                s.all_count[b - kBins] = c;
+                s.all_count[b - kBins] = over_blocks(&s.bin_count[buffer][b - kBins]);
             }
         }
         __syncthreads();
@@ -643,13 +657,16 @@ __device__ void gather_picked(Row<T>& row) {
     DrawShared& s = row.s;
     static_assert(kRanked <= kDrawThreads, "a thread an id");
     if (threadIdx.x >= kRanked) return;
-    int at = threadIdx.x, b = 0;
-    for (; b < row.blocks; ++b) {
-        const int n = static_cast<int>(peer_u32(&s.pick_n, b));
-        if (at < n) break;
-        at -= n;
-    }
-    if (b < row.blocks) {
+    int n[kMostBlocks], at = threadIdx.x, b = -1;
+#pragma unroll
+    for (int o = 0; o < kMostBlocks; ++o) n[o] = o < row.blocks ? static_cast<int>(peer_u32(&s.pick_n, o)) : 0;
+#pragma unroll
+    for (int o = 0; o < kMostBlocks; ++o)
+        if (b < 0) {
+            if (at < n[o]) b = o;
+            else at -= n[o];
+        }
+    if (b >= 0) {
         const uint32_t k = peer_u32(&s.pick_key[at], b);
         s.rank_key[threadIdx.x] = k;
         s.rank_id[threadIdx.x] = static_cast<int>(peer_u32(&s.pick_id[at], b));
@@ -1087,8 +1104,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         if (by_p && !by_k && bin == kBins && guess) {
             // About where the cut lies, from the counts of the rest's bins: a bin's ids at its middle.
             for (int b = tid; b < kGuessBins; b += kDrawThreads) {
-                uint32_t c = 0;
-                for (int o = 0; o < a.blocks; ++o) c += peer_u32(&s.guess[b], o);
+                const uint32_t c = row.over_blocks(&s.guess[b]);
                 const float middle = rest_bins.by_key ? near_value : 2.f * (rest_bins.top - (b + 0.5f) / rest_bins.per);
                 s.all_guess[b] = static_cast<float>(c) * expf((middle - most_value) / heat);
             }
