@@ -33,8 +33,9 @@ struct alignas(sizeof(T) * N) Lump {
 // ---- penalties, biases, masks -------------------------------------------------------
 // A block takes a slice of a row.  It counts the row's history into shared memory, as far as it lies in the slice, and then passes over
 // the slice once, the logits of which are on their way meanwhile.  Bound by memory: a logit read and written, a bit of a mask; in place, only what changes.
-// A cluster that goes over a history once, each block a part, and counts into one another's shared memory, waits for the block with the frequent ids: 251 rows of 128,256
-// with 12,500 ids each TIMES.
+// 251 rows of 128,256 bf16 with histories of 12,500 ids, 300 biases and masks: 109 us (22 at the rate of a copy); 44 of it with short histories and nothing else, the rest counting, masks and
+// biases.  A cluster that goes over a history once, each block a part, and counts into one another's shared memory waits for the block with the frequent ids: 266 us, when counting by
+// each block took 220.  Slices of half the size, four blocks to an SM: 173 us where 145.  One row of 128,256 with 911 ids: 3.8 us, all latency.
 constexpr int kAdjustThreads = 512, kMostSlice = 16384;
 constexpr int kSpare = 8;                        // ids of the lump in front of a slice
 constexpr uint32_t kSaid = 0x80000000u;          // of a count: the id is in the prompt
@@ -245,6 +246,11 @@ cudaError_t adjust(AdjustArgs a, int64_t rows, cudaStream_t stream) {
 // ranks them one by one and draws.  Otherwise (a flat distribution of which much is kept) the rest's bins say about where the cut lies, a second pass sums
 // what is above exactly and lists the ids around, and bins of these alone find it.  Where the guess was wrong, or too many ids are alike, bins over ever narrower intervals of
 // all ids do.  What is near, and the guess, go by the logits' mean and deviation; they decide how long it takes and not what comes out.
+//
+// 251 rows of 128,256 bf16 with top_p 0.9 of a flat distribution: 220 us (10 at the rate of a copy): two passes of 25 to 40 instructions an id, of which 12 in 64 bits, and one of fetching; the instructions
+// bound them.  64 rows of 151,665 fp32 as they are: 32 us.  47 rows of their own wishes: 61.  One row of 50,256 with top_k 50 and top_p 0.95: 18 us, some 12 barriers and exchanges of the cluster.
+// What it took: sums of 64 bits in shared memory by pieces of 32 (as one addition of 64, a loop of comparisons and exchanges, 23,900 us); one thread a place and no branch in the
+// exponential; places found by all warps of a block (by the one whose ids they are among: 60 us more); no conversions and no moving of bits between keys and logits.
 constexpr int kMostBlocks = 8, kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kBins = 256, kGuessBins = 512, kRanked = 512, kPieces = 4;
 constexpr uint32_t kLowest = 0x007FFFFFu;        // key of -infinity
 constexpr uint32_t kHighest = 0xFF800000u;       // key of +infinity

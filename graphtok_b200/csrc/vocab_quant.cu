@@ -53,7 +53,7 @@ struct PackArgs {
     int64_t zeros_stride;
 };
 
-// A warp a pair of units, done once for a table: every byte read and written once, but bytes by bytes.
+// A warp a pair of units, done once for a table: every byte read and written once, but codes byte by byte.
 __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackArgs a) {
     after_previous();
     const int lane = threadIdx.x & 31;
@@ -180,6 +180,7 @@ struct LogitsArgs {
     int rows;                      // of hidden states, at most 8 NT
     int split, split_log;          // warps that share a tile
     bool staged;                   // hidden states fit into shared memory
+    bool pairs;                    // two of them lie on 4 bytes
     int buffers;                   // of partial sums
 };
 
@@ -221,6 +222,7 @@ template <> struct Half16<false> {
 __device__ __forceinline__ uint32_t hidden_pair(const LogitsArgs& a, int n, int64_t col) {
     if (n >= a.rows) return 0;
     const uint16_t* row = a.hidden + n * a.hidden_stride;
+    if (a.pairs) return col < a.width ? *reinterpret_cast<const uint32_t*>(row + col) : 0;
     const uint32_t low = col < a.width ? row[col] : 0, high = col + 1 < a.width ? row[col + 1] : 0;
     return high << 16 | low;
 }
@@ -242,8 +244,10 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
 
 // Up to 8 NT rows of hidden states.  Warps take 64 rows of the table and every `split`th unit of the width; those that share rows add up through
 // shared memory when they are done with them.  Codes come from memory straight into the lanes that multiply with them, kAhead steps before they are
-// needed, across the ends of rows; hidden states lie in shared memory in the order of operands.  What bounds it: memory, and not far below the integer units, which make
-// two codes of a word in 3.5 operations (shift, and-or twice; the subtraction is another unit's) at half of an SM's rate.
+// needed, across the ends of rows; hidden states lie in shared memory in the order of operands.  With 32 x 64 codes an SM's quarter has to do: 56 shifts and and-ors, which go at a warp
+// in two clocks, 32 subtractions in the unit beside it, NT times 8 products of 16 x 8 x 16 of 8 clocks each, and waits 186 clocks for its share of memory.
+// It takes 310 with one row of 128,256 x 4096 in groups of 128: 72 us, 3.7 TB/s (42 at the rate of a copy); 50,256 x 768 11 us.  Four warps a quarter are too few to hide the chain from
+// shift to product, and registers do not allow more.  Lots of 32 rows took 88 us (addresses, scales and waits for half as much), an integer division a lot 13 more.
 template <bool BF16, int NT, int SUBS, bool ZEROS, typename Out>
 __global__ void __launch_bounds__(kThreads, 1) few_rows_kernel(const __grid_constant__ LogitsArgs a) {
     using H = Half16<BF16>;
@@ -299,10 +303,19 @@ __global__ void __launch_bounds__(kThreads, 1) few_rows_kernel(const __grid_cons
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) fetch(lot[s]);
     if (a.staged) {
-        for (int i = tid; i < a.units * 4 * NT * 32; i += kThreads) {
-            const int l = i & 31, nt = (i >> 5) % NT, step = (i >> 5) / NT;
-            const int64_t col = step * 16 + 2 * (l & 3);
-            staged[i] = make_uint2(hidden_pair(a, nt * 8 + l / 4, col), hidden_pair(a, nt * 8 + l / 4, col + 8));
+        constexpr int kAtOnce = 8;             // under way a thread
+        const int all = a.units * 4 * NT * 32;
+        for (int from = tid; from < all; from += kThreads * kAtOnce) {
+            uint2 v[kAtOnce];
+#pragma unroll
+            for (int q = 0; q < kAtOnce; ++q) {
+                const int i = from + q * kThreads, l = i & 31, nt = (i >> 5) % NT, step = (i >> 5) / NT;
+                const int64_t col = step * 16 + 2 * (l & 3);
+                if (i < all) v[q] = make_uint2(hidden_pair(a, nt * 8 + l / 4, col), hidden_pair(a, nt * 8 + l / 4, col + 8));
+            }
+#pragma unroll
+            for (int q = 0; q < kAtOnce; ++q)
+                if (from + q * kThreads < all) staged[from + q * kThreads] = v[q];
         }
         __syncthreads();
     }
@@ -391,7 +404,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_rows_kernel(const __grid_cons
 
 int few_smem(int nt, int units, bool staged, int buffers) { return buffers * kWarps * 8 * nt * kPartLine * 4 + (staged ? units * 4 * nt * 32 * 8 : 0); }
 constexpr int kMostSmem = 227 * 1024;
-// Above them the kernel for more (13 rows of 151,665 x 2560: 95 us here and 131 there; 17 would be two passes here).
+// More rows than 8, and in groups of less than 128 columns than these, go to the other kernel.  (In groups of 128: 128,256 x 4096, 16 rows 113 us here and 111 there; 50,256 x 768 17.8 and
+// 12.3.  Of 64: 151,665 x 2560, 13 rows 100 and 122.  Of 32: 128,256 x 4096, 16 rows 112 and 17 there 330; 50,256 x 768 18 and 21.)
 constexpr int kFewRows = 16;
 
 template <bool BF16, int NT, int SUBS, bool ZEROS, typename Out>
@@ -413,11 +427,14 @@ cudaError_t few_rows(const LogitsArgs& a, int nt, int blocks, cudaStream_t strea
 
 // ---- products with more rows --------------------------------------------------------------
 // As for few rows, with the matrix instruction that takes 256 of the table's rows at a time, two blocks of a cluster half of them each, and all hidden states as columns.
-// Eight warps of a block make 16-bit operands of codes, in registers, and put them into tensor memory, from where the instruction takes them: a stage holds 128 rows x 64 columns.
-// Hidden states come to shared memory by tiled copies, each block half of the rows.  A group's product is taken out of tensor memory by eight more warps and added, with its
-// scale, to sums in registers, while the next group's goes to the other half of the accumulators.
+// A stage is 128 rows x 128 columns of a block.  One warp copies codes to shared memory, one hidden states (each block half of the rows, by tiled copies).  Eight warps, or four, make
+// 16-bit operands of codes, in registers, and put them into tensor memory, from where the instruction takes them.  A group's product is taken out of tensor memory by eight
+// more warps and added, with its scale, to sums in registers, while the next group's goes to the other half of the accumulators.
 //
-// Bound by reading the codes up to some 60 rows, and beyond by this taking out: a row of hidden states costs an addition for each row of the table and group.
+// Groups of 128 and 47 rows of 128,256 x 4096: 126 us (46 at the rate of a copy), 128 rows 139: what the threads hand one another costs some 550 clocks for 64 columns, whatever the rows.  Groups of 32 and
+// 125 rows of 151,665 x 2048: 210 us, taking out, an addition for each hidden state, row of the table and group.  What it took: products issued by one thread in a straight line (as a loop of
+// branches, by that thread or by a whole warp that elects one for each, a stage took two to four times as long); no copy of a loaded register that waits for the load; stages of 128 columns
+// (of 64: 150 us, and 307 in groups of 32).  The warps' own products of 16 x 8 x 16 for up to 64 rows, hidden states streamed through shared memory, took 381 us for 47 rows.
 constexpr int kManyStages = 4, kTakers = 8, kCodeStages = 10, kAheadMeta = 8;
 // Warps that make operands.  In groups of 32 columns the taking out is what is slow, and more of them are in its way: 125 rows of 151,665 x 2048 236 us with eight,
 // 212 with four; in groups of 128, 47 rows of 128,256 x 4096, 128 and 171.
@@ -838,7 +855,7 @@ const char* table_logits(const Matrix& hidden, const Table4& t, const Matrix& ou
     for (int64_t row = 0; row < hidden.rows;) {
         const int64_t left = hidden.rows - row;
         const bool few = few_smem(2, a.units, true, 1) <= kMostSmem;           // two tiles of eight rows are at hand
-        if (left > (few ? kFewRows : 8) && whole) {
+        if (left > (few && t.group < 128 ? kFewRows : 8) && whole) {
             // Rows in equal parts, as a part of few rows costs about what one of many does.
             const int rows = static_cast<int>(div_up(left, div_up(left, kMostColumns))), needed = (rows + 15) / 16 * 8;
             const int columns = needed <= 32 ? needed : needed <= 48 ? 48 : 64;
@@ -855,6 +872,7 @@ const char* table_logits(const Matrix& hidden, const Table4& t, const Matrix& ou
             continue;
         }
         const int nt = left > 8 && few ? 2 : 1;
+        a.pairs = reinterpret_cast<uintptr_t>(hidden.data) % 4 == 0 && hidden.stride % 2 == 0 && hidden.cols % 2 == 0;
         a.staged = few_smem(nt, a.units, true, 1) <= kMostSmem;
         a.buffers = few_smem(nt, a.units, a.staged, 2) <= kMostSmem ? 2 : 1;
         a.rows = static_cast<int>(std::min<int64_t>(left, 8 * nt));
