@@ -535,20 +535,21 @@ struct Row {                       // a block's share of a row
         for (int i = 0; m; ++i, m >>= piece) atomicAdd(&s.pieces[i][b], static_cast<uint32_t>(m) & ((1u << piece) - 1));
     }
     // (behind a barrier)
-    __device__ void tell_bins(int buffer) {
+    __device__ void tell_bins(int buffer, bool masses) {
         for (int b = threadIdx.x; b < kBins; b += kDrawThreads) {
+            s.bin_count[buffer][b] = s.count[b];
+            if (!masses) continue;
             uint64_t m = 0;
 #pragma unroll
             for (int i = kPieces - 1; i >= 0; --i) m = (m << piece) + s.pieces[i][b];
             s.bin_mass[buffer][b] = m;
-            s.bin_count[buffer][b] = s.count[b];
         }
     }
     // (behind the cluster's barrier)
-    __device__ void gather_bins(int buffer) {
+    __device__ void gather_bins(int buffer, bool masses) {
         for (int b = threadIdx.x; b < 2 * kBins; b += kDrawThreads) {
             if (b < kBins) {
-                s.all_mass[b] = over_blocks(&s.bin_mass[buffer][b]);
+                if (masses) s.all_mass[b] = over_blocks(&s.bin_mass[buffer][b]);
             } else {
                 s.all_count[b - kBins] = over_blocks(&s.bin_count[buffer][b - kBins]);
             }
@@ -739,9 +740,9 @@ __device__ __forceinline__ Cut find_cut(Row<T> row, bool by_mass, uint64_t targe
             });
         }
         __syncthreads();
-        row.tell_bins(buffer);
+        row.tell_bins(buffer, by_mass);
         sm100::cluster_sync();
-        row.gather_bins(buffer);
+        row.gather_bins(buffer, by_mass);
         buffer ^= 1;
         const int bin = locate(s, by_mass, target, above);
         if (bin == kBins) {
@@ -960,6 +961,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     const float near_value = value_of(near);
     float rest_end = fmaxf(mean - 3.f * deviation, near_value - 64.f * fmaxf(1.f, heat));
     if (!(rest_end < near_value)) rest_end = near_value - 1.f;
+    const bool weigh = by_p && !by_k;          // the first cut goes by masses, not by numbers
     const bool cuts = by_k || by_p || by_min, guess = by_p && !by_k && near > kLowest + 1 && near < kHighest;
     const Bins<kBins> near_bins(near, row.top, false);
     const Bins<kGuessBins> rest_bins(kLowest + 1, guess ? near - 1 : kLowest + 1, false, rest_end);
@@ -1001,7 +1003,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
                     if (at < a.listed) row.list_key[at] = __float_as_uint(x[q]);
                     else {
                         atomicAdd(&s.count[near_bins(x[q])], 1u);
-                        row.add_mass(near_bins(x[q]), static_cast<uint64_t>(m[q] - kWholeBits));
+                        if (weigh) row.add_mass(near_bins(x[q]), static_cast<uint64_t>(m[q] - kWholeBits));
                     }
                 }
         });
@@ -1010,7 +1012,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
             const float x = __uint_as_float(row.list_key[i]);
             const int b = near_bins(x);
             atomicAdd(&s.count[b], 1u);
-            row.add_mass(b, row.mass(x));
+            if (weigh) row.add_mass(b, row.mass(x));
         }
     }
     mine = warp_sum(mine);
@@ -1018,11 +1020,11 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     uint64_t before = 0;
     if (cuts) {
         __syncthreads();
-        row.tell_bins(0);
+        row.tell_bins(0, weigh);
     }
     const uint64_t total = row.template over_cluster<false>(lane == 0 ? mine : 0, &before);
     if (cuts) {
-        row.gather_bins(0);
+        row.gather_bins(0, weigh);
     }
 
     const auto logprob = [&](float x) {
@@ -1076,8 +1078,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
                 bool keep = here;
                 if (by_k) {
                     keep = keep && placed.place[tid] < top_k;
-                    const uint64_t some = row.template over_warps<false>(keep ? m : 0);
-                    if (tid == 0) s.word[2] = some;
+                    if (here && placed.place[tid] == min(top_k, n) - 1) s.word[2] = placed.in_front[tid] + m;
                     __syncthreads();
                     kept = s.word[2];
                 }

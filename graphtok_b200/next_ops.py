@@ -228,6 +228,12 @@ def _logits_of(logits):
 
 def _pointer(name, t, dtype, shape, index, keep):
     """Address of `t`, one element next to the other, with what keeps its memory alive in `keep`."""
+    try:                                                     # as it mostly is
+        if t.get_device() == index and t.dtype is dtype and t.shape == shape and t.is_contiguous() and not t.is_neg():
+            keep.append(t)
+            return t.data_ptr()
+    except (AttributeError, RuntimeError):
+        pass
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == index and t.layout is torch.strided):
         _on_gpu(keep[0], **{name: t})
     if t.dtype != dtype:
@@ -244,7 +250,7 @@ def _wish(name, value, shape, index, keep, dtype=torch.float32):
     """(a value for each row or 0, one for all)"""
     if not isinstance(value, torch.Tensor):
         return 0, value
-    if value.dtype != dtype or value.shape != shape:
+    if value.dtype is not dtype or value.shape != shape:
         raise ValueError("%s must be a number or %s %s" % (name, str(dtype)[6:], list(shape)))
     return _pointer(name, value, dtype, shape, index, keep), None
 
