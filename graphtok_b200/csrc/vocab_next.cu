@@ -248,7 +248,8 @@ cudaError_t adjust(AdjustArgs a, int64_t rows, cudaStream_t stream) {
 // all ids do.  What is near, and the guess, go by the logits' mean and deviation; they decide how long it takes and not what comes out.
 //
 // 251 rows of 128,256 bf16 with top_p 0.9 of a flat distribution: 220 us (10 at the rate of a copy): two passes of 25 to 40 instructions an id, of which 12 in 64 bits, and one of fetching; the instructions
-// bound them.  64 rows of 151,665 fp32 as they are: 32 us.  47 rows of their own wishes: 61.  One row of 50,256 with top_k 50 and top_p 0.95: 18 us, some 12 barriers and exchanges of the cluster.
+// bound them.  64 rows of 151,665 fp32 as they are: 32 us.  47 rows of their own wishes: 61.  One row of 50,256 with top_k 50 and top_p 0.95: 14 us, six barriers of the cluster and
+// what is said across them; with 32 warps a block, where a block has an SM to itself, 17.
 // What it took: sums of 64 bits in shared memory by pieces of 32 (as one addition of 64, a loop of comparisons and exchanges, 23,900 us); one thread a place and no branch in the
 // exponential; places found by all warps of a block (by the one whose ids they are among: 60 us more); no conversions and no moving of bits between keys and logits.
 constexpr int kMostBlocks = 8, kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kBins = 256, kGuessBins = 512, kRanked = 512, kPieces = 4;

@@ -190,10 +190,17 @@ template <> struct Half16<true> {
     static constexpr uint32_t kBase = 0x43004300u;             // 128 + code, twice
     static __device__ __forceinline__ float lower_half(uint32_t w) { return __uint_as_float(w << 16); }
     static __device__ __forceinline__ float upper_half(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-    static __device__ __forceinline__ uint32_t pair(uint32_t zero) { return kBase + (zero << 16 | zero); }
-    static __device__ __forceinline__ uint32_t minus(uint32_t a, uint32_t b) {
-        const __nv_bfloat162 r = __hsub2(reinterpret_cast<const __nv_bfloat162&>(a), reinterpret_cast<const __nv_bfloat162&>(b));
-        return reinterpret_cast<const uint32_t&>(r);
+    // What is taken from the codes of the upper and of the lower row, twice.
+    static __device__ __forceinline__ uint32_t upper_zero(uint32_t zero) { return kBase + (zero << 16 | zero); }
+    static __device__ __forceinline__ uint32_t lower_zero(uint32_t zero) { return upper_zero(zero); }
+    // The lane's four operand pairs of a word.  A code becomes the lowest bits of 128's mantissa, which has no room for one that lies higher.
+    static __device__ __forceinline__ void operands(uint32_t w, uint32_t upper, uint32_t lower, uint32_t* q) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const uint32_t a = (w >> (4 * p) & 0x000F000Fu) | kBase, &b = p & 1 ? lower : upper;
+            const __nv_bfloat162 r = __hsub2(reinterpret_cast<const __nv_bfloat162&>(a), reinterpret_cast<const __nv_bfloat162&>(b));
+            q[p] = reinterpret_cast<const uint32_t&>(r);
+        }
     }
     static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint2 b) {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -206,10 +213,19 @@ template <> struct Half16<false> {
     static constexpr uint32_t kBase = 0x64006400u;             // 1024 + code, twice
     static __device__ __forceinline__ float lower_half(uint32_t w) { return __low2float(reinterpret_cast<const __half2&>(w)); }
     static __device__ __forceinline__ float upper_half(uint32_t w) { return __high2float(reinterpret_cast<const __half2&>(w)); }
-    static __device__ __forceinline__ uint32_t pair(uint32_t zero) { return kBase + (zero << 16 | zero); }
-    static __device__ __forceinline__ uint32_t minus(uint32_t a, uint32_t b) {
-        const __half2 r = __hsub2(reinterpret_cast<const __half2&>(a), reinterpret_cast<const __half2&>(b));
-        return reinterpret_cast<const uint32_t&>(r);
+    static __device__ __forceinline__ uint32_t upper_zero(uint32_t zero) { return kBase + (zero << 16 | zero); }
+    static __device__ __forceinline__ uint32_t lower_zero(uint32_t zero) { return 0xD400D400u + (zero << 20 | zero << 4); }         // -(64 + zero), twice
+    // 1024's mantissa has room for a code four bits up, too: 1024 + 16 q, of which a 16th less 64 + zero is exact.  One shift in place of three.
+    static __device__ __forceinline__ void operands(uint32_t w, uint32_t upper, uint32_t lower, uint32_t* q) {
+        const uint32_t sixteenth = 0x2C002C00u;
+#pragma unroll
+        for (int p = 0; p < 4; p += 2) {
+            const uint32_t v = w >> (4 * p), a = (v & 0x000F000Fu) | kBase, b = (v & 0x00F000F0u) | kBase;
+            const __half2 r = __hsub2(reinterpret_cast<const __half2&>(a), reinterpret_cast<const __half2&>(upper));
+            const __half2 t = __hfma2(reinterpret_cast<const __half2&>(b), reinterpret_cast<const __half2&>(sixteenth), reinterpret_cast<const __half2&>(lower));
+            q[p] = reinterpret_cast<const uint32_t&>(r);
+            q[p + 1] = reinterpret_cast<const uint32_t&>(t);
+        }
     }
     static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint2 b) {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -244,9 +260,9 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
 
 // Up to 8 NT rows of hidden states.  Warps take 64 rows of the table and every `split`th unit of the width; those that share rows add up through
 // shared memory when they are done with them.  Codes come from memory straight into the lanes that multiply with them, kAhead steps before they are
-// needed, across the ends of rows; hidden states lie in shared memory in the order of operands.  With 32 x 64 codes an SM's quarter has to do: 56 shifts and and-ors, which go at a warp
+// needed, across the ends of rows; hidden states lie in shared memory in the order of operands.  With 32 x 64 codes an SM's quarter has to do: 56 shifts and and-ors (40 in fp16), which go at a warp
 // in two clocks, 32 subtractions in the unit beside it, NT times 8 products of 16 x 8 x 16 of 8 clocks each, and waits 186 clocks for its share of memory.
-// It takes 310 with one row of 128,256 x 4096 in groups of 128: 72 us, 3.7 TB/s (42 at the rate of a copy); 50,256 x 768 11 us.  Four warps a quarter are too few to hide the chain from
+// It takes 310 with one row of 128,256 x 4096 in groups of 128: 73 us, 3.7 TB/s (42 at the rate of a copy); 50,256 x 768 in fp16 10.5 us.  Four warps a quarter are too few to hide the chain from
 // shift to product, and registers do not allow more.  Lots of 32 rows took 88 us (addresses, scales and waits for half as much), an integer division a lot 13 more.
 template <bool BF16, int NT, int SUBS, bool ZEROS, typename Out>
 __global__ void __launch_bounds__(kThreads, 1) few_rows_kernel(const __grid_constant__ LogitsArgs a) {
@@ -346,16 +362,14 @@ __global__ void __launch_bounds__(kThreads, 1) few_rows_kernel(const __grid_cons
 #pragma unroll
                 for (int half = 0; half < kHalves; ++half) {
                     float sum[NT][4] = {};
-                    uint32_t base[2];
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) base[r] = H::pair(ZEROS ? l.zero[half / 2][ZEROS ? sub : 0] >> (16 * (half & 1) + 8 * r) & 15 : 8);
+                    const uint32_t zeros = ZEROS ? l.zero[half / 2][ZEROS ? sub : 0] >> (16 * (half & 1)) : 0x0808u, upper_zero = H::upper_zero(zeros & 15),
+                                   lower_zero = H::lower_zero(zeros >> 8 & 15);
 #pragma unroll
                     for (int k = 0; k < kSteps; ++k) {
                         const int word = sub * kSteps + k;
                         const uint32_t w = word == 0 ? l.code[half].x : word == 1 ? l.code[half].y : word == 2 ? l.code[half].z : l.code[half].w;
                         uint32_t q[4];
-#pragma unroll
-                        for (int p = 0; p < 4; ++p) q[p] = H::minus((w >> (4 * p) & 0x000F000Fu) | H::kBase, base[p & 1]);
+                        H::operands(w, upper_zero, lower_zero, q);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) H::mma(sum[nt], q, b[k][nt]);
                     }
@@ -405,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_rows_kernel(const __grid_cons
 int few_smem(int nt, int units, bool staged, int buffers) { return buffers * kWarps * 8 * nt * kPartLine * 4 + (staged ? units * 4 * nt * 32 * 8 : 0); }
 constexpr int kMostSmem = 227 * 1024;
 // More rows than 8, and in groups of less than 128 columns than these, go to the other kernel.  (In groups of 128: 128,256 x 4096, 16 rows 113 us here and 111 there; 50,256 x 768 17.8 and
-// 12.3.  Of 64: 151,665 x 2560, 13 rows 100 and 122.  Of 32: 128,256 x 4096, 16 rows 112 and 17 there 330; 50,256 x 768 18 and 21.)
+// 12.3.  Of 64: 151,665 x 2560 in fp16, 13 rows 91 and 122.  Of 32: 128,256 x 4096, 16 rows 112 and 17 there 330; 50,256 x 768 18 and 21.)
 constexpr int kFewRows = 16;
 
 template <bool BF16, int NT, int SUBS, bool ZEROS, typename Out>
@@ -583,9 +597,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(many_threads(TWO), 1
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const uint32_t w = k == 0 ? code[half].x : k == 1 ? code[half].y : k == 2 ? code[half].z : code[half].w;
-#pragma unroll
-                        for (int p = 0; p < 4; ++p)
-                            q[half][4 * k + p] = H::minus((w >> (4 * p) & 0x000F000Fu) | H::kBase, H::pair(z[h][TWO ? k >> 1 : 0] >> (16 * half + 8 * (p & 1)) & 15));
+                        const uint32_t zeros = z[h][TWO ? k >> 1 : 0] >> (16 * half);
+                        H::operands(w, H::upper_zero(zeros & 15), H::lower_zero(zeros >> 8 & 15), &q[half][4 * k]);
                     }
                 if (h == 0) {
                     if (handed) hand_over();
