@@ -614,6 +614,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(many_threads(TWO), 1
             handed = full_of_pair + 8 * s;
         }
         if (handed && ok) hand_over();
+        if (!ok) tmem_stored();                // (before tensor memory is given back)
     } else if (warp < kMakers + kTakers) {
         // Products to sums: a warp 32 rows and half of the columns.
         const int quarter = warp & 3, half = (warp - kMakers) >> 2;
