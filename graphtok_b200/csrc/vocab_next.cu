@@ -237,8 +237,10 @@ cudaError_t adjust(AdjustArgs a, int64_t rows, cudaStream_t stream) {
 // the ids, at which the running sum of kept masses is more than u times their sum.
 //
 // A cluster of blocks takes a row.  Where it fits they hold it in shared memory and it is read from memory once; where rows are many, fewer blocks take longer shares,
-// which they read again from L2, and wait for one another less.  Masses are whole numbers, 2^F for the largest, computed in 64 bits and off by 2^-43
-// relative: their sums are exact, do not depend on the order of summation, and where the cuts lie is what arithmetic in 64 bits says.  All three cuts are
+// which they read again from L2, and wait for one another less.  Masses are whole numbers, 2^F for the largest, computed in 64 bits, off by 2^-43
+// relative and rounded to a unit: their sums are exact and do not depend on the order of summation, nor on how many blocks take a row.  F is 46 for up to 2^16 ids, one less for
+// each doubling up to 43 at 2^19, so that sums have 62 bits: all roundings together are 2^-25 of a row's total at most (2^-29 for 128,256 ids).  With more ids F goes by the row, which takes one pass
+// more: as fine as its total allows, up to 50, and the roundings are 2^-27 of it at most.  All three cuts are
 // stretches from the top of one order and so is what they have in common; a cut is the last id that is kept.
 //
 // What a row costs is the exponentials: 11 operations in 64 bits an id, of which an SM does two warps' in a clock.  One pass over all ids gives the total; most rows
@@ -252,18 +254,21 @@ cudaError_t adjust(AdjustArgs a, int64_t rows, cudaStream_t stream) {
 // what is said across them; with 32 warps a block, where a block has an SM to itself, 17.
 // What it took: sums of 64 bits in shared memory by pieces of 32 (as one addition of 64, a loop of comparisons and exchanges, 23,900 us); one thread a place and no branch in the
 // exponential; places found by all warps of a block (by the one whose ids they are among: 60 us more); no conversions and no moving of bits between keys and logits.
-constexpr int kMostBlocks = 8, kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kBins = 256, kGuessBins = 512, kRanked = 512, kPieces = 4;
+constexpr int kMostBlocks = 8, kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kBins = 256, kGuessBins = 512, kRanked = 512, kPieces = 5;
 constexpr uint32_t kLowest = 0x007FFFFFu;        // key of -infinity
 constexpr uint32_t kHighest = 0xFF800000u;       // key of +infinity
 constexpr uint32_t kNone = 0xFFFFFFFFu;          // of a NaN
 constexpr int64_t kWholeBits = 0x4338000000000000ll;             // 1.5 * 2^52: behind sums with it whole numbers stand in the lower bits
+constexpr int kOneUnit = 1 << 19;                // ids of a row up to which F goes by their number alone
+constexpr int kFinest = 50;                      // F at most
+constexpr int kMostShare = 1 << 21;              // ids of a block at most: kPieces pieces make a mass of kFinest bits
 
 struct DrawArgs {
     const void* logits;
     int64_t stride;
     int vocab, segment;            // ids; ids of a warp, a multiple of 32
     int blocks;                    // of a row
-    int fixed;                     // F
+    int fixed;                     // F, in a row of more than kOneUnit ids at least
     int piece;                     // bits of a mass that are added up at a time, in 32: share of a block times 2^piece is no more than 2^32
     int listed;                    // ids that a block can list
     bool held;                     // in shared memory
@@ -811,7 +816,8 @@ __device__ __forceinline__ uint64_t place_of(double u, uint64_t kept) {
     return at < kept ? at : kept - 1;
 }
 
-template <typename T>
+// FINE: rows of more than kOneUnit ids, each with a unit of its own.
+template <typename T, bool FINE>
 __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_constant__ DrawArgs a) {
     extern __shared__ uint4 smem[];
     DrawShared& s = *reinterpret_cast<DrawShared*>(smem);
@@ -936,12 +942,33 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         }
     }
     row.top_value = static_cast<double>(most_value);
-    {
+    int fixed = a.fixed;
+    const auto set_floor = [&] {
         // a logit whose mass is a quarter of a unit, and that it is one that the table's exponents go down to
-        const double down = row.top_value - (a.fixed + 2) * 0.69314718055994531 * static_cast<double>(heat);
+        const double down = row.top_value - (fixed + 2) * 0.69314718055994531 * static_cast<double>(heat);
         row.floor = __double2float_rd(down);
         const double y = (static_cast<double>(row.floor) - row.top_value) * row.steps;
         row.plain = row.top < kHighest && down > -3.4e38 && y <= row.least && y > -32.0 * 900;
+    };
+    set_floor();
+    if constexpr (FINE) {
+        // So many ids that units for all of them alike would be coarse: the total says how fine they may be (it is the same whatever the blocks are).
+        uint64_t mine = 0;
+        row.some([&](const float (&x)[Row<T>::kAtOnce], int) {
+            int64_t m[Row<T>::kAtOnce];
+            row.masses(x, m);
+#pragma unroll
+            for (int q = 0; q < Row<T>::kAtOnce; ++q) mine += static_cast<uint64_t>(m[q] - kWholeBits);
+        });
+        const uint64_t coarse = row.template over_cluster<false>(mine) + a.vocab;
+        int finer = 0;
+        while (fixed + finer < kFinest && coarse << (finer + 1) <= 1ull << 61) ++finer;
+        fixed += finer;
+        row.largest <<= finer;
+        row.least = -32.0 * (fixed + 1);
+        if (tid < 32) s.power[tid] *= static_cast<double>(1 << finer);
+        __syncthreads();
+        set_floor();
     }
 
     const bool by_k = !one && top_k > 0 && top_k < a.vocab, by_p = !one && top_p < 1.f, by_min = !one && min_p > 0.f && row.top < kHighest;
@@ -1030,7 +1057,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
 
     const auto logprob = [&](float x) {
         const double down = row.top == kHighest ? 0.0 : (static_cast<double>(x) - row.top_value) / static_cast<double>(heat);
-        return static_cast<float>(down - log(static_cast<double>(total)) + a.fixed * 0.69314718055994531);
+        return static_cast<float>(down - log(static_cast<double>(total)) + fixed * 0.69314718055994531);
     };
     if (one) {
         if (block == 0 && tid == 0) {
@@ -1127,7 +1154,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
                     const float o = __shfl_up_sync(~0u, run, d);
                     if (tid >= d) run += o;
                 }
-                const float want = static_cast<float>(static_cast<double>(target - above) * exp2(-static_cast<double>(a.fixed)));
+                const float want = static_cast<float>(static_cast<double>(target - above) * exp2(-static_cast<double>(fixed)));
                 const uint32_t reached = __ballot_sync(~0u, run >= want);
                 if (tid == (reached ? __ffs(reached) - 1 : 31)) {
                     float at = run - part;
@@ -1256,7 +1283,7 @@ cudaError_t draw(const DrawArgs& a, int64_t rows, cudaStream_t stream) {
     // Blocks that find an SM each are to have one: no two of them fit.
     int smem = static_cast<int>(sizeof(DrawShared)) + a.listed * 8 + (a.held ? a.segment * kDrawWarps * 4 : 0);
     if (rows * a.blocks <= alone(a.blocks)) smem = std::max(smem, 116 * 1024);
-    auto* kernel = draw_kernel<T>;
+    auto* kernel = a.vocab > kOneUnit ? draw_kernel<T, true> : draw_kernel<T, false>;
     if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024)) return e;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(rows * a.blocks));
@@ -1329,11 +1356,12 @@ const char* sample(const SampleCall& c) {
     // one (1.75 for rows in one block), in as many rounds as it takes.  (47 rows with top-k, top-p and min-p: 76, 49, 42 and 55 us in 1, 2, 4 and 8 blocks; 1 row 75, 45, 31
     // and 24; 251 rows 134, 131, 156 and 221.)
     a.blocks = 1;
+    while (div_up(a.vocab, a.blocks) > kMostShare) a.blocks *= 2;
     const auto cost = [&](int blocks) {
         const int64_t all = c.logits.rows * blocks;
         return (8 + 35 * (a.vocab / 128256.0) / blocks) * (all <= alone(blocks) ? 1 : (blocks == 1 ? 1.75 : 1.5) * div_up(all, 296));
     };
-    for (int blocks = 2; blocks <= kMostBlocks; blocks *= 2)
+    for (int blocks = 2 * a.blocks; blocks <= kMostBlocks; blocks *= 2)
         if (cost(blocks) < cost(a.blocks)) a.blocks = blocks;
     a.segment = static_cast<int>(round_up(div_up(a.vocab, a.blocks * kDrawWarps), 32));
     const auto bits = [](int64_t n) {
@@ -1341,9 +1369,9 @@ const char* sample(const SampleCall& c) {
         while ((1ll << b) < n) ++b;
         return b;
     };
-    // Sums of a row's masses have at most 62 bits, and a mass no more than kPieces pieces.
+    // Sums of a row's masses have at most 62 bits, and a mass no more than kPieces pieces; F depends on the ids alone, not on how many blocks take them.
     a.piece = std::min(16, 32 - bits(a.segment * kDrawWarps));
-    a.fixed = std::min({46, 62 - bits(a.vocab), kPieces * a.piece - 1});
+    a.fixed = std::min(46, 62 - bits(a.vocab));
     for (int i = 0; i < 32; ++i) a.power[i] = std::exp2(a.fixed + i / 32.0);
     // Two blocks to an SM.
     constexpr int64_t kRoom = 113 * 1024 - sizeof(DrawShared);

@@ -1,0 +1,64 @@
+"""The operators from hidden states to ids where it is easy to go wrong: the largest vocabularies, arguments that lie over one another, on a B200."""
+import math
+
+import pytest
+import torch
+
+from test_next_ops import check_draw, model_logits
+from test_vocab_ops import BF16, F32, gen, randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(built):
+    from graphtok_b200 import next_ops
+    return next_ops
+
+
+# ---- an id a row -----------------------------------------------------------------------
+@pytest.mark.parametrize("vocab,depth", [(1 << 24, 25.0), (1 << 24, 17.25), (3000001, 20.0), ((1 << 19) + 1, 18.0), (1 << 19, 18.0)])
+def test_a_flat_tail_far_below_one_logit(ops, vocab, depth):
+    """One likely id, and all others alike and so unlikely that a mass is a few units or none: their share is drawn and cut as it should be, and whatever the number of rows.
+
+    A mass is rounded to a unit of the largest, which is 2^-43 up to 2^19 ids and 2^-50 here beyond (the total is near 1): together they are off by
+    at most 2^19 * 2^-44 and 2^24 * 2^-51, both within 2^-25; masses and u * total are off by 2^-43 and 2^-53 relative."""
+    likely, off = vocab // 13, 2.0 ** -25
+    row = torch.full((1, vocab), -depth, device="cuda")
+    row[0, likely] = 0.0
+    m = math.exp(-depth)
+    total = 1 + (vocab - 1) * m
+    tail = 1 - 1 / total
+    upto = lambda i: ((i + 1) * m + (1 - m if i >= likely else 0)) / total          # noqa: E731
+    points = [0.0, tail / 20, 0.5, 1 - 0.8 * tail, 1 - tail / 3, 1 - 2.0 ** -53]
+    seen = {}
+    for n in (1, 3, 148):
+        u = torch.tensor([points[i % len(points)] for i in range(n)], dtype=torch.float64, device="cuda")
+        ids, logprobs = ops.sample(row.expand(n, vocab), u)
+        for i, (got, logprob) in enumerate(zip(ids.tolist(), logprobs.tolist())):
+            at = points[i % len(points)]
+            assert upto(got - 1) <= at + off and upto(got) >= at - off, (n, at, got)
+            want = math.log((1.0 if got == likely else m) / total)
+            assert abs(logprob - want) <= 1.01 * off + abs(want) * 2.0 ** -24 * 1.01
+            assert seen.setdefault(at, (got, logprob)) == (got, logprob)
+    # a cut inside the tail: the last kept id says where
+    share = float(torch.tensor(1 - 0.4 * tail, dtype=F32))
+    for n in (1, 148):
+        ids, _ = ops.sample(row.expand(n, vocab), torch.full((n,), 1 - 2.0 ** -53, dtype=torch.float64, device="cuda"), top_p=share)
+        got = ids.tolist()
+        assert len(set(got)) == 1 and abs((1 + (got[0] + (got[0] < likely)) * m) / total - share) <= off + 2 * m
+        assert seen.setdefault("cut", got[0]) == got[0]
+
+
+# (blocks of a row for each: 1, 1, 2, 2, 4, 4, 8; none of the shares fits into shared memory)
+@pytest.mark.parametrize("n,vocab,dtype", [(251, 30000, BF16), (160, 50257, F32), (100, 60000, F32), (40, 100000, BF16), (30, 100000, F32), (20, 151665, BF16), (3, 262144, F32)])
+def test_shares_that_are_read_again_from_memory(ops, n, vocab, dtype):
+    """In each number of blocks: flat rows of which much is kept, and rows that begin anywhere in 16 bytes."""
+    for i, wish in enumerate(((1.0, 0, 0.9, 0.0), (0.9, 40, 0.95, 0.0), (1.0, 0, 1.0, 0.0))):
+        logits = model_logits(n + i, n, vocab, dtype)
+        logits[::7] *= 0.01                                  # next to flat
+        u = torch.rand(n, generator=gen(i), device="cuda")
+        ids = check_draw(ops, logits, u, *wish)
+        room = torch.empty(n, vocab + 3, dtype=dtype, device="cuda")
+        room[:, 1:1 + vocab] = logits
+        assert torch.equal(ops.sample(room[:, 1:1 + vocab], u, temperature=wish[0], top_k=wish[1], top_p=wish[2], min_p=wish[3])[0], ids)
