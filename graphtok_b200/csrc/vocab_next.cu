@@ -1057,7 +1057,8 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
 
     const auto logprob = [&](float x) {
         const double down = row.top == kHighest ? 0.0 : (static_cast<double>(x) - row.top_value) / static_cast<double>(heat);
-        return static_cast<float>(down - log(static_cast<double>(total)) + fixed * 0.69314718055994531);
+        // (the total in parts of the largest, which is exact and 1 at least: an id that has all of it gets 0, and none more)
+        return static_cast<float>(down - log(static_cast<double>(total) * __hiloint2double((1023 - fixed) << 20, 0)));
     };
     if (one) {
         if (block == 0 && tid == 0) {

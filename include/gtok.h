@@ -341,7 +341,7 @@ int32_t gtok_x_adjust_logits(const gtok_x_adjustment* args);
 /* An id for each row of logits [n, vocab] (vocab at most 2^24).  With m = exp((l - max) / temperature), ids go in order of falling logits, equal ones in order of rising ids.  The first top_k
  * are kept (all, where it is 0 or less); of these the fewest whose m make up at least top_p of theirs (all, where it is 1 or more; one, where it is 0 or less); of these the ones with m >= min_p;
  * the first in any case.  ids[i] is the first id, in the order of ids, at which the running sum of the kept m exceeds u[i] times their sum (u from 0, below 1); logprobs[i] is
- * the logarithm of its share of all m, kept or not.  Temperature 0 gives the first id and logprob 0.  Sums of masses are exact sums of whole
+ * the logarithm of its share of all m, kept or not, and never above 0.  Temperature 0 gives the first id and logprob 0.  Sums of masses are exact sums of whole
  * numbers, whatever the order and the number of rows; a mass is off by 2^-43 relative, and rounding it to a whole number takes 2^-25 of a row's total at most from all masses together (2^-29 for
  * 128,256 ids).
  * -infinity is never drawn; a row of nothing else gives id -1 and logprob -infinity.  A row with a NaN, or whose temperature is negative or not finite, whose u is outside its range

@@ -62,3 +62,21 @@ def test_shares_that_are_read_again_from_memory(ops, n, vocab, dtype):
         room = torch.empty(n, vocab + 3, dtype=dtype, device="cuda")
         room[:, 1:1 + vocab] = logits
         assert torch.equal(ops.sample(room[:, 1:1 + vocab], u, temperature=wish[0], top_k=wish[1], top_p=wish[2], min_p=wish[3])[0], ids)
+
+
+@pytest.mark.parametrize("n,vocab", [(5, 128256), (5, 151665), (3, 50256), (200, 40000), (4, 7), (2, 600000)])
+def test_no_logprob_is_above_0(ops, n, vocab):
+    """An id that is alone, as a grammar often leaves one, has all of the mass: logprob 0 to the bit, whatever the logit; and others' are not above it."""
+    logits = torch.full((n, vocab), -math.inf, device="cuda")
+    value = torch.tensor([0.0, 7.3, -100.1, 3e38, -3.4e38], device="cuda")[torch.arange(n, device="cuda") % 5]
+    place = torch.randint(0, vocab, (n,), generator=gen(n), device="cuda")
+    logits[torch.arange(n, device="cuda"), place] = value
+    u = torch.rand(n, generator=gen(n + 1), device="cuda")
+    for wish in (dict(), dict(top_k=1), dict(top_k=50, top_p=0.9), dict(top_p=0.9, temperature=0.7), dict(min_p=0.1), dict(top_p=0.0)):
+        ids, logprobs = ops.sample(logits, u, **wish)
+        assert torch.equal(ids.long(), place) and (logprobs.view(torch.int32) == 0).all(), wish
+    # all but the least that numbers tell apart
+    logits.fill_(-36.0)
+    logits[torch.arange(n, device="cuda"), place] = 0.0
+    for wish in (dict(), dict(top_k=1), dict(top_p=0.9), dict(temperature=0.2)):
+        assert (ops.sample(logits, u, **wish)[1] <= 0).all(), wish
