@@ -11,7 +11,8 @@ several streams at once.
     ids, logprobs = sample(logits, torch.rand(len(logits), device="cuda"), temperature=0.8, top_p=0.95)
     text = tokenizer.decode(...)
 
-None of them has a gradient: where one would be asked for, and for dual tensors, they refuse.  torch.compile and torch.export do not look into the operators:
+None of them has a gradient: where one would be asked for, by logits, hidden states, biases, penalties or wishes, they refuse, as they do for dual tensors.  A table in 4 bits is a constant:
+weights and scales that it is made of may require a gradient, and get none from it.  torch.compile and torch.export do not look into the operators:
 compiled code calls them through torch.compiler.disable, between its graphs.
 """
 import ctypes
@@ -152,6 +153,7 @@ def pack_table(codes, scales, zeros=None, group=128):
     if scales.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError("scales must be bfloat16 or float16, not %s" % scales.dtype)
     vocab, width = codes.shape
+    _no_tangents(scales)
     if scales.shape != (vocab, -(-width // group)) or (zeros is not None and zeros.shape != scales.shape):
         raise ValueError("scales and zeros must be [vocab, ceil(width / group)]")
     return _there(index, _pack, _rows(codes), _rows(scales.detach()), None if zeros is None else _rows(zeros), group, index)
@@ -176,6 +178,7 @@ def quantize_table(weight, group=128, zeros=False, dtype=None):
         dtype = torch.bfloat16 if weight.dtype == torch.float32 else weight.dtype
     if dtype not in (torch.bfloat16, torch.float16):
         raise TypeError("dtype must be bfloat16 or float16")
+    _no_tangents(weight)
     return _there(index, _quantize, _rows(weight.detach()), group, bool(zeros), dtype, index)
 
 
@@ -275,7 +278,7 @@ def adjust_logits(logits, ids=None, offsets=None, prompt_lengths=None, repetitio
                  allowed_rows[i] (int32 [n]; negative: none; beyond m: nothing is allowed), or mask i without them
 
     repetition (above 0), presence, frequency: a number, or float32 [n].  out: where to write, `logits` itself included; else a new tensor is returned."""
-    _no_gradient("adjust_logits", logits, bias, out)
+    _no_gradient("adjust_logits", logits, repetition, presence, frequency, bias, out)
     index = _on_gpu(logits, logits=logits)
     _logits_of(logits)
     n, vocab = logits.shape
@@ -363,7 +366,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
 
     temperature, top_p, min_p: a number, or float32 [n]; top_k: a number, or int32 [n].  Where the cuts lie and which id is hit is decided by
     whole numbers of up to 50 bits in place of the m, off by no more than 2^-43 relative and, all of a row's together, 2^-25 of their sum.  A row of -inf only gives id -1 and logprob -inf; a row with a NaN, or one of a tensor's values that makes no sense (a negative temperature, a `u` of 1), gives id -1 and logprob NaN."""
-    _no_gradient("sample", logits)
+    _no_gradient("sample", logits, u, temperature, top_p, min_p)
     index = _on_gpu(logits, logits=logits, u=u)
     _logits_of(logits)
     shape, keep = logits.shape[:1], [logits]

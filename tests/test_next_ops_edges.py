@@ -3,6 +3,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from test_next_ops import check_draw, model_logits
 from test_vocab_ops import BF16, F32, gen, randn
@@ -80,3 +81,16 @@ def test_no_logprob_is_above_0(ops, n, vocab):
     logits[torch.arange(n, device="cuda"), place] = 0.0
     for wish in (dict(), dict(top_k=1), dict(top_p=0.9), dict(temperature=0.2)):
         assert (ops.sample(logits, u, **wish)[1] <= 0).all(), wish
+
+
+# ---- tables in 4 bits -----------------------------------------------------------------------
+def test_a_table_is_a_constant(ops):
+    """Of weights that are being trained, and of no dual ones."""
+    weight = randn(gen(1), 40, 64)
+    want = ops.quantize_table(weight).data
+    assert torch.equal(ops.quantize_table(torch.nn.Parameter(weight)).data, want)
+    codes, scales = torch.zeros(40, 64, dtype=torch.uint8, device="cuda"), torch.ones(40, 1, device="cuda").to(BF16)
+    with forward_ad.dual_level():
+        for call in (lambda: ops.quantize_table(forward_ad.make_dual(weight, weight)), lambda: ops.pack_table(codes, forward_ad.make_dual(scales, scales))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
