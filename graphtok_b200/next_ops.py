@@ -277,7 +277,7 @@ def adjust_logits(logits, ids=None, offsets=None, prompt_lengths=None, repetitio
     masks        allowed: int32 [m, ceil(vocab / 32)], or without the m one for all rows; where bit id % 32 of word id // 32 is 0 the logit becomes -inf, whatever it was.  Row i has mask
                  allowed_rows[i] (int32 [n]; negative: none; beyond m: nothing is allowed), or mask i without them
 
-    repetition (above 0), presence, frequency: a number, or float32 [n].  out: where to write, `logits` itself included; else a new tensor is returned."""
+    repetition (above 0), presence, frequency: a number, or float32 [n]; they need `ids`.  out: where to write, `logits` itself included; else a new tensor is returned."""
     _no_gradient("adjust_logits", logits, repetition, presence, frequency, bias, out)
     index = _on_gpu(logits, logits=logits)
     _logits_of(logits)
@@ -306,6 +306,10 @@ def adjust_logits(logits, ids=None, offsets=None, prompt_lengths=None, repetitio
         freq = 0.0 if frequency_at or one is None else _number("frequency", one)
     elif prompt_lengths is not None:
         raise ValueError("prompt_lengths without ids")
+    else:
+        for name, value, none in (("repetition", repetition, 1.0), ("presence", presence, 0.0), ("frequency", frequency, 0.0)):
+            if isinstance(value, torch.Tensor) or value != none:
+                raise ValueError("%s without ids" % name)
     if (bias_ids is None) != (bias is None):
         raise ValueError("bias_ids and bias go together")
     if bias is not None:

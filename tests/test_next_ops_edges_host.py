@@ -35,3 +35,17 @@ def test_gradients_of_penalties_and_wishes_are_refused(ops):
             call(leaf)
         with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
             call(forward_ad.make_dual(torch.ones(2), torch.ones(2)))
+
+
+def test_penalties_without_a_history_are_refused(ops, monkeypatch):
+    """They would change nothing, whatever they say.  (The checks behind the GPU's are reached as on one.)"""
+    monkeypatch.setattr(ops, "_on_gpu", lambda first, **others: 0)
+    monkeypatch.setattr(ops, "_there", lambda index, f, *args: args[-1])
+    logits = torch.zeros(2, 5)
+    for name, none in (("repetition", 1.0), ("presence", 0.0), ("frequency", 0.0)):
+        for value in (1.2, -1.0, float("nan"), float("inf"), torch.ones(2), torch.ones(3)):
+            with pytest.raises(ValueError, match=name + " without ids"):
+                ops.adjust_logits(logits, **{name: value})
+        assert ops.adjust_logits(logits, **{name: none}) and ops.adjust_logits(logits, **{name: int(none)})
+    with pytest.raises(ValueError, match="prompt_lengths without ids"):
+        ops.adjust_logits(logits, prompt_lengths=torch.zeros(2, dtype=torch.int32))
