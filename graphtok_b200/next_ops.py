@@ -265,6 +265,16 @@ def _number(name, value, least=-_MOST, most=_MOST):
     return value
 
 
+def _lies_over(rows, t):
+    """Whether a row of `rows` has memory with `t`, whose elements follow one another, in common."""
+    n, cols = rows.shape
+    size, begin, long = rows.element_size(), t.data_ptr() - rows.data_ptr(), t.numel() * t.element_size()
+    line = rows.stride(0) * size if n > 1 else cols * size
+    if not (n and long) or begin + long <= 0 or begin >= (n - 1) * line + cols * size:
+        return False
+    return not (begin >= 0 and cols * size <= begin % line <= line - long)           # (between two rows)
+
+
 def adjust_logits(logits, ids=None, offsets=None, prompt_lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias_ids=None, bias=None, allowed=None,
                   allowed_rows=None, out=None):
     """Logits [n, vocab] (float32, bfloat16 or float16) as the requests that they answer ask for them, in this order:
@@ -277,7 +287,8 @@ def adjust_logits(logits, ids=None, offsets=None, prompt_lengths=None, repetitio
     masks        allowed: int32 [m, ceil(vocab / 32)], or without the m one for all rows; where bit id % 32 of word id // 32 is 0 the logit becomes -inf, whatever it was.  Row i has mask
                  allowed_rows[i] (int32 [n]; negative: none; beyond m: nothing is allowed), or mask i without them
 
-    repetition (above 0), presence, frequency: a number, or float32 [n]; they need `ids`.  out: where to write, `logits` itself included; else a new tensor is returned."""
+    repetition (above 0), presence, frequency: a number, or float32 [n]; they need `ids`.  out: where to write, `logits` itself included, apart from all other
+    arguments; else a new tensor is returned."""
     _no_gradient("adjust_logits", logits, repetition, presence, frequency, bias, out)
     index = _on_gpu(logits, logits=logits)
     _logits_of(logits)
@@ -340,6 +351,9 @@ def adjust_logits(logits, ids=None, offsets=None, prompt_lengths=None, repetitio
         same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride() and not logits.is_neg()
         if not same and _overlap(_rows(logits), out):
             raise ValueError("out and logits overlap")
+        for t in keep[1:]:                                   # (blocks would read what others have written)
+            if _lies_over(out, t):
+                raise ValueError("out overlaps another argument")
     result = _there(index, _adjust, logits, out, index, keep, (flat_at, n_ids, bits, entries, offsets_at, prompts_at, rho_at, presence_at, frequency_at, rho, pres, freq, 0,
                                                               bias_ids_at, bias_at, bias_stride, allowed_at, rows_at, count, stride))
     if out is not None:

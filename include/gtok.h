@@ -309,7 +309,7 @@ int32_t gtok_x_table4_pack(const gtok_x_table4* table, const uint8_t* codes, int
 int32_t gtok_x_table4_quantize(const gtok_x_table4* table, const gtok_x_matrix* weight, void* cuda_stream);
 int32_t gtok_x_table4_logits(const gtok_x_matrix* hidden, const gtok_x_table4* table, const gtok_x_matrix* out, void* cuda_stream);
 
-/* Changes to logits [n, vocab], in fp32 and rounded once; `out` has their type and is their memory, with the same stride, or apart from it.  In this order:
+/* Changes to logits [n, vocab], in fp32 and rounded once; `out` has their type and is their memory, with the same stride, or apart from it; it is apart from all else.  In this order:
  *   ids of the row's history: l > 0 becomes l / repetition, others l * repetition; then, for ids that come `count` > 0 times behind the row's first
  *     prompt_lengths (all of them without it), l - frequency * count - presence.  Row i's history is ids[offsets[i]] to ids[offsets[i + 1] - 1] (of `n_ids` in all; `offsets` NULL: none); ids
  *     outside the vocabulary are left out

@@ -49,3 +49,33 @@ def test_penalties_without_a_history_are_refused(ops, monkeypatch):
         assert ops.adjust_logits(logits, **{name: none}) and ops.adjust_logits(logits, **{name: int(none)})
     with pytest.raises(ValueError, match="prompt_lengths without ids"):
         ops.adjust_logits(logits, prompt_lengths=torch.zeros(2, dtype=torch.int32))
+
+
+def test_what_lies_over_an_output(ops):
+    """Against the bytes themselves: every place and length of a list before, in, between and behind the rows of a matrix."""
+    room = torch.zeros(120, dtype=torch.uint8)
+    for n, cols, line in ((1, 10, 10), (1, 10, 30), (3, 10, 10), (3, 10, 17), (2, 4, 30), (0, 5, 5), (2, 1, 1)):
+        rows = room[20:20 + max(n - 1, 0) * line + cols].as_strided((n, cols), (line, 1), 20)
+        taken = {20 + r * line + c for r in range(n) for c in range(cols)}
+        for begin in range(90):
+            for long in (0, 1, 2, 6, 7, 8, 25):
+                assert ops._lies_over(rows, room[begin:begin + long]) == bool(taken & set(range(begin, begin + long))), (n, cols, line, begin, long)
+    wide = torch.zeros(40, dtype=torch.int64)
+    assert ops._lies_over(room[:64].view(torch.float32).view(2, 8), room[60:]) and not ops._lies_over(room[:64].view(torch.float32).view(2, 8), room[64:])
+    assert ops._lies_over(wide.view(torch.float32).view(2, 40), wide[39:]) and not ops._lies_over(wide[:20].view(torch.float32).view(2, 20), wide[20:])
+
+
+def test_an_output_over_another_argument_is_refused(ops, monkeypatch):
+    monkeypatch.setattr(ops, "_on_gpu", lambda first, **others: -1)          # (tensors of the host say that they are on GPU -1)
+    monkeypatch.setattr(ops, "_there", lambda index, f, *args: args[1])
+    room = torch.zeros(400)
+    out, behind = room[:120].view(6, 20), room[120:]
+    logits = torch.zeros(6, 20)
+    ints = lambda t, *shape: t[:torch.Size(shape).numel()].view(torch.int32).view(shape)          # noqa: E731
+    for at in (room, room[100:], room[119:]):
+        for named in (dict(ids=ints(at, 4), offsets=torch.zeros(7, dtype=torch.int32)), dict(ids=torch.zeros(4, dtype=torch.int32), offsets=ints(at, 7)), dict(bias=at[:12].view(6, 2), bias_ids=torch.zeros(6, 2).int()),
+                      dict(bias=torch.zeros(6, 2), bias_ids=ints(at, 6, 2)), dict(allowed=ints(at, 6, 1)), dict(allowed=torch.zeros(2, 1).int(), allowed_rows=ints(at, 6)),
+                      dict(ids=torch.zeros(4, dtype=torch.int32), offsets=torch.zeros(7, dtype=torch.int32), repetition=at[:6])):
+            with pytest.raises(ValueError, match="overlaps another argument"):
+                ops.adjust_logits(logits, out=out, **named)
+    assert ops.adjust_logits(logits, out=out, bias=behind[:12].view(6, 2), bias_ids=ints(behind[12:], 6, 2)) is out
