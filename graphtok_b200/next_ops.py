@@ -348,7 +348,8 @@ def adjust_logits(logits, ids=None, offsets=None, prompt_lengths=None, repetitio
         _on_gpu(logits, out=out)
         if out.shape != logits.shape or out.dtype != logits.dtype or (vocab > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < vocab) or out.is_neg():
             raise ValueError("out must have the logits' shape and type, the elements of a row next to one another and rows apart, and be no view of negated ones")
-        same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride() and not logits.is_neg()
+        # (what one row or one column is apart from the next says nothing)
+        same = (out.data_ptr() == logits.data_ptr() and (n < 2 or out.stride(0) == logits.stride(0)) and (vocab < 2 or out.stride(1) == logits.stride(1)) and not logits.is_neg())
         if not same and _overlap(_rows(logits), out):
             raise ValueError("out and logits overlap")
         for t in keep[1:]:                                   # (blocks would read what others have written)

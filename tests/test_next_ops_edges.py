@@ -94,3 +94,15 @@ def test_a_table_is_a_constant(ops):
         for call in (lambda: ops.quantize_table(forward_ad.make_dual(weight, weight)), lambda: ops.pack_table(codes, forward_ad.make_dual(scales, scales))):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+# ---- penalties, biases, masks -----------------------------------------------------------------
+def test_one_row_in_place_through_two_views(ops):
+    """The last positions of one text: a view of [1, positions, vocab] and one of a single row have different strides."""
+    room = randn(gen(2), 1, 3, 1001)
+    logits, out = room[:, -1], room[0, -1:]
+    allowed = torch.randint(-2 ** 31, 2 ** 31, (32,), generator=gen(3), device="cuda", dtype=torch.int64).int()
+    want = ops.adjust_logits(logits, allowed=allowed)
+    rest = room[:, :-1].clone()
+    assert logits.stride() != out.stride() and ops.adjust_logits(logits, allowed=allowed, out=out) is out
+    assert torch.equal(out, want) and torch.equal(room[:, :-1], rest) and torch.isinf(want).any()

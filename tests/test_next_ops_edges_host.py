@@ -79,3 +79,14 @@ def test_an_output_over_another_argument_is_refused(ops, monkeypatch):
             with pytest.raises(ValueError, match="overlaps another argument"):
                 ops.adjust_logits(logits, out=out, **named)
     assert ops.adjust_logits(logits, out=out, bias=behind[:12].view(6, 2), bias_ids=ints(behind[12:], 6, 2)) is out
+
+
+def test_one_row_is_its_own_memory_whatever_its_stride_says(ops, monkeypatch):
+    monkeypatch.setattr(ops, "_on_gpu", lambda first, **others: -1)
+    monkeypatch.setattr(ops, "_there", lambda index, f, *args: args[1])
+    room = torch.zeros(3, 4, 5)
+    for logits, out in ((room[:1, 0], room[0, :1]), (room[0, :1], room[:1, 0]), (room[:, :1, 0], room[:, 0, :1]), (room[:0, 0], room[:0, 0])):
+        assert logits.shape == out.shape and ops.adjust_logits(logits, out=out) is out
+    for logits, out in ((room[:2, 0], room[0, :2]), (room[:1, 0], room.view(-1)[1:6].view(1, 5))):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.adjust_logits(logits, out=out)
