@@ -8,8 +8,10 @@ several streams at once.
     table = quantize_table(out_table)                          # once
     logits = table_logits(hidden, table)                       # a step: a hidden state for each request
     adjust_logits(logits, ids, offsets, repetition=1.1, out=logits)
-    ids, logprobs = sample(logits, torch.rand(len(logits), device="cuda"), temperature=0.8, top_p=0.95)
-    text = tokenizer.decode(...)
+    new, logprobs = sample(logits, torch.rand(len(logits), device="cuda"), temperature=0.8, top_p=0.95)
+    for answer, i in zip(answers, new.tolist()):
+        answer += [i] if i >= 0 else []                        # (-1: nothing was allowed)
+    text = tokenizer.decode(answers[0])                        # of a whole one; a part may end within a character: decode_bytes
 
 None of them has a gradient: where one would be asked for, by logits, hidden states, biases, penalties or wishes, they refuse, as they do for dual tensors.  A table in 4 bits is a constant:
 weights and scales that it is made of may require a gradient, and get none from it.  torch.compile and torch.export do not look into the operators:

@@ -1,5 +1,7 @@
 """The operators from hidden states to ids where it is easy to go wrong: the largest vocabularies, arguments that lie over one another, on a B200."""
 import math
+import os
+import textwrap
 
 import pytest
 import torch
@@ -106,3 +108,33 @@ def test_one_row_in_place_through_two_views(ops):
     rest = room[:, :-1].clone()
     assert logits.stride() != out.stride() and ops.adjust_logits(logits, allowed=allowed, out=out) is out
     assert torch.equal(out, want) and torch.equal(room[:, :-1], rest) and torch.isinf(want).any()
+
+
+# ---- together -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("where", ["INTEGRATION.md", "docstring"])
+def test_the_step_that_is_shown_runs(ops, where):
+    """As it is written, for two requests of which one's mask leaves nothing, and ids that are not whole characters."""
+    from conftest import ROOT, tiny_vocab
+    from graphtok_b200.gpu_bpe_tokenizer import Tokenizer
+    if where == "docstring":
+        lines = [line for line in ops.__doc__.splitlines() if line.startswith("    ")]
+        shown = textwrap.dedent("\n".join(lines))
+    else:
+        with open(os.path.join(ROOT, where)) as f:
+            shown = next(block.split("```")[0] for block in f.read().split("```python\n") if "next_ops.sample" in block.split("```")[0])
+    tok = Tokenizer(tiny_vocab("llama3"))
+    ids, offsets = tok.encode_batch_to_device(["some text to go on from", "and another one"])
+    some = next(i for i in range(tok.vocab_size) if tok.decode_bytes([i])[0] >= 0x80)
+    weight = randn(gen(5), tok.vocab_size, 64) * 0.3
+    masks = torch.zeros(2, -(-tok.vocab_size // 32), dtype=torch.int32, device="cuda")
+    masks[0, some // 32] = 1 << (some % 32) if some % 32 < 31 else -2 ** 31
+    names = dict(vars(ops), next_ops=ops, torch=torch, tokenizer=tok, ids=ids, offsets=offsets, hidden=randn(gen(6), 2, 64).to(BF16), out_table=weight, answers=[[], []], masks=masks,
+                 states=torch.arange(2, dtype=torch.int32, device="cuda"), prompts=offsets.diff().int(), heat=torch.ones(2, device="cuda"))
+    if where == "docstring":
+        names["tokenizer"].decode = tok.decode_bytes           # (of a whole answer, which one id is not)
+    exec(shown, names)
+    answers = names["answers"]
+    if where == "docstring":
+        assert [len(a) for a in answers] == [1, 1] and names["text"] == tok.decode_bytes(answers[0])
+    else:
+        assert answers == [[some], []] and names["part"] == tok.decode_bytes([some]) and names["new"].tolist() == [some, -1] and names["logprobs"].tolist() == [0.0, -math.inf]
