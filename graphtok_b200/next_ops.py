@@ -93,7 +93,8 @@ def _no_gradient(what, *tensors):
 # ---- tables in 4 bits -------------------------------------------------------------
 class QuantizedTable:
     """A table [vocab, width] in 4 bits, as `quantize_table` and `pack_table` make it: a scale in `dtype` (bfloat16 or float16), and with `zeros` a
-    zero, for every `group` columns of a row.  It lies in `data`, one uint8 tensor, in an order of its own; `to`, copy.deepcopy and torch.save work as on tensors."""
+    zero, for every `group` columns of a row.  It lies in `data`, one uint8 tensor, in an order of its own; `to`, copy.deepcopy, torch.save and (where this module has been
+    imported) torch.load work as on tensors."""
 
     def __init__(self, vocab, width, group, dtype, zeros, device, data=None):
         self.vocab, self.width, self.group, self.dtype, self.zeros = vocab, width, group, dtype, zeros
@@ -130,6 +131,9 @@ class QuantizedTable:
 
     def __repr__(self):
         return "QuantizedTable(%d x %d, group=%d, dtype=%s, zeros=%s, device=%s)" % (self.vocab, self.width, self.group, self.dtype, self.zeros, self.device)
+
+
+torch.serialization.add_safe_globals([QuantizedTable])         # torch.load makes one from its sizes and its memory, which are looked at, and nothing else
 
 
 def _group(group):

@@ -90,3 +90,25 @@ def test_one_row_is_its_own_memory_whatever_its_stride_says(ops, monkeypatch):
     for logits, out in ((room[:2, 0], room[0, :2]), (room[:1, 0], room.view(-1)[1:6].view(1, 5))):
         with pytest.raises(ValueError, match="overlap"):
             ops.adjust_logits(logits, out=out)
+
+
+@pytest.mark.parametrize("dtype,zeros", [(torch.bfloat16, False), (torch.float16, True)])
+def test_tables_are_loaded_as_tensors_are(ops, tmp_path, dtype, zeros):
+    """By torch.load as it is called, beside tensors; and not of another size than theirs."""
+    import pickle
+    table = ops.QuantizedTable(40, 100, 32, dtype, zeros, "cpu")
+    table.data.copy_(torch.randint(0, 256, table.data.shape, generator=torch.Generator().manual_seed(1), dtype=torch.uint8))
+    torch.save({"out": table, "in": torch.ones(3)}, tmp_path / "model")
+    for named in ({}, dict(map_location="cpu"), dict(weights_only=True), dict(weights_only=False), dict(mmap=True)):
+        kept = torch.load(tmp_path / "model", **named)["out"]
+        assert isinstance(kept, ops.QuantizedTable) and torch.equal(kept.data, table.data)
+        assert (kept.shape, kept.group, kept.dtype, kept.zeros) == (table.shape, 32, dtype, zeros)
+    for sizes in ((41, 100, 32), (40, 129, 32), (40, 100, 64), (0, 100, 32), (40, 100, 33)):
+        class Wrong(ops.QuantizedTable):
+            def __reduce__(self):
+                return ops.QuantizedTable, (*sizes, dtype, zeros, None, self.data)
+        wrong = Wrong(40, 100, 32, dtype, zeros, None, table.data)
+        torch.save(wrong, tmp_path / "wrong")
+        if ops._lib().gtok_x_table4_bytes(*sizes, zeros) != table.data.numel():
+            with pytest.raises((ValueError, ops.GTokError, pickle.UnpicklingError)):
+                torch.load(tmp_path / "wrong")
