@@ -89,7 +89,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackA
 // ---- from weights -------------------------------------------------------------------
 // Without zeros: s = max |w| / 7, q = round(w / s) + 8 from 0 to 15.  With zeros: s = (max(w, 0) - min(w, 0)) / 15, b = round(-min(w, 0) / s),
 // q = round(w / s) + b.  Ties to even.  s is rounded to the table's 16 bits first and the codes are of what was rounded; a group of zeros, or
-// one whose scale rounds to 0, has scale 0.  A group with a NaN or an infinity gets the scale NaN.
+// one whose scale rounds to 0, has scale 0.  A group with a NaN or an infinity, or whose scale is beyond the largest of the table's type (in fp16 that of weights from 7 or 15 times 65,520 on), gets
+// the scale NaN.
 struct QuantizeArgs {
     Table4 t;
     Table4Plan p;
@@ -132,7 +133,8 @@ __global__ void __launch_bounds__(256) quantize_kernel(const __grid_constant__ Q
         }
         if (lane == 0) {
             // (in two parts, as the difference of two large numbers may be none)
-            const float s = to_float<T>(from_float<T>((a.t.zeros ? high / 15.f - low / 15.f : fmaxf(high, -low) / 7.f) + bad));
+            float s = to_float<T>(from_float<T>((a.t.zeros ? high / 15.f - low / 15.f : fmaxf(high, -low) / 7.f) + bad));
+            s += s - s;                        // (0, or NaN for an infinite one)
             const int b = a.t.zeros ? (s > 0.f ? static_cast<int>(fminf(fmaxf(rintf(-low / s), 0.f), 15.f)) : 0) : 8;
             scale[r][g - g0] = s;
             zero[r][g - g0] = b;

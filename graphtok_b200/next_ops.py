@@ -174,7 +174,8 @@ def _pack(codes, scales, zeros, group, index):
 
 def quantize_table(weight, group=128, zeros=False, dtype=None):
     """A `QuantizedTable` of `weight` [vocab, width] (float32, bfloat16 or float16), rounded to the nearest of 16 values a group: of 15 on both sides of 0, or with `zeros` of
-    16 between the group's least and largest, 0 among them.  dtype: of the scales and of the hidden states to come, weight's by default (bfloat16 for float32)."""
+    16 between the group's least and largest, 0 among them.  dtype: of the scales and of the hidden states to come, weight's by default (bfloat16 for float32).
+    A group with a NaN, an infinity or more than its scale's type can say gives NaN."""
     group = _group(group)
     index = _on_gpu(weight, weight=weight)
     _table_shape("weight", weight)

@@ -293,7 +293,8 @@ int32_t gtok_x_vocab_loss_backward(const gtok_x_vocab_loss* args);
  * gtok_x_table4_bytes, aligned to 256 bytes, in an order of its own.
  *   pack       from codes (a byte each, of which the low four bits count; rows `codes_stride` apart), scales [vocab, groups of a row] of the table's type, and zeros likewise
  *   quantize   from weights of any type: without zeros s = max |w| / 7, q = round(w / s) + 8; with zeros s = (max(w, 0) - min(w, 0)) / 15, b = round(-min(w, 0) / s),
- *              q = round(w / s) + b; s is rounded to the table's type first, ties go to even, q is held to 0 to 15.  A group with a NaN or an infinity has NaN for a scale
+ *              q = round(w / s) + b; s is rounded to the table's type first, ties go to even, q is held to 0 to 15.  A group with a NaN or an
+ *              infinity, or whose scale would be infinite in the table's type, has NaN for a scale
  *   logits     out[i, v] = sum over the groups of s * (sum over the group's columns of (q - b) * hidden[i, k]), for hidden states of the table's type; out is fp32 or of
  *              that type.  Products are exact and summed in fp32, in an order that depends on the sizes alone.  A row's hidden states touch no other row */
 typedef struct {

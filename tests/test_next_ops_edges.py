@@ -8,7 +8,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 from test_next_ops import check_draw, model_logits
-from test_vocab_ops import BF16, F32, gen, randn
+from test_vocab_ops import BF16, F16, F32, gen, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +138,26 @@ def test_the_step_that_is_shown_runs(ops, where):
         assert [len(a) for a in answers] == [1, 1] and names["text"] == tok.decode_bytes(answers[0])
     else:
         assert answers == [[some], []] and names["part"] == tok.decode_bytes([some]) and names["new"].tolist() == [some, -1] and names["logprobs"].tolist() == [0.0, -math.inf]
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_groups_whose_scale_is_too_large(ops, zeros):
+    """Weights of fp32 beyond what scales in fp16 can say: NaN for the whole group, as where a weight is infinite, and the largest that can be said is."""
+    weight = randn(gen(8), 64, 256)
+    bad = weight.clone()
+    least = 65520.0 * (15 if zeros else 7)                     # rounds to infinity in fp16, what is below does not
+    bad[3, 64:128] = least * 1.0001
+    bad[40, 192] = -1e38
+    weight[3, 70] = weight[40, 200] = math.nan
+    got, want = ops.quantize_table(bad, group=64, zeros=zeros, dtype=F16), ops.quantize_table(weight, group=64, zeros=zeros, dtype=F16)
+    eye = torch.eye(256, device="cuda").half()
+    rows = torch.zeros(64, dtype=torch.bool, device="cuda")
+    rows[3] = rows[40] = True
+    for table in (got, want):
+        values = ops.table_logits(eye, table).T
+        assert values[rows].isnan().all() and values[~rows].isfinite().all()
+    assert torch.equal(got.data, want.data)                    # (a group that is NaN is one whatever it was)
+    bad[3, 64:128] = least * 0.9999
+    bad[40, 192] = 1.0
+    values = ops.table_logits(eye, ops.quantize_table(bad, group=64, zeros=zeros, dtype=F16)).T
+    assert values.isfinite().all() and ((values - bad).abs()[3, 64:128] <= 65504.0 * (1.0 if zeros else 0.5) + least * 2.0 ** -11).all()
