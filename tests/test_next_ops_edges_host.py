@@ -1,4 +1,8 @@
 """Refusals of the operators from hidden states to ids that need no GPU: they come before anything is looked for on one."""
+import ctypes
+import os
+import subprocess
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -112,3 +116,39 @@ def test_tables_are_loaded_as_tensors_are(ops, tmp_path, dtype, zeros):
         if ops._lib().gtok_x_table4_bytes(*sizes, zeros) != table.data.numel():
             with pytest.raises((ValueError, ops.GTokError, pickle.UnpicklingError)):
                 torch.load(tmp_path / "wrong")
+
+
+def places(struct, at=0, head=""):
+    """(name, offset, size) of all that is in a ctypes struct, matrices by their parts."""
+    for name, kind in struct._fields_:
+        field = getattr(struct, name)
+        if hasattr(kind, "_fields_"):
+            yield from places(kind, at + field.offset, head + name + ".")
+        else:
+            yield head + name, at + field.offset, field.size
+
+
+def test_structs_and_packed_structs_are_what_a_c_compiler_makes_of_the_header(ops, tmp_path):
+    """Every member's place and size; and each value of a packed struct, which the calls use, is in the member of its turn."""
+    from conftest import ROOT
+    kinds = {"gtok_x_table4": ops._Table4, "gtok_x_adjustment": ops._Adjustment, "gtok_x_draw": ops._Draw}
+    lines = ["printf(\"%s %%zu\\n\", sizeof(%s));" % (c, c) for c in kinds]
+    for c, struct in kinds.items():
+        lines += ["printf(\"%s %s %%zu %%zu\\n\", offsetof(%s, %s), sizeof(((%s*)0)->%s));" % (c, name, c, name, c, name) for name, _, _ in places(struct)]
+    (tmp_path / "sizes.c").write_text('#include <stddef.h>\n#include <stdio.h>\n#include "gtok.h"\nint main(void) {\n%s\nreturn 0;\n}\n' % "\n".join(lines))
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), "-o", str(tmp_path / "sizes"), str(tmp_path / "sizes.c")], check=True)
+    said = subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout.splitlines()
+    want = ["%s %d" % (c, ctypes.sizeof(struct)) for c, struct in kinds.items()]
+    want += ["%s %s %d %d" % (c, *place) for c, struct in kinds.items() for place in places(struct)]
+    assert said == want
+    for packed, struct in ((ops._ADJUSTMENT, ops._Adjustment), (ops._DRAW, ops._Draw)):
+        names = [name for name, _, _ in places(struct)]
+        memory = bytearray(ctypes.sizeof(struct))
+        assert packed.size == len(memory)
+        packed.pack_into(memory, 0, *range(1, len(names) + 1))
+        got = struct.from_buffer(memory)
+        for i, name in enumerate(names):
+            value = got
+            for part in name.split("."):
+                value = getattr(value, part)
+            assert value == i + 1, name
