@@ -370,7 +370,7 @@ struct Row {                       // a block's share of a row
     const float* held;             // NULL: in memory
     const T* in;
     int first, count, segment;     // first id, ids, ids of a warp
-    int blocks, piece, listed;
+    int blocks, piece;
     uint32_t* list_key;
     int* list_id;
     uint32_t top;                  // key of the largest
@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     const double u = a.wide_u ? static_cast<const double*>(a.u)[r] : static_cast<double>(static_cast<const float*>(a.u)[r]);
 
     Row<T> row{s, a.held ? held : nullptr, static_cast<const T*>(a.logits) + r * a.stride + first, first, max(0, min(share, a.vocab - first)), a.segment, a.blocks, a.piece,
-               a.listed, lists, reinterpret_cast<int*>(lists + a.listed), 0, uint64_t{1} << a.fixed, 0.0, 46.166241308446829 / static_cast<double>(heat), -32.0 * (a.fixed + 1),
+               lists, reinterpret_cast<int*>(lists + a.listed), 0, uint64_t{1} << a.fixed, 0.0, 46.166241308446829 / static_cast<double>(heat), -32.0 * (a.fixed + 1),
                0.f, true, 0};
     if (tid < 32) s.power[tid] = a.power[tid];
     if (tid == 0) s.list_n = 0;

@@ -269,7 +269,6 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
 template <bool BF16, int NT, int SUBS, bool ZEROS, typename Out>
 __global__ void __launch_bounds__(kThreads, 1) few_rows_kernel(const __grid_constant__ LogitsArgs a) {
     using H = Half16<BF16>;
-    using T = typename H::type;
     extern __shared__ uint4 smem[];
     constexpr int kPart = 8 * NT * kPartLine;                  // floats of a warp's partial sums
     float* parts = reinterpret_cast<float*>(smem);             // [buffers][kWarps][kPart]
