@@ -7,7 +7,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
-from test_next_ops import check_draw, model_logits
+from test_next_ops import check_draw, check_logits, model_logits
 from test_vocab_ops import BF16, F16, F32, gen, randn
 
 pytestmark = pytest.mark.gpu
@@ -161,3 +161,78 @@ def test_groups_whose_scale_is_too_large(ops, zeros):
     bad[40, 192] = 1.0
     values = ops.table_logits(eye, ops.quantize_table(bad, group=64, zeros=zeros, dtype=F16)).T
     assert values.isfinite().all() and ((values - bad).abs()[3, 64:128] <= 65504.0 * (1.0 if zeros else 0.5) + least * 2.0 ** -11).all()
+
+
+# ---- the largest, and what every share of a row takes part in ---------------------------------------
+@pytest.mark.parametrize("n,vocab,dtype", [(1, 128256, BF16), (20, 50257, F32), (70, 9000, F16), (60, 100001, BF16), (251, 20000, BF16), (251, 50257, F32), (2, 600001, F32)])
+def test_greedy_rows_in_every_number_of_blocks(ops, n, vocab, dtype):
+    """The first of the largest, wherever it lies: at both ends, once and many times."""
+    logits = randn(gen(n), n, vocab).to(dtype)
+    rows = torch.arange(n, device="cuda")
+    top = float(logits.max()) + 1
+    logits[rows[::3], torch.randint(0, vocab, (len(rows[::3]),), generator=gen(n + 1), device="cuda")] = top
+    logits[rows[1::3], vocab - 1] = top
+    logits[::5, 0] = top
+    u = torch.rand(n, generator=gen(n + 2), device="cuda")
+    want = (logits == logits.amax(1, keepdim=True)).int().argmax(1)
+    shares = torch.log_softmax(logits.double(), 1)[rows, want]
+    for wish, logprobs in ((dict(temperature=0.0), torch.zeros_like(shares)), (dict(temperature=0.0, top_k=5, top_p=0.5, min_p=0.3), torch.zeros_like(shares)), (dict(top_k=1), shares),
+                           (dict(top_p=0.0), shares), (dict(min_p=1.5), shares)):
+        ids, got = ops.sample(logits, u, **wish)
+        assert torch.equal(ids.long(), want), wish
+        # (2^-25 of the total in whole numbers; the softmax in 64 bits)
+        assert ((got.double() - logprobs).abs() <= logprobs.abs() * 2.0 ** -24 * 1.01 + 1.01 * 2.0 ** -25).all(), wish
+
+
+def test_as_many_rows_as_there_may_be(ops):
+    n = 1 << 20
+    logits = randn(gen(4), n, 3)
+    u = torch.rand(n, generator=gen(5), device="cuda", dtype=torch.float64)
+    ids, _ = ops.sample(logits, u)
+    ends = torch.softmax(logits.double(), 1).cumsum(1)
+    sure = (ends - u[:, None]).abs().amin(1) > 1e-9              # (the others are borders, of which 64 bits may say either)
+    assert torch.equal(ids.long()[sure], (ends <= u[:, None]).sum(1)[sure]) and sure.sum() > n - 100
+    allowed = torch.randint(0, 8, (n, 1), generator=gen(6), device="cuda").int()
+    got = ops.adjust_logits(logits, torch.arange(n, device="cuda").int() % 3, torch.arange(n + 1, device="cuda").int(), presence=1.0, allowed=allowed)
+    want = logits.clone()
+    want[torch.arange(n, device="cuda"), torch.arange(n, device="cuda") % 3] -= 1
+    assert torch.equal(got, want.masked_fill((allowed >> torch.arange(3, device="cuda").int()) % 2 == 0, -math.inf))
+    more = torch.zeros(n + 1, 1, device="cuda")
+    for call in (lambda: ops.sample(more, more[:, 0]), lambda: ops.adjust_logits(more)):
+        with pytest.raises(ValueError, match="2\\^20"):
+            call()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_adjust_logits_of_the_largest_vocabulary(ops, dtype):
+    n, vocab = 2, 1 << 24
+    logits = randn(gen(7), n, vocab).to(dtype)
+    ends = torch.tensor([0, 1, 15, 16383, 16384, 16391, vocab // 2, vocab - 16385, vocab - 9, vocab - 1], dtype=torch.int32, device="cuda")
+    ids = torch.cat([ends, ends, ends.flip(0), torch.randint(0, vocab, (5000,), generator=gen(8), device="cuda").int()])
+    allowed = torch.randint(-2 ** 31, 2 ** 31, (1, vocab // 32), generator=gen(9), device="cuda", dtype=torch.int64).int()
+    bias = torch.arange(10, device="cuda") * 0.5
+    got = ops.adjust_logits(logits, ids, torch.tensor([0, 10, len(ids)], dtype=torch.int32, device="cuda"), frequency=0.25, bias_ids=ends, bias=bias, allowed=allowed,
+                            allowed_rows=torch.tensor([-1, 0], dtype=torch.int32, device="cuda"))
+    want = logits.float()
+    for r, some in enumerate((ids[:10], ids[10:])):
+        want[r] -= 0.25 * torch.bincount(some, minlength=vocab)
+        want[r, ends.long()] += bias
+    bit = (allowed[0, :, None] >> torch.arange(32, device="cuda", dtype=torch.int32) & 1).flatten() != 0
+    want[1].masked_fill_(~bit, -math.inf)
+    # (frequencies and biases are quarters: one rounding of fp32 at each of two steps, in the same order, and one to the type)
+    assert torch.equal(got, want.to(dtype))
+
+
+@pytest.mark.parametrize("n", [1, 12, 40])
+def test_tables_of_more_than_4_gib(ops, n):
+    """Places of codes and scales beyond 32 bits: rows all over the table against the formula."""
+    vocab, width = (1 << 23) + 77, 1024
+    codes = torch.randint(0, 16, (vocab, width), generator=gen(10), device="cuda", dtype=torch.uint8)
+    scales = (torch.rand(vocab, width // 64, generator=gen(11), device="cuda") + 0.5).to(BF16)
+    table = ops.pack_table(codes, scales, group=64)
+    assert table.data.numel() > 1 << 32
+    hidden = randn(gen(12), n, width).to(BF16)
+    rows = torch.cat([torch.arange(2000, device="cuda"), torch.randint(0, vocab, (4000,), generator=gen(13), device="cuda"), torch.arange(vocab - 2000, vocab, device="cuda")])
+    got = ops.table_logits(hidden, table)[:, rows]
+    values = scales[rows].double().repeat_interleave(64, 1) * (codes[rows].double() - 8)
+    check_logits(got, hidden, values, 64)
