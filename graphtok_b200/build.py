@@ -56,7 +56,8 @@ def source_hash():
 
 
 def vocab_source_hash():
-    """The same of the operators on a model's tables (profiles/embed_kernels.md, profiles/vocab_products.md)."""
+    """The same of the operators on a model's tables (profiles/embed_kernels.md, profiles/vocab_products.md,
+    profiles/next_kernels.md)."""
     return _hash_of(VOCAB_SOURCES)
 
 

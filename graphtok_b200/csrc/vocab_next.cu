@@ -35,7 +35,8 @@ struct alignas(sizeof(T) * N) Lump {
 // the slice once, the logits of which are on their way meanwhile.  Bound by memory: a logit read and written, a bit of a mask; in place, only what changes.
 // 251 rows of 128,256 bf16 with histories of 12,500 ids, 300 biases and masks: 109 us (22 at the rate of a copy); 44 of it with short histories and nothing else, the rest counting, masks and
 // biases.  A cluster that goes over a history once, each block a part, and counts into one another's shared memory waits for the block with the frequent ids: 266 us, when counting by
-// each block took 220.  Slices of half the size, four blocks to an SM: 173 us where 145.  One row of 128,256 with 911 ids: 3.8 us, all latency.
+// each block took 220.  Slices of half the size, four blocks to an SM: 173 us where 145.  At the 40 registers that three blocks to an SM leave, whole lumps spill 50 to 108 bytes; with two
+// blocks, 64 registers and next to no spills it is 117 us, 47 rows of 151,665 fp32 25.2 where 25.8.  One row of 128,256 with 911 ids: 3.7 us, all latency.
 constexpr int kAdjustThreads = 512, kMostSlice = 16384;
 constexpr int kSpare = 8;                        // ids of the lump in front of a slice
 constexpr uint32_t kSaid = 0x80000000u;          // of a count: the id is in the prompt
@@ -249,9 +250,10 @@ cudaError_t adjust(AdjustArgs a, int64_t rows, cudaStream_t stream) {
 // what is above exactly and lists the ids around, and bins of these alone find it.  Where the guess was wrong, or too many ids are alike, bins over ever narrower intervals of
 // all ids do.  What is near, and the guess, go by the logits' mean and deviation; they decide how long it takes and not what comes out.
 //
-// 251 rows of 128,256 bf16 with top_p 0.9 of a flat distribution: 220 us (10 at the rate of a copy): two passes of 25 to 40 instructions an id, of which 12 in 64 bits, and one of fetching; the instructions
-// bound them.  64 rows of 151,665 fp32 as they are: 32 us.  47 rows of their own wishes: 61.  One row of 50,256 with top_k 50 and top_p 0.95: 14 us, six barriers of the cluster and
-// what is said across them; with 32 warps a block, where a block has an SM to itself, 17.
+// 251 rows of 128,256 bf16 with top_p 0.9 of a flat distribution: 223 us (10 at the rate of a copy): 146 instructions an id in a pass that fetches and two of exponentials and bins, with issue slots in use 64 % of the time by
+// six to seven warps a scheduler.  64 rows of 151,665 fp32 as they are: 33 us, 57 instructions an id in two passes, slots in use 51 %.  47 rows of their own wishes: 61.  One row of 50,256 with top_k 50
+// and top_p 0.95: 14.6 us, a chain of steps of which each waits for the one before; its four barriers of the cluster are 0.9 of it (0.23 each, by themselves).  With 32 warps a block, where a
+// block has an SM to itself, 17.  One row of 2^20 ids as they are: 68 us, 45 without the pass that looks for its unit.
 // What it took: sums of 64 bits in shared memory by pieces of 32 (as one addition of 64, a loop of comparisons and exchanges, 23,900 us); one thread a place and no branch in the
 // exponential; places found by all warps of a block (by the one whose ids they are among: 60 us more); no conversions and no moving of bits between keys and logits.
 constexpr int kMostBlocks = 8, kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kBins = 256, kGuessBins = 512, kRanked = 512, kPieces = 5;

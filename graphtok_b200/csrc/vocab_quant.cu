@@ -265,7 +265,7 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
 // needed, across the ends of rows; hidden states lie in shared memory in the order of operands.  With 32 x 64 codes an SM's quarter has to do: 56 shifts and and-ors (40 in fp16), which go at a warp
 // in two clocks, 32 subtractions in the unit beside it, NT times 8 products of 16 x 8 x 16 of 8 clocks each, and waits 186 clocks for its share of memory.
 // It takes 310 with one row of 128,256 x 4096 in groups of 128: 73 us, 3.7 TB/s (42 at the rate of a copy); 50,256 x 768 in fp16 10.5 us.  Four warps a quarter are too few to hide the chain from
-// shift to product, and registers do not allow more.  Lots of 32 rows took 88 us (addresses, scales and waits for half as much), an integer division a lot 13 more.
+// shift to product, and registers do not allow more (with 9 to 16 rows up to 112 bytes of a thread's are spilled as it is).  Lots of 32 rows took 88 us (addresses, scales and waits for half as much), an integer division a lot 13 more.
 template <bool BF16, int NT, int SUBS, bool ZEROS, typename Out>
 __global__ void __launch_bounds__(kThreads, 1) few_rows_kernel(const __grid_constant__ LogitsArgs a) {
     using H = Half16<BF16>;
@@ -420,7 +420,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_rows_kernel(const __grid_cons
 int few_smem(int nt, int units, bool staged, int buffers) { return buffers * kWarps * 8 * nt * kPartLine * 4 + (staged ? units * 4 * nt * 32 * 8 : 0); }
 constexpr int kMostSmem = 227 * 1024;
 // More rows than 8, and in groups of less than 128 columns than these, go to the other kernel.  (In groups of 128: 128,256 x 4096, 16 rows 113 us here and 111 there; 50,256 x 768 17.8 and
-// 12.3.  Of 64: 151,665 x 2560 in fp16, 13 rows 91 and 122.  Of 32: 128,256 x 4096, 16 rows 112 and 17 there 330; 50,256 x 768 18 and 21.)
+// 12.3.  Of 64: 151,665 x 2560 in fp16, 13 rows 91 and 122.  Of 32, 17 rows in two passes here and there: 50,256 x 768 30 and 21, x 2048
+// 54 and 48, 5,000 x 4096 37 and 31, but 128,256 x 4096 205 and 330: for 17 to 32 rows of the largest tables the rule takes the slower one.)
 constexpr int kFewRows = 16;
 
 template <bool BF16, int NT, int SUBS, bool ZEROS, typename Out>
@@ -447,12 +448,13 @@ cudaError_t few_rows(const LogitsArgs& a, int nt, int blocks, cudaStream_t strea
 // more warps and added, with its scale, to sums in registers, while the next group's goes to the other half of the accumulators.
 //
 // Groups of 128 and 47 rows of 128,256 x 4096: 126 us (46 at the rate of a copy), 128 rows 139: what the threads hand one another costs some 550 clocks for 64 columns, whatever the rows.  Groups of 32 and
-// 125 rows of 151,665 x 2048: 210 us, taking out, an addition for each hidden state, row of the table and group.  What it took: products issued by one thread in a straight line (as a loop of
+// 125 rows of 151,665 x 2048: 212 us; 17 of 128,256 x 4096: 330.  That is 0.36 us for a group of a tile whatever the rows, so neither taking out nor adding bounds it; what is left is the way from a
+// product to the next one that may use its accumulator, of which there are two.  593 tiles are eight for each pair of blocks and a ninth for one.  What it took: products issued by one thread in a straight line (as a loop of
 // branches, by that thread or by a whole warp that elects one for each, a stage took two to four times as long); no copy of a loaded register that waits for the load; stages of 128 columns
 // (of 64: 150 us, and 307 in groups of 32).  The warps' own products of 16 x 8 x 16 for up to 64 rows, hidden states streamed through shared memory, took 381 us for 47 rows.
 constexpr int kManyStages = 4, kTakers = 8, kCodeStages = 10, kAheadMeta = 8;
-// Warps that make operands.  In groups of 32 columns the taking out is what is slow, and more of them are in its way: 125 rows of 151,665 x 2048 236 us with eight,
-// 212 with four; in groups of 128, 47 rows of 128,256 x 4096, 128 and 171.
+// Warps that make operands.  In groups of 32 columns they are not what is waited for, and more of them are in the way: 125 rows of 151,665 x 2048 236 us with eight,
+// 212 with four (fewer rows were not timed); in groups of 128, 47 rows of 128,256 x 4096, 128 and 171.
 __host__ __device__ constexpr int makers(bool two) { return two ? 4 : 8; }
 __host__ __device__ constexpr int many_threads(bool two) { return 32 * (makers(two) + kTakers + 3); }
 constexpr int kMostColumns = 128;          // of hidden states
