@@ -391,7 +391,8 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     Temperature 0: the first id in that order, logprob 0.
 
     temperature, top_p, min_p: a number, or float32 [n]; top_k: a number, or int32 [n].  Where the cuts lie and which id is hit is decided by
-    whole numbers of up to 50 bits in place of the m, off by no more than 2^-43 relative and, all of a row's together, 2^-25 of their sum.  A row of -inf only gives id -1 and logprob -inf; a row with a NaN, or one of a tensor's values that makes no sense (a negative temperature, a `u` of 1), gives id -1 and logprob NaN."""
+    whole numbers of up to 50 bits in place of the m, off by no more than 2^-43 relative and, all of a row's together, 2^-25 of their sum.  A row of -inf only gives
+    id -1 and logprob -inf; a row with a NaN, or one of a tensor's values that makes no sense (a negative temperature, a `u` of 1), gives id -1 and logprob NaN."""
     _no_gradient("sample", logits, u, temperature, top_p, min_p)
     index = _on_gpu(logits, logits=logits, u=u)
     _logits_of(logits)

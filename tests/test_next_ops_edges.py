@@ -236,3 +236,18 @@ def test_tables_of_more_than_4_gib(ops, n):
     got = ops.table_logits(hidden, table)[:, rows]
     values = scales[rows].double().repeat_interleave(64, 1) * (codes[rows].double() - 8)
     check_logits(got, hidden, values, 64)
+
+
+@pytest.mark.parametrize("n,vocab", [(6, 600001), (6, (1 << 21) + 5)])
+def test_rows_with_units_of_their_own(ops, n, vocab):
+    """More than 2^19 ids: all alike, infinities, lowest values, few ids left, nothing left and a NaN, in one call."""
+    g = gen(vocab)
+    logits = randn(g, n, vocab) * 3
+    logits[0] = 2.5
+    logits[1, torch.randint(0, vocab, (1000,), generator=g, device="cuda")] = math.inf
+    logits[2] = torch.where(torch.rand(vocab, generator=g, device="cuda") < 1e-4, logits[2], torch.finfo(F32).min)
+    logits[3] = -math.inf
+    logits[4, vocab // 2] = math.nan
+    u = torch.tensor([0.3, 0.71, 0.5, 0.5, 0.5, 0.93], device="cuda")
+    for wish in ((1.0, 0, 1.0, 0.0), (0.7, 50, 0.9, 0.0), (1.0, 0, 0.75, 0.0), (1.0, 100000, 1.0, 0.0), (1.5, 0, 1.0, 0.02), (1e-30, 0, 0.9, 0.0), (1e30, 0, 0.4, 0.0), (1.0, 1, 1.0, 0.0)):
+        check_draw(ops, logits, u, *wish)
